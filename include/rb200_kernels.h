@@ -376,6 +376,85 @@ RB200_API int rb200k_transpose(const uint8_t* arena, const rb200_pointwise_sampl
                      uint8_t* out, const int32_t out_dims[3], void* stream);
 
 /* ---------------------------------------------------------------------------------------
+ * Head operators: matrix product with epilogue, linear cross entropy, gradient norm
+ * ------------------------------------------------------------------------------------- */
+
+/* What a training or serving step does with the arrays the operators above make: the image batch (float16 NCHW, or
+ * bfloat16 made from it) goes through matrix products, the class indices of the label reader or of the box encoder
+ * (int32) go into a loss, the gradients of both are clipped. The reference leaves this to the framework it feeds.
+ *
+ * Matrices are row-major: element (i, j) at data[i * ld + j], ld in elements. All pointers are device pointers. Rows
+ * that start on 16-byte boundaries (base address and ld * element size multiples of 16) are read in place; any other
+ * operand of a matrix product is first copied into the workspace. Workspaces hold nothing of value between calls and
+ * need no initialisation; two calls that can run at the same time need two workspaces. Results do not depend on
+ * timing: no floating-point atomics are used. Every wait inside these kernels is bounded (see "Bounded waits"); trouble
+ * goes to `status` or, where that is NULL, to the library-wide status word. */
+enum { RB200_BF16 = 16 };   /* element type of the head operators besides RB200_FP16 / RB200_FP32 (not a rocAL type) */
+enum { RB200_ACT_NONE = 0, RB200_ACT_RELU = 1, RB200_ACT_GELU = 2, RB200_ACT_SILU = 3 };
+
+/* out = act(x weight^T + bias) + residual. GELU is z * Phi(z) with the error function. Sums in 32 bits, one rounding
+ * to the element type at the end. residual has residual_rows rows (a divisor of rows): row i of the result takes row
+ * i % residual_rows, so a table of positions is added to every image of a batch. preact, if given, receives
+ * x weight^T + bias rounded to the element type; the backward pass of an activation needs it. */
+typedef struct rb200_linear_params {
+    int32_t dtype;               /* RB200_FP16 or RB200_BF16, of every matrix and vector here */
+    int32_t activation;          /* RB200_ACT_* */
+    int64_t rows, in_features, out_features;   /* >= 0, >= 1, >= 1; at most 2^30 */
+    const void* x;               /* [rows][in_features]         */
+    int64_t ldx;
+    const void* weight;          /* [out_features][in_features] */
+    int64_t ldw;
+    const void* bias;            /* [out_features] or NULL      */
+    const void* residual;        /* [residual_rows][out_features] or NULL */
+    int64_t ldr, residual_rows;
+    void* out;                   /* [rows][out_features]        */
+    int64_t ldo;
+    void* preact;                /* [rows][out_features] or NULL */
+    int64_t ldp;
+    void* workspace;
+    uint64_t workspace_bytes;
+    int32_t* status;             /* device word or NULL */
+} rb200_linear_params;
+
+/* Bytes of workspace that the call with these parameters needs (0 for invalid ones; pointers may still be NULL, but
+ * their alignment and that of the leading dimensions counts). */
+RB200_API uint64_t rb200k_linear_workspace_bytes(const rb200_linear_params* params);
+RB200_API int rb200k_linear(const rb200_linear_params* params, void* stream);
+/* Self-test of the bounded waits, as rb200k_resample_probe: the copies of the contracted axis' blocks (64 elements)
+ * from skip_block on are left out, and waits give up after wait_cycles. */
+RB200_API int rb200k_linear_probe(const rb200_linear_params* params, void* stream, uint64_t wait_cycles, int skip_block);
+
+/* The gradients, each of them only where its pointer is given: with dz = dout * act'(preact),
+ * dx = dz weight, dweight = dz^T x, dbias = column sums of dz, dresidual = sums of dout over the rows that shared a
+ * residual row. */
+typedef struct rb200_linear_backward_params {
+    int32_t dtype, activation;
+    int64_t rows, in_features, out_features;
+    const void* dout;            /* [rows][out_features] */
+    int64_t lddo;
+    const void* x;               /* for dweight */
+    int64_t ldx;
+    const void* weight;          /* for dx */
+    int64_t ldw;
+    const void* preact;          /* with an activation other than none */
+    int64_t ldp;
+    int64_t residual_rows;       /* for dresidual */
+    void* dx;                    /* [rows][in_features] or NULL */
+    int64_t lddx;
+    void* dweight;               /* [out_features][in_features] or NULL */
+    int64_t lddw;
+    void* dbias;                 /* [out_features] or NULL */
+    void* dresidual;             /* [residual_rows][out_features] or NULL */
+    int64_t lddr;
+    void* workspace;
+    uint64_t workspace_bytes;
+    int32_t* status;
+} rb200_linear_backward_params;
+
+RB200_API uint64_t rb200k_linear_backward_workspace_bytes(const rb200_linear_backward_params* params);
+RB200_API int rb200k_linear_backward(const rb200_linear_backward_params* params, void* stream);
+
+/* ---------------------------------------------------------------------------------------
  * Overlapping launches
  * ------------------------------------------------------------------------------------- */
 

@@ -66,6 +66,30 @@ class NormalizeParams(ctypes.Structure):
                 ("arena_bytes", ctypes.c_uint64), ("out_bytes", ctypes.c_uint64)]
 
 
+def _fields(spec):
+    """"p data, q ld, i n" -> ctypes fields; p pointer, q int64, i int32, u uint64, f float, d double."""
+    kinds = {"p": c_void_p, "q": ctypes.c_int64, "i": ctypes.c_int32, "u": ctypes.c_uint64, "f": ctypes.c_float, "d": ctypes.c_double}
+    return [(name, kinds[kind]) for kind, name in (part.split() for part in spec.split(","))]
+
+
+class LinearParams(ctypes.Structure):
+    _fields_ = _fields("i dtype, i activation, q rows, q in_features, q out_features, p x, q ldx, p weight, q ldw, p bias, p residual, "
+                       "q ldr, q residual_rows, p out, q ldo, p preact, q ldp, p workspace, u workspace_bytes, p status")
+
+
+class LinearBackwardParams(ctypes.Structure):
+    _fields_ = _fields("i dtype, i activation, q rows, q in_features, q out_features, p dout, q lddo, p x, q ldx, p weight, q ldw, "
+                       "p preact, q ldp, q residual_rows, p dx, q lddx, p dweight, q lddw, p dbias, p dresidual, q lddr, "
+                       "p workspace, u workspace_bytes, p status")
+
+
+for _name, _params in (("linear", LinearParams), ("linear_backward", LinearBackwardParams)):
+    _f = getattr(lib, "rb200k_%s_workspace_bytes" % _name)
+    _f.argtypes, _f.restype = [ctypes.POINTER(_params)], c_uint64
+    _f = getattr(lib, "rb200k_" + _name)
+    _f.argtypes, _f.restype = [ctypes.POINTER(_params), c_void_p], c_int
+lib.rb200k_linear_probe.argtypes = [ctypes.POINTER(LinearParams), c_void_p, c_uint64, c_int]
+lib.rb200k_linear_probe.restype = c_int
 lib.rb200k_normalize_scratch_bytes.argtypes = [c_int, c_int, c_int, c_int]
 lib.rb200k_normalize_scratch_bytes.restype = ctypes.c_size_t
 lib.rb200k_normalize.argtypes = [c_void_p, c_void_p, c_void_p, c_int, ctypes.POINTER(NormalizeParams), c_void_p, ctypes.c_size_t, c_void_p]

@@ -1,0 +1,225 @@
+// Host side of the matrix products (gemm.cuh): tensor maps, how a product is cut, the plain-epilogue instances, and the
+// small kernels around them (joining split products, packing operands).
+#include "gemm.cuh"
+
+namespace rb200 {
+
+int device_info(DeviceInfo* out) {
+    int dev = 0, rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+    if (rc) return rc;
+    static int sms[64];   // a property of the device; every writer writes the same value
+    if (dev < 0 || dev >= 64) {
+        set_error("device %d: only devices 0..63 are supported", dev);
+        return RB200_E_LIMIT;
+    }
+    int v = __atomic_load_n(&sms[dev], __ATOMIC_RELAXED);
+    if (!v) {
+        rc = check_cuda(cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
+        if (rc) return rc;
+        __atomic_store_n(&sms[dev], v, __ATOMIC_RELAXED);
+    }
+    out->sms = v;
+    return RB200_OK;
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiled encode_tiled() {
+    static EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            p = nullptr;
+        }
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return fn;
+}
+
+int make_map(CUtensorMap* map, const Operand& o, bool bf16, int box_rows, const char* what) {
+    EncodeTiled fn = encode_tiled();
+    if (!fn) {
+        set_error("%s: the driver has no cuTensorMapEncodeTiled", what);
+        return RB200_E_CUDA;
+    }
+    const cuuint64_t dims[2] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows};
+    // the pitch of a single row is never used, but has to be a legal one
+    const cuuint64_t pitch[1] = {(cuuint64_t)(o.rows > 1 ? o.ld : round_up(o.cols, 8)) * 2};
+    const cuuint32_t box[2] = {(cuuint32_t)kTileK, (cuuint32_t)box_rows};
+    const cuuint32_t one[2] = {1, 1};
+    const CUresult rc = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(o.data), dims, pitch,
+                           box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) {
+        set_error("%s: cuTensorMapEncodeTiled refused a %d x %d operand of pitch %lld (%d)", what, o.rows, o.cols, o.ld, (int)rc);
+        return RB200_E_CUDA;
+    }
+    return RB200_OK;
+}
+
+GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed, bool may_split) {
+    GemmPlan p;
+    p.cg = 1;
+    p.kblocks = (k + kTileK - 1) / kTileK;
+    p.splits = 1;
+    const int unit = b_transposed ? 64 : 32;
+    double best = 0;
+    p.bn = kTileNMax;
+    for (int bn = kTileNMax; bn >= unit; bn -= unit) {
+        const long long tiles = ((m + kTileM * p.cg - 1) / (kTileM * p.cg)) * (long long)((n + bn - 1) / bn);
+        const long long slots = dev.sms / p.cg, waves = (tiles + slots - 1) / slots;
+        const double cost = (double)waves * (bn + 32);
+        if (best == 0 || cost < best * 0.98) {
+            best = cost;
+            p.bn = bn;
+        }
+    }
+    p.tiles_m = (m + kTileM * p.cg - 1) / (kTileM * p.cg);
+    p.tiles_n = (n + p.bn - 1) / p.bn;
+    const long long tiles = (long long)p.tiles_m * p.tiles_n;
+    if (may_split && tiles * 2 <= dev.sms && p.kblocks >= 16) {
+        long long s = dev.sms / tiles;
+        if (s > p.kblocks / 8) s = p.kblocks / 8;
+        if (s > 1) p.splits = (int)s;
+    }
+    p.kblocks_per_split = (p.kblocks + p.splits - 1) / p.splits;
+    p.splits = (p.kblocks + p.kblocks_per_split - 1) / p.kblocks_per_split;   // none of them empty
+    return p;
+}
+
+int gemm_args(GemmArgs* g, bool bf16, const Operand& a, const Operand& b, const Operand* b_alt, const int* b_select, const GemmPlan& plan,
+              const EpiArgs& e, const GemmWait& wait, const char* what) {
+    const int m = a.outer(), n = b.outer();
+    g->a_box_rows = kTileM;
+    if (!a.transposed && m < kTileM) g->a_box_rows = (int)round_up(m, 8);
+    const int bn_cta = plan.bn / plan.cg;
+    int rc = make_map(&g->a, a, bf16, a.transposed ? kTileK : g->a_box_rows, what);
+    if (rc) return rc;
+    rc = make_map(&g->b, b, bf16, b.transposed ? kTileK : bn_cta, what);
+    if (rc) return rc;
+    g->b_alt = g->b;
+    g->b_select = b_select;
+    if (b_alt) {
+        rc = make_map(&g->b_alt, *b_alt, bf16, b.transposed ? kTileK : bn_cta, what);
+        if (rc) return rc;
+    }
+    g->m = m;
+    g->n = n;
+    g->bn = plan.bn;
+    g->tiles_m = plan.tiles_m;
+    g->tiles_n = plan.tiles_n;
+    g->splits = plan.splits;
+    g->kblocks = plan.kblocks;
+    g->kblocks_per_split = plan.kblocks_per_split;
+    g->idesc = tc::instr_desc(bf16, a.transposed, b.transposed, kTileM * plan.cg, plan.bn);
+    g->stage_bytes = (uint32_t)(kTileM + bn_cta) * kTileK * 2;
+    const uint32_t room = 196608;   // of the 227 KB: the ring
+    g->stages = room / g->stage_bytes;
+    if (g->stages > 12) g->stages = 12;
+    g->status = wait.status ? wait.status : default_status_word();
+    if (!g->status) {
+        set_error("%s: the library-wide status word could not be found", what);
+        return RB200_E_CUDA;
+    }
+    g->wait_cycles = wait.cycles ? wait.cycles : kDefaultWaitCycles;
+    g->skip_block = wait.skip_block;
+    g->e = e;
+    return RB200_OK;
+}
+
+int gemm_store(int kind, bool bf16, const Operand& a, const Operand& b, const Operand* b_alt, const int* b_select, const GemmPlan& plan,
+               const EpiArgs& e, const GemmWait& wait, cudaStream_t stream, const char* what) {
+    if (kind == GEMM_KK) return gemm_launch<EPI_STORE, false, false>(bf16, a, b, b_alt, b_select, plan, e, wait, stream, what);
+    if (kind == GEMM_KN) return gemm_launch<EPI_STORE, false, true>(bf16, a, b, b_alt, b_select, plan, e, wait, stream, what);
+    return gemm_launch<EPI_STORE, true, true>(bf16, a, b, b_alt, b_select, plan, e, wait, stream, what);
+}
+
+// ---- joining split products -----------------------------------------------------------------------------
+// Pieces are added in their order, so the result does not depend on which CTA finished first.
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ part, int splits, long long stride, long long ldacc, int m, int n,
+                                                   EpiArgs e) {
+    const long long groups = (n + 3) / 4, total = groups * m;
+    const float alpha = e.alpha_const * (e.alpha ? *e.alpha : 1.0f);
+    for (long long t = blockIdx.x * 256ll + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
+        const int row = (int)(t / groups), col = (int)(t - row * groups) * 4;
+        const float* p = part + row * ldacc + col;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s = 0; s < splits; s++) {
+            const float4 f = *reinterpret_cast<const float4*>(p + s * stride);
+            v[0] += f.x;
+            v[1] += f.y;
+            v[2] += f.z;
+            v[3] += f.w;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (col + i >= n) break;
+            float z = v[i] * alpha;
+            if (e.bias) z += Elem<T>::to_float(reinterpret_cast<const T*>(e.bias)[col + i]);
+            if (e.preact) reinterpret_cast<T*>(e.preact)[row * e.ldp + col + i] = Elem<T>::from_float(z);
+            z = act_value(z, e.act);
+            if (e.residual) z += Elem<T>::to_float(reinterpret_cast<const T*>(e.residual)[(long long)(row % e.residual_rows) * e.ldr + col + i]);
+            reinterpret_cast<T*>(e.out)[row * e.ldo + col + i] = Elem<T>::from_float(z);
+        }
+    }
+}
+
+size_t gemm_partial_bytes(const GemmPlan& plan, int m, int n) {
+    return plan.splits > 1 ? (size_t)plan.splits * m * round_up(n, 4) * sizeof(float) : 0;
+}
+
+int gemm_join(bool bf16, const float* partials, int splits, int m, int n, const EpiArgs& e, cudaStream_t stream, const char* what) {
+    const long long ldacc = round_up(n, 4), total = ldacc / 4 * m;
+    const long long blocks = (total + 255) / 256;
+    const unsigned grid = (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16);
+    if (bf16)
+        join_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(partials, splits, ldacc * m, ldacc, m, n, e);
+    else
+        join_kernel<__half><<<grid, 256, 0, stream>>>(partials, splits, ldacc * m, ldacc, m, n, e);
+    RB200_CHECK_LAUNCH(what);
+    return RB200_OK;
+}
+
+int gemm_store_joined(int kind, bool bf16, const Operand& a, const Operand& b, const Operand* b_alt, const int* b_select, const GemmPlan& plan,
+                      EpiArgs e, void* partials, const GemmWait& wait, cudaStream_t stream, const char* what) {
+    if (plan.splits == 1) return gemm_store(kind, bf16, a, b, b_alt, b_select, plan, e, wait, stream, what);
+    const int m = a.outer(), n = b.outer();
+    EpiArgs part = {};
+    part.acc_out = (float*)partials;
+    part.ldacc = round_up(n, 4);
+    part.acc_split_stride = part.ldacc * m;
+    part.alpha_const = 1.0f;
+    int rc = gemm_store(kind, bf16, a, b, b_alt, b_select, plan, part, wait, stream, what);
+    if (rc) return rc;
+    return gemm_join(bf16, (const float*)partials, plan.splits, m, n, e, stream, what);
+}
+
+// ---- packing --------------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) pack_kernel(const uint16_t* __restrict__ src, long long lds, int rows, int cols, uint16_t* __restrict__ dst,
+                                                   long long ldd) {
+    const long long groups = (cols + 7) / 8, total = groups * rows;
+    for (long long t = blockIdx.x * 256ll + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
+        const long long row = t / groups;
+        const int col = (int)(t - row * groups) * 8;
+        const uint16_t* p = src + row * lds + col;
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (col + i < cols) w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+        *reinterpret_cast<uint4*>(dst + row * ldd + col) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+int pack_rows(const Operand& src, void* dst, long long ldd, cudaStream_t stream, const char* what) {
+    const long long total = (long long)((src.cols + 7) / 8) * src.rows, blocks = (total + 255) / 256;
+    pack_kernel<<<(unsigned)(blocks < 148 * 32 ? blocks : 148 * 32), 256, 0, stream>>>((const uint16_t*)src.data, src.ld, src.rows, src.cols,
+                                                                                     (uint16_t*)dst, ldd);
+    RB200_CHECK_LAUNCH(what);
+    return RB200_OK;
+}
+
+}  // namespace rb200

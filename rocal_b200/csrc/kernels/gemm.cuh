@@ -1,0 +1,589 @@
+// Matrix products C[m][n] = sum_k A[m][k] B[n][k] of 16-bit operands with fp32 accumulation on the fifth-generation
+// tensor cores, and what is done with the accumulators before they leave the chip (EPI_*). One persistent kernel:
+//   warp 0      copies operand tiles (128-byte swizzle) into a ring of shared-memory stages,
+//   warp 1      issues the products of a stage (64 contracted elements) into one of two TMEM accumulators,
+//   warps 4-11  read the other accumulator, 32 columns at a time (thread = row), and run the epilogue, so that the
+//               epilogue of a tile overlaps the products of the next.
+// CG = 2: two CTAs (a cluster) work on one tile of 256 rows; each holds its 128 rows of A and half of the B tile, so a
+// tile needs half the shared-memory traffic per product.
+// Either operand may have the contracted axis contiguous (K-major) or the other one (MN-major): the backward products
+// need no transposed copies. Rows and columns beyond the matrices arrive as zeros and are not stored.
+#pragma once
+
+#include "tensor_core.cuh"
+
+namespace rb200 {
+
+constexpr int kTileM = 128, kTileK = 64, kTileNMax = 256;
+constexpr int kGemmThreads = 384, kEpiWarps = 8;
+
+enum { EPI_LINEAR = 0, EPI_STORE = 1, EPI_CE_STATS = 2, EPI_CE_GRAD = 3 };
+enum { ACT_NONE = RB200_ACT_NONE, ACT_RELU = RB200_ACT_RELU, ACT_GELU = RB200_ACT_GELU, ACT_SILU = RB200_ACT_SILU };
+
+// What the epilogues read and write; the fields an epilogue does not name are unused.
+struct EpiArgs {
+    void* out;                // LINEAR, STORE (final): T[m][ldo]; CE_GRAD: T[m][ldo]
+    long long ldo;
+    const void* bias;         // LINEAR, CE_*: T[n] or null
+    const void* residual;     // LINEAR: T[residual_rows][ldr], row i % residual_rows, or null
+    long long ldr;
+    int residual_rows;
+    void* preact;             // LINEAR: T[m][ldp] or null
+    long long ldp;
+    int act;
+    int vec_out, vec_res, vec_pre;   // 1: the rows of that array start on 16-byte boundaries
+    // STORE: value = acc + acc_in; to acc_out (fp32) if that is set, else alpha * value to out.
+    const float* acc_in;
+    float* acc_out;
+    long long ldacc, acc_split_stride;
+    const float* alpha;       // device scalar or null (= 1)
+    float alpha_const;
+    // CE: labels of the rows, the first class of this launch, the ignored label.
+    const int32_t* labels;
+    int class0, ignore_index;
+    float smooth_on, smooth_off;   // 1 - smoothing, smoothing / classes
+    float* part;              // STATS: [parts][m] maxima, then [parts][m] sums, then (smoothing) [parts][m] sums of z
+    int parts, want_zsum;
+    float* zlabel;            // STATS: [m] the label's z
+    const float* stats;       // GRAD: [2][m] maximum and sum
+    const float* coef;        // GRAD: [m] per-row factor or null (= 1)
+};
+
+struct GemmArgs {
+    CUtensorMap a, b, b_alt;   // b_alt replaces b when *b_select is not 0
+    const int* b_select;
+    int m, n;
+    int bn;                    // columns of a tile
+    int tiles_m, tiles_n, splits;
+    int kblocks, kblocks_per_split;
+    int a_box_rows;            // rows of a K-major A copy
+    uint32_t idesc, stage_bytes, stages;
+    int* status;
+    unsigned long long wait_cycles;
+    int skip_block;            // copies of the k-blocks from this one on are left out (-1: none)
+    EpiArgs e;
+};
+
+// ---- 16-bit elements ---------------------------------------------------------------------------------
+template <typename T>
+struct Elem;
+template <>
+struct Elem<__half> {
+    static __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+};
+template <>
+struct Elem<__nv_bfloat16> {
+    static __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t w) {
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    }
+};
+
+__device__ __forceinline__ float act_value(float z, int act) {
+    switch (act) {
+        case ACT_RELU: return z < 0.0f ? 0.0f : z;   // NaN stays
+        case ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678f));
+        case ACT_SILU: return z / (1.0f + __expf(-z));
+        default: return z;
+    }
+}
+__device__ __forceinline__ float act_slope(float z, int act) {
+    switch (act) {
+        case ACT_RELU: return z > 0.0f ? 1.0f : z <= 0.0f ? 0.0f : z;   // NaN stays
+        case ACT_GELU: return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * 0.39894228f * __expf(-0.5f * z * z);
+        case ACT_SILU: {
+            const float g = 1.0f / (1.0f + __expf(-z));
+            return g * (1.0f + z * (1.0f - g));
+        }
+        default: return 1.0f;
+    }
+}
+
+// Columns [col, col + 32) of one row, `count` of them inside the matrix.
+template <typename T>
+__device__ __forceinline__ void store32(T* row, int col, int count, bool vec, const float (&v)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+        if (vec && i + 8 <= count) {
+            uint4 w = make_uint4(Elem<T>::pack(v[i], v[i + 1]), Elem<T>::pack(v[i + 2], v[i + 3]), Elem<T>::pack(v[i + 4], v[i + 5]),
+                                 Elem<T>::pack(v[i + 6], v[i + 7]));
+            *reinterpret_cast<uint4*>(row + col + i) = w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (i + j < count) row[col + i + j] = Elem<T>::from_float(v[i + j]);
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void add32(const T* row, int col, int count, bool vec, float (&v)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+        if (vec && i + 8 <= count) {
+            const uint4 w = __ldg(reinterpret_cast<const uint4*>(row + col + i));
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float2 f = Elem<T>::unpack(u[j]);
+                v[i + 2 * j] += f.x;
+                v[i + 2 * j + 1] += f.y;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (i + j < count) v[i + j] += Elem<T>::to_float(row[col + i + j]);
+        }
+    }
+}
+
+// Running maximum and sum of exp(z - maximum) of one row. A maximum of -inf (every class masked so far) is replaced by
+// 0 in the differences, so that masked classes add exp(-inf) = 0 and no -inf - -inf arises. NaN reaches the sum.
+struct RunningSoftmax {
+    float m, s;
+};
+__device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <typename T, int EPI>
+__device__ __forceinline__ void epilogue_bias(const GemmArgs& g, int col, float* strip, int lane) {
+    if (EPI == EPI_STORE) return;
+    float b = 0.0f;
+    if (g.e.bias && col + lane < g.n) b = Elem<T>::to_float(reinterpret_cast<const T*>(g.e.bias)[col + lane]);
+    __syncwarp();
+    strip[lane] = b;
+    __syncwarp();
+}
+
+template <typename T, bool A_MN, bool B_MN, int EPI, int CG>
+__global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmArgs g) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * 16 + 2 * 2 + 1];
+    __shared__ uint32_t tmem_addr_s;
+    __shared__ int gave_up_s;
+    __shared__ float strips[kEpiWarps][32];
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = CG == 2 ? tc::cta_rank() : 0;
+    const uint32_t smem0 = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t bar0 = tc::smem_u32(bars);
+    const int S = (int)g.stages;
+    auto full = [&](int s) { return bar0 + 8u * s; };
+    auto empty = [&](int s) { return bar0 + 8u * (16 + s); };
+    auto acc_full = [&](int b) { return bar0 + 8u * (32 + b); };
+    auto acc_empty = [&](int b) { return bar0 + 8u * (34 + b); };
+    const uint32_t drained = bar0 + 8u * 36;
+
+    if (threadIdx.x == 0) {
+        gave_up_s = 0;
+        for (int s = 0; s < S; s++) {
+            tc::bar_init(full(s), 1);
+            tc::bar_init(empty(s), 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            tc::bar_init(acc_full(b), 1);
+            tc::bar_init(acc_empty(b), kEpiWarps * CG);
+        }
+        tc::bar_init(drained, 1);
+        tc::bar_init_fence();
+        tc::prefetch_map(&g.a);
+        tc::prefetch_map(&g.b);
+    }
+    if (warp == 2) tc::tmem_alloc<CG>(tc::smem_u32(&tmem_addr_s));
+    tc::fence_before();
+    if constexpr (CG == 2)
+        tc::cluster_sync();
+    else
+        __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = tmem_addr_s;
+    const tc::Patience patience = {&gave_up_s, g.status, g.wait_cycles};
+
+    const long long tiles = (long long)g.tiles_m * g.tiles_n * g.splits;
+    const long long first = blockIdx.x / CG, step = gridDim.x / CG;
+    // Tiles in bands of 8 tile rows, row fastest: the tiles in flight share their operands in L2.
+    auto place = [&](long long t, int& mb, int& nb, int& sp) {
+        const long long per = (long long)g.tiles_m * g.tiles_n;
+        sp = (int)(t / per);
+        const long long r = t - sp * per;
+        const long long band = r / (8ll * g.tiles_n);
+        const int rows = min(8, g.tiles_m - (int)band * 8);
+        const int q = (int)(r - band * 8 * g.tiles_n);
+        nb = q / rows;
+        mb = (int)band * 8 + q - nb * rows;
+    };
+    const int bn_cta = g.bn / CG;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const CUtensorMap* map_b = (g.b_select && *g.b_select) ? &g.b_alt : &g.b;
+            int s = 0;
+            uint32_t phase = 0;
+            long long filled = 0;
+            bool ok = true;
+            for (long long t = first; t < tiles && ok; t += step) {
+                int mb, nb, sp;
+                place(t, mb, nb, sp);
+                const int m0 = mb * (kTileM * CG) + (int)rank * kTileM, n0 = nb * g.bn + (int)rank * bn_cta;
+                const int k_end = min(g.kblocks, (sp + 1) * g.kblocks_per_split);
+                for (int kb = sp * g.kblocks_per_split; kb < k_end; kb++) {
+                    ok = tc::bar_wait(empty(s), phase ^ 1, patience);
+                    if (!ok) break;
+                    const uint32_t sa = smem0 + s * g.stage_bytes, sb = sa + kTileM * kTileK * 2;
+                    uint32_t bar = full(s);
+                    if constexpr (CG == 2) bar = tc::map_to_rank(bar, 0);
+                    if (rank == 0) {
+                        const uint32_t a_bytes = A_MN ? kTileM * kTileK * 2 : g.a_box_rows * kTileK * 2;
+                        tc::bar_expect(full(s), CG * (a_bytes + bn_cta * kTileK * 2));
+                    }
+                    if (g.skip_block < 0 || kb < g.skip_block) {
+                        if constexpr (A_MN) {
+                            tc::tma_load<CG>(sa, &g.a, m0, kb * kTileK, bar);
+                            tc::tma_load<CG>(sa + 64 * kTileK * 2, &g.a, m0 + 64, kb * kTileK, bar);
+                        } else {
+                            tc::tma_load<CG>(sa, &g.a, kb * kTileK, m0, bar);
+                        }
+                        if constexpr (B_MN) {
+                            for (int j = 0; j < bn_cta; j += 64) tc::tma_load<CG>(sb + j * kTileK * 2, map_b, n0 + j, kb * kTileK, bar);
+                        } else {
+                            tc::tma_load<CG>(sb, map_b, kb * kTileK, n0, bar);
+                        }
+                    }
+                    filled++;
+                    if (++s == S) {
+                        s = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+            if (!ok && rank == 0) {   // copies still on their way into this CTA's (and its peer's) stages
+                for (int i = 0; i < S && i < filled; i++) {
+                    if (s == 0) {
+                        s = S;
+                        phase ^= 1;
+                    }
+                    s--;
+                    tc::bar_drain(full(s), phase, g.wait_cycles);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            int s = 0, buf = 0;
+            uint32_t phase = 0, acc_phase = 0;
+            bool ok = true, issued = false;
+            for (long long t = first; t < tiles && ok; t += step) {
+                int mb, nb, sp;
+                place(t, mb, nb, sp);
+                const int k_begin = sp * g.kblocks_per_split, k_end = min(g.kblocks, (sp + 1) * g.kblocks_per_split);
+                ok = tc::bar_wait(acc_empty(buf), acc_phase ^ 1, patience);
+                if (!ok) break;
+                tc::fence_after();
+                const uint32_t d = tmem + buf * kTileNMax;
+                for (int kb = k_begin; kb < k_end; kb++) {
+                    ok = tc::bar_wait(full(s), phase, patience);
+                    if (!ok) break;
+                    tc::fence_after();
+                    const uint32_t sa = smem0 + s * g.stage_bytes, sb = sa + kTileM * kTileK * 2;
+                    const uint64_t da = tc::operand_desc(sa, A_MN, 64 * kTileK * 2), db = tc::operand_desc(sb, B_MN, 64 * kTileK * 2);
+#pragma unroll
+                    for (int k = 0; k < kTileK / 16; k++)
+                        tc::mma_f16<CG>(d, da + k * (A_MN ? 2048 >> 4 : 32 >> 4), db + k * (B_MN ? 2048 >> 4 : 32 >> 4), g.idesc,
+                                        (kb > k_begin || k > 0) ? 1u : 0u);
+                    issued = true;
+                    tc::mma_commit<CG>(empty(s));
+                    if (++s == S) {
+                        s = 0;
+                        phase ^= 1;
+                    }
+                }
+                if (!ok) break;
+                tc::mma_commit<CG>(acc_full(buf));
+                buf ^= 1;
+                acc_phase ^= buf == 0;
+            }
+            if (!ok && issued) {   // products still running when the CTA gives up
+                tc::mma_commit<CG>(drained);
+                tc::bar_drain(drained, 0, g.wait_cycles);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        const int ew = warp - 4, quarter = warp & 3, half = ew >> 2;
+        float* strip = strips[ew];
+        int buf = 0;
+        uint32_t acc_phase = 0;
+        for (long long t = first; t < tiles; t += step) {
+            int mb, nb, sp;
+            place(t, mb, nb, sp);
+            // the lanes leave together: what follows needs whole warps
+            if (!__all_sync(0xFFFFFFFFu, tc::bar_wait(acc_full(buf), acc_phase, patience))) break;
+            tc::fence_after();
+            const int row = mb * (kTileM * CG) + (int)rank * kTileM + quarter * 32 + lane;
+            const bool row_ok = row < g.m;
+            const int n0 = nb * g.bn;
+            const uint32_t acc = tmem + buf * kTileNMax + ((uint32_t)(quarter * 32) << 16);
+
+            int label = -1, res_row = 0;
+            bool counted = false;
+            float cmax = 0.0f, cscale = 0.0f;
+            RunningSoftmax run = {-INFINITY, 0.0f};
+            float zsum = 0.0f;
+            if constexpr (EPI == EPI_CE_STATS || EPI == EPI_CE_GRAD) {
+                if (row_ok) {
+                    label = g.e.labels[row];
+                    counted = label != g.e.ignore_index;
+                    label -= g.e.class0;
+                }
+                if constexpr (EPI == EPI_CE_GRAD) {
+                    if (counted) {
+                        cmax = finite_max(g.e.stats[row]);
+                        cscale = (g.e.coef ? g.e.coef[row] : 1.0f) * 32768.0f;
+                    }
+                }
+            }
+            float inv_sum = 0.0f;
+            if constexpr (EPI == EPI_CE_GRAD) {
+                if (counted) inv_sum = 1.0f / g.e.stats[(long long)g.m + row];
+            }
+            if constexpr (EPI == EPI_LINEAR) {
+                if (g.e.residual && row_ok) res_row = row % g.e.residual_rows;
+            }
+            float alpha = 1.0f;
+            if constexpr (EPI == EPI_STORE) alpha = g.e.alpha_const * (g.e.alpha ? *g.e.alpha : 1.0f);
+
+            for (int c = half * 32; c < g.bn; c += 64) {
+                const int col = n0 + c, count = g.n - col;   // columns of this strip inside the matrix (may be <= 0)
+                uint32_t raw[32];
+                tc::tmem_load32(acc + c, raw);
+                epilogue_bias<T, EPI>(g, col, strip, lane);
+                tc::tmem_wait();
+                if (count <= 0) continue;
+                float v[32];
+#pragma unroll
+                for (int i = 0; i < 32; i++) v[i] = __uint_as_float(raw[i]);
+                if constexpr (EPI != EPI_STORE) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 b = *reinterpret_cast<const float4*>(strip + i);
+                        v[i] += b.x;
+                        v[i + 1] += b.y;
+                        v[i + 2] += b.z;
+                        v[i + 3] += b.w;
+                    }
+                }
+                if constexpr (EPI == EPI_LINEAR) {
+                    if (row_ok) {
+                        if (g.e.preact)
+                            store32(reinterpret_cast<T*>(g.e.preact) + (long long)row * g.e.ldp, col, count, g.e.vec_pre, v);
+                        if (g.e.act != ACT_NONE) {
+#pragma unroll
+                            for (int i = 0; i < 32; i++) v[i] = act_value(v[i], g.e.act);
+                        }
+                        if (g.e.residual)
+                            add32(reinterpret_cast<const T*>(g.e.residual) + (long long)res_row * g.e.ldr, col, count, g.e.vec_res, v);
+                        store32(reinterpret_cast<T*>(g.e.out) + (long long)row * g.e.ldo, col, count, g.e.vec_out, v);
+                    }
+                }
+                if constexpr (EPI == EPI_STORE) {
+                    if (row_ok) {
+                        const long long at = (long long)row * g.e.ldacc + col;
+                        if (g.e.acc_in) {
+#pragma unroll
+                            for (int i = 0; i < 32; i++)
+                                if (i < count) v[i] += g.e.acc_in[at + i];
+                        }
+                        if (g.e.acc_out) {
+                            float* o = g.e.acc_out + (long long)sp * g.e.acc_split_stride + at;
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4) {   // ldacc is a multiple of 4: the row's padding takes the rest
+                                if (i < count) *reinterpret_cast<float4*>(o + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; i++) v[i] *= alpha;
+                            store32(reinterpret_cast<T*>(g.e.out) + (long long)row * g.e.ldo, col, count, g.e.vec_out, v);
+                        }
+                    }
+                }
+                if constexpr (EPI == EPI_CE_STATS) {
+                    if (row_ok && label >= col && label < col + 32 && label < g.n) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++)
+                            if (label == col + i) g.e.zlabel[row] = v[i];
+                    }
+                    float top = run.m;
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        if (i >= count) v[i] = -INFINITY;
+                        top = fmaxf(top, v[i]);
+                    }
+                    if (g.e.want_zsum) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++)
+                            if (i < count) zsum += v[i];
+                    }
+                    const float base = finite_max(top);
+                    run.s *= exp2f((run.m - base) * kLog2e);
+                    run.m = top;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 32; i++) sum += exp2f((v[i] - base) * kLog2e);
+                    run.s += sum;
+                }
+                if constexpr (EPI == EPI_CE_GRAD) {
+                    if (row_ok) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            float p = exp2f((v[i] - cmax) * kLog2e) * inv_sum - g.e.smooth_off;
+                            if (label == col + i) p -= g.e.smooth_on;
+                            v[i] = counted ? p * cscale : 0.0f;
+                        }
+                        store32(reinterpret_cast<T*>(g.e.out) + (long long)row * g.e.ldo, col, count, g.e.vec_out, v);
+                    }
+                }
+            }
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::bar_arrive_cluster(CG == 2 ? tc::map_to_rank(acc_empty(buf), 0) : acc_empty(buf));
+            if constexpr (EPI == EPI_CE_STATS) {
+                if (row_ok) {
+                    const long long plane = (long long)g.e.parts * g.m, at = (long long)(2 * nb + half) * g.m + row;
+                    g.e.part[at] = run.m;
+                    g.e.part[plane + at] = run.s;
+                    if (g.e.want_zsum) g.e.part[2 * plane + at] = zsum;
+                }
+            }
+            buf ^= 1;
+            acc_phase ^= buf == 0;
+        }
+        __syncwarp();
+    }
+    tc::fence_before();
+    if constexpr (CG == 2)
+        tc::cluster_sync();
+    else
+        __syncthreads();
+    tc::fence_after();
+    if (warp == 2) tc::tmem_free<CG>(tmem);
+}
+
+// ---- host side -----------------------------------------------------------------------------------------
+// One operand: `rows` x `cols` elements, row r at data + r * ld, columns contiguous. transposed = false: rows are the
+// product's m or n, columns its contracted axis; true: the other way round.
+struct Operand {
+    const void* data;
+    long long ld;
+    int rows, cols;
+    bool transposed;
+    int outer() const { return transposed ? cols : rows; }
+    int inner() const { return transposed ? rows : cols; }
+};
+
+struct DeviceInfo {
+    int sms;
+};
+int device_info(DeviceInfo* out);   // of the current device; 0 or an error code
+int make_map(CUtensorMap* map, const Operand& o, bool bf16, int box_rows, const char* what);
+// Rows on 16-byte boundaries, as a tensor-map copy needs them.
+static inline bool map_ready(const Operand& o) {
+    return ((uintptr_t)o.data & 15) == 0 && (o.rows <= 1 || (o.ld & 7) == 0);
+}
+
+// How a product is cut: columns per tile, CTAs per tile, pieces of the contracted axis.
+struct GemmPlan {
+    int bn, cg, splits, tiles_m, tiles_n, kblocks, kblocks_per_split;
+};
+GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed, bool may_split);
+
+template <typename T, bool A_MN, bool B_MN, int EPI, int CG>
+int gemm_launch_as(const GemmArgs& g, const DeviceInfo& dev, cudaStream_t stream, const char* what) {
+    auto* kernel = gemm_kernel<T, A_MN, B_MN, EPI, CG>;
+    const size_t smem = (size_t)g.stages * g.stage_bytes + 1024;
+    int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), what);
+    if (rc) return rc;
+    const long long tiles = (long long)g.tiles_m * g.tiles_n * g.splits, slots = dev.sms / CG;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((tiles < slots ? tiles : slots) * CG));
+    cfg.blockDim = dim3(kGemmThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CG;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = CG == 2 ? 1 : 0;
+    rc = check_cuda(cudaLaunchKernelEx(&cfg, kernel, g), what);
+    if (rc) return rc;
+    count_launch();
+    return RB200_OK;
+}
+
+// Waits of a product: default limit, no self-test.
+struct GemmWait {
+    int* status;
+    unsigned long long cycles;
+    int skip_block;
+};
+
+// Fills the launch block. Both operands are map_ready.
+int gemm_args(GemmArgs* g, bool bf16, const Operand& a, const Operand& b, const Operand* b_alt, const int* b_select, const GemmPlan& plan,
+              const EpiArgs& e, const GemmWait& wait, const char* what);
+
+template <int EPI, bool A_MN, bool B_MN>
+int gemm_launch(bool bf16, const Operand& a, const Operand& b, const Operand* b_alt, const int* b_select, const GemmPlan& plan, const EpiArgs& e,
+                const GemmWait& wait, cudaStream_t stream, const char* what) {
+    GemmArgs g;
+    DeviceInfo dev;
+    int rc = device_info(&dev);
+    if (rc) return rc;
+    rc = gemm_args(&g, bf16, a, b, b_alt, b_select, plan, e, wait, what);
+    if (rc) return rc;
+    if (plan.cg == 2)
+        return bf16 ? gemm_launch_as<__nv_bfloat16, A_MN, B_MN, EPI, 2>(g, dev, stream, what)
+                    : gemm_launch_as<__half, A_MN, B_MN, EPI, 2>(g, dev, stream, what);
+    return bf16 ? gemm_launch_as<__nv_bfloat16, A_MN, B_MN, EPI, 1>(g, dev, stream, what)
+                : gemm_launch_as<__half, A_MN, B_MN, EPI, 1>(g, dev, stream, what);
+}
+
+// The products with a plain epilogue (gemm.cu): x w^T (KK), dz w (KN), dz^T x (NN: both operands transposed).
+enum { GEMM_KK = 0, GEMM_KN = 1, GEMM_NN = 2 };
+int gemm_store(int kind, bool bf16, const Operand& a, const Operand& b, const Operand* b_alt, const int* b_select, const GemmPlan& plan,
+               const EpiArgs& e, const GemmWait& wait, cudaStream_t stream, const char* what);
+// The same including the second launch that joins the pieces of a split product. `partials`: gemm_partial_bytes of the plan.
+size_t gemm_partial_bytes(const GemmPlan& plan, int m, int n);
+int gemm_store_joined(int kind, bool bf16, const Operand& a, const Operand& b, const Operand* b_alt, const int* b_select, const GemmPlan& plan,
+                      EpiArgs e, void* partials, const GemmWait& wait, cudaStream_t stream, const char* what);
+// Joins the pieces: sum over splits, then bias, activation, residual (or alpha) and the conversion.
+int gemm_join(bool bf16, const float* partials, int splits, int m, int n, const EpiArgs& e, cudaStream_t stream, const char* what);
+// dst[rows][ldd] = src, for operands whose rows no tensor map can describe.
+int pack_rows(const Operand& src, void* dst, long long ldd, cudaStream_t stream, const char* what);
+
+static inline long long round_up(long long v, long long to) { return (v + to - 1) / to * to; }
+
+// Carves 256-byte aligned pieces out of a workspace; with base == nullptr it only counts.
+struct Carver {
+    uint8_t* base;
+    size_t used = 0;
+    explicit Carver(void* b) : base((uint8_t*)b) {}
+    void* take(size_t bytes) {
+        void* p = base ? base + used : nullptr;
+        used += (size_t)round_up((long long)bytes, 256);
+        return p;
+    }
+};
+
+}  // namespace rb200

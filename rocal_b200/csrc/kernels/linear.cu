@@ -1,0 +1,476 @@
+// rb200k_linear: out = act(x W^T + b) + r, and its gradients. The products run on the tensor cores (gemm.cuh); the
+// passes over the gradient of the output that the products do not make (activation slope, column sums, sums over rows
+// that share a residual row) are memory-bound and made by rows_kernel in one sweep.
+#include "gemm.cuh"
+
+namespace rb200 {
+
+// ---- sweeps over a gradient matrix ------------------------------------------------------------------------
+// Rows j, j + period, j + 2 period, ... of `src` are summed into partial sums [chunk][j][column] in 32 bits; with
+// `preact` the elements are first multiplied by the activation's slope, and with `dst` what was read (multiplied) is
+// written, in the element type. A block takes 256 columns (a warp reads 512 contiguous bytes of a row) and a chunk of
+// the repeats, 8 rows at a time; its 8 row sums meet in shared memory, chunks meet in sum_chunks_kernel, always in the
+// same order.
+struct RowsArgs {
+    const void* src;
+    long long lds;
+    const void* preact;
+    long long ldp;
+    void* dst;
+    long long ldd;
+    float* part;              // [chunks][period][ldpart] or null
+    long long ldpart;
+    int rows, cols, period, chunks, per_chunk;   // per_chunk: repeats of a chunk
+    int act, vec_src, vec_pre;
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int count, bool vec, float (&v)[8]) {
+    if (vec && count >= 8) {
+        const uint4 w = *reinterpret_cast<const uint4*>(p);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = Elem<T>::unpack(u[i]);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = i < count ? Elem<T>::to_float(p[i]) : 0.0f;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) rows_kernel(RowsArgs a) {
+    __shared__ float sums[8][256 + 8];
+    const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
+    const int col = blockIdx.x * 256 + lane * 8, count = a.cols - col;
+    const long long units = (long long)a.period * a.chunks;
+    for (long long u = blockIdx.y; u < units; u += gridDim.y) {
+        const int chunk = (int)(u / a.period), j = (int)(u - (long long)chunk * a.period);
+        const int repeats = a.rows / a.period;
+        const int t_end = min(repeats, (chunk + 1) * a.per_chunk);
+        float acc[8] = {};
+        if (count > 0) {
+            for (int t = chunk * a.per_chunk + sub; t < t_end; t += 8) {
+                const long long row = (long long)t * a.period + j;
+                float v[8];
+                load8(reinterpret_cast<const T*>(a.src) + row * a.lds + col, count, a.vec_src, v);
+                if (a.preact) {
+                    float z[8];
+                    load8(reinterpret_cast<const T*>(a.preact) + row * a.ldp + col, count, a.vec_pre, z);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[i] *= act_slope(z[i], a.act);
+                }
+                if (a.dst) {   // the destination's rows are padded to whole vectors
+                    *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.dst) + row * a.ldd + col) =
+                        make_uint4(Elem<T>::pack(v[0], v[1]), Elem<T>::pack(v[2], v[3]), Elem<T>::pack(v[4], v[5]), Elem<T>::pack(v[6], v[7]));
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) acc[i] += v[i];
+            }
+        }
+        if (a.part) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) sums[sub][lane * 8 + i] = acc[i];
+            __syncthreads();
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) s += sums[i][threadIdx.x];
+            const int c = blockIdx.x * 256 + threadIdx.x;
+            if (c < a.cols) a.part[u * a.ldpart + c] = s;
+            __syncthreads();
+        }
+    }
+}
+
+// out[j][c] = sum over planes of part[plane][j][c].
+template <typename T>
+__global__ void __launch_bounds__(256) sum_chunks_kernel(const float* __restrict__ part, long long ldpart, int planes, int rows, int cols, T* out,
+                                                         long long ldo) {
+    __shared__ float sums[8][33];
+    const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+    for (int j = blockIdx.y; j < rows; j += gridDim.y) {
+        float s = 0.0f;
+        if (col < cols)
+            for (int p = sub; p < planes; p += 8) s += part[((long long)p * rows + j) * ldpart + col];
+        sums[sub][lane] = s;
+        __syncthreads();
+        if (sub == 0 && col < cols) {
+#pragma unroll
+            for (int i = 1; i < 8; i++) s += sums[i][lane];
+            out[j * ldo + col] = Elem<T>::from_float(s);
+        }
+        __syncthreads();
+    }
+}
+
+// How many pieces the repeats are cut into: about four blocks an SM, at least 32 repeats a piece.
+static void cut_rows(RowsArgs* a, int sms) {
+    const int repeats = a->rows / a->period;
+    const long long blocks = (long long)((a->cols + 255) / 256) * a->period;
+    long long chunks = (4ll * sms + blocks - 1) / blocks;
+    if (chunks > (repeats + 31) / 32) chunks = (repeats + 31) / 32;
+    if (chunks < 1) chunks = 1;
+    a->per_chunk = (int)((repeats + chunks - 1) / chunks);
+    a->chunks = (repeats + a->per_chunk - 1) / a->per_chunk;
+}
+
+static int rows_launch(bool bf16, const RowsArgs& a, cudaStream_t stream, const char* what) {
+    const long long units = (long long)a.period * a.chunks;
+    const dim3 grid((unsigned)((a.cols + 255) / 256), (unsigned)(units < 32768 ? units : 32768));
+    if (bf16)
+        rows_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(a);
+    else
+        rows_kernel<__half><<<grid, 256, 0, stream>>>(a);
+    RB200_CHECK_LAUNCH(what);
+    return RB200_OK;
+}
+
+static int sum_chunks(bool bf16, const float* part, long long ldpart, int planes, int rows, int cols, void* out, long long ldo, cudaStream_t stream,
+                      const char* what) {
+    const dim3 grid((unsigned)((cols + 31) / 32), (unsigned)(rows < 32768 ? rows : 32768));
+    if (bf16)
+        sum_chunks_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(part, ldpart, planes, rows, cols, (__nv_bfloat16*)out, ldo);
+    else
+        sum_chunks_kernel<__half><<<grid, 256, 0, stream>>>(part, ldpart, planes, rows, cols, (__half*)out, ldo);
+    RB200_CHECK_LAUNCH(what);
+    return RB200_OK;
+}
+
+size_t column_sums_bytes(int rows, int cols, int sms) {
+    RowsArgs a = {};
+    a.rows = rows;
+    a.cols = cols;
+    a.period = 1;
+    cut_rows(&a, sms);
+    return (size_t)a.chunks * round_up(cols, 4) * sizeof(float);
+}
+
+int column_sums(bool bf16, const Operand& src, void* out, void* workspace, int sms, cudaStream_t stream, const char* what) {
+    RowsArgs a = {};
+    a.src = src.data;
+    a.lds = src.ld;
+    a.rows = src.rows;
+    a.cols = src.cols;
+    a.period = 1;
+    a.vec_src = map_ready(src);
+    a.part = (float*)workspace;
+    a.ldpart = round_up(src.cols, 4);
+    cut_rows(&a, sms);
+    int rc = rows_launch(bf16, a, stream, what);
+    if (rc) return rc;
+    return sum_chunks(bf16, a.part, a.ldpart, a.chunks, 1, src.cols, out, 0, stream, what);
+}
+
+// ---- argument checks ------------------------------------------------------------------------------------
+constexpr long long kMaxExtent = 1ll << 30;
+
+static int check_shape(const char* what, int dtype, int act, long long rows, long long in, long long out) {
+    if (dtype != RB200_FP16 && dtype != RB200_BF16) {
+        set_error("%s: dtype %d is neither RB200_FP16 nor RB200_BF16", what, dtype);
+        return RB200_E_INVALID;
+    }
+    if (act < RB200_ACT_NONE || act > RB200_ACT_SILU) {
+        set_error("%s: activation %d is not one of RB200_ACT_*", what, act);
+        return RB200_E_INVALID;
+    }
+    if (rows < 0 || in < 1 || out < 1) {
+        set_error("%s: rows %lld, in_features %lld, out_features %lld", what, rows, in, out);
+        return RB200_E_INVALID;
+    }
+    if (rows > kMaxExtent || in > kMaxExtent || out > kMaxExtent) {
+        set_error("%s: %lld x %lld x %lld exceeds 2^30 in one extent", what, rows, in, out);
+        return RB200_E_LIMIT;
+    }
+    return RB200_OK;
+}
+
+// A matrix argument: present, its rows not overlapping, its elements on their own boundaries.
+static int check_matrix(const char* what, const char* name, const void* data, long long ld, long long rows, long long cols) {
+    if (!data) {
+        set_error("%s: %s is null", what, name);
+        return RB200_E_INVALID;
+    }
+    if ((uintptr_t)data & 1) {
+        set_error("%s: %s is not aligned to its elements", what, name);
+        return RB200_E_INVALID;
+    }
+    if (rows > 1 && (ld < cols || ld > (1ll << 38))) {
+        set_error("%s: leading dimension %lld of %s, %lld columns", what, ld, name, cols);
+        return RB200_E_INVALID;
+    }
+    return RB200_OK;
+}
+
+static int check_workspace(const char* what, const void* ws, uint64_t have, uint64_t need) {
+    if (need == 0) return RB200_OK;
+    if (!ws || have < need) {
+        set_error("%s: the workspace has %llu bytes, the call needs %llu", what, (unsigned long long)(ws ? have : 0), (unsigned long long)need);
+        return RB200_E_INVALID;
+    }
+    if ((uintptr_t)ws & 255) {
+        set_error("%s: the workspace must be 256-byte aligned", what);
+        return RB200_E_INVALID;
+    }
+    return RB200_OK;
+}
+
+static Operand operand(const void* data, long long ld, long long rows, long long cols, bool transposed) {
+    Operand o = {data, ld, (int)rows, (int)cols, transposed};
+    return o;
+}
+
+// An operand as the product reads it: in place, or from a packed copy in the workspace.
+struct Packed {
+    Operand src, use;
+    bool copy;
+};
+static Packed plan_pack(const Operand& o, Carver* c) {
+    Packed p = {o, o, !map_ready(o)};
+    if (p.copy) {
+        p.use.ld = round_up(o.cols, 8);
+        p.use.data = c->take((size_t)p.use.ld * o.rows * 2);
+    }
+    return p;
+}
+static int do_pack(const Packed& p, cudaStream_t stream, const char* what) {
+    return p.copy ? pack_rows(p.src, const_cast<void*>(p.use.data), p.use.ld, stream, what) : RB200_OK;
+}
+
+// ---- forward ------------------------------------------------------------------------------------------------
+struct LinearPlan {
+    Packed x, w;
+    GemmPlan gemm;
+    void* partials;
+    size_t bytes;
+};
+static LinearPlan plan_linear(const rb200_linear_params& p, const DeviceInfo& dev, void* ws) {
+    LinearPlan l;
+    Carver c(ws);
+    l.x = plan_pack(operand(p.x, p.ldx, p.rows, p.in_features, false), &c);
+    l.w = plan_pack(operand(p.weight, p.ldw, p.out_features, p.in_features, false), &c);
+    l.gemm = gemm_plan(dev, (int)p.rows, (int)p.out_features, (int)p.in_features, false, true);
+    l.partials = c.take(gemm_partial_bytes(l.gemm, (int)p.rows, (int)p.out_features));
+    l.bytes = c.used;
+    return l;
+}
+
+static int linear_run(const rb200_linear_params* p, void* stream_v, GemmWait wait) {
+    const char* what = "rb200k_linear";
+    if (!p) {
+        set_error("%s: params is null", what);
+        return RB200_E_INVALID;
+    }
+    int rc = check_shape(what, p->dtype, p->activation, p->rows, p->in_features, p->out_features);
+    if (rc) return rc;
+    if (p->rows == 0) return RB200_OK;
+    if ((rc = check_matrix(what, "x", p->x, p->ldx, p->rows, p->in_features))) return rc;
+    if ((rc = check_matrix(what, "weight", p->weight, p->ldw, p->out_features, p->in_features))) return rc;
+    if ((rc = check_matrix(what, "out", p->out, p->ldo, p->rows, p->out_features))) return rc;
+    if (p->bias && (rc = check_matrix(what, "bias", p->bias, 0, 1, p->out_features))) return rc;
+    if (p->preact && (rc = check_matrix(what, "preact", p->preact, p->ldp, p->rows, p->out_features))) return rc;
+    if (p->residual) {
+        if (p->residual_rows < 1 || p->rows % p->residual_rows) {
+            set_error("%s: residual_rows %lld does not divide rows %lld", what, (long long)p->residual_rows, (long long)p->rows);
+            return RB200_E_INVALID;
+        }
+        if ((rc = check_matrix(what, "residual", p->residual, p->ldr, p->residual_rows, p->out_features))) return rc;
+    }
+    DeviceInfo dev;
+    if ((rc = device_info(&dev))) return rc;
+    const LinearPlan l = plan_linear(*p, dev, p->workspace);
+    if ((rc = check_workspace(what, p->workspace, p->workspace_bytes, l.bytes))) return rc;
+    cudaStream_t stream = (cudaStream_t)stream_v;
+    const bool bf16 = p->dtype == RB200_BF16;
+    if ((rc = do_pack(l.x, stream, what)) || (rc = do_pack(l.w, stream, what))) return rc;
+    EpiArgs e = {};
+    e.out = p->out;
+    e.ldo = p->ldo;
+    e.bias = p->bias;
+    e.residual = p->residual;
+    e.ldr = p->ldr;
+    e.residual_rows = (int)p->residual_rows;
+    e.preact = p->preact;
+    e.ldp = p->ldp;
+    e.act = p->activation;
+    e.alpha_const = 1.0f;
+    e.vec_out = map_ready(operand(p->out, p->ldo, p->rows, p->out_features, false));
+    e.vec_res = map_ready(operand(p->residual, p->ldr, p->residual_rows, p->out_features, false));
+    e.vec_pre = map_ready(operand(p->preact, p->ldp, p->rows, p->out_features, false));
+    wait.status = p->status;
+    if (l.gemm.splits > 1) {
+        EpiArgs part = {};
+        part.acc_out = (float*)l.partials;
+        part.ldacc = round_up(p->out_features, 4);
+        part.acc_split_stride = part.ldacc * p->rows;
+        part.alpha_const = 1.0f;
+        if ((rc = gemm_store(GEMM_KK, bf16, l.x.use, l.w.use, nullptr, nullptr, l.gemm, part, wait, stream, what))) return rc;
+        return gemm_join(bf16, (const float*)l.partials, l.gemm.splits, (int)p->rows, (int)p->out_features, e, stream, what);
+    }
+    return gemm_launch<EPI_LINEAR, false, false>(bf16, l.x.use, l.w.use, nullptr, nullptr, l.gemm, e, wait, stream, what);
+}
+
+// ---- backward -----------------------------------------------------------------------------------------------
+struct LinearBackwardPlan {
+    Packed x, w;
+    Operand dz;               // [rows][out]: dout itself, or the copy that rows_kernel writes
+    bool own_dz, sums;        // sums: rows_kernel makes the column sums
+    RowsArgs bias_rows, res_rows;
+    GemmPlan gx, gw;
+    void *px, *pw;
+    size_t bytes;
+};
+static LinearBackwardPlan plan_backward(const rb200_linear_backward_params& p, const DeviceInfo& dev, void* ws) {
+    LinearBackwardPlan l = {};
+    Carver c(ws);
+    const int n = (int)p.rows, k = (int)p.in_features, m = (int)p.out_features;
+    const Operand dout = operand(p.dout, p.lddo, p.rows, p.out_features, false);
+    const bool products = p.dx || p.dweight;
+    l.own_dz = products && (p.activation != RB200_ACT_NONE || !map_ready(dout));
+    l.dz = dout;
+    if (l.own_dz) {
+        l.dz.ld = round_up(m, 8);
+        l.dz.data = c.take((size_t)l.dz.ld * n * 2);
+    }
+    if (p.dx) {
+        l.w = plan_pack(operand(p.weight, p.ldw, m, k, true), &c);
+        l.gx = gemm_plan(dev, n, k, m, true, true);
+        l.px = c.take(gemm_partial_bytes(l.gx, n, k));
+    }
+    if (p.dweight) {
+        l.x = plan_pack(operand(p.x, p.ldx, n, k, true), &c);
+        l.gw = gemm_plan(dev, m, k, n, true, true);
+        l.pw = c.take(gemm_partial_bytes(l.gw, m, k));
+    }
+    RowsArgs a = {};
+    a.src = p.dout;
+    a.lds = p.lddo;
+    a.rows = n;
+    a.cols = m;
+    a.vec_src = map_ready(dout);
+    a.ldpart = round_up(m, 4);
+    if (p.dresidual) {
+        l.res_rows = a;
+        l.res_rows.period = (int)p.residual_rows;
+        cut_rows(&l.res_rows, dev.sms);
+        l.res_rows.part = (float*)c.take((size_t)l.res_rows.chunks * l.res_rows.period * a.ldpart * sizeof(float));
+    }
+    // without an activation the column sums are the sums of the residual's sums: no second sweep
+    l.sums = p.dbias && (p.activation != RB200_ACT_NONE || !p.dresidual);
+    l.bias_rows = a;
+    l.bias_rows.period = 1;
+    cut_rows(&l.bias_rows, dev.sms);
+    if (p.activation != RB200_ACT_NONE) {
+        l.bias_rows.preact = p.preact;
+        l.bias_rows.ldp = p.ldp;
+        l.bias_rows.act = p.activation;
+        l.bias_rows.vec_pre = map_ready(operand(p.preact, p.ldp, p.rows, p.out_features, false));
+    }
+    if (l.own_dz) {
+        l.bias_rows.dst = const_cast<void*>(l.dz.data);
+        l.bias_rows.ldd = l.dz.ld;
+    }
+    if (l.sums) l.bias_rows.part = (float*)c.take((size_t)l.bias_rows.chunks * a.ldpart * sizeof(float));
+    l.bytes = c.used;
+    return l;
+}
+
+static int clear_matrix(void* data, long long ld, long long rows, long long cols, cudaStream_t stream, const char* what) {
+    return check_cuda(cudaMemset2DAsync(data, (size_t)(rows > 1 ? ld : cols) * 2, 0, (size_t)cols * 2, (size_t)rows, stream), what);
+}
+
+static int backward_run(const rb200_linear_backward_params* p, void* stream_v) {
+    const char* what = "rb200k_linear_backward";
+    if (!p) {
+        set_error("%s: params is null", what);
+        return RB200_E_INVALID;
+    }
+    int rc = check_shape(what, p->dtype, p->activation, p->rows, p->in_features, p->out_features);
+    if (rc) return rc;
+    cudaStream_t stream = (cudaStream_t)stream_v;
+    const long long n = p->rows, k = p->in_features, m = p->out_features;
+    if (p->dweight && (rc = check_matrix(what, "dweight", p->dweight, p->lddw, m, k))) return rc;
+    if (p->dbias && (rc = check_matrix(what, "dbias", p->dbias, 0, 1, m))) return rc;
+    if (p->dresidual) {
+        if (p->residual_rows < 1 || n % p->residual_rows) {
+            set_error("%s: residual_rows %lld does not divide rows %lld", what, (long long)p->residual_rows, n);
+            return RB200_E_INVALID;
+        }
+        if ((rc = check_matrix(what, "dresidual", p->dresidual, p->lddr, p->residual_rows, m))) return rc;
+    }
+    if (n == 0) {   // nothing flows back: the sums over no rows are zero
+        if (p->dweight && (rc = clear_matrix(p->dweight, p->lddw, m, k, stream, what))) return rc;
+        if (p->dbias && (rc = clear_matrix(p->dbias, 0, 1, m, stream, what))) return rc;
+        if (p->dresidual && (rc = clear_matrix(p->dresidual, p->lddr, p->residual_rows, m, stream, what))) return rc;
+        return RB200_OK;
+    }
+    if ((rc = check_matrix(what, "dout", p->dout, p->lddo, n, m))) return rc;
+    if (p->dx && ((rc = check_matrix(what, "weight", p->weight, p->ldw, m, k)) || (rc = check_matrix(what, "dx", p->dx, p->lddx, n, k)))) return rc;
+    if (p->dweight && (rc = check_matrix(what, "x", p->x, p->ldx, n, k))) return rc;
+    if (p->activation != RB200_ACT_NONE && (p->dx || p->dweight || p->dbias) && (rc = check_matrix(what, "preact", p->preact, p->ldp, n, m)))
+        return rc;
+    DeviceInfo dev;
+    if ((rc = device_info(&dev))) return rc;
+    const LinearBackwardPlan l = plan_backward(*p, dev, p->workspace);
+    if ((rc = check_workspace(what, p->workspace, p->workspace_bytes, l.bytes))) return rc;
+    const bool bf16 = p->dtype == RB200_BF16;
+    if (p->dresidual) {
+        const RowsArgs& r = l.res_rows;
+        if ((rc = rows_launch(bf16, r, stream, what))) return rc;
+        if ((rc = sum_chunks(bf16, r.part, r.ldpart, r.chunks, r.period, (int)m, p->dresidual, p->lddr, stream, what))) return rc;
+        if (p->dbias && !l.sums &&
+            (rc = sum_chunks(bf16, r.part, r.ldpart, r.chunks * r.period, 1, (int)m, p->dbias, 0, stream, what)))
+            return rc;
+    }
+    if (l.sums || l.own_dz) {
+        const RowsArgs& r = l.bias_rows;
+        if ((rc = rows_launch(bf16, r, stream, what))) return rc;
+        if (l.sums && (rc = sum_chunks(bf16, r.part, r.ldpart, r.chunks, 1, (int)m, p->dbias, 0, stream, what))) return rc;
+    }
+    const GemmWait wait = {p->status, 0, -1};
+    EpiArgs e = {};
+    e.alpha_const = 1.0f;
+    if (p->dx) {
+        if ((rc = do_pack(l.w, stream, what))) return rc;
+        e.out = p->dx;
+        e.ldo = p->lddx;
+        e.vec_out = map_ready(operand(p->dx, p->lddx, n, k, false));
+        if ((rc = gemm_store_joined(GEMM_KN, bf16, l.dz, l.w.use, nullptr, nullptr, l.gx, e, l.px, wait, stream, what))) return rc;
+    }
+    if (p->dweight) {
+        if ((rc = do_pack(l.x, stream, what))) return rc;
+        e.out = p->dweight;
+        e.ldo = p->lddw;
+        e.vec_out = map_ready(operand(p->dweight, p->lddw, m, k, false));
+        Operand dzt = l.dz;
+        dzt.transposed = true;
+        if ((rc = gemm_store_joined(GEMM_NN, bf16, dzt, l.x.use, nullptr, nullptr, l.gw, e, l.pw, wait, stream, what))) return rc;
+    }
+    return RB200_OK;
+}
+
+}  // namespace rb200
+
+using namespace rb200;
+
+extern "C" uint64_t rb200k_linear_workspace_bytes(const rb200_linear_params* p) {
+    DeviceInfo dev;
+    if (!p || check_shape("rb200k_linear_workspace_bytes", p->dtype, p->activation, p->rows, p->in_features, p->out_features) || p->rows == 0 ||
+        device_info(&dev))
+        return 0;
+    return plan_linear(*p, dev, nullptr).bytes;
+}
+extern "C" int rb200k_linear(const rb200_linear_params* p, void* stream) { return linear_run(p, stream, GemmWait{nullptr, 0, -1}); }
+extern "C" int rb200k_linear_probe(const rb200_linear_params* p, void* stream, uint64_t wait_cycles, int skip_block) {
+    return linear_run(p, stream, GemmWait{nullptr, wait_cycles, skip_block});
+}
+extern "C" uint64_t rb200k_linear_backward_workspace_bytes(const rb200_linear_backward_params* p) {
+    DeviceInfo dev;
+    if (!p || check_shape("rb200k_linear_backward_workspace_bytes", p->dtype, p->activation, p->rows, p->in_features, p->out_features) ||
+        p->rows == 0 || (p->dresidual && (p->residual_rows < 1 || p->rows % p->residual_rows)) || device_info(&dev))
+        return 0;
+    return plan_backward(*p, dev, nullptr).bytes;
+}
+extern "C" int rb200k_linear_backward(const rb200_linear_backward_params* p, void* stream) { return backward_run(p, stream); }

@@ -10,7 +10,8 @@ import numpy as np
 import torch
 
 from . import tables as T
-from ._lib import (BoxEncoderParams, BoxMatcherParams, NormalizeParams, PointwiseParams, ResampleParams, WarpParams, check, lib)
+from ._lib import (BoxEncoderParams, BoxMatcherParams, LinearBackwardParams, LinearParams, NormalizeParams, PointwiseParams,
+                   ResampleParams, WarpParams, check, lib)
 
 _TORCH_DTYPE = {T.FP32: torch.float32, T.FP16: torch.float16, T.UINT8: torch.uint8}
 
@@ -236,3 +237,169 @@ def transpose(arena, samples, perm, out_dims, out=None, d_samples=None, stream=N
     check(lib.rb200k_transpose(arena.data_ptr(), d_samples.data_ptr(), n, pm, out.data_ptr(), od, _stream_ptr(stream)),
           "rb200k_transpose")
     return out
+
+
+# ---- head operators -----------------------------------------------------------------------------
+# Tensors may live on any device; the call runs there, on `stream` or that device's current stream, and takes its
+# workspace from torch's allocator on that stream.
+_HEAD_DTYPE = {torch.float16: T.FP16, torch.bfloat16: T.BF16}
+
+
+class _on:
+    """The device and stream of a head operator's launch."""
+
+    def __init__(self, device, stream):
+        self.device, self.stream = device, stream
+        self.away = device.index != torch.cuda.current_device()
+
+    def __enter__(self):
+        self.guards = []
+        if self.away:
+            self.guards.append(torch.cuda.device(self.device))
+        if self.stream is not None:
+            if self.stream.device != self.device:
+                raise ValueError("the stream is on %s, the tensors are on %s" % (self.stream.device, self.device))
+            self.guards.append(torch.cuda.stream(self.stream))
+        for g in self.guards:
+            g.__enter__()
+        s = self.stream if self.stream is not None else torch.cuda.current_stream(self.device)
+        return s.cuda_stream
+
+    def __exit__(self, *exc):
+        for g in reversed(self.guards):
+            g.__exit__(*exc)
+        return False
+
+
+def _matrix(t, name, like, cols=None):
+    """A 2-d tensor on the device and of the type of `like`, its rows contiguous and not overlapping (copied if need be)."""
+    if t.dim() != 2:
+        raise ValueError("%s has %d dimensions, a matrix is needed" % (name, t.dim()))
+    if t.dtype != like.dtype or t.device != like.device:
+        raise ValueError("%s is %s on %s, the input is %s on %s" % (name, t.dtype, t.device, like.dtype, like.device))
+    if cols is not None and t.shape[1] != cols:
+        raise ValueError("%s has %d columns, %d are needed" % (name, t.shape[1], cols))
+    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t
+
+
+def _vector(t, name, like, n):
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError("%s has shape %s, (%d,) is needed" % (name, tuple(t.shape), n))
+    if t.dtype != like.dtype or t.device != like.device:
+        raise ValueError("%s is %s on %s, the input is %s on %s" % (name, t.dtype, t.device, like.dtype, like.device))
+    return t.contiguous()
+
+
+def _head_input(x, weight):
+    """Element type of a head operator and its (x, weight) as matrices."""
+    if not x.is_cuda:
+        raise ValueError("x is on %s: the head operators run on a GPU" % x.device)
+    if x.dtype not in _HEAD_DTYPE:
+        raise ValueError("x is %s: the head operators take float16 and bfloat16" % x.dtype)
+    x = _matrix(x, "x", x)
+    return _HEAD_DTYPE[x.dtype], x, _matrix(weight, "weight", x, x.shape[1])
+
+
+def _output(out, name, shape, like):
+    if out is None:
+        return torch.empty(shape, dtype=like.dtype, device=like.device)
+    if tuple(out.shape) != tuple(shape) or out.dtype != like.dtype or out.device != like.device:
+        raise ValueError("%s is %s %s on %s, needed: %s %s on %s" % (name, tuple(out.shape), out.dtype, out.device, tuple(shape),
+                                                                    like.dtype, like.device))
+    if out.dim() == 2 and ((out.stride(1) != 1 and out.shape[1] > 1) or (out.shape[0] > 1 and out.stride(0) < out.shape[1])):
+        raise ValueError("%s needs contiguous rows that do not overlap" % name)
+    return out
+
+
+def _workspace(p, sizer, device):
+    need = sizer(ctypes.byref(p))
+    if not need:
+        return None
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    p.workspace, p.workspace_bytes = ws.data_ptr(), need
+    return ws
+
+
+def _activation(name):
+    if name not in T.ACTIVATIONS:
+        raise ValueError("activation %r: one of %s is needed" % (name, ", ".join(T.ACTIVATIONS)))
+    return T.ACTIVATIONS[name]
+
+
+def linear(x, weight, bias=None, residual=None, activation="none", out=None, want_preact=False, stream=None, status=None, probe=None):
+    """rb200k_linear: act(x weight^T + bias) + residual for x [n, k], weight [m, k], bias [m], residual [r, m] with r a
+    divisor of n (row i takes residual row i % r), all float16 or all bfloat16. Returns [n, m], with want_preact also
+    the value before the activation. probe=(wait_cycles, skip_block) launches through rb200k_linear_probe."""
+    dtype, x, weight = _head_input(x, weight)
+    n, k = x.shape
+    m = weight.shape[0]
+    act = _activation(activation)
+    if bias is not None:
+        bias = _vector(bias, "bias", x, m)
+    if residual is not None:
+        residual = _matrix(residual, "residual", x, m)
+        if residual.shape[0] == 0 and n or residual.shape[0] and n % residual.shape[0]:
+            raise ValueError("residual has %d rows, which do not divide the %d rows of x" % (residual.shape[0], n))
+    with _on(x.device, stream) as s:
+        out = _output(out, "out", (n, m), x)
+        pre = torch.empty((n, m), dtype=x.dtype, device=x.device) if want_preact else None
+        if n:
+            p = LinearParams(dtype, act, n, k, m, x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0))
+            p.out, p.ldo = out.data_ptr(), out.stride(0)
+            if bias is not None:
+                p.bias = bias.data_ptr()
+            if residual is not None:
+                p.residual, p.ldr, p.residual_rows = residual.data_ptr(), residual.stride(0), residual.shape[0]
+            if pre is not None:
+                p.preact, p.ldp = pre.data_ptr(), m
+            if status is not None:
+                p.status = status.data_ptr()
+            ws = _workspace(p, lib.rb200k_linear_workspace_bytes, x.device)  # noqa: F841  (alive until the launch)
+            if probe is not None:
+                check(lib.rb200k_linear_probe(ctypes.byref(p), s, int(probe[0]), int(probe[1])), "rb200k_linear_probe")
+            else:
+                check(lib.rb200k_linear(ctypes.byref(p), s), "rb200k_linear")
+    return (out, pre) if want_preact else out
+
+
+def linear_backward(dout, x, weight, preact=None, activation="none", residual_rows=0, need=(True, True, True, True), stream=None,
+                    status=None):
+    """rb200k_linear_backward: (dx, dweight, dbias, dresidual), None where `need` is false. dresidual takes residual_rows."""
+    dtype, x, weight = _head_input(x, weight)
+    n, k = x.shape
+    m = weight.shape[0]
+    act = _activation(activation)
+    dout = _matrix(dout, "dout", x, m)
+    if dout.shape[0] != n:
+        raise ValueError("dout has %d rows, x has %d" % (dout.shape[0], n))
+    if act and (need[0] or need[1] or need[2]):
+        if preact is None:
+            raise ValueError("the backward pass of an activation needs preact")
+        preact = _matrix(preact, "preact", x, m)
+        if preact.shape[0] != n:
+            raise ValueError("preact has %d rows, x has %d" % (preact.shape[0], n))
+    if need[3] and (residual_rows < 1 or n % residual_rows):
+        raise ValueError("residual_rows %d does not divide the %d rows" % (residual_rows, n))
+    shapes = ((n, k), (m, k), (m,), (residual_rows, m))
+    with _on(x.device, stream) as s:
+        grads = [torch.empty(shape, dtype=x.dtype, device=x.device) if want else None for shape, want in zip(shapes, need)]
+        dx, dw, db, dr = grads
+        p = LinearBackwardParams(dtype, act, n, k, m, dout.data_ptr(), dout.stride(0), x.data_ptr(), x.stride(0), weight.data_ptr(),
+                                 weight.stride(0))
+        if act and preact is not None:
+            p.preact, p.ldp = preact.data_ptr(), preact.stride(0)
+        if dx is not None:
+            p.dx, p.lddx = dx.data_ptr(), k
+        if dw is not None:
+            p.dweight, p.lddw = dw.data_ptr(), k
+        if db is not None:
+            p.dbias = db.data_ptr()
+        if dr is not None:
+            p.dresidual, p.lddr, p.residual_rows = dr.data_ptr(), m, residual_rows
+        if status is not None:
+            p.status = status.data_ptr()
+        ws = _workspace(p, lib.rb200k_linear_backward_workspace_bytes, x.device)  # noqa: F841
+        check(lib.rb200k_linear_backward(ctypes.byref(p), s), "rb200k_linear_backward")
+    return tuple(grads)

@@ -76,3 +76,57 @@ class ROCALClassificationIterator(ROCALGenericIterator):
 
     def reset(self):
         self.loader.reset()
+
+
+# ---- the head of a training or serving step, on the batches above -----------------------------------
+# Differentiable by torch.autograd, once. Float16 and bfloat16 CUDA tensors; everything runs on the tensors' device, on
+# its current stream.
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        from .. import kernels
+        act = activation != "none"
+        y = kernels.linear(x, weight, bias, residual, activation, want_preact=act)
+        y, pre = y if act else (y, None)
+        ctx.save_for_backward(x, weight, pre)
+        ctx.activation = activation
+        ctx.residual_rows = 0 if residual is None else residual.shape[0]
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        from .. import kernels
+        x, weight, pre = ctx.saved_tensors
+        need = list(ctx.needs_input_grad[:4])
+        whole = need[3] and ctx.residual_rows == x.shape[0]      # nothing is summed: the gradient goes through as it is
+        need[3] = need[3] and not whole
+        grads = kernels.linear_backward(dout, x, weight, pre, ctx.activation, ctx.residual_rows, need) if any(need) else (None,) * 4
+        return grads[0], grads[1], grads[2], dout if whole else grads[3], None
+
+
+def linear(x, weight, bias=None, residual=None, activation="none"):
+    """act(x weight^T + bias) + residual, the matrix product with its epilogue in one kernel: a projection of image
+    patches with their position table, a hidden layer or the scores of a classifier.
+
+    x [..., k]; weight [m, k]; bias [m]; residual: the trailing dimensions of the result, repeated over the leading ones
+    (a position table [196, m] for x [images, 196, k]); activation "none", "relu", "gelu" (with the error function) or
+    "silu". All float16 or all bfloat16; sums in 32 bits, one rounding at the end. Returns [..., m]."""
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError("x %s does not go with weight %s" % (tuple(x.shape), tuple(weight.shape)))
+    shape = tuple(x.shape[:-1]) + (weight.shape[0],)
+    if residual is not None:
+        if residual.dim() < 1 or residual.dim() > len(shape) or tuple(residual.shape) != shape[len(shape) - residual.dim():]:
+            if not (residual.dim() == 2 and x.dim() == 2 and residual.shape[1] == shape[1]):
+                raise ValueError("residual %s is not a tail of the result's shape %s" % (tuple(residual.shape), shape))
+        residual = residual.reshape(-1, shape[-1])
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
+        y = _Linear.apply(x2, weight, bias, residual, activation)
+    else:
+        from .. import kernels
+        y = kernels.linear(x2, weight, bias, residual, activation)
+    return y if x.dim() == 2 else y.reshape(shape)
