@@ -454,6 +454,51 @@ typedef struct rb200_linear_backward_params {
 RB200_API uint64_t rb200k_linear_backward_workspace_bytes(const rb200_linear_backward_params* params);
 RB200_API int rb200k_linear_backward(const rb200_linear_backward_params* params, void* stream);
 
+/* Softmax cross entropy of a linear classifier without keeping the scores. With z = x weight^T + bias (rows x classes,
+ * never stored whole: pieces of it are made, used and overwritten), lse_i = log sum_j exp z_ij and s = label_smoothing:
+ *   loss_i = lse_i - (1 - s) z_{i, label_i} - s / classes * sum_j z_ij
+ * A row whose label equals ignore_index does not count: its loss is 0 and nothing flows back from or into it, whatever its
+ * features hold (the padding of a last batch, anchors that matched nothing). A label that is neither ignore_index nor
+ * a class makes the row's loss NaN. Classes may be masked by a bias of -inf or of the type's lowest value. Reductions:
+ * NONE = one loss a row, SUM, MEAN = over the rows that count, 0 if none does. 32-bit sums; loss and stats are fp32. */
+enum { RB200_REDUCE_NONE = 0, RB200_REDUCE_MEAN = 1, RB200_REDUCE_SUM = 2 };
+typedef struct rb200_linear_ce_params {
+    int32_t dtype;               /* RB200_FP16 or RB200_BF16, of x, weight, bias and their gradients */
+    int32_t reduction;
+    int64_t rows, features, classes;           /* >= 0, >= 1, >= 1; at most 2^30 */
+    const void* x;               /* [rows][features]    */
+    int64_t ldx;
+    const void* weight;          /* [classes][features] */
+    int64_t ldw;
+    const void* bias;            /* [classes] or NULL   */
+    const void* labels;          /* [rows], integers of label_bytes bytes */
+    int32_t label_bytes;         /* 4 or 8 */
+    float label_smoothing;       /* 0 .. 1 */
+    int64_t ignore_index;
+    float* loss;                 /* NONE: [rows], else one value (forward only) */
+    float* stats;                /* [2][rows]: each row's largest score and sum of exp(z - that) - written by the
+                                    forward pass, read by the backward pass */
+    int32_t* info;               /* [4]: rows that count, 1 if a row that does not count holds inf or NaN, two reserved
+                                    words - written by the forward pass, read by the backward pass */
+    /* backward pass only: */
+    const float* dloss;          /* gradient of the loss: NONE: [rows], else one value */
+    void* dx;                    /* [rows][features] or NULL    */
+    int64_t lddx;
+    void* dweight;               /* [classes][features] or NULL */
+    int64_t lddw;
+    void* dbias;                 /* [classes] or NULL           */
+    void* workspace;
+    uint64_t workspace_bytes;
+    int32_t* status;             /* device word or NULL */
+} rb200_linear_ce_params;
+
+RB200_API uint64_t rb200k_linear_ce_workspace_bytes(const rb200_linear_ce_params* params);
+RB200_API int rb200k_linear_ce(const rb200_linear_ce_params* params, void* stream);
+/* The gradients whose pointers are given. The scores are made again, in pieces of at most about 256 MB of the element
+ * type (pieces of the classes, or of the rows where there are more of those). */
+RB200_API uint64_t rb200k_linear_ce_backward_workspace_bytes(const rb200_linear_ce_params* params);
+RB200_API int rb200k_linear_ce_backward(const rb200_linear_ce_params* params, void* stream);
+
 /* ---------------------------------------------------------------------------------------
  * Overlapping launches
  * ------------------------------------------------------------------------------------- */

@@ -83,7 +83,14 @@ class LinearBackwardParams(ctypes.Structure):
                        "p workspace, u workspace_bytes, p status")
 
 
-for _name, _params in (("linear", LinearParams), ("linear_backward", LinearBackwardParams)):
+class LinearCeParams(ctypes.Structure):
+    _fields_ = _fields("i dtype, i reduction, q rows, q features, q classes, p x, q ldx, p weight, q ldw, p bias, p labels, "
+                       "i label_bytes, f label_smoothing, q ignore_index, p loss, p stats, p info, p dloss, p dx, q lddx, p dweight, "
+                       "q lddw, p dbias, p workspace, u workspace_bytes, p status")
+
+
+for _name, _params in (("linear", LinearParams), ("linear_backward", LinearBackwardParams), ("linear_ce", LinearCeParams),
+                       ("linear_ce_backward", LinearCeParams)):
     _f = getattr(lib, "rb200k_%s_workspace_bytes" % _name)
     _f.argtypes, _f.restype = [ctypes.POINTER(_params)], c_uint64
     _f = getattr(lib, "rb200k_" + _name)

@@ -143,7 +143,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ part, int splits, long long stride, long long ldacc, int m, int n,
                                                    EpiArgs e) {
     const long long groups = (n + 3) / 4, total = groups * m;
-    const float alpha = e.alpha_const * (e.alpha ? *e.alpha : 1.0f);
+    const float alpha = e.scale.value();
     for (long long t = blockIdx.x * 256ll + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
         const int row = (int)(t / groups), col = (int)(t - row * groups) * 4;
         const float* p = part + row * ldacc + col;
@@ -154,6 +154,18 @@ __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ par
             v[1] += f.y;
             v[2] += f.z;
             v[3] += f.w;
+        }
+        const long long at = row * ldacc + col;
+        if (e.acc_in) {
+            const float4 f = *reinterpret_cast<const float4*>(e.acc_in + at);
+            v[0] += f.x;
+            v[1] += f.y;
+            v[2] += f.z;
+            v[3] += f.w;
+        }
+        if (e.acc_out) {
+            *reinterpret_cast<float4*>(e.acc_out + at) = make_float4(v[0], v[1], v[2], v[3]);
+            continue;
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -192,7 +204,6 @@ int gemm_store_joined(int kind, bool bf16, const Operand& a, const Operand& b, c
     part.acc_out = (float*)partials;
     part.ldacc = round_up(n, 4);
     part.acc_split_stride = part.ldacc * m;
-    part.alpha_const = 1.0f;
     int rc = gemm_store(kind, bf16, a, b, b_alt, b_select, plan, part, wait, stream, what);
     if (rc) return rc;
     return gemm_join(bf16, (const float*)partials, plan.splits, m, n, e, stream, what);

@@ -20,6 +20,15 @@ constexpr int kGemmThreads = 384, kEpiWarps = 8;
 enum { EPI_LINEAR = 0, EPI_STORE = 1, EPI_CE_STATS = 2, EPI_CE_GRAD = 3 };
 enum { ACT_NONE = RB200_ACT_NONE, ACT_RELU = RB200_ACT_RELU, ACT_GELU = RB200_ACT_GELU, ACT_SILU = RB200_ACT_SILU };
 
+// A factor that is partly known on the device only: constant * *scalar / max(1, *count).
+struct Scale {
+    float constant;
+    const float* scalar;   // or null (= 1)
+    const int* count;      // or null (= 1)
+    __host__ __device__ Scale(float c = 1.0f, const float* s = nullptr, const int* n = nullptr) : constant(c), scalar(s), count(n) {}
+    __device__ float value() const { return constant * (scalar ? *scalar : 1.0f) / (count ? (float)max(1, *count) : 1.0f); }
+};
+
 // What the epilogues read and write; the fields an epilogue does not name are unused.
 struct EpiArgs {
     void* out;                // LINEAR, STORE (final): T[m][ldo]; CE_GRAD: T[m][ldo]
@@ -32,20 +41,22 @@ struct EpiArgs {
     long long ldp;
     int act;
     int vec_out, vec_res, vec_pre;   // 1: the rows of that array start on 16-byte boundaries
-    // STORE: value = acc + acc_in; to acc_out (fp32) if that is set, else alpha * value to out.
+    // STORE: value = acc + acc_in; to acc_out (fp32) if that is set, else scale * value to out.
     const float* acc_in;
     float* acc_out;
     long long ldacc, acc_split_stride;
-    const float* alpha;       // device scalar or null (= 1)
-    float alpha_const;
-    // CE: labels of the rows, the first class of this launch, the ignored label.
-    const int32_t* labels;
-    int class0, ignore_index;
+    Scale scale;
+    // CE: labels of the rows (4- or 8-byte integers), all classes and the first one of this launch, the ignored label.
+    const void* labels;
+    int label_bytes, classes, class0;
+    long long ignore_index;
     float smooth_on, smooth_off;   // 1 - smoothing, smoothing / classes
     float* part;              // STATS: [parts][m] maxima, then [parts][m] sums, then (smoothing) [parts][m] sums of z
     int parts, want_zsum;
     float* zlabel;            // STATS: [m] the label's z
-    const float* stats;       // GRAD: [2][m] maximum and sum
+    int* clear;               // STATS: four words to be zeroed, or null
+    const float* stats;       // GRAD: maxima, and stats_stride further the sums
+    long long stats_stride;
     const float* coef;        // GRAD: [m] per-row factor or null (= 1)
 };
 
@@ -154,6 +165,19 @@ struct RunningSoftmax {
 };
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
 constexpr float kLog2e = 1.4426950408889634f;
+// exp(d) for a difference d <= 0 (or NaN): one special-function operation, 2^-22 relative.
+__device__ __forceinline__ float exp_diff(float d) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * kLog2e));
+    return r;
+}
+
+// The class of a row and whether it counts; -1 for a label that is no class.
+__device__ __forceinline__ int load_label(const void* labels, int bytes, long long row, long long ignore_index, int classes, bool* counted) {
+    const long long v = bytes == 8 ? reinterpret_cast<const long long*>(labels)[row] : reinterpret_cast<const int32_t*>(labels)[row];
+    *counted = v != ignore_index;
+    return v >= 0 && v < classes ? (int)v : -1;
+}
 
 template <typename T, int EPI>
 __device__ __forceinline__ void epilogue_bias(const GemmArgs& g, int col, float* strip, int lane) {
@@ -207,6 +231,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         __syncthreads();
     tc::fence_after();
     const uint32_t tmem = tmem_addr_s;
+    if (EPI == EPI_CE_STATS && g.e.clear && blockIdx.x == 0 && threadIdx.x < 4) g.e.clear[threadIdx.x] = 0;
     const tc::Patience patience = {&gave_up_s, g.status, g.wait_cycles};
 
     const long long tiles = (long long)g.tiles_m * g.tiles_n * g.splits;
@@ -342,9 +367,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             float zsum = 0.0f;
             if constexpr (EPI == EPI_CE_STATS || EPI == EPI_CE_GRAD) {
                 if (row_ok) {
-                    label = g.e.labels[row];
-                    counted = label != g.e.ignore_index;
-                    label -= g.e.class0;
+                    label = load_label(g.e.labels, g.e.label_bytes, row, g.e.ignore_index, g.e.classes, &counted);
+                    label = label < g.e.class0 ? -1 : label - g.e.class0;
                 }
                 if constexpr (EPI == EPI_CE_GRAD) {
                     if (counted) {
@@ -355,13 +379,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             }
             float inv_sum = 0.0f;
             if constexpr (EPI == EPI_CE_GRAD) {
-                if (counted) inv_sum = 1.0f / g.e.stats[(long long)g.m + row];
+                if (counted) inv_sum = 1.0f / g.e.stats[g.e.stats_stride + row];
             }
             if constexpr (EPI == EPI_LINEAR) {
                 if (g.e.residual && row_ok) res_row = row % g.e.residual_rows;
             }
             float alpha = 1.0f;
-            if constexpr (EPI == EPI_STORE) alpha = g.e.alpha_const * (g.e.alpha ? *g.e.alpha : 1.0f);
+            if constexpr (EPI == EPI_STORE) alpha = g.e.scale.value();
 
             for (int c = half * 32; c < g.bn; c += 64) {
                 const int col = n0 + c, count = g.n - col;   // columns of this strip inside the matrix (may be <= 0)
@@ -435,18 +459,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                             if (i < count) zsum += v[i];
                     }
                     const float base = finite_max(top);
-                    run.s *= exp2f((run.m - base) * kLog2e);
+                    run.s *= exp_diff(run.m - base);
                     run.m = top;
                     float sum = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 32; i++) sum += exp2f((v[i] - base) * kLog2e);
+                    for (int i = 0; i < 32; i++) sum += exp_diff(v[i] - base);
                     run.s += sum;
                 }
                 if constexpr (EPI == EPI_CE_GRAD) {
                     if (row_ok) {
 #pragma unroll
                         for (int i = 0; i < 32; i++) {
-                            float p = exp2f((v[i] - cmax) * kLog2e) * inv_sum - g.e.smooth_off;
+                            float p = exp_diff(v[i] - cmax) * inv_sum - g.e.smooth_off;
                             if (label == col + i) p -= g.e.smooth_on;
                             v[i] = counted ? p * cscale : 0.0f;
                         }
@@ -567,10 +591,20 @@ int gemm_store(int kind, bool bf16, const Operand& a, const Operand& b, const Op
 size_t gemm_partial_bytes(const GemmPlan& plan, int m, int n);
 int gemm_store_joined(int kind, bool bf16, const Operand& a, const Operand& b, const Operand* b_alt, const int* b_select, const GemmPlan& plan,
                       EpiArgs e, void* partials, const GemmWait& wait, cudaStream_t stream, const char* what);
-// Joins the pieces: sum over splits, then bias, activation, residual (or alpha) and the conversion.
+// Joins the pieces: sum over splits (and acc_in), to acc_out, or scaled with bias, activation and residual to out.
 int gemm_join(bool bf16, const float* partials, int splits, int m, int n, const EpiArgs& e, cudaStream_t stream, const char* what);
 // dst[rows][ldd] = src, for operands whose rows no tensor map can describe.
 int pack_rows(const Operand& src, void* dst, long long ldd, cudaStream_t stream, const char* what);
+
+// Column sums of a matrix (linear.cu): chunks planes of ldpart partial sums, joined (with other planes) by sum_chunks.
+struct ColumnSums {
+    int chunks;
+    long long ldpart;
+};
+ColumnSums plan_column_sums(int rows, int cols, int sms);
+int column_partials(bool bf16, const Operand& src, float* part, int sms, cudaStream_t stream, const char* what);
+int sum_chunks(bool bf16, const float* part, long long ldpart, int planes, int rows, int cols, void* out, long long ldo, const Scale& scale,
+               cudaStream_t stream, const char* what);
 
 static inline long long round_up(long long v, long long to) { return (v + to - 1) / to * to; }
 

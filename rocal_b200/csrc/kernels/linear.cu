@@ -1,7 +1,7 @@
 // rb200k_linear: out = act(x W^T + b) + r, and its gradients. The products run on the tensor cores (gemm.cuh); the
 // passes over the gradient of the output that the products do not make (activation slope, column sums, sums over rows
 // that share a residual row) are memory-bound and made by rows_kernel in one sweep.
-#include "gemm.cuh"
+#include "matrix_args.cuh"
 
 namespace rb200 {
 
@@ -85,12 +85,13 @@ __global__ void __launch_bounds__(256) rows_kernel(RowsArgs a) {
     }
 }
 
-// out[j][c] = sum over planes of part[plane][j][c].
+// out[j][c] = scale * sum over planes of part[plane][j][c].
 template <typename T>
 __global__ void __launch_bounds__(256) sum_chunks_kernel(const float* __restrict__ part, long long ldpart, int planes, int rows, int cols, T* out,
-                                                         long long ldo) {
+                                                         long long ldo, Scale scale) {
     __shared__ float sums[8][33];
     const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+    const float factor = scale.value();
     for (int j = blockIdx.y; j < rows; j += gridDim.y) {
         float s = 0.0f;
         if (col < cols)
@@ -100,7 +101,7 @@ __global__ void __launch_bounds__(256) sum_chunks_kernel(const float* __restrict
         if (sub == 0 && col < cols) {
 #pragma unroll
             for (int i = 1; i < 8; i++) s += sums[i][lane];
-            out[j * ldo + col] = Elem<T>::from_float(s);
+            out[j * ldo + col] = Elem<T>::from_float(s * factor);
         }
         __syncthreads();
     }
@@ -128,27 +129,28 @@ static int rows_launch(bool bf16, const RowsArgs& a, cudaStream_t stream, const 
     return RB200_OK;
 }
 
-static int sum_chunks(bool bf16, const float* part, long long ldpart, int planes, int rows, int cols, void* out, long long ldo, cudaStream_t stream,
-                      const char* what) {
+int sum_chunks(bool bf16, const float* part, long long ldpart, int planes, int rows, int cols, void* out, long long ldo, const Scale& scale,
+               cudaStream_t stream, const char* what) {
     const dim3 grid((unsigned)((cols + 31) / 32), (unsigned)(rows < 32768 ? rows : 32768));
     if (bf16)
-        sum_chunks_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(part, ldpart, planes, rows, cols, (__nv_bfloat16*)out, ldo);
+        sum_chunks_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(part, ldpart, planes, rows, cols, (__nv_bfloat16*)out, ldo, scale);
     else
-        sum_chunks_kernel<__half><<<grid, 256, 0, stream>>>(part, ldpart, planes, rows, cols, (__half*)out, ldo);
+        sum_chunks_kernel<__half><<<grid, 256, 0, stream>>>(part, ldpart, planes, rows, cols, (__half*)out, ldo, scale);
     RB200_CHECK_LAUNCH(what);
     return RB200_OK;
 }
 
-size_t column_sums_bytes(int rows, int cols, int sms) {
+ColumnSums plan_column_sums(int rows, int cols, int sms) {
     RowsArgs a = {};
     a.rows = rows;
     a.cols = cols;
     a.period = 1;
     cut_rows(&a, sms);
-    return (size_t)a.chunks * round_up(cols, 4) * sizeof(float);
+    ColumnSums c = {a.chunks, round_up(cols, 4)};
+    return c;
 }
 
-int column_sums(bool bf16, const Operand& src, void* out, void* workspace, int sms, cudaStream_t stream, const char* what) {
+int column_partials(bool bf16, const Operand& src, float* part, int sms, cudaStream_t stream, const char* what) {
     RowsArgs a = {};
     a.src = src.data;
     a.lds = src.ld;
@@ -156,87 +158,20 @@ int column_sums(bool bf16, const Operand& src, void* out, void* workspace, int s
     a.cols = src.cols;
     a.period = 1;
     a.vec_src = map_ready(src);
-    a.part = (float*)workspace;
+    a.part = part;
     a.ldpart = round_up(src.cols, 4);
     cut_rows(&a, sms);
-    int rc = rows_launch(bf16, a, stream, what);
-    if (rc) return rc;
-    return sum_chunks(bf16, a.part, a.ldpart, a.chunks, 1, src.cols, out, 0, stream, what);
+    return rows_launch(bf16, a, stream, what);
 }
 
-// ---- argument checks ------------------------------------------------------------------------------------
-constexpr long long kMaxExtent = 1ll << 30;
-
 static int check_shape(const char* what, int dtype, int act, long long rows, long long in, long long out) {
-    if (dtype != RB200_FP16 && dtype != RB200_BF16) {
-        set_error("%s: dtype %d is neither RB200_FP16 nor RB200_BF16", what, dtype);
-        return RB200_E_INVALID;
-    }
+    int rc = check_dtype(what, dtype);
+    if (rc) return rc;
     if (act < RB200_ACT_NONE || act > RB200_ACT_SILU) {
         set_error("%s: activation %d is not one of RB200_ACT_*", what, act);
         return RB200_E_INVALID;
     }
-    if (rows < 0 || in < 1 || out < 1) {
-        set_error("%s: rows %lld, in_features %lld, out_features %lld", what, rows, in, out);
-        return RB200_E_INVALID;
-    }
-    if (rows > kMaxExtent || in > kMaxExtent || out > kMaxExtent) {
-        set_error("%s: %lld x %lld x %lld exceeds 2^30 in one extent", what, rows, in, out);
-        return RB200_E_LIMIT;
-    }
-    return RB200_OK;
-}
-
-// A matrix argument: present, its rows not overlapping, its elements on their own boundaries.
-static int check_matrix(const char* what, const char* name, const void* data, long long ld, long long rows, long long cols) {
-    if (!data) {
-        set_error("%s: %s is null", what, name);
-        return RB200_E_INVALID;
-    }
-    if ((uintptr_t)data & 1) {
-        set_error("%s: %s is not aligned to its elements", what, name);
-        return RB200_E_INVALID;
-    }
-    if (rows > 1 && (ld < cols || ld > (1ll << 38))) {
-        set_error("%s: leading dimension %lld of %s, %lld columns", what, ld, name, cols);
-        return RB200_E_INVALID;
-    }
-    return RB200_OK;
-}
-
-static int check_workspace(const char* what, const void* ws, uint64_t have, uint64_t need) {
-    if (need == 0) return RB200_OK;
-    if (!ws || have < need) {
-        set_error("%s: the workspace has %llu bytes, the call needs %llu", what, (unsigned long long)(ws ? have : 0), (unsigned long long)need);
-        return RB200_E_INVALID;
-    }
-    if ((uintptr_t)ws & 255) {
-        set_error("%s: the workspace must be 256-byte aligned", what);
-        return RB200_E_INVALID;
-    }
-    return RB200_OK;
-}
-
-static Operand operand(const void* data, long long ld, long long rows, long long cols, bool transposed) {
-    Operand o = {data, ld, (int)rows, (int)cols, transposed};
-    return o;
-}
-
-// An operand as the product reads it: in place, or from a packed copy in the workspace.
-struct Packed {
-    Operand src, use;
-    bool copy;
-};
-static Packed plan_pack(const Operand& o, Carver* c) {
-    Packed p = {o, o, !map_ready(o)};
-    if (p.copy) {
-        p.use.ld = round_up(o.cols, 8);
-        p.use.data = c->take((size_t)p.use.ld * o.rows * 2);
-    }
-    return p;
-}
-static int do_pack(const Packed& p, cudaStream_t stream, const char* what) {
-    return p.copy ? pack_rows(p.src, const_cast<void*>(p.use.data), p.use.ld, stream, what) : RB200_OK;
+    return check_extents(what, rows, "in_features", in, "out_features", out);
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------
@@ -295,7 +230,6 @@ static int linear_run(const rb200_linear_params* p, void* stream_v, GemmWait wai
     e.preact = p->preact;
     e.ldp = p->ldp;
     e.act = p->activation;
-    e.alpha_const = 1.0f;
     e.vec_out = map_ready(operand(p->out, p->ldo, p->rows, p->out_features, false));
     e.vec_res = map_ready(operand(p->residual, p->ldr, p->residual_rows, p->out_features, false));
     e.vec_pre = map_ready(operand(p->preact, p->ldp, p->rows, p->out_features, false));
@@ -305,7 +239,6 @@ static int linear_run(const rb200_linear_params* p, void* stream_v, GemmWait wai
         part.acc_out = (float*)l.partials;
         part.ldacc = round_up(p->out_features, 4);
         part.acc_split_stride = part.ldacc * p->rows;
-        part.alpha_const = 1.0f;
         if ((rc = gemm_store(GEMM_KK, bf16, l.x.use, l.w.use, nullptr, nullptr, l.gemm, part, wait, stream, what))) return rc;
         return gemm_join(bf16, (const float*)l.partials, l.gemm.splits, (int)p->rows, (int)p->out_features, e, stream, what);
     }
@@ -377,10 +310,6 @@ static LinearBackwardPlan plan_backward(const rb200_linear_backward_params& p, c
     return l;
 }
 
-static int clear_matrix(void* data, long long ld, long long rows, long long cols, cudaStream_t stream, const char* what) {
-    return check_cuda(cudaMemset2DAsync(data, (size_t)(rows > 1 ? ld : cols) * 2, 0, (size_t)cols * 2, (size_t)rows, stream), what);
-}
-
 static int backward_run(const rb200_linear_backward_params* p, void* stream_v) {
     const char* what = "rb200k_linear_backward";
     if (!p) {
@@ -419,19 +348,18 @@ static int backward_run(const rb200_linear_backward_params* p, void* stream_v) {
     if (p->dresidual) {
         const RowsArgs& r = l.res_rows;
         if ((rc = rows_launch(bf16, r, stream, what))) return rc;
-        if ((rc = sum_chunks(bf16, r.part, r.ldpart, r.chunks, r.period, (int)m, p->dresidual, p->lddr, stream, what))) return rc;
+        if ((rc = sum_chunks(bf16, r.part, r.ldpart, r.chunks, r.period, (int)m, p->dresidual, p->lddr, Scale(), stream, what))) return rc;
         if (p->dbias && !l.sums &&
-            (rc = sum_chunks(bf16, r.part, r.ldpart, r.chunks * r.period, 1, (int)m, p->dbias, 0, stream, what)))
+            (rc = sum_chunks(bf16, r.part, r.ldpart, r.chunks * r.period, 1, (int)m, p->dbias, 0, Scale(), stream, what)))
             return rc;
     }
     if (l.sums || l.own_dz) {
         const RowsArgs& r = l.bias_rows;
         if ((rc = rows_launch(bf16, r, stream, what))) return rc;
-        if (l.sums && (rc = sum_chunks(bf16, r.part, r.ldpart, r.chunks, 1, (int)m, p->dbias, 0, stream, what))) return rc;
+        if (l.sums && (rc = sum_chunks(bf16, r.part, r.ldpart, r.chunks, 1, (int)m, p->dbias, 0, Scale(), stream, what))) return rc;
     }
     const GemmWait wait = {p->status, 0, -1};
     EpiArgs e = {};
-    e.alpha_const = 1.0f;
     if (p->dx) {
         if ((rc = do_pack(l.w, stream, what))) return rc;
         e.out = p->dx;

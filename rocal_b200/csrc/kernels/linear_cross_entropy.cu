@@ -1,0 +1,535 @@
+// rb200k_linear_ce: softmax cross entropy of x W^T + b, forward and backward, without the rows x classes matrix.
+//   forward   one product whose epilogue keeps, for every row and half tile of classes, the largest score and the sum
+//             of exp(score - largest); ce_merge_kernel joins them (and makes the loss). The scores stay on the chip.
+//   backward  piece by piece: the product again, its epilogue turning scores into (softmax - target) in the element type, then
+//             that piece times W and transposed times x. Pieces are cut along the longer of classes and rows; the
+//             gradient that sums over pieces is accumulated in 32 bits.
+// Pieces hold (softmax - target) * c_i * 2^15 with |c_i| <= 1, so that a probability of 2^-29 is still a normal fp16;
+// the common factor (2^-15, the loss gradient, 1 / count) is applied to the 32-bit sums.
+#include "matrix_args.cuh"
+
+namespace rb200 {
+
+constexpr size_t kStatBytes = 64u << 20;     // partial maxima and sums of one launch
+constexpr size_t kPieceBytes = 256u << 20;   // scores' gradients of one piece
+
+// ---- forward: joining the partial statistics ----------------------------------------------------------------
+struct MergeArgs {
+    const float* part;      // [parts][rows] maxima, sums, sums of z
+    int parts, want_zsum;
+    const float* zlabel;
+    const void* labels;
+    int label_bytes, classes, rows, reduction;
+    long long ignore_index;
+    float smoothing;
+    int first, last;        // piece of the classes: the first starts the statistics, the last makes the loss
+    float* stats;           // [2][rows]
+    float* zsum;            // [rows], between pieces
+    float* loss;
+    int* info;
+    double* block_sums;
+};
+
+__device__ __forceinline__ void join(RunningSoftmax& a, float m, float s) {
+    const float top = fmaxf(a.m, m), base = finite_max(top);
+    a.s = a.s * exp_diff(a.m - base) + s * exp_diff(m - base);
+    a.m = top;
+}
+
+__global__ void __launch_bounds__(256) ce_merge_kernel(MergeArgs a) {
+    __shared__ float sm[8][33], ss[8][33], sz[8][33];
+    __shared__ double sums[256];
+    __shared__ int last_block;
+    const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
+    const int row = blockIdx.x * 32 + lane;
+    const long long plane = (long long)a.parts * a.rows;
+    RunningSoftmax r = {-INFINITY, 0.0f};
+    float z = 0.0f;
+    if (row < a.rows) {
+        for (int p = sub; p < a.parts; p += 8) {
+            const long long at = (long long)p * a.rows + row;
+            join(r, a.part[at], a.part[plane + at]);
+            if (a.want_zsum) z += a.part[2 * plane + at];
+        }
+    }
+    sm[sub][lane] = r.m;
+    ss[sub][lane] = r.s;
+    sz[sub][lane] = z;
+    __syncthreads();
+    if (sub == 0) {
+        bool counted = false, dirty = false;
+        double mine = 0.0;
+        if (row < a.rows) {
+            for (int i = 1; i < 8; i++) {
+                join(r, sm[i][lane], ss[i][lane]);
+                z += sz[i][lane];
+            }
+            if (!a.first) {
+                join(r, a.stats[row], a.stats[a.rows + row]);
+                if (a.want_zsum) z += a.zsum[row];
+            }
+            if (!a.last) {
+                if (a.want_zsum) a.zsum[row] = z;
+            } else {
+                const int label = load_label(a.labels, a.label_bytes, row, a.ignore_index, a.classes, &counted);
+                float loss = 0.0f;
+                if (counted) {
+                    if (label < 0) {
+                        r.m = r.s = loss = nanf("");
+                    } else {
+                        const float lse = logf(r.s);   // above the maximum
+                        loss = (1.0f - a.smoothing) * (lse + (r.m - a.zlabel[row]));
+                        if (a.want_zsum) loss += a.smoothing * (lse + (r.m - z / (float)a.classes));
+                    }
+                } else {
+                    dirty = !(isfinite(r.m) && isfinite(r.s));
+                }
+                mine = loss;
+                if (a.reduction == RB200_REDUCE_NONE) a.loss[row] = loss;
+            }
+            a.stats[row] = r.m;
+            a.stats[a.rows + row] = r.s;
+        }
+        if (a.last) {
+            const unsigned n = __popc(__ballot_sync(0xFFFFFFFFu, counted));
+            const bool any = __any_sync(0xFFFFFFFFu, dirty);
+#pragma unroll
+            for (int d = 16; d; d >>= 1) mine += __shfl_down_sync(0xFFFFFFFFu, mine, d);
+            if (lane == 0) {
+                if (n) atomicAdd(a.info, (int)n);
+                if (any) atomicOr(a.info + 1, 1);
+                if (a.reduction != RB200_REDUCE_NONE) {
+                    a.block_sums[blockIdx.x] = mine;
+                    __threadfence();
+                    last_block = atomicAdd(a.info + 2, 1) == (int)gridDim.x - 1;
+                }
+            }
+        }
+    }
+    if (!a.last || a.reduction == RB200_REDUCE_NONE) return;
+    __syncthreads();
+    if (!last_block) return;
+    // the block that finished last adds the others' sums, always in the same order
+    __threadfence();
+    double s = 0.0;
+    for (unsigned b = threadIdx.x; b < gridDim.x; b += 256) s += __ldcg(a.block_sums + b);
+    sums[threadIdx.x] = s;
+    __syncthreads();
+    for (int d = 128; d; d >>= 1) {
+        if (threadIdx.x < d) sums[threadIdx.x] += sums[threadIdx.x + d];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        const int count = atomicAdd(a.info, 0);
+        *a.loss = (float)(a.reduction == RB200_REDUCE_MEAN ? sums[0] / (double)max(1, count) : sums[0]);
+    }
+}
+
+// ---- backward: per-row factors --------------------------------------------------------------------------------
+// NONE: c_i = g_i / G and the common factor G, the power of two above the largest finite |g_i| of a counted row (so
+// the division is exact). One block: rows are few next to the products' work.
+__global__ void __launch_bounds__(1024) ce_factors_kernel(const float* __restrict__ dloss, const void* labels, int label_bytes, int classes,
+                                                          long long ignore_index, int rows, float* coef, float* factor) {
+    __shared__ float tops[32];
+    __shared__ float inv_s;
+    float top = 0.0f;
+    for (int i = threadIdx.x; i < rows; i += 1024) {
+        bool counted;
+        load_label(labels, label_bytes, i, ignore_index, classes, &counted);
+        const float g = fabsf(dloss[i]);
+        if (counted && g <= 3.4028235e38f) top = fmaxf(top, g);
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 32; i++) top = fmaxf(top, tops[i]);
+        // both the factor and its inverse stay normal: exponents -100 .. 100
+        int e = top > 0.0f ? ilogbf(top) + 1 : 0;
+        e = max(-100, min(100, e));
+        *factor = ldexpf(1.0f, e);
+        inv_s = ldexpf(1.0f, -e);
+    }
+    __syncthreads();
+    const float inv = inv_s;
+    for (int i = threadIdx.x; i < rows; i += 1024) coef[i] = dloss[i] * inv;
+}
+
+// Rows that do not count but hold inf or NaN would reach dweight as 0 * NaN: a copy of x with those rows zeroed, made
+// only if the forward pass found any.
+__global__ void __launch_bounds__(256) ce_clean_kernel(const int* info, const uint16_t* __restrict__ x, long long ldx, int rows, int cols,
+                                                       const void* labels, int label_bytes, int classes, long long ignore_index,
+                                                       uint16_t* __restrict__ out, long long ldo) {
+    if (info[1] == 0) return;
+    const long long groups = ldo / 8, total = groups * rows;
+    for (long long t = blockIdx.x * 256ll + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
+        const long long row = t / groups;
+        const int col = (int)(t - row * groups) * 8;
+        bool counted;
+        load_label(labels, label_bytes, row, ignore_index, classes, &counted);
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (counted) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (col + i < cols) w[i >> 1] |= (uint32_t)x[row * ldx + col + i] << (16 * (i & 1));
+        }
+        *reinterpret_cast<uint4*>(out + row * ldo + col) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// ---- argument checks --------------------------------------------------------------------------------------------
+static int check_sizes(const char* what, const rb200_linear_ce_params& p) {
+    int rc = check_dtype(what, p.dtype);
+    if (rc) return rc;
+    if (p.reduction < RB200_REDUCE_NONE || p.reduction > RB200_REDUCE_SUM) {
+        set_error("%s: reduction %d is not one of RB200_REDUCE_*", what, p.reduction);
+        return RB200_E_INVALID;
+    }
+    if (p.label_bytes != 4 && p.label_bytes != 8) {
+        set_error("%s: labels of %d bytes (4 or 8)", what, p.label_bytes);
+        return RB200_E_INVALID;
+    }
+    if (!(p.label_smoothing >= 0.0f && p.label_smoothing <= 1.0f)) {
+        set_error("%s: label_smoothing %g outside [0, 1]", what, p.label_smoothing);
+        return RB200_E_INVALID;
+    }
+    return check_extents(what, p.rows, "features", p.features, "classes", p.classes);
+}
+
+static int check_common(const char* what, const rb200_linear_ce_params& p) {
+    int rc;
+    if ((rc = check_matrix(what, "x", p.x, p.ldx, p.rows, p.features))) return rc;
+    if ((rc = check_matrix(what, "weight", p.weight, p.ldw, p.classes, p.features))) return rc;
+    if (p.bias && (rc = check_matrix(what, "bias", p.bias, 0, 1, p.classes))) return rc;
+    if (!p.labels || !p.stats || !p.info) {
+        set_error("%s: labels, stats or info is null", what);
+        return RB200_E_INVALID;
+    }
+    if (((uintptr_t)p.labels & (p.label_bytes - 1)) || (((uintptr_t)p.stats | (uintptr_t)p.info) & 3)) {
+        set_error("%s: labels, stats or info is not aligned to its elements", what);
+        return RB200_E_INVALID;
+    }
+    return RB200_OK;
+}
+
+static EpiArgs label_args(const rb200_linear_ce_params& p) {
+    EpiArgs e = {};
+    e.labels = p.labels;
+    e.label_bytes = p.label_bytes;
+    e.classes = (int)p.classes;
+    e.ignore_index = p.ignore_index;
+    e.smooth_on = 1.0f - p.label_smoothing;
+    e.smooth_off = p.label_smoothing / (float)p.classes;
+    return e;
+}
+static const uint8_t* at_row(const void* p, long long ld, long long row) { return (const uint8_t*)p + row * ld * 2; }
+
+// ---- forward ------------------------------------------------------------------------------------------------------
+struct StatsPlan {
+    Packed x, w;
+    int piece;              // classes of one launch
+    size_t part_bytes;
+    float *part, *zlabel, *zsum;
+    double* block_sums;
+    size_t bytes;
+};
+static GemmPlan stats_gemm(const rb200_linear_ce_params& p, const DeviceInfo& dev, int classes) {
+    return gemm_plan(dev, (int)p.rows, classes, (int)p.features, false, false);
+}
+static StatsPlan plan_stats(const rb200_linear_ce_params& p, const DeviceInfo& dev, void* ws) {
+    StatsPlan s;
+    Carver c(ws);
+    s.x = plan_pack(operand(p.x, p.ldx, p.rows, p.features, false), &c);
+    s.w = plan_pack(operand(p.weight, p.ldw, p.classes, p.features, false), &c);
+    // a half tile of 16 columns is the smallest that a plan makes; a piece keeps whole tiles of every width
+    const size_t per_part = (size_t)p.rows * 3 * sizeof(float);
+    long long parts = (long long)(kStatBytes / per_part);
+    if (parts < 2) parts = 2;
+    long long piece = parts / 2 * 32 / kTileNMax * kTileNMax;
+    if (piece < kTileNMax) piece = kTileNMax;
+    s.piece = (int)(piece < p.classes ? piece : p.classes);
+    const long long most = 2ll * stats_gemm(p, dev, s.piece).tiles_n;
+    const long long rest = p.classes % s.piece ? 2ll * stats_gemm(p, dev, (int)(p.classes % s.piece)).tiles_n : 0;
+    s.part_bytes = (size_t)(most > rest ? most : rest) * per_part;
+    s.part = (float*)c.take(s.part_bytes);
+    s.zlabel = (float*)c.take((size_t)p.rows * sizeof(float));
+    s.zsum = (float*)c.take((size_t)p.rows * sizeof(float));
+    s.block_sums = (double*)c.take((size_t)((p.rows + 31) / 32) * sizeof(double));
+    s.bytes = c.used;
+    return s;
+}
+
+static int ce_forward(const rb200_linear_ce_params* p, cudaStream_t stream) {
+    const char* what = "rb200k_linear_ce";
+    if (!p) {
+        set_error("%s: params is null", what);
+        return RB200_E_INVALID;
+    }
+    int rc = check_sizes(what, *p);
+    if (rc) return rc;
+    if (p->rows == 0) {
+        if (p->info && (rc = check_cuda(cudaMemsetAsync(p->info, 0, 16, stream), what))) return rc;
+        if (p->loss && p->reduction != RB200_REDUCE_NONE) return check_cuda(cudaMemsetAsync(p->loss, 0, 4, stream), what);
+        return RB200_OK;
+    }
+    if ((rc = check_common(what, *p))) return rc;
+    if (!p->loss || ((uintptr_t)p->loss & 3)) {
+        set_error("%s: loss is null or not aligned", what);
+        return RB200_E_INVALID;
+    }
+    DeviceInfo dev;
+    if ((rc = device_info(&dev))) return rc;
+    const StatsPlan s = plan_stats(*p, dev, p->workspace);
+    if ((rc = check_workspace(what, p->workspace, p->workspace_bytes, s.bytes))) return rc;
+    const bool bf16 = p->dtype == RB200_BF16;
+    if ((rc = do_pack(s.x, stream, what)) || (rc = do_pack(s.w, stream, what))) return rc;
+    const GemmWait wait = {p->status, 0, -1};
+    for (long long c0 = 0; c0 < p->classes; c0 += s.piece) {
+        const int classes = (int)(p->classes - c0 < s.piece ? p->classes - c0 : s.piece);
+        const GemmPlan plan = stats_gemm(*p, dev, classes);
+        EpiArgs e = label_args(*p);
+        e.bias = p->bias ? at_row(p->bias, 1, c0) : nullptr;
+        e.class0 = (int)c0;
+        e.part = s.part;
+        e.parts = 2 * plan.tiles_n;
+        e.want_zsum = p->label_smoothing > 0.0f;
+        e.zlabel = s.zlabel;
+        e.clear = p->info;
+        const Operand w = operand(at_row(s.w.use.data, s.w.use.ld, c0), s.w.use.ld, classes, p->features, false);
+        if ((rc = gemm_launch<EPI_CE_STATS, false, false>(bf16, s.x.use, w, nullptr, nullptr, plan, e, wait, stream, what))) return rc;
+        MergeArgs m = {};
+        m.part = s.part;
+        m.parts = e.parts;
+        m.want_zsum = e.want_zsum;
+        m.zlabel = s.zlabel;
+        m.labels = p->labels;
+        m.label_bytes = p->label_bytes;
+        m.classes = (int)p->classes;
+        m.rows = (int)p->rows;
+        m.reduction = p->reduction;
+        m.ignore_index = p->ignore_index;
+        m.smoothing = p->label_smoothing;
+        m.first = c0 == 0;
+        m.last = c0 + classes == p->classes;
+        m.stats = p->stats;
+        m.zsum = s.zsum;
+        m.loss = p->loss;
+        m.info = p->info;
+        m.block_sums = s.block_sums;
+        ce_merge_kernel<<<(unsigned)((p->rows + 31) / 32), 256, 0, stream>>>(m);
+        RB200_CHECK_LAUNCH(what);
+    }
+    return RB200_OK;
+}
+
+// ---- backward -----------------------------------------------------------------------------------------------------
+struct GradPlan {
+    Packed x, w;
+    Operand clean;              // x without the rows that do not count
+    bool by_rows;               // pieces are cut along the rows
+    int piece, pieces;
+    long long ldd;              // of the piece's gradients
+    void* dz;
+    float *coef, *factor;
+    float* sum;                 // 32-bit sums over pieces: dx (pieces of classes) or dweight (pieces of rows)
+    long long ldsum;
+    void *px, *pw;              // partial products
+    int col_chunks;             // partial sums that a piece makes at most
+    float* col_part;
+    size_t bytes;
+};
+static int piece_rows(const rb200_linear_ce_params& p, const GradPlan& g, int i) {
+    if (!g.by_rows) return (int)p.rows;
+    const long long left = p.rows - (long long)i * g.piece;
+    return (int)(left < g.piece ? left : g.piece);
+}
+static int piece_classes(const rb200_linear_ce_params& p, const GradPlan& g, int i) {
+    if (g.by_rows) return (int)p.classes;
+    const long long left = p.classes - (long long)i * g.piece;
+    return (int)(left < g.piece ? left : g.piece);
+}
+static GradPlan plan_grad(const rb200_linear_ce_params& p, const DeviceInfo& dev, void* ws) {
+    GradPlan g = {};
+    Carver c(ws);
+    const int k = (int)p.features;
+    g.x = plan_pack(operand(p.x, p.ldx, p.rows, k, false), &c);
+    g.w = plan_pack(operand(p.weight, p.ldw, p.classes, k, false), &c);
+    g.by_rows = p.rows > p.classes;
+    const long long longer = g.by_rows ? p.rows : p.classes, shorter = g.by_rows ? p.classes : p.rows;
+    long long piece = (long long)(kPieceBytes / 2) / shorter / kTileNMax * kTileNMax;
+    if (piece < kTileNMax) piece = kTileNMax;
+    if (piece < longer) {   // pieces of about one size
+        const long long pieces = (longer + piece - 1) / piece;
+        piece = round_up((longer + pieces - 1) / pieces, kTileNMax);
+    }
+    g.piece = (int)(piece < longer ? piece : longer);
+    g.pieces = (int)((longer + g.piece - 1) / g.piece);
+    g.ldd = round_up(piece_classes(p, g, 0), 8);
+    g.dz = c.take((size_t)g.ldd * piece_rows(p, g, 0) * 2);
+    if (p.reduction == RB200_REDUCE_NONE) {
+        g.coef = (float*)c.take((size_t)p.rows * sizeof(float));
+        g.factor = (float*)c.take(sizeof(float));
+    }
+    if (p.dweight) {
+        g.clean = operand(nullptr, round_up(k, 8), p.rows, k, true);
+        g.clean.data = c.take((size_t)g.clean.ld * p.rows * 2);
+    }
+    g.ldsum = round_up(k, 4);
+    if (g.pieces > 1 && (g.by_rows ? p.dweight : p.dx)) g.sum = (float*)c.take((size_t)shorter * g.ldsum * sizeof(float));
+    // the last piece is the only one of another size
+    size_t px = 0, pw = 0, pc = 0;
+    for (int i = 0; i < g.pieces; i += g.pieces > 1 ? g.pieces - 1 : 1) {
+        const int rows = piece_rows(p, g, i), classes = piece_classes(p, g, i);
+        const size_t bx = gemm_partial_bytes(gemm_plan(dev, rows, k, classes, true, true), rows, k);
+        const size_t bw = gemm_partial_bytes(gemm_plan(dev, classes, k, rows, true, true), classes, k);
+        if (bx > px) px = bx;
+        if (bw > pw) pw = bw;
+        const ColumnSums cs = plan_column_sums(rows, classes, dev.sms);
+        if (cs.chunks > g.col_chunks) g.col_chunks = cs.chunks;   // a smaller piece may be cut into more chunks
+        if (cs.chunks * (size_t)cs.ldpart > pc) pc = cs.chunks * (size_t)cs.ldpart;
+    }
+    if (p.dx) g.px = c.take(px);
+    if (p.dweight) g.pw = c.take(pw);
+    // pieces of the rows keep theirs until the last one, packed behind one another
+    if (p.dbias) g.col_part = (float*)c.take((g.by_rows ? (size_t)g.col_chunks * g.pieces * round_up(p.classes, 4) : pc) * sizeof(float));
+    g.bytes = c.used;
+    return g;
+}
+
+static int ce_backward(const rb200_linear_ce_params* p, cudaStream_t stream) {
+    const char* what = "rb200k_linear_ce_backward";
+    if (!p) {
+        set_error("%s: params is null", what);
+        return RB200_E_INVALID;
+    }
+    int rc = check_sizes(what, *p);
+    if (rc) return rc;
+    const long long n = p->rows, v = p->classes, k = p->features;
+    if (p->dweight && (rc = check_matrix(what, "dweight", p->dweight, p->lddw, v, k))) return rc;
+    if (p->dbias && (rc = check_matrix(what, "dbias", p->dbias, 0, 1, v))) return rc;
+    if (n == 0) {
+        if (p->dweight && (rc = clear_matrix(p->dweight, p->lddw, v, k, stream, what))) return rc;
+        if (p->dbias && (rc = clear_matrix(p->dbias, 0, 1, v, stream, what))) return rc;
+        return RB200_OK;
+    }
+    if (!p->dx && !p->dweight && !p->dbias) return RB200_OK;
+    if ((rc = check_common(what, *p))) return rc;
+    if (p->dx && (rc = check_matrix(what, "dx", p->dx, p->lddx, n, k))) return rc;
+    if (!p->dloss || ((uintptr_t)p->dloss & 3)) {
+        set_error("%s: dloss is null or not aligned", what);
+        return RB200_E_INVALID;
+    }
+    DeviceInfo dev;
+    if ((rc = device_info(&dev))) return rc;
+    const GradPlan g = plan_grad(*p, dev, p->workspace);
+    if ((rc = check_workspace(what, p->workspace, p->workspace_bytes, g.bytes))) return rc;
+    const bool bf16 = p->dtype == RB200_BF16;
+    const GemmWait wait = {p->status, 0, -1};
+    if ((rc = do_pack(g.x, stream, what)) || (rc = do_pack(g.w, stream, what))) return rc;
+    const bool none = p->reduction == RB200_REDUCE_NONE;
+    if (none) {
+        ce_factors_kernel<<<1, 1024, 0, stream>>>(p->dloss, p->labels, p->label_bytes, (int)v, p->ignore_index, (int)n, g.coef, g.factor);
+        RB200_CHECK_LAUNCH(what);
+    }
+    if (p->dweight) {
+        const long long blocks = (g.clean.ld / 8 * n + 255) / 256;
+        ce_clean_kernel<<<(unsigned)(blocks < 8 * dev.sms ? blocks : 8 * dev.sms), 256, 0, stream>>>(
+            p->info, (const uint16_t*)p->x, p->ldx, (int)n, (int)k, p->labels, p->label_bytes, (int)v, p->ignore_index,
+            (uint16_t*)const_cast<void*>(g.clean.data), g.clean.ld);
+        RB200_CHECK_LAUNCH(what);
+    }
+    const Scale scale(1.0f / 32768.0f, none ? g.factor : p->dloss, p->reduction == RB200_REDUCE_MEAN ? p->info : nullptr);
+    int planes = 0;   // of partial column sums so far
+    for (int i = 0; i < g.pieces; i++) {
+        const int rows = piece_rows(*p, g, i), classes = piece_classes(*p, g, i);
+        const long long r0 = g.by_rows ? (long long)i * g.piece : 0, c0 = g.by_rows ? 0 : (long long)i * g.piece;
+        const Operand x = operand(at_row(g.x.use.data, g.x.use.ld, r0), g.x.use.ld, rows, k, false);
+        const Operand w = operand(at_row(g.w.use.data, g.w.use.ld, c0), g.w.use.ld, classes, k, false);
+        Operand dz = operand(g.dz, g.ldd, rows, classes, false);
+        EpiArgs e = label_args(*p);
+        e.labels = (const uint8_t*)p->labels + r0 * p->label_bytes;
+        e.bias = p->bias ? at_row(p->bias, 1, c0) : nullptr;
+        e.class0 = (int)c0;
+        e.stats = p->stats + r0;
+        e.stats_stride = n;
+        e.coef = none ? g.coef + r0 : nullptr;
+        e.out = g.dz;
+        e.ldo = g.ldd;
+        e.vec_out = 1;
+        const GemmPlan plan = gemm_plan(dev, rows, classes, (int)k, false, false);
+        if ((rc = gemm_launch<EPI_CE_GRAD, false, false>(bf16, x, w, nullptr, nullptr, plan, e, wait, stream, what))) return rc;
+        const bool first = i == 0, last = i == g.pieces - 1;
+        if (p->dx) {
+            EpiArgs o = {};
+            Operand wt = w;
+            wt.transposed = true;
+            if (g.by_rows || g.pieces == 1) {
+                o.out = const_cast<uint8_t*>(at_row(p->dx, p->lddx, r0));
+                o.ldo = p->lddx;
+            } else {   // a piece of the classes gives a summand of dx
+                o.acc_in = first ? nullptr : g.sum;
+                o.acc_out = last ? nullptr : g.sum;
+                o.ldacc = g.ldsum;
+                o.out = p->dx;
+                o.ldo = p->lddx;
+            }
+            o.vec_out = map_ready(operand(o.out, o.ldo, rows, k, false));
+            o.scale = scale;
+            if ((rc = gemm_store_joined(GEMM_KN, bf16, dz, wt, nullptr, nullptr, gemm_plan(dev, rows, (int)k, classes, true, true), o, g.px, wait,
+                                        stream, what)))
+                return rc;
+        }
+        if (p->dweight) {
+            EpiArgs o = {};
+            Operand xt = x, clean = g.clean, dzt = dz;
+            xt.transposed = dzt.transposed = true;
+            clean.data = at_row(clean.data, clean.ld, r0);
+            clean.rows = rows;
+            if (!g.by_rows || g.pieces == 1) {
+                o.out = const_cast<uint8_t*>(at_row(p->dweight, p->lddw, c0));
+                o.ldo = p->lddw;
+            } else {
+                o.acc_in = first ? nullptr : g.sum;
+                o.acc_out = last ? nullptr : g.sum;
+                o.ldacc = g.ldsum;
+                o.out = p->dweight;
+                o.ldo = p->lddw;
+            }
+            o.vec_out = map_ready(operand(o.out, o.ldo, classes, k, false));
+            o.scale = scale;
+            if ((rc = gemm_store_joined(GEMM_NN, bf16, dzt, xt, &clean, p->info + 1, gemm_plan(dev, classes, (int)k, rows, true, true), o, g.pw,
+                                        wait, stream, what)))
+                return rc;
+        }
+        if (p->dbias) {
+            const ColumnSums cs = plan_column_sums(rows, classes, dev.sms);
+            if (!g.by_rows) planes = 0;
+            if ((rc = column_partials(bf16, dz, g.col_part + planes * cs.ldpart, dev.sms, stream, what))) return rc;
+            planes += cs.chunks;
+            if (!g.by_rows || last) {
+                if ((rc = sum_chunks(bf16, g.col_part, cs.ldpart, planes, 1, classes, const_cast<uint8_t*>(at_row(p->dbias, 1, c0)), 0, scale,
+                                     stream, what)))
+                    return rc;
+            }
+        }
+    }
+    return RB200_OK;
+}
+
+}  // namespace rb200
+
+using namespace rb200;
+
+extern "C" uint64_t rb200k_linear_ce_workspace_bytes(const rb200_linear_ce_params* p) {
+    DeviceInfo dev;
+    if (!p || check_sizes("rb200k_linear_ce_workspace_bytes", *p) || p->rows == 0 || device_info(&dev)) return 0;
+    return plan_stats(*p, dev, nullptr).bytes;
+}
+extern "C" int rb200k_linear_ce(const rb200_linear_ce_params* p, void* stream) { return ce_forward(p, (cudaStream_t)stream); }
+extern "C" uint64_t rb200k_linear_ce_backward_workspace_bytes(const rb200_linear_ce_params* p) {
+    DeviceInfo dev;
+    if (!p || check_sizes("rb200k_linear_ce_backward_workspace_bytes", *p) || p->rows == 0 || device_info(&dev)) return 0;
+    return plan_grad(*p, dev, nullptr).bytes;
+}
+extern "C" int rb200k_linear_ce_backward(const rb200_linear_ce_params* p, void* stream) { return ce_backward(p, (cudaStream_t)stream); }

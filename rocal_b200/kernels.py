@@ -10,7 +10,8 @@ import numpy as np
 import torch
 
 from . import tables as T
-from ._lib import (BoxEncoderParams, BoxMatcherParams, LinearBackwardParams, LinearParams, NormalizeParams, PointwiseParams,
+from ._lib import (BoxEncoderParams, BoxMatcherParams, LinearBackwardParams, LinearCeParams,
+                   LinearParams, NormalizeParams, PointwiseParams,
                    ResampleParams, WarpParams, check, lib)
 
 _TORCH_DTYPE = {T.FP32: torch.float32, T.FP16: torch.float16, T.UINT8: torch.uint8}
@@ -402,4 +403,71 @@ def linear_backward(dout, x, weight, preact=None, activation="none", residual_ro
             p.status = status.data_ptr()
         ws = _workspace(p, lib.rb200k_linear_backward_workspace_bytes, x.device)  # noqa: F841
         check(lib.rb200k_linear_backward(ctypes.byref(p), s), "rb200k_linear_backward")
+    return tuple(grads)
+
+
+def _ce_params(x, weight, labels, bias, ignore_index, label_smoothing, reduction):
+    """(parameter block, tensors that it points into) of a linear cross entropy."""
+    dtype, x, weight = _head_input(x, weight)
+    n, k = x.shape
+    v = weight.shape[0]
+    if reduction not in T.REDUCTIONS:
+        raise ValueError("reduction %r: one of %s is needed" % (reduction, ", ".join(T.REDUCTIONS)))
+    if labels.dim() != 1 or labels.shape[0] != n or labels.device != x.device or labels.dtype not in (torch.int32, torch.int64):
+        raise ValueError("labels are %s %s on %s, needed: int32 or int64 of shape (%d,) on %s"
+                         % (labels.dtype, tuple(labels.shape), labels.device, n, x.device))
+    labels = labels.contiguous()
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError("label_smoothing %r outside [0, 1]" % (label_smoothing,))
+    p = LinearCeParams(dtype, T.REDUCTIONS[reduction], n, k, v, x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0))
+    if bias is not None:
+        bias = _vector(bias, "bias", x, v)
+        p.bias = bias.data_ptr()
+    p.labels, p.label_bytes, p.label_smoothing, p.ignore_index = labels.data_ptr(), labels.element_size(), label_smoothing, ignore_index
+    return p, (x, weight, labels, bias)
+
+
+def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, label_smoothing=0.0, reduction="mean", stream=None, status=None):
+    """rb200k_linear_ce: the cross entropy of the scores x weight^T + bias for x [n, k], weight [v, k], labels [n] (int32 or
+    int64), without making the [n, v] scores. Returns (loss, stats, info): the loss is fp32, [n] or a scalar; stats and info
+    go to linear_cross_entropy_backward."""
+    p, held = _ce_params(x, weight, labels, bias, ignore_index, label_smoothing, reduction)
+    x, n = held[0], p.rows
+    with _on(x.device, stream) as s:
+        loss = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=x.device)
+        stats = torch.empty((2, n), dtype=torch.float32, device=x.device)
+        info = torch.empty((4,), dtype=torch.int32, device=x.device)
+        p.loss, p.stats, p.info = loss.data_ptr(), stats.data_ptr(), info.data_ptr()
+        if status is not None:
+            p.status = status.data_ptr()
+        ws = _workspace(p, lib.rb200k_linear_ce_workspace_bytes, x.device)  # noqa: F841
+        check(lib.rb200k_linear_ce(ctypes.byref(p), s), "rb200k_linear_ce")
+    return loss, stats, info
+
+
+def linear_cross_entropy_backward(dloss, x, weight, labels, stats, info, bias=None, ignore_index=-100, label_smoothing=0.0,
+                                  reduction="mean", need=(True, True, True), stream=None, status=None):
+    """rb200k_linear_ce_backward: (dx, dweight, dbias), None where `need` is false. dloss: fp32, of the loss's shape."""
+    p, held = _ce_params(x, weight, labels, bias, ignore_index, label_smoothing, reduction)
+    x, n, k, v = held[0], p.rows, p.features, p.classes
+    if dloss.dtype != torch.float32 or dloss.device != x.device or tuple(dloss.shape) != ((n,) if reduction == "none" else ()):
+        raise ValueError("dloss is %s %s on %s, it has to be like the loss" % (dloss.dtype, tuple(dloss.shape), dloss.device))
+    if tuple(stats.shape) != (2, n) or stats.dtype != torch.float32 or tuple(info.shape) != (4,) or info.dtype != torch.int32 or \
+            stats.device != x.device or info.device != x.device or not stats.is_contiguous() or not info.is_contiguous():
+        raise ValueError("stats and info are not those of this forward pass")
+    dloss = dloss.contiguous()
+    with _on(x.device, stream) as s:
+        grads = [torch.empty(shape, dtype=x.dtype, device=x.device) if want else None for shape, want in zip(((n, k), (v, k), (v,)), need)]
+        dx, dw, db = grads
+        p.dloss, p.stats, p.info = dloss.data_ptr(), stats.data_ptr(), info.data_ptr()
+        if dx is not None:
+            p.dx, p.lddx = dx.data_ptr(), k
+        if dw is not None:
+            p.dweight, p.lddw = dw.data_ptr(), k
+        if db is not None:
+            p.dbias = db.data_ptr()
+        if status is not None:
+            p.status = status.data_ptr()
+        ws = _workspace(p, lib.rb200k_linear_ce_backward_workspace_bytes, x.device)  # noqa: F841
+        check(lib.rb200k_linear_ce_backward(ctypes.byref(p), s), "rb200k_linear_ce_backward")
     return tuple(grads)

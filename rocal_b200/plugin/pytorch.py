@@ -130,3 +130,44 @@ def linear(x, weight, bias=None, residual=None, activation="none"):
         from .. import kernels
         y = kernels.linear(x2, weight, bias, residual, activation)
     return y if x.dim() == 2 else y.reshape(shape)
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, labels, bias, ignore_index, label_smoothing, reduction):
+        from .. import kernels
+        loss, stats, info = kernels.linear_cross_entropy(x, weight, labels, bias, ignore_index, label_smoothing, reduction)
+        ctx.save_for_backward(x, weight, labels, bias, stats, info)
+        ctx.how = (ignore_index, label_smoothing, reduction)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        from .. import kernels
+        x, weight, labels, bias, stats, info = ctx.saved_tensors
+        need = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3])
+        dx, dw, db = kernels.linear_cross_entropy_backward(dloss, x, weight, labels, stats, info, bias, *ctx.how, need)
+        return dx, dw, None, db, None, None, None
+
+
+def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
+    """Softmax cross entropy of the scores x weight^T + bias against class indices, without keeping the scores: forward
+    and backward pass make them piece by piece. For the labels of the iterators above, of Pipeline.get_image_labels() and of
+    the box encoder (the anchors' classes, int32).
+
+    x [..., k] and weight [v, k], bias [v]: all float16 or all bfloat16; labels [...]: int32 or int64. Rows whose label is
+    ignore_index (samples that pad the last batch, anchors that matched nothing) have loss 0 and take no part in any
+    gradient, whatever their features hold; any other label outside 0 .. v-1 makes the row's loss NaN. A class is masked by
+    a bias of -inf or of the type's lowest value. reduction "mean" (over the rows that count; 0 if none does), "sum" or
+    "none" (the shape of labels). The loss is float32."""
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or tuple(labels.shape) != tuple(x.shape[:-1]):
+        raise ValueError("x %s, weight %s and labels %s do not go together" % (tuple(x.shape), tuple(weight.shape), tuple(labels.shape)))
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    flat = labels if labels.dim() == 1 else labels.reshape(-1)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        loss = _LinearCrossEntropy.apply(x2, weight, flat, bias, ignore_index, label_smoothing, reduction)
+    else:
+        from .. import kernels
+        loss = kernels.linear_cross_entropy(x2, weight, flat, bias, ignore_index, label_smoothing, reduction)[0]
+    return loss.reshape(labels.shape) if reduction == "none" else loss
