@@ -499,6 +499,26 @@ RB200_API int rb200k_linear_ce(const rb200_linear_ce_params* params, void* strea
 RB200_API uint64_t rb200k_linear_ce_backward_workspace_bytes(const rb200_linear_ce_params* params);
 RB200_API int rb200k_linear_ce_backward(const rb200_linear_ce_params* params, void* stream);
 
+/* Global norm of a step's gradients and clipping. With N = inv_scale * sqrt(sum of all squares over all tensors) and
+ * c = min(1, max_norm / (N + 1e-6)), every tensor's out = grad * (inv_scale * c), and *norm = N. inv_scale undoes the loss scale
+ * of float16 training (1 otherwise). out may be grad itself (same type; nothing is written when inv_scale * c is 1) or
+ * another array; no two outputs overlap, and no output overlaps another tensor's gradients (refused). Squares are added
+ * in 64 bits, in an order that only depends on the tensors' sizes. A gradient with inf gives N = inf and c = 0, one
+ * with NaN gives NaN everywhere. No alignment beyond the elements' own is needed; 16-byte boundaries are faster. Empty
+ * tensors are skipped. `tensors` is a HOST array, not retained after return. */
+typedef struct rb200_grad_tensor {
+    const void* grad;
+    void* out;
+    int64_t count;               /* elements */
+    int32_t grad_dtype;          /* RB200_FP32, RB200_FP16 or RB200_BF16 */
+    int32_t out_dtype;           /* grad_dtype or RB200_FP32 */
+} rb200_grad_tensor;
+
+/* Bytes of workspace for this many tensors (any sizes). */
+RB200_API uint64_t rb200k_grad_clip_workspace_bytes(int num_tensors);
+RB200_API int rb200k_grad_clip(const rb200_grad_tensor* tensors, int num_tensors, float max_norm, float inv_scale, float* norm,
+                     void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------------------------------
  * Overlapping launches
  * ------------------------------------------------------------------------------------- */

@@ -95,6 +95,9 @@ for _name, _params in (("linear", LinearParams), ("linear_backward", LinearBackw
     _f.argtypes, _f.restype = [ctypes.POINTER(_params)], c_uint64
     _f = getattr(lib, "rb200k_" + _name)
     _f.argtypes, _f.restype = [ctypes.POINTER(_params), c_void_p], c_int
+lib.rb200k_grad_clip_workspace_bytes.argtypes, lib.rb200k_grad_clip_workspace_bytes.restype = [c_int], c_uint64
+lib.rb200k_grad_clip.argtypes = [c_void_p, c_int, ctypes.c_float, ctypes.c_float, c_void_p, c_void_p, c_uint64, c_void_p]
+lib.rb200k_grad_clip.restype = c_int
 lib.rb200k_linear_probe.argtypes = [ctypes.POINTER(LinearParams), c_void_p, c_uint64, c_int]
 lib.rb200k_linear_probe.restype = c_int
 lib.rb200k_normalize_scratch_bytes.argtypes = [c_int, c_int, c_int, c_int]

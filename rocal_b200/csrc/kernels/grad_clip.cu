@@ -1,0 +1,348 @@
+// rb200k_grad_clip: norm over many tensors and clipping. Two sweeps, both bound by memory: the first adds the squares,
+// the second multiplies. The tensors' table travels in the launch's own parameters (no copy, nothing to keep alive, and
+// a captured graph holds it). Tensors are cut into chunks of one size, which blocks take in turn; the second sweep walks
+// the chunks backwards, so that what the first one read last is still in L2.
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "gemm.cuh"
+
+namespace rb200 {
+
+constexpr int kClipThreads = 256, kClipBlocksPerSm = 8;
+constexpr int kClipMaxBlocks = 148 * kClipBlocksPerSm;   // partial sums a launch leaves at most
+
+struct ClipEntry {
+    const void* grad;
+    void* out;
+    long long count;
+    int chunk0;         // of this tensor, counted over the launch's table
+    short grad_dtype, out_dtype;
+};
+template <int CAP>
+struct ClipTable {
+    ClipEntry e[CAP];
+    int n, chunks;
+    int chunk;          // elements
+};
+
+template <int CAP>
+__device__ __forceinline__ int find_tensor(const ClipTable<CAP>& t, int c) {
+    int lo = 0, hi = t.n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (t.e[mid].chunk0 <= c)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    return lo;
+}
+
+template <typename T>
+struct Values;   // of one 16-byte vector
+template <>
+struct Values<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void get(const uint4& w, float* v) {
+        v[0] = __uint_as_float(w.x);
+        v[1] = __uint_as_float(w.y);
+        v[2] = __uint_as_float(w.z);
+        v[3] = __uint_as_float(w.w);
+    }
+    static __device__ __forceinline__ uint4 put(const float* v) {
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    }
+    static __device__ __forceinline__ float to_float(float v) { return v; }
+    static __device__ __forceinline__ float from_float(float v) { return v; }
+};
+template <typename T>
+struct Values16 {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void get(const uint4& w, float* v) {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = Elem<T>::unpack(u[i]);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
+    static __device__ __forceinline__ uint4 put(const float* v) {
+        return make_uint4(Elem<T>::pack(v[0], v[1]), Elem<T>::pack(v[2], v[3]), Elem<T>::pack(v[4], v[5]), Elem<T>::pack(v[6], v[7]));
+    }
+    static __device__ __forceinline__ float to_float(T v) { return Elem<T>::to_float(v); }
+    static __device__ __forceinline__ T from_float(float v) { return Elem<T>::from_float(v); }
+};
+template <>
+struct Values<__half> : Values16<__half> {};
+template <>
+struct Values<__nv_bfloat16> : Values16<__nv_bfloat16> {};
+
+// ---- sum of squares ---------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ double square_sum(const T* p, int count) {
+    constexpr int N = Values<T>::N;
+    double s = 0.0;
+    const int head = min(count, (int)(((16 - ((uintptr_t)p & 15)) & 15) / sizeof(T)));   // up to the 16-byte boundary
+    if ((int)threadIdx.x < head) {
+        const double v = Values<T>::to_float(p[threadIdx.x]);
+        s = v * v;
+    }
+    p += head;
+    count -= head;
+    const uint4* q = reinterpret_cast<const uint4*>(p);
+    const int vectors = count / N;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < vectors; i += kClipThreads) {
+        float v[N];
+        Values<T>::get(__ldg(q + i), v);
+#pragma unroll
+        for (int j = 0; j < N; j++) s += (double)v[j] * (double)v[j];
+    }
+    const int tail = vectors * N + threadIdx.x;
+    if (tail < count) {
+        const double v = Values<T>::to_float(p[tail]);
+        s += v * v;
+    }
+    return s;
+}
+
+// The block's sum, in thread 0.
+__device__ __forceinline__ double block_sum(double s, double* shared) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
+    if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = s;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        for (int i = 1; i < kClipThreads / 32; i++) s += shared[i];
+    return s;
+}
+
+template <int CAP>
+__global__ void __launch_bounds__(kClipThreads) clip_norm_kernel(const __grid_constant__ ClipTable<CAP> t, double* partial) {
+    __shared__ double shared[kClipThreads / 32];
+    double s = 0.0;
+    for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+        const ClipEntry& e = t.e[find_tensor(t, c)];
+        const long long begin = (long long)(c - e.chunk0) * t.chunk;
+        const int count = (int)min((long long)t.chunk, e.count - begin);
+        if (e.grad_dtype == RB200_FP32)
+            s += square_sum(reinterpret_cast<const float*>(e.grad) + begin, count);
+        else if (e.grad_dtype == RB200_FP16)
+            s += square_sum(reinterpret_cast<const __half*>(e.grad) + begin, count);
+        else
+            s += square_sum(reinterpret_cast<const __nv_bfloat16*>(e.grad) + begin, count);
+    }
+    s = block_sum(s, shared);
+    if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+
+// ---- multiplication -----------------------------------------------------------------------------------------
+template <typename T, typename O>
+__device__ __forceinline__ void scale_chunk(const T* g, O* o, int count, float factor) {
+    constexpr int N = Values<T>::N;
+    if ((((uintptr_t)g | (uintptr_t)o) & 15) == 0) {
+        const int vectors = count / N;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < vectors; i += kClipThreads) {
+            float v[N];
+            Values<T>::get(reinterpret_cast<const uint4*>(g)[i], v);
+#pragma unroll
+            for (int j = 0; j < N; j++) v[j] *= factor;
+#pragma unroll
+            for (int j = 0; j < N; j += Values<O>::N) reinterpret_cast<uint4*>(o)[i * (N / Values<O>::N) + j / Values<O>::N] = Values<O>::put(v + j);
+        }
+        g += vectors * N;
+        o += vectors * N;
+        count -= vectors * N;
+    }
+#pragma unroll 8
+    for (int i = threadIdx.x; i < count; i += kClipThreads) o[i] = Values<O>::from_float(Values<T>::to_float(g[i]) * factor);
+}
+
+template <int CAP>
+__global__ void __launch_bounds__(kClipThreads) clip_scale_kernel(const __grid_constant__ ClipTable<CAP> t, const double* __restrict__ partial,
+                                                                  int partials, float max_norm, float inv_scale, float* norm) {
+    __shared__ double shared[kClipThreads / 32];
+    __shared__ float factor_s;
+    double s = 0.0;
+    for (int i = threadIdx.x; i < partials; i += kClipThreads) s += partial[i];
+    s = block_sum(s, shared);
+    if (threadIdx.x == 0) {
+        const float n = (float)(sqrt(s) * (double)inv_scale);
+        const float c = max_norm / (n + 1e-6f);
+        factor_s = (c > 1.0f ? 1.0f : c) * inv_scale;   // NaN stays
+        if (norm && blockIdx.x == 0) *norm = n;
+    }
+    __syncthreads();
+    const float factor = factor_s;
+    for (int i = blockIdx.x; i < t.chunks; i += gridDim.x) {
+        const int c = t.chunks - 1 - i;
+        const ClipEntry& e = t.e[find_tensor(t, c)];
+        const long long begin = (long long)(c - e.chunk0) * t.chunk;
+        const int count = (int)min((long long)t.chunk, e.count - begin);
+        if (factor == 1.0f && e.out == e.grad) continue;
+        if (e.grad_dtype == RB200_FP32) {
+            scale_chunk(reinterpret_cast<const float*>(e.grad) + begin, reinterpret_cast<float*>(e.out) + begin, count, factor);
+        } else if (e.grad_dtype == RB200_FP16) {
+            const __half* g = reinterpret_cast<const __half*>(e.grad) + begin;
+            if (e.out_dtype == RB200_FP32)
+                scale_chunk(g, reinterpret_cast<float*>(e.out) + begin, count, factor);
+            else
+                scale_chunk(g, reinterpret_cast<__half*>(e.out) + begin, count, factor);
+        } else {
+            const __nv_bfloat16* g = reinterpret_cast<const __nv_bfloat16*>(e.grad) + begin;
+            if (e.out_dtype == RB200_FP32)
+                scale_chunk(g, reinterpret_cast<float*>(e.out) + begin, count, factor);
+            else
+                scale_chunk(g, reinterpret_cast<__nv_bfloat16*>(e.out) + begin, count, factor);
+        }
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------
+constexpr int kClipSmall = 16, kClipMedium = 192, kClipLarge = 960;   // 960 entries: 30 KB of launch parameters
+
+template <int CAP>
+static int clip_table_launch(const ClipEntry* entries, int n, int chunks, int chunk, bool scale, double* partial, int partials, float max_norm,
+                             float inv_scale, float* norm, int blocks, cudaStream_t stream) {
+    ClipTable<CAP> t;
+    for (int i = 0; i < n; i++) t.e[i] = entries[i];
+    t.n = n;
+    t.chunks = chunks;
+    t.chunk = chunk;
+    if (scale)
+        clip_scale_kernel<CAP><<<blocks, kClipThreads, 0, stream>>>(t, partial, partials, max_norm, inv_scale, norm);
+    else
+        clip_norm_kernel<CAP><<<blocks, kClipThreads, 0, stream>>>(t, partial);
+    RB200_CHECK_LAUNCH("rb200k_grad_clip");
+    return RB200_OK;
+}
+
+static size_t clip_bytes(int dtype) { return dtype == RB200_FP32 ? 4 : 2; }
+
+// No output meets another output or another tensor's gradients.
+static bool outputs_disjoint(const std::vector<ClipEntry>& v) {
+    struct Range {
+        uintptr_t begin, end;
+        bool out;
+        size_t owner;
+    };
+    std::vector<Range> r;
+    r.reserve(2 * v.size());
+    for (size_t i = 0; i < v.size(); i++) {
+        const uintptr_t g = (uintptr_t)v[i].grad, o = (uintptr_t)v[i].out;
+        r.push_back({o, o + v[i].count * clip_bytes(v[i].out_dtype), true, i});
+        if (g != o) r.push_back({g, g + v[i].count * clip_bytes(v[i].grad_dtype), false, i});
+    }
+    std::sort(r.begin(), r.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+    uintptr_t out_end = 0, any_end = 0;   // of the ranges so far
+    for (const Range& a : r) {
+        if (a.begin < out_end || (a.out && a.begin < any_end)) return false;
+        if (a.out) out_end = std::max(out_end, a.end);
+        any_end = std::max(any_end, a.end);
+    }
+    return true;
+}
+
+static int clip_run(const rb200_grad_tensor* tensors, int n, float max_norm, float inv_scale, float* norm, void* ws, uint64_t ws_bytes,
+                    cudaStream_t stream) {
+    const char* what = "rb200k_grad_clip";
+    if (n < 0 || (n && !tensors) || !norm || ((uintptr_t)norm & 3)) {
+        set_error("%s: null pointer, misaligned norm or negative count", what);
+        return RB200_E_INVALID;
+    }
+    if (!(max_norm >= 0.0f) || !(inv_scale > 0.0f && inv_scale <= 3.4028235e38f)) {
+        set_error("%s: max_norm %g, inv_scale %g", what, max_norm, inv_scale);
+        return RB200_E_INVALID;
+    }
+    std::vector<ClipEntry> v;
+    v.reserve(n);
+    long long total = 0;
+    for (int i = 0; i < n; i++) {
+        const rb200_grad_tensor& t = tensors[i];
+        if (t.count == 0) continue;
+        if (t.count < 0 || t.count > (1ll << 40) || !t.grad || !t.out) {
+            set_error("%s: tensor %d is null or has %lld elements", what, i, (long long)t.count);
+            return RB200_E_INVALID;
+        }
+        if ((t.grad_dtype != RB200_FP32 && t.grad_dtype != RB200_FP16 && t.grad_dtype != RB200_BF16) ||
+            (t.out_dtype != t.grad_dtype && t.out_dtype != RB200_FP32)) {
+            set_error("%s: tensor %d: types %d -> %d", what, i, t.grad_dtype, t.out_dtype);
+            return RB200_E_INVALID;
+        }
+        if ((uintptr_t)t.grad % clip_bytes(t.grad_dtype) || (uintptr_t)t.out % clip_bytes(t.out_dtype)) {
+            set_error("%s: tensor %d is not aligned to its elements", what, i);
+            return RB200_E_INVALID;
+        }
+        v.push_back({t.grad, t.out, t.count, 0, (short)t.grad_dtype, (short)t.out_dtype});
+        total += t.count;
+    }
+    if (total == 0) return check_cuda(cudaMemsetAsync(norm, 0, sizeof(float), stream), what);
+    for (const ClipEntry& e : v)
+        if (e.out == e.grad && e.out_dtype != e.grad_dtype) {
+            set_error("%s: an output in place of gradients of another type", what);
+            return RB200_E_INVALID;
+        }
+    if (!outputs_disjoint(v)) {
+        set_error("%s: an output overlaps another output or another tensor's gradients", what);
+        return RB200_E_INVALID;
+    }
+    const uint64_t need = rb200k_grad_clip_workspace_bytes(n);
+    if (!ws || ws_bytes < need || ((uintptr_t)ws & 15)) {
+        set_error("%s: the workspace has %llu bytes, the call needs %llu, 16-byte aligned", what, (unsigned long long)(ws ? ws_bytes : 0),
+                  (unsigned long long)need);
+        return RB200_E_INVALID;
+    }
+    DeviceInfo dev;
+    int rc = device_info(&dev);
+    if (rc) return rc;
+    const int most = std::min(dev.sms * kClipBlocksPerSm, kClipMaxBlocks);
+    // chunks: enough of them for every block, between 2048 elements (a block's vectors once) and 32768
+    long long chunk = round_up((total + most - 1) / most, 2048);
+    chunk = std::min(chunk, 32768ll);
+    while (total / chunk > (1ll << 30)) chunk *= 2;
+    double* partial = (double*)ws;
+    int partials = 0;
+    for (int pass = 0; pass < 2; pass++) {
+        const size_t tables = (v.size() + kClipLarge - 1) / kClipLarge;
+        for (size_t k = 0; k < tables; k++) {
+            const size_t b = pass ? tables - 1 - k : k;   // the second sweep starts with the last table
+            ClipEntry* first = v.data() + b * kClipLarge;
+            const int count = (int)std::min<size_t>(kClipLarge, v.size() - b * kClipLarge);
+            int chunks = 0;
+            for (int i = 0; i < count; i++) {
+                first[i].chunk0 = chunks;
+                chunks += (int)((first[i].count + chunk - 1) / chunk);
+            }
+            const int blocks = std::min(chunks, most);
+            auto* launch = count <= kClipSmall ? clip_table_launch<kClipSmall>
+                                               : count <= kClipMedium ? clip_table_launch<kClipMedium> : clip_table_launch<kClipLarge>;
+            rc = launch(first, count, chunks, (int)chunk, pass == 1, pass ? partial : partial + partials, partials, max_norm, inv_scale,
+                        k == 0 ? norm : nullptr, blocks, stream);
+            if (rc) return rc;
+            if (pass == 0) partials += blocks;
+        }
+    }
+    return RB200_OK;
+}
+
+}  // namespace rb200
+
+using namespace rb200;
+
+extern "C" uint64_t rb200k_grad_clip_workspace_bytes(int num_tensors) {
+    if (num_tensors <= 0) return 0;
+    return (uint64_t)((num_tensors + kClipLarge - 1) / kClipLarge) * kClipMaxBlocks * sizeof(double);
+}
+extern "C" int rb200k_grad_clip(const rb200_grad_tensor* tensors, int num_tensors, float max_norm, float inv_scale, float* norm, void* workspace,
+                                uint64_t workspace_bytes, void* stream) {
+    try {
+        return clip_run(tensors, num_tensors, max_norm, inv_scale, norm, workspace, workspace_bytes, (cudaStream_t)stream);
+    } catch (const std::bad_alloc&) {
+        set_error("rb200k_grad_clip: out of host memory");
+        return RB200_E_LIMIT;
+    }
+}

@@ -471,3 +471,67 @@ def linear_cross_entropy_backward(dloss, x, weight, labels, stats, info, bias=No
         ws = _workspace(p, lib.rb200k_linear_ce_backward_workspace_bytes, x.device)  # noqa: F841
         check(lib.rb200k_linear_ce_backward(ctypes.byref(p), s), "rb200k_linear_ce_backward")
     return tuple(grads)
+
+
+_GRAD_DTYPE = {torch.float32: T.FP32, torch.float16: T.FP16, torch.bfloat16: T.BF16}
+
+
+def _dense(t):
+    """Whether the elements fill a contiguous stretch of memory, in whatever order of the dimensions."""
+    order = sorted(range(t.dim()), key=lambda d: -t.stride(d))
+    return t.is_contiguous() or t.permute(order).is_contiguous()
+
+
+def grad_clip(grads, max_norm, out=None, inv_scale=1.0, stream=None):
+    """rb200k_grad_clip: the norm (fp32 scalar tensor) of inv_scale * all of `grads`, and each of them times inv_scale * min(1,
+    max_norm / (norm + 1e-6)) - in place, or written to the tensors of `out` (the gradients' types or float32)."""
+    grads = list(grads)
+    targets = grads if out is None else list(out)
+    if not grads:
+        raise ValueError("no gradients")
+    device = grads[0].device
+    if not grads[0].is_cuda:
+        raise ValueError("the gradients are on %s: the head operators run on a GPU" % device)
+    if len(targets) != len(grads):
+        raise ValueError("%d outputs for %d gradients" % (len(targets), len(grads)))
+    copies = []                        # (view with gaps, the dense tensor that stands for it)
+    types = _GRAD_DTYPE
+    for both in ((grads,) if out is None else (grads, targets)):
+        for t in both:
+            if t.dtype not in types or t.device != device or t.layout != torch.strided:
+                raise ValueError("a tensor is %s %s on %s; float32, float16 or bfloat16 on %s are needed" % (t.layout, t.dtype, t.device, device))
+    with _on(device, stream) as s:
+        if out is None:
+            if not all(map(torch.Tensor.is_contiguous, grads)):
+                dense = [t if _dense(t) else t.contiguous() for t in grads]
+                copies = [(t, d) for t, d in zip(grads, dense) if d is not t]
+                grads = targets = dense
+        else:
+            for g, o in zip(grads, targets):
+                if g.shape != o.shape or (o.dtype != g.dtype and o.dtype != torch.float32):
+                    raise ValueError("an output is %s %s for a gradient %s %s" % (tuple(o.shape), o.dtype, tuple(g.shape), g.dtype))
+            if not (all(map(torch.Tensor.is_contiguous, grads)) and all(map(torch.Tensor.is_contiguous, targets))):
+                pairs = []
+                for g, o in zip(grads, targets):
+                    if g.is_contiguous() and o.is_contiguous() or g.stride() == o.stride() and _dense(g):
+                        pairs.append((g, o))
+                        continue
+                    d = o if o.is_contiguous() else torch.empty(o.shape, dtype=o.dtype, device=device)
+                    if d is not o:
+                        copies.append((o, d))
+                    pairs.append((g.contiguous(), d))
+                grads, targets = [g for g, _ in pairs], [o for _, o in pairs]
+        n = len(grads)
+        table = np.empty(n, dtype=T.GRAD_TENSOR)
+        table["grad"] = list(map(torch.Tensor.data_ptr, grads))
+        table["out"] = table["grad"] if targets is grads else list(map(torch.Tensor.data_ptr, targets))
+        table["count"] = list(map(torch.Tensor.numel, grads))
+        table["grad_dtype"] = [types[t.dtype] for t in grads]
+        table["out_dtype"] = table["grad_dtype"] if targets is grads else [types[t.dtype] for t in targets]
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        need = lib.rb200k_grad_clip_workspace_bytes(n)
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        check(lib.rb200k_grad_clip(table.ctypes.data, n, max_norm, inv_scale, norm.data_ptr(), ws.data_ptr(), need, s), "rb200k_grad_clip")
+        for view, dense in copies:
+            view.copy_(dense)
+    return norm

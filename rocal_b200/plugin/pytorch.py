@@ -171,3 +171,23 @@ def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, label_
         from .. import kernels
         loss = kernels.linear_cross_entropy(x2, weight, flat, bias, ignore_index, label_smoothing, reduction)[0]
     return loss.reshape(labels.shape) if reduction == "none" else loss
+
+
+def clip_grad_norm(grads, max_norm, out=None, inv_scale=1.0):
+    """The norm over all tensors of `grads` (times inv_scale, the inverse of a loss scale), and the clipping to it: every
+    tensor is multiplied by inv_scale * min(1, max_norm / (norm + 1e-6)), in place or into the tensors of `out` (of the
+    gradients' types, or float32 copies for a 32-bit optimiser). Float32, float16 and bfloat16 CUDA tensors of any
+    shapes, mixed, on one device. Returns the norm, a float32 scalar on the device; nothing is read back.
+    A gradient with inf gives the norm inf and the factor 0, one with NaN gives NaN, as torch.nn.utils.clip_grad_norm_."""
+    from .. import kernels
+    with torch.no_grad():
+        return kernels.grad_clip(grads, max_norm, out, inv_scale)
+
+
+def clip_grad_norm_(parameters, max_norm, inv_scale=1.0):
+    """clip_grad_norm of the parameters' gradients, in place; parameters without one are passed over."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.zeros((), device=parameters[0].device if parameters else "cuda")
+    return clip_grad_norm(grads, max_norm, inv_scale=inv_scale)

@@ -31,9 +31,10 @@ WARP_SAMPLE = np.dtype([
 
 BOX_WINDOW = np.dtype([("l", "<f4"), ("t", "<f4"), ("r", "<f4"), ("b", "<f4"), ("mirror_h", "<i4"), ("mirror_v", "<i4"),
                        ("reserved", "<i4", (2,))], align=True)
+GRAD_TENSOR = np.dtype([("grad", "<u8"), ("out", "<u8"), ("count", "<i8"), ("grad_dtype", "<i4"), ("out_dtype", "<i4")], align=True)
 BOX_RULE_QUARTER_AREA, BOX_RULE_CENTRE = 0, 1
 
 assert RESAMPLE_SAMPLE.itemsize == 64 and POINTWISE_SAMPLE.itemsize == 64 and WARP_SAMPLE.itemsize == 64
-assert BOX_WINDOW.itemsize == 32
+assert BOX_WINDOW.itemsize == 32 and GRAD_TENSOR.itemsize == 32
 
 NP_DTYPE = {FP32: np.float32, FP16: np.float16, UINT8: np.uint8}
