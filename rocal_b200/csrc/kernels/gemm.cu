@@ -7,18 +7,28 @@ namespace rb200 {
 int device_info(DeviceInfo* out) {
     int dev = 0, rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
     if (rc) return rc;
-    static int sms[64];   // a property of the device; every writer writes the same value
     if (dev < 0 || dev >= 64) {
         set_error("device %d: only devices 0..63 are supported", dev);
         return RB200_E_LIMIT;
     }
-    int v = __atomic_load_n(&sms[dev], __ATOMIC_RELAXED);
+    // properties of the device; every writer writes the same values
+    static int sms[64];
+    static int* words[64];
+    int v = __atomic_load_n(&sms[dev], __ATOMIC_ACQUIRE);
     if (!v) {
         rc = check_cuda(cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
         if (rc) return rc;
-        __atomic_store_n(&sms[dev], v, __ATOMIC_RELAXED);
+        int* word = default_status_word();
+        if (!word) {
+            set_error("the library-wide status word could not be found");
+            return RB200_E_CUDA;
+        }
+        __atomic_store_n(&words[dev], word, __ATOMIC_RELAXED);
+        __atomic_store_n(&sms[dev], v, __ATOMIC_RELEASE);
     }
     out->sms = v;
+    out->index = dev;
+    out->status = __atomic_load_n(&words[dev], __ATOMIC_RELAXED);
     return RB200_OK;
 }
 
@@ -39,72 +49,104 @@ static EncodeTiled encode_tiled() {
     return fn;
 }
 
-int make_map(CUtensorMap* map, const Operand& o, bool bf16, int box_rows, const char* what) {
+int make_map(CUtensorMap* map, const void* data, long long ld, long long rows, long long cols, int bytes, bool bf16, int box_bytes,
+             int box_rows, const char* what) {
     EncodeTiled fn = encode_tiled();
     if (!fn) {
         set_error("%s: the driver has no cuTensorMapEncodeTiled", what);
         return RB200_E_CUDA;
     }
-    const cuuint64_t dims[2] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows};
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
     // the pitch of a single row is never used, but has to be a legal one
-    const cuuint64_t pitch[1] = {(cuuint64_t)(o.rows > 1 ? o.ld : round_up(o.cols, 8)) * 2};
-    const cuuint32_t box[2] = {(cuuint32_t)kTileK, (cuuint32_t)box_rows};
+    const cuuint64_t pitch[1] = {(cuuint64_t)(rows > 1 ? ld : round_up(cols, 16 / bytes)) * bytes};
+    const cuuint32_t box[2] = {(cuuint32_t)(box_bytes / bytes), (cuuint32_t)box_rows};
     const cuuint32_t one[2] = {1, 1};
-    const CUresult rc = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(o.data), dims, pitch,
-                           box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUtensorMapDataType type =
+        bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUresult rc = fn(map, type, 2, const_cast<void*>(data), dims, pitch, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (rc != CUDA_SUCCESS) {
-        set_error("%s: cuTensorMapEncodeTiled refused a %d x %d operand of pitch %lld (%d)", what, o.rows, o.cols, o.ld, (int)rc);
+        set_error("%s: cuTensorMapEncodeTiled refused a %lld x %lld matrix of pitch %lld (%d)", what, rows, cols, ld, (int)rc);
         return RB200_E_CUDA;
     }
     return RB200_OK;
 }
 
+// A model of the kernel's time in clocks, good enough to order the ways of cutting a product:
+//   a k-block of a tile takes the longer of the tensor cores' time (bn clocks: 128 rows per SM and 8192 products a
+//   clock) and the copies' (about 100 bytes of operands per SM and clock);
+//   a tile also keeps the epilogue warps busy (about 10 clocks a column), which counts where it is the longest;
+//   the last tile's epilogue is not hidden, and pieces of the contracted axis have to be joined by another launch.
 GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed, bool may_split) {
-    GemmPlan p;
-    p.cg = 1;
-    p.kblocks = (k + kTileK - 1) / kTileK;
-    p.splits = 1;
-    const int unit = b_transposed ? 64 : 32;
-    double best = 0;
-    p.bn = kTileNMax;
-    for (int bn = kTileNMax; bn >= unit; bn -= unit) {
-        const long long tiles = ((m + kTileM * p.cg - 1) / (kTileM * p.cg)) * (long long)((n + bn - 1) / bn);
-        const long long slots = dev.sms / p.cg, waves = (tiles + slots - 1) / slots;
-        const double cost = (double)waves * (bn + 32);
-        if (best == 0 || cost < best * 0.98) {
-            best = cost;
-            p.bn = bn;
+    GemmPlan best = {};
+    double best_cost = 0;
+    const int kblocks = (k + kTileK - 1) / kTileK;
+    for (int cg = 2; cg >= 1; cg--) {
+        if (cg == 2 && m <= kTileM) continue;
+        const int unit = (b_transposed ? 64 : 32) * cg, slots = dev.sms / cg;
+        const int tiles_m = (m + kTileM * cg - 1) / (kTileM * cg);
+        for (int bn = kTileNMax; bn >= unit; bn -= unit) {
+            const int tiles_n = (n + bn - 1) / bn;
+            if (bn > unit && (n + bn - unit - 1) / (bn - unit) == tiles_n && bn - unit >= n) continue;   // wider than the matrix
+            const long long tiles = (long long)tiles_m * tiles_n;
+            const double copies = (kTileM + bn / cg) * 128 / 100.0, block = copies > bn ? copies : bn, epilogue = 10.0 * bn + 500;
+            // one piece, or as many as the free SMs take in one or two rounds
+            long long choices[3] = {1, 1, 1};
+            if (may_split && kblocks >= 16) {
+                for (int r = 1; r <= 2; r++) {
+                    long long s = r * slots / tiles;
+                    if (s > kblocks / 8) s = kblocks / 8;
+                    choices[r] = s > 1 ? s : 1;
+                }
+            }
+            for (long long s : choices) {
+                const int per = (int)((kblocks + s - 1) / s), splits = (kblocks + per - 1) / per;   // none of them empty
+                const long long waves = (tiles * splits + slots - 1) / slots;
+                const double work = per * block + 300;
+                double cost = waves * (work > epilogue / 2 ? work : epilogue / 2) + epilogue + 1000;
+                if (splits > 1) cost += 6000 + 8.0 * splits * m * n / 2500;   // partial sums: about 2500 bytes a clock
+                if (best_cost == 0 || cost < best_cost * 0.99) {
+                    best_cost = cost;
+                    best = {bn, cg, splits, tiles_m, tiles_n, kblocks, per};
+                }
+            }
         }
     }
-    p.tiles_m = (m + kTileM * p.cg - 1) / (kTileM * p.cg);
-    p.tiles_n = (n + p.bn - 1) / p.bn;
-    const long long tiles = (long long)p.tiles_m * p.tiles_n;
-    if (may_split && tiles * 2 <= dev.sms && p.kblocks >= 16) {
-        long long s = dev.sms / tiles;
-        if (s > p.kblocks / 8) s = p.kblocks / 8;
-        if (s > 1) p.splits = (int)s;
-    }
-    p.kblocks_per_split = (p.kblocks + p.splits - 1) / p.splits;
-    p.splits = (p.kblocks + p.kblocks_per_split - 1) / p.kblocks_per_split;   // none of them empty
-    return p;
+    return best;
 }
 
-int gemm_args(GemmArgs* g, bool bf16, const Operand& a, const Operand& b, const Operand* b_alt, const int* b_select, const GemmPlan& plan,
-              const EpiArgs& e, const GemmWait& wait, const char* what) {
+int gemm_args(GemmArgs* g, const DeviceInfo& dev, bool bf16, const Operand& a, const Operand& b, const Operand* b_alt, const int* b_select,
+              const GemmPlan& plan, const EpiArgs& e, const GemmWait& wait, const char* what) {
     const int m = a.outer(), n = b.outer();
     g->a_box_rows = kTileM;
     if (!a.transposed && m < kTileM) g->a_box_rows = (int)round_up(m, 8);
-    const int bn_cta = plan.bn / plan.cg;
-    int rc = make_map(&g->a, a, bf16, a.transposed ? kTileK : g->a_box_rows, what);
+    const int bn_cta = plan.bn / plan.cg, b_box = b.transposed ? kTileK : bn_cta;
+    int rc = make_map(&g->a, a.data, a.ld, a.rows, a.cols, 2, bf16, 128, a.transposed ? kTileK : g->a_box_rows, what);
     if (rc) return rc;
-    rc = make_map(&g->b, b, bf16, b.transposed ? kTileK : bn_cta, what);
+    rc = make_map(&g->b, b.data, b.ld, b.rows, b.cols, 2, bf16, 128, b_box, what);
     if (rc) return rc;
-    g->b_alt = g->b;
-    g->b_select = b_select;
-    if (b_alt) {
-        rc = make_map(&g->b_alt, *b_alt, bf16, b.transposed ? kTileK : bn_cta, what);
-        if (rc) return rc;
+    g->b_select = b_alt ? b_select : nullptr;
+    if (b_alt && (rc = make_map(&g->b_alt, b_alt->data, b_alt->ld, b_alt->rows, b_alt->cols, 2, bf16, 128, b_box, what))) return rc;
+    g->e = e;
+    // results leave through tensor maps where their rows start on 16-byte boundaries
+    auto mappable = [](const void* p, long long ld, int bytes, long long rows) {
+        return p && ((uintptr_t)p & 15) == 0 && (rows <= 1 || ld * bytes % 16 == 0);
+    };
+    g->e.map_out = g->e.map_pre = 0;
+    if (e.acc_out) {
+        // the rows behind a piece are the next piece's: only whole groups of 32 rows leave that way (gemm_kernel)
+        if (mappable(e.acc_out, e.ldacc, 4, 2) && (long long)plan.splits * m <= INT32_MAX) {
+            g->e.map_out = 1;
+            rc = make_map(&g->out, e.acc_out, e.ldacc, (long long)plan.splits * m, e.ldacc, 4, bf16, 128, 32, what);
+        }
+    } else if (mappable(e.out, e.ldo, 2, m)) {
+        g->e.map_out = 1;
+        rc = make_map(&g->out, e.out, e.ldo, m, n, 2, bf16, 64, 32, what);
+    }
+    if (rc) return rc;
+    if (mappable(e.preact, e.ldp, 2, m)) {
+        g->e.map_pre = 1;
+        if ((rc = make_map(&g->pre, e.preact, e.ldp, m, n, 2, bf16, 64, 32, what))) return rc;
     }
     g->m = m;
     g->n = n;
@@ -116,17 +158,11 @@ int gemm_args(GemmArgs* g, bool bf16, const Operand& a, const Operand& b, const 
     g->kblocks_per_split = plan.kblocks_per_split;
     g->idesc = tc::instr_desc(bf16, a.transposed, b.transposed, kTileM * plan.cg, plan.bn);
     g->stage_bytes = (uint32_t)(kTileM + bn_cta) * kTileK * 2;
-    const uint32_t room = 196608;   // of the 227 KB: the ring
-    g->stages = room / g->stage_bytes;
+    g->stages = kRingBytes / g->stage_bytes;
     if (g->stages > 12) g->stages = 12;
-    g->status = wait.status ? wait.status : default_status_word();
-    if (!g->status) {
-        set_error("%s: the library-wide status word could not be found", what);
-        return RB200_E_CUDA;
-    }
+    g->status = wait.status ? wait.status : dev.status;
     g->wait_cycles = wait.cycles ? wait.cycles : kDefaultWaitCycles;
     g->skip_block = wait.skip_block;
-    g->e = e;
     return RB200_OK;
 }
 
@@ -173,7 +209,13 @@ __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ par
             float z = v[i] * alpha;
             if (e.bias) z += Elem<T>::to_float(reinterpret_cast<const T*>(e.bias)[col + i]);
             if (e.preact) reinterpret_cast<T*>(e.preact)[row * e.ldp + col + i] = Elem<T>::from_float(z);
-            z = act_value(z, e.act);
+            v[i] = z;
+        }
+        act_value4(v, e.act);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (col + i >= n) break;
+            float z = v[i];
             if (e.residual) z += Elem<T>::to_float(reinterpret_cast<const T*>(e.residual)[(long long)(row % e.residual_rows) * e.ldr + col + i]);
             reinterpret_cast<T*>(e.out)[row * e.ldo + col + i] = Elem<T>::from_float(z);
         }

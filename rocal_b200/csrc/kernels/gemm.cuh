@@ -2,10 +2,12 @@
 // tensor cores, and what is done with the accumulators before they leave the chip (EPI_*). One persistent kernel:
 //   warp 0      copies operand tiles (128-byte swizzle) into a ring of shared-memory stages,
 //   warp 1      issues the products of a stage (64 contracted elements) into one of two TMEM accumulators,
-//   warps 4-11  read the other accumulator, 32 columns at a time (thread = row), and run the epilogue, so that the
-//               epilogue of a tile overlaps the products of the next.
+//   warps 4-11  two groups of four; each group reads its own accumulator, 32 columns at a time (thread = row), and
+//               runs the epilogue of every other tile, so that the epilogues of two tiles overlap each other's latency
+//               and the products of the tiles behind them. Results pass through shared memory (32 columns of a warp's
+//               32 rows) and leave as tensor-map stores.
 // CG = 2: two CTAs (a cluster) work on one tile of 256 rows; each holds its 128 rows of A and half of the B tile, so a
-// tile needs half the shared-memory traffic per product.
+// tile of 256 columns takes 128 bytes of operands per SM and clock at the full rate of the tensor cores instead of 192.
 // Either operand may have the contracted axis contiguous (K-major) or the other one (MN-major): the backward products
 // need no transposed copies. Rows and columns beyond the matrices arrive as zeros and are not stored.
 #pragma once
@@ -16,6 +18,8 @@ namespace rb200 {
 
 constexpr int kTileM = 128, kTileK = 64, kTileNMax = 256;
 constexpr int kGemmThreads = 384, kEpiWarps = 8;
+constexpr int kStageBytes = 4096;            // of an epilogue warp: 32 lines of 128 bytes
+constexpr int kRingBytes = 196608;           // of the 227 KB: operand stages
 
 enum { EPI_LINEAR = 0, EPI_STORE = 1, EPI_CE_STATS = 2, EPI_CE_GRAD = 3 };
 enum { ACT_NONE = RB200_ACT_NONE, ACT_RELU = RB200_ACT_RELU, ACT_GELU = RB200_ACT_GELU, ACT_SILU = RB200_ACT_SILU };
@@ -40,7 +44,8 @@ struct EpiArgs {
     void* preact;             // LINEAR: T[m][ldp] or null
     long long ldp;
     int act;
-    int vec_out, vec_res, vec_pre;   // 1: the rows of that array start on 16-byte boundaries
+    int vec_res;              // 1: the residual's rows start on 16-byte boundaries
+    int map_out, map_pre;     // 1: out / preact (acc_out) have tensor maps (GemmArgs)
     // STORE: value = acc + acc_in; to acc_out (fp32) if that is set, else scale * value to out.
     const float* acc_in;
     float* acc_out;
@@ -62,6 +67,7 @@ struct EpiArgs {
 
 struct GemmArgs {
     CUtensorMap a, b, b_alt;   // b_alt replaces b when *b_select is not 0
+    CUtensorMap out, pre;      // of the results, 32 rows x 32 columns (where e.map_out, e.map_pre)
     const int* b_select;
     int m, n;
     int bn;                    // columns of a tile
@@ -101,42 +107,85 @@ struct Elem<__nv_bfloat16> {
     }
 };
 
-__device__ __forceinline__ float act_value(float z, int act) {
-    switch (act) {
-        case ACT_RELU: return z < 0.0f ? 0.0f : z;   // NaN stays
-        case ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678f));
-        case ACT_SILU: return z / (1.0f + __expf(-z));
-        default: return z;
+// Upper tail of the normal distribution over its density shape: R(a) = Q(a) exp(a^2 / 2) for a in [0, 6], a polynomial
+// of degree 12 in a / 3 - 1 fitted for the least relative error (2.3e-6 evaluated in fp32). Beyond 6, where z Q(z) is
+// below 6e-9, R(6) stands in. Two values at a time.
+__device__ __forceinline__ float2 tail_ratio(float2 a) {
+    constexpr float c[13] = {0.121513851f,   -0.103198029f, 0.0824128985f,  -0.0624807179f,   0.0450092852f,  -0.0303888023f, 0.020790372f,
+                             -0.0161429029f, 0.00893525127f, -0.000628449256f, 0.00143634493f, -0.00477083307f, 0.0022911916f};
+    const float2 t = fma2(make_float2(fminf(a.x, 6.0f), fminf(a.y, 6.0f)), make_float2(1.0f / 3.0f, 1.0f / 3.0f), make_float2(-1.0f, -1.0f));
+    float2 r = make_float2(c[12], c[12]);
+#pragma unroll
+    for (int i = 11; i >= 0; i--) r = fma2(r, t, make_float2(c[i], c[i]));
+    return r;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// z Phi(z) = max(z, 0) - |z| Q(|z|): one exponential and no division, accurate in the negative tail as well.
+// |z| is held at 40, where the exponential is 0, so that infinities give 0 and inf; NaN passes through the maximum.
+__device__ __forceinline__ float2 gelu2(float2 z) {
+    const float2 a = make_float2(fminf(fabsf(z.x), 40.0f), fminf(fabsf(z.y), 40.0f));
+    const float2 h = mul2(a, mul2(a, make_float2(-0.72134752f, -0.72134752f)));
+    const float2 e = make_float2(exp2_fast(h.x), exp2_fast(h.y));
+    const float2 q = mul2(mul2(a, e), tail_ratio(a));
+    return make_float2((z.x < 0.0f ? 0.0f : z.x) - q.x, (z.y < 0.0f ? 0.0f : z.y) - q.y);
+}
+// Phi(z) + z phi(z)
+__device__ __forceinline__ float2 gelu_slope2(float2 z) {
+    const float2 a = make_float2(fminf(fabsf(z.x), 40.0f), fminf(fabsf(z.y), 40.0f));
+    const float2 h = mul2(a, mul2(a, make_float2(-0.72134752f, -0.72134752f)));
+    const float2 e = make_float2(exp2_fast(h.x), exp2_fast(h.y));
+    // |z| phi - Q, which the sign of z turns into the distance from 1 or from 0
+    const float2 r = tail_ratio(a);
+    const float2 d = mul2(e, fma2(a, make_float2(0.39894228f, 0.39894228f), make_float2(-r.x, -r.y)));
+    return make_float2(z.x < 0.0f ? -d.x : z.x >= 0.0f ? 1.0f + d.x : z.x, z.y < 0.0f ? -d.y : z.y >= 0.0f ? 1.0f + d.y : z.y);
+}
+__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + exp2_fast(z * -1.4426950408889634f)); }
+
+// Four values at a time, so that the branch on the activation is taken once for them.
+__device__ __forceinline__ void act_value4(float* v, int act) {
+    if (act == ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = v[i] < 0.0f ? 0.0f : v[i];   // NaN stays
+    } else if (act == ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const float2 r = gelu2(make_float2(v[i], v[i + 1]));
+            v[i] = r.x;
+            v[i + 1] = r.y;
+        }
+    } else if (act == ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] *= sigmoid(v[i]);
     }
 }
-__device__ __forceinline__ float act_slope(float z, int act) {
-    switch (act) {
-        case ACT_RELU: return z > 0.0f ? 1.0f : z <= 0.0f ? 0.0f : z;   // NaN stays
-        case ACT_GELU: return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * 0.39894228f * __expf(-0.5f * z * z);
-        case ACT_SILU: {
-            const float g = 1.0f / (1.0f + __expf(-z));
-            return g * (1.0f + z * (1.0f - g));
+__device__ __forceinline__ void act_slope4(float* v, int act) {   // z -> slope
+    if (act == ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = v[i] > 0.0f ? 1.0f : v[i] <= 0.0f ? 0.0f : v[i];   // NaN stays
+    } else if (act == ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const float2 r = gelu_slope2(make_float2(v[i], v[i + 1]));
+            v[i] = r.x;
+            v[i + 1] = r.y;
         }
-        default: return 1.0f;
+    } else if (act == ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float g = sigmoid(v[i]);
+            v[i] = g * fmaf(v[i], 1.0f - g, 1.0f);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = 1.0f;
     }
 }
 
-// Columns [col, col + 32) of one row, `count` of them inside the matrix.
-template <typename T>
-__device__ __forceinline__ void store32(T* row, int col, int count, bool vec, const float (&v)[32]) {
-#pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-        if (vec && i + 8 <= count) {
-            uint4 w = make_uint4(Elem<T>::pack(v[i], v[i + 1]), Elem<T>::pack(v[i + 2], v[i + 3]), Elem<T>::pack(v[i + 4], v[i + 5]),
-                                 Elem<T>::pack(v[i + 6], v[i + 7]));
-            *reinterpret_cast<uint4*>(row + col + i) = w;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (i + j < count) row[col + i + j] = Elem<T>::from_float(v[i + j]);
-        }
-    }
-}
+// Adds columns [col, col + 32) of one row to v, `count` of them inside the matrix.
 template <typename T>
 __device__ __forceinline__ void add32(const T* row, int col, int count, bool vec, float (&v)[32]) {
 #pragma unroll
@@ -156,6 +205,57 @@ __device__ __forceinline__ void add32(const T* row, int col, int count, bool vec
                 if (i + j < count) v[i + j] += Elem<T>::to_float(row[col + i + j]);
         }
     }
+}
+
+// ---- results through shared memory -----------------------------------------------------------------------
+// A warp's 32 rows x 32 columns lie in shared memory line by line in the swizzle of a tensor-map store: threads write their
+// own line without bank conflicts, and the store reads the block as it lies. Element type: lines of 64 bytes, two areas
+// that take turns (16-byte piece j of line r at place j ^ (r / 2 & 3)); fp32: lines of 128 bytes, one area (j ^ (r & 7)).
+__device__ __forceinline__ uint32_t staged16(uint32_t area, int line, int piece) { return area + line * 64 + ((piece ^ (line >> 1 & 3)) << 4); }
+__device__ __forceinline__ uint32_t staged32(uint32_t area, int line, int piece) { return area + line * 128 + ((piece ^ (line & 7)) << 4); }
+__device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void stage32(uint32_t area, int lane, const float (&v)[32]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        st_shared16(staged16(area, lane, i), Elem<T>::pack(v[8 * i], v[8 * i + 1]), Elem<T>::pack(v[8 * i + 2], v[8 * i + 3]),
+                    Elem<T>::pack(v[8 * i + 4], v[8 * i + 5]), Elem<T>::pack(v[8 * i + 6], v[8 * i + 7]));
+}
+template <>
+__device__ __forceinline__ void stage32<float>(uint32_t area, int lane, const float (&v)[32]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        st_shared16(staged32(area, lane, i), __float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                    __float_as_uint(v[4 * i + 3]));
+}
+// All but the last N stores have read their area.
+template <int N>
+__device__ __forceinline__ void stage_wait(int lane) {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+    __syncwarp();
+}
+__device__ __forceinline__ void stage_flush(uint32_t area, const CUtensorMap* map, int col, int row, int lane) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(col), "r"(row), "r"(area)
+                     : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+}
+// The same for rows that no tensor map can describe: a warp writes one row's columns at a time.
+template <typename T>
+__device__ __forceinline__ void stage_copy(uint32_t area, T* out, long long ld, int col, int cols, int row, int rows, int lane) {
+    __syncwarp();
+#pragma unroll 4
+    for (int r = 0; r < rows; r++) {
+        uint16_t w;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(staged16(area, r, lane >> 3) + (lane & 7) * 2) : "memory");
+        if (lane < cols) reinterpret_cast<uint16_t*>(out + (long long)(row + r) * ld + col)[lane] = w;
+    }
+    __syncwarp();
 }
 
 // Running maximum and sum of exp(z - maximum) of one row. A maximum of -inf (every class masked so far) is replaced by
@@ -179,23 +279,13 @@ __device__ __forceinline__ int load_label(const void* labels, int bytes, long lo
     return v >= 0 && v < classes ? (int)v : -1;
 }
 
-template <typename T, int EPI>
-__device__ __forceinline__ void epilogue_bias(const GemmArgs& g, int col, float* strip, int lane) {
-    if (EPI == EPI_STORE) return;
-    float b = 0.0f;
-    if (g.e.bias && col + lane < g.n) b = Elem<T>::to_float(reinterpret_cast<const T*>(g.e.bias)[col + lane]);
-    __syncwarp();
-    strip[lane] = b;
-    __syncwarp();
-}
-
 template <typename T, bool A_MN, bool B_MN, int EPI, int CG>
 __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmArgs g) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[2 * 16 + 2 * 2 + 1];
     __shared__ uint32_t tmem_addr_s;
     __shared__ int gave_up_s;
-    __shared__ float strips[kEpiWarps][32];
+    __shared__ __align__(16) T bias_s[kEpiWarps][2][32];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = CG == 2 ? tc::cta_rank() : 0;
@@ -216,7 +306,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         }
         for (int b = 0; b < 2; b++) {
             tc::bar_init(acc_full(b), 1);
-            tc::bar_init(acc_empty(b), kEpiWarps * CG);
+            tc::bar_init(acc_empty(b), kEpiWarps / 2 * CG);
         }
         tc::bar_init(drained, 1);
         tc::bar_init_fence();
@@ -345,100 +435,129 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         }
         __syncwarp();
     } else if (warp >= 4) {
-        const int ew = warp - 4, quarter = warp & 3, half = ew >> 2;
-        float* strip = strips[ew];
-        int buf = 0;
+        const int ew = warp - 4, quarter = warp & 3, group = ew >> 2;   // group 0: even tiles and accumulator 0
+        const uint32_t area = smem0 + kRingBytes + ew * kStageBytes;
+        const uint32_t acc = tmem + group * kTileNMax + ((uint32_t)(quarter * 32) << 16);
+        const int in_tile = (int)rank * kTileM + quarter * 32;
         uint32_t acc_phase = 0;
-        for (long long t = first; t < tiles; t += step) {
+        int turn = 0;   // which of the staging areas is next
+        float scale = 1.0f;
+        if constexpr (EPI == EPI_STORE) scale = g.e.scale.value();
+        for (long long t = first + group * step; t < tiles; t += 2 * step) {
             int mb, nb, sp;
             place(t, mb, nb, sp);
-            // the lanes leave together: what follows needs whole warps
-            if (!__all_sync(0xFFFFFFFFu, tc::bar_wait(acc_full(buf), acc_phase, patience))) break;
-            tc::fence_after();
-            const int row = mb * (kTileM * CG) + (int)rank * kTileM + quarter * 32 + lane;
+            const int row0 = mb * (kTileM * CG) + in_tile, row = row0 + lane;
             const bool row_ok = row < g.m;
-            const int n0 = nb * g.bn;
-            const uint32_t acc = tmem + buf * kTileNMax + ((uint32_t)(quarter * 32) << 16);
+            const int n0 = nb * g.bn, n1 = min(n0 + g.bn, g.n);
 
+            // what does not depend on the products is fetched before the wait for them
             int label = -1, res_row = 0;
             bool counted = false;
-            float cmax = 0.0f, cscale = 0.0f;
+            float cmax = 0.0f, cscale = 0.0f, inv_sum = 0.0f, zsum = 0.0f;
             RunningSoftmax run = {-INFINITY, 0.0f};
-            float zsum = 0.0f;
             if constexpr (EPI == EPI_CE_STATS || EPI == EPI_CE_GRAD) {
                 if (row_ok) {
                     label = load_label(g.e.labels, g.e.label_bytes, row, g.e.ignore_index, g.e.classes, &counted);
                     label = label < g.e.class0 ? -1 : label - g.e.class0;
                 }
-                if constexpr (EPI == EPI_CE_GRAD) {
-                    if (counted) {
-                        cmax = finite_max(g.e.stats[row]);
-                        cscale = (g.e.coef ? g.e.coef[row] : 1.0f) * 32768.0f;
-                    }
-                }
             }
-            float inv_sum = 0.0f;
             if constexpr (EPI == EPI_CE_GRAD) {
-                if (counted) inv_sum = 1.0f / g.e.stats[g.e.stats_stride + row];
+                if (counted) {
+                    cmax = finite_max(g.e.stats[row]);
+                    inv_sum = 1.0f / g.e.stats[g.e.stats_stride + row];
+                    cscale = (g.e.coef ? g.e.coef[row] : 1.0f) * 32768.0f;
+                }
             }
             if constexpr (EPI == EPI_LINEAR) {
                 if (g.e.residual && row_ok) res_row = row % g.e.residual_rows;
             }
-            float alpha = 1.0f;
-            if constexpr (EPI == EPI_STORE) alpha = g.e.scale.value();
+            // the bias of 32 columns, one lane each, is fetched a strip ahead and passed around in shared memory
+            auto fetch_bias = [&](int c) {
+                return EPI != EPI_STORE && g.e.bias && n0 + c + lane < n1 ? reinterpret_cast<const T*>(g.e.bias)[n0 + c + lane]
+                                                                          : Elem<T>::from_float(0.0f);
+            };
+            T bias_next = fetch_bias(0);
 
-            for (int c = half * 32; c < g.bn; c += 64) {
-                const int col = n0 + c, count = g.n - col;   // columns of this strip inside the matrix (may be <= 0)
-                uint32_t raw[32];
-                tc::tmem_load32(acc + c, raw);
-                epilogue_bias<T, EPI>(g, col, strip, lane);
-                tc::tmem_wait();
-                if (count <= 0) continue;
+            // the lanes leave together: what follows needs whole warps
+            if (!__all_sync(0xFFFFFFFFu, tc::bar_wait(acc_full(group), acc_phase, patience))) break;
+            acc_phase ^= 1;
+            tc::fence_after();
+
+            auto body = [&](const uint32_t (&raw)[32], int c) {
+                const int col = n0 + c, count = n1 - col;   // columns of this strip inside the matrix (may be <= 0)
+                T* bias = bias_s[ew][c >> 5 & 1];
+                if constexpr (EPI != EPI_STORE) {
+                    bias[lane] = bias_next;
+                    bias_next = fetch_bias(c + 32);
+                    __syncwarp();
+                }
+                if (count <= 0) return;
                 float v[32];
 #pragma unroll
                 for (int i = 0; i < 32; i++) v[i] = __uint_as_float(raw[i]);
                 if constexpr (EPI != EPI_STORE) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 b = *reinterpret_cast<const float4*>(strip + i);
-                        v[i] += b.x;
-                        v[i + 1] += b.y;
-                        v[i + 2] += b.z;
-                        v[i + 3] += b.w;
+                    for (int i = 0; i < 32; i += 8) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(bias + i);
+                        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const float2 s = add2(make_float2(v[i + 2 * j], v[i + 2 * j + 1]), Elem<T>::unpack(u[j]));
+                            v[i + 2 * j] = s.x;
+                            v[i + 2 * j + 1] = s.y;
+                        }
                     }
                 }
+                auto leave = [&](const CUtensorMap* map, bool mapped, void* out, long long ld) {
+                    if (row0 >= g.m) return;
+                    const uint32_t half = area + turn * (kStageBytes / 2);
+                    turn ^= 1;
+                    stage_wait<1>(lane);
+                    stage32<T>(half, lane, v);
+                    if (mapped)
+                        stage_flush(half, map, col, row0, lane);
+                    else
+                        stage_copy(half, reinterpret_cast<T*>(out), ld, col, min(32, count), row0, min(32, g.m - row0), lane);
+                };
                 if constexpr (EPI == EPI_LINEAR) {
-                    if (row_ok) {
-                        if (g.e.preact)
-                            store32(reinterpret_cast<T*>(g.e.preact) + (long long)row * g.e.ldp, col, count, g.e.vec_pre, v);
-                        if (g.e.act != ACT_NONE) {
+                    if (g.e.preact) leave(&g.pre, g.e.map_pre, g.e.preact, g.e.ldp);
+                    if (g.e.act != ACT_NONE) {
 #pragma unroll
-                            for (int i = 0; i < 32; i++) v[i] = act_value(v[i], g.e.act);
-                        }
-                        if (g.e.residual)
-                            add32(reinterpret_cast<const T*>(g.e.residual) + (long long)res_row * g.e.ldr, col, count, g.e.vec_res, v);
-                        store32(reinterpret_cast<T*>(g.e.out) + (long long)row * g.e.ldo, col, count, g.e.vec_out, v);
+                        for (int i = 0; i < 32; i += 4) act_value4(v + i, g.e.act);
                     }
+                    if (g.e.residual && row_ok)
+                        add32(reinterpret_cast<const T*>(g.e.residual) + (long long)res_row * g.e.ldr, col, count, g.e.vec_res, v);
+                    leave(&g.out, g.e.map_out, g.e.out, g.e.ldo);
                 }
                 if constexpr (EPI == EPI_STORE) {
-                    if (row_ok) {
-                        const long long at = (long long)row * g.e.ldacc + col;
-                        if (g.e.acc_in) {
+                    if (g.e.acc_in && row_ok) {
+                        const float* p = g.e.acc_in + (long long)row * g.e.ldacc + col;   // ldacc is a multiple of 4
 #pragma unroll
-                            for (int i = 0; i < 32; i++)
-                                if (i < count) v[i] += g.e.acc_in[at + i];
-                        }
-                        if (g.e.acc_out) {
-                            float* o = g.e.acc_out + (long long)sp * g.e.acc_split_stride + at;
-#pragma unroll
-                            for (int i = 0; i < 32; i += 4) {   // ldacc is a multiple of 4: the row's padding takes the rest
-                                if (i < count) *reinterpret_cast<float4*>(o + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                        for (int i = 0; i < 32; i += 4) {
+                            if (i < count) {
+                                const float4 f = *reinterpret_cast<const float4*>(p + i);
+                                v[i] += f.x;
+                                v[i + 1] += f.y;
+                                v[i + 2] += f.z;
+                                v[i + 3] += f.w;
                             }
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 32; i++) v[i] *= alpha;
-                            store32(reinterpret_cast<T*>(g.e.out) + (long long)row * g.e.ldo, col, count, g.e.vec_out, v);
                         }
+                    }
+                    if (g.e.acc_out) {   // pieces of a split product lie behind one another as rows of one matrix
+                        if (g.e.map_out && row0 + 32 <= g.m) {
+                            stage_wait<0>(lane);
+                            stage32<float>(area, lane, v);
+                            stage_flush(area, &g.out, col, sp * g.m + row0, lane);
+                        } else if (row_ok) {
+                            float* o = g.e.acc_out + (long long)sp * g.e.acc_split_stride + (long long)row * g.e.ldacc + col;
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4)   // a row's padding takes the rest
+                                if (i < count) *reinterpret_cast<float4*>(o + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; i++) v[i] *= scale;
+                        leave(&g.out, g.e.map_out, g.e.out, g.e.ldo);
                     }
                 }
                 if constexpr (EPI == EPI_CE_STATS) {
@@ -447,51 +566,76 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                         for (int i = 0; i < 32; i++)
                             if (label == col + i) g.e.zlabel[row] = v[i];
                     }
-                    float top = run.m;
-#pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        if (i >= count) v[i] = -INFINITY;
-                        top = fmaxf(top, v[i]);
-                    }
                     if (g.e.want_zsum) {
 #pragma unroll
                         for (int i = 0; i < 32; i++)
                             if (i < count) zsum += v[i];
                     }
+                    if (count < 32) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++)
+                            if (i >= count) v[i] = -INFINITY;
+                    }
+                    float top = run.m;
+#pragma unroll
+                    for (int i = 0; i < 32; i++) top = fmaxf(top, v[i]);
                     const float base = finite_max(top);
                     run.s *= exp_diff(run.m - base);
                     run.m = top;
-                    float sum = 0.0f;
+                    float2 sum = make_float2(0.0f, 0.0f);
+                    const float2 off = make_float2(-base, -base), unit = make_float2(kLog2e, kLog2e);
 #pragma unroll
-                    for (int i = 0; i < 32; i++) sum += exp_diff(v[i] - base);
-                    run.s += sum;
+                    for (int i = 0; i < 32; i += 2) {
+                        const float2 d = mul2(add2(make_float2(v[i], v[i + 1]), off), unit);
+                        sum = add2(sum, make_float2(exp2_fast(d.x), exp2_fast(d.y)));
+                    }
+                    run.s += sum.x + sum.y;
                 }
                 if constexpr (EPI == EPI_CE_GRAD) {
-                    if (row_ok) {
+                    const float2 off = make_float2(-cmax, -cmax), unit = make_float2(kLog2e, kLog2e);
+                    const float2 inv = make_float2(inv_sum, inv_sum), smooth = make_float2(-g.e.smooth_off, -g.e.smooth_off);
 #pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            float p = exp_diff(v[i] - cmax) * inv_sum - g.e.smooth_off;
-                            if (label == col + i) p -= g.e.smooth_on;
-                            v[i] = counted ? p * cscale : 0.0f;
-                        }
-                        store32(reinterpret_cast<T*>(g.e.out) + (long long)row * g.e.ldo, col, count, g.e.vec_out, v);
+                    for (int i = 0; i < 32; i += 2) {
+                        const float2 d = mul2(add2(make_float2(v[i], v[i + 1]), off), unit);
+                        const float2 p = fma2(make_float2(exp2_fast(d.x), exp2_fast(d.y)), inv, smooth);
+                        v[i] = p.x;
+                        v[i + 1] = p.y;
                     }
+                    if (label >= col && label < col + 32) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++)
+                            if (label == col + i) v[i] -= g.e.smooth_on;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[i] = counted ? v[i] * cscale : 0.0f;
+                    leave(&g.out, true, nullptr, 0);
+                }
+            };
+            uint32_t even[32], odd[32];   // the strip at work and the one on its way
+            tc::tmem_load32(acc, even);
+            for (int c = 0; c < g.bn; c += 64) {
+                tc::tmem_wait();
+                if (c + 32 < g.bn) tc::tmem_load32(acc + c + 32, odd);
+                body(even, c);
+                if (c + 32 < g.bn) {
+                    tc::tmem_wait();
+                    if (c + 64 < g.bn) tc::tmem_load32(acc + c + 64, even);
+                    body(odd, c + 32);
                 }
             }
             tc::fence_before();
             __syncwarp();
-            if (lane == 0) tc::bar_arrive_cluster(CG == 2 ? tc::map_to_rank(acc_empty(buf), 0) : acc_empty(buf));
+            if (lane == 0) tc::bar_arrive_cluster(CG == 2 ? tc::map_to_rank(acc_empty(group), 0) : acc_empty(group));
             if constexpr (EPI == EPI_CE_STATS) {
                 if (row_ok) {
-                    const long long plane = (long long)g.e.parts * g.m, at = (long long)(2 * nb + half) * g.m + row;
+                    const long long plane = (long long)g.e.parts * g.m, at = (long long)nb * g.m + row;
                     g.e.part[at] = run.m;
                     g.e.part[plane + at] = run.s;
                     if (g.e.want_zsum) g.e.part[2 * plane + at] = zsum;
                 }
             }
-            buf ^= 1;
-            acc_phase ^= buf == 0;
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the results are out before the CTA ends
         __syncwarp();
     }
     tc::fence_before();
@@ -516,10 +660,13 @@ struct Operand {
 };
 
 struct DeviceInfo {
-    int sms;
+    int sms, index;
+    int* status;              // the library-wide status word
 };
 int device_info(DeviceInfo* out);   // of the current device; 0 or an error code
-int make_map(CUtensorMap* map, const Operand& o, bool bf16, int box_rows, const char* what);
+// A map of boxes box_bytes wide (128 or 64, the swizzle's width too); bytes: of an element, 2 or 4 (fp32).
+int make_map(CUtensorMap* map, const void* data, long long ld, long long rows, long long cols, int bytes, bool bf16, int box_bytes, int box_rows,
+             const char* what);
 // Rows on 16-byte boundaries, as a tensor-map copy needs them.
 static inline bool map_ready(const Operand& o) {
     return ((uintptr_t)o.data & 15) == 0 && (o.rows <= 1 || (o.ld & 7) == 0);
@@ -534,9 +681,14 @@ GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed
 template <typename T, bool A_MN, bool B_MN, int EPI, int CG>
 int gemm_launch_as(const GemmArgs& g, const DeviceInfo& dev, cudaStream_t stream, const char* what) {
     auto* kernel = gemm_kernel<T, A_MN, B_MN, EPI, CG>;
-    const size_t smem = (size_t)g.stages * g.stage_bytes + 1024;
-    int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), what);
-    if (rc) return rc;
+    constexpr size_t smem = kRingBytes + kEpiWarps * kStageBytes + 1024;
+    static unsigned long long ready;   // a bit for each device whose kernel has its shared-memory limit
+    int rc;
+    if (!(__atomic_load_n(&ready, __ATOMIC_RELAXED) >> dev.index & 1)) {
+        rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), what);
+        if (rc) return rc;
+        __atomic_fetch_or(&ready, 1ull << dev.index, __ATOMIC_RELAXED);
+    }
     const long long tiles = (long long)g.tiles_m * g.tiles_n * g.splits, slots = dev.sms / CG;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((tiles < slots ? tiles : slots) * CG));
@@ -564,7 +716,7 @@ struct GemmWait {
 };
 
 // Fills the launch block. Both operands are map_ready.
-int gemm_args(GemmArgs* g, bool bf16, const Operand& a, const Operand& b, const Operand* b_alt, const int* b_select, const GemmPlan& plan,
+int gemm_args(GemmArgs* g, const DeviceInfo& dev, bool bf16, const Operand& a, const Operand& b, const Operand* b_alt, const int* b_select, const GemmPlan& plan,
               const EpiArgs& e, const GemmWait& wait, const char* what);
 
 template <int EPI, bool A_MN, bool B_MN>
@@ -574,7 +726,7 @@ int gemm_launch(bool bf16, const Operand& a, const Operand& b, const Operand* b_
     DeviceInfo dev;
     int rc = device_info(&dev);
     if (rc) return rc;
-    rc = gemm_args(&g, bf16, a, b, b_alt, b_select, plan, e, wait, what);
+    rc = gemm_args(&g, dev, bf16, a, b, b_alt, b_select, plan, e, wait, what);
     if (rc) return rc;
     if (plan.cg == 2)
         return bf16 ? gemm_launch_as<__nv_bfloat16, A_MN, B_MN, EPI, 2>(g, dev, stream, what)

@@ -60,8 +60,10 @@ __global__ void __launch_bounds__(256) rows_kernel(RowsArgs a) {
                 if (a.preact) {
                     float z[8];
                     load8(reinterpret_cast<const T*>(a.preact) + row * a.ldp + col, count, a.vec_pre, z);
+                    act_slope4(z, a.act);
+                    act_slope4(z + 4, a.act);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) v[i] *= act_slope(z[i], a.act);
+                    for (int i = 0; i < 8; i++) v[i] *= z[i];
                 }
                 if (a.dst) {   // the destination's rows are padded to whole vectors
                     *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.dst) + row * a.ldd + col) =
@@ -230,9 +232,7 @@ static int linear_run(const rb200_linear_params* p, void* stream_v, GemmWait wai
     e.preact = p->preact;
     e.ldp = p->ldp;
     e.act = p->activation;
-    e.vec_out = map_ready(operand(p->out, p->ldo, p->rows, p->out_features, false));
     e.vec_res = map_ready(operand(p->residual, p->ldr, p->residual_rows, p->out_features, false));
-    e.vec_pre = map_ready(operand(p->preact, p->ldp, p->rows, p->out_features, false));
     wait.status = p->status;
     if (l.gemm.splits > 1) {
         EpiArgs part = {};
@@ -364,15 +364,13 @@ static int backward_run(const rb200_linear_backward_params* p, void* stream_v) {
         if ((rc = do_pack(l.w, stream, what))) return rc;
         e.out = p->dx;
         e.ldo = p->lddx;
-        e.vec_out = map_ready(operand(p->dx, p->lddx, n, k, false));
-        if ((rc = gemm_store_joined(GEMM_KN, bf16, l.dz, l.w.use, nullptr, nullptr, l.gx, e, l.px, wait, stream, what))) return rc;
+            if ((rc = gemm_store_joined(GEMM_KN, bf16, l.dz, l.w.use, nullptr, nullptr, l.gx, e, l.px, wait, stream, what))) return rc;
     }
     if (p->dweight) {
         if ((rc = do_pack(l.x, stream, what))) return rc;
         e.out = p->dweight;
         e.ldo = p->lddw;
-        e.vec_out = map_ready(operand(p->dweight, p->lddw, m, k, false));
-        Operand dzt = l.dz;
+            Operand dzt = l.dz;
         dzt.transposed = true;
         if ((rc = gemm_store_joined(GEMM_NN, bf16, dzt, l.x.use, nullptr, nullptr, l.gw, e, l.pw, wait, stream, what))) return rc;
     }

@@ -1,5 +1,5 @@
 // rb200k_linear_ce: softmax cross entropy of x W^T + b, forward and backward, without the rows x classes matrix.
-//   forward   one product whose epilogue keeps, for every row and half tile of classes, the largest score and the sum
+//   forward   one product whose epilogue keeps, for every row and tile of classes, the largest score and the sum
 //             of exp(score - largest); ce_merge_kernel joins them (and makes the loss). The scores stay on the chip.
 //   backward  piece by piece: the product again, its epilogue turning scores into (softmax - target) in the element type, then
 //             that piece times W and transposed times x. Pieces are cut along the longer of classes and rows; the
@@ -242,15 +242,14 @@ static StatsPlan plan_stats(const rb200_linear_ce_params& p, const DeviceInfo& d
     Carver c(ws);
     s.x = plan_pack(operand(p.x, p.ldx, p.rows, p.features, false), &c);
     s.w = plan_pack(operand(p.weight, p.ldw, p.classes, p.features, false), &c);
-    // a half tile of 16 columns is the smallest that a plan makes; a piece keeps whole tiles of every width
+    // a tile has 32 columns at least
     const size_t per_part = (size_t)p.rows * 3 * sizeof(float);
     long long parts = (long long)(kStatBytes / per_part);
-    if (parts < 2) parts = 2;
-    long long piece = parts / 2 * 32 / kTileNMax * kTileNMax;
+    long long piece = parts * 32 / kTileNMax * kTileNMax;
     if (piece < kTileNMax) piece = kTileNMax;
     s.piece = (int)(piece < p.classes ? piece : p.classes);
-    const long long most = 2ll * stats_gemm(p, dev, s.piece).tiles_n;
-    const long long rest = p.classes % s.piece ? 2ll * stats_gemm(p, dev, (int)(p.classes % s.piece)).tiles_n : 0;
+    const long long most = stats_gemm(p, dev, s.piece).tiles_n;
+    const long long rest = p.classes % s.piece ? stats_gemm(p, dev, (int)(p.classes % s.piece)).tiles_n : 0;
     s.part_bytes = (size_t)(most > rest ? most : rest) * per_part;
     s.part = (float*)c.take(s.part_bytes);
     s.zlabel = (float*)c.take((size_t)p.rows * sizeof(float));
@@ -292,7 +291,7 @@ static int ce_forward(const rb200_linear_ce_params* p, cudaStream_t stream) {
         e.bias = p->bias ? at_row(p->bias, 1, c0) : nullptr;
         e.class0 = (int)c0;
         e.part = s.part;
-        e.parts = 2 * plan.tiles_n;
+        e.parts = plan.tiles_n;
         e.want_zsum = p->label_smoothing > 0.0f;
         e.zlabel = s.zlabel;
         e.clear = p->info;
@@ -456,7 +455,6 @@ static int ce_backward(const rb200_linear_ce_params* p, cudaStream_t stream) {
         e.coef = none ? g.coef + r0 : nullptr;
         e.out = g.dz;
         e.ldo = g.ldd;
-        e.vec_out = 1;
         const GemmPlan plan = gemm_plan(dev, rows, classes, (int)k, false, false);
         if ((rc = gemm_launch<EPI_CE_GRAD, false, false>(bf16, x, w, nullptr, nullptr, plan, e, wait, stream, what))) return rc;
         const bool first = i == 0, last = i == g.pieces - 1;
@@ -474,7 +472,6 @@ static int ce_backward(const rb200_linear_ce_params* p, cudaStream_t stream) {
                 o.out = p->dx;
                 o.ldo = p->lddx;
             }
-            o.vec_out = map_ready(operand(o.out, o.ldo, rows, k, false));
             o.scale = scale;
             if ((rc = gemm_store_joined(GEMM_KN, bf16, dz, wt, nullptr, nullptr, gemm_plan(dev, rows, (int)k, classes, true, true), o, g.px, wait,
                                         stream, what)))
@@ -496,7 +493,6 @@ static int ce_backward(const rb200_linear_ce_params* p, cudaStream_t stream) {
                 o.out = p->dweight;
                 o.ldo = p->lddw;
             }
-            o.vec_out = map_ready(operand(o.out, o.ldo, classes, k, false));
             o.scale = scale;
             if ((rc = gemm_store_joined(GEMM_NN, bf16, dzt, xt, &clean, p->info + 1, gemm_plan(dev, classes, (int)k, rows, true, true), o, g.pw,
                                         wait, stream, what)))
