@@ -49,24 +49,22 @@ static EncodeTiled encode_tiled() {
     return fn;
 }
 
-int make_map(CUtensorMap* map, const void* data, long long ld, long long rows, long long cols, int bytes, bool bf16, int box_bytes,
-             int box_rows, const char* what) {
+int make_map(CUtensorMap* map, const Operand& o, bool bf16, int box_rows, const char* what) {
     EncodeTiled fn = encode_tiled();
     if (!fn) {
         set_error("%s: the driver has no cuTensorMapEncodeTiled", what);
         return RB200_E_CUDA;
     }
-    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t dims[2] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows};
     // the pitch of a single row is never used, but has to be a legal one
-    const cuuint64_t pitch[1] = {(cuuint64_t)(rows > 1 ? ld : round_up(cols, 16 / bytes)) * bytes};
-    const cuuint32_t box[2] = {(cuuint32_t)(box_bytes / bytes), (cuuint32_t)box_rows};
+    const cuuint64_t pitch[1] = {(cuuint64_t)(o.rows > 1 ? o.ld : round_up(o.cols, 8)) * 2};
+    const cuuint32_t box[2] = {(cuuint32_t)kTileK, (cuuint32_t)box_rows};
     const cuuint32_t one[2] = {1, 1};
-    const CUtensorMapDataType type =
-        bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    const CUresult rc = fn(map, type, 2, const_cast<void*>(data), dims, pitch, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult rc = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(o.data), dims, pitch,
+                           box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (rc != CUDA_SUCCESS) {
-        set_error("%s: cuTensorMapEncodeTiled refused a %lld x %lld matrix of pitch %lld (%d)", what, rows, cols, ld, (int)rc);
+        set_error("%s: cuTensorMapEncodeTiled refused a %d x %d operand of pitch %lld (%d)", what, o.rows, o.cols, o.ld, (int)rc);
         return RB200_E_CUDA;
     }
     return RB200_OK;
@@ -121,33 +119,17 @@ int gemm_args(GemmArgs* g, const DeviceInfo& dev, bool bf16, const Operand& a, c
     g->a_box_rows = kTileM;
     if (!a.transposed && m < kTileM) g->a_box_rows = (int)round_up(m, 8);
     const int bn_cta = plan.bn / plan.cg, b_box = b.transposed ? kTileK : bn_cta;
-    int rc = make_map(&g->a, a.data, a.ld, a.rows, a.cols, 2, bf16, 128, a.transposed ? kTileK : g->a_box_rows, what);
+    int rc = make_map(&g->a, a, bf16, a.transposed ? kTileK : g->a_box_rows, what);
     if (rc) return rc;
-    rc = make_map(&g->b, b.data, b.ld, b.rows, b.cols, 2, bf16, 128, b_box, what);
+    rc = make_map(&g->b, b, bf16, b_box, what);
     if (rc) return rc;
     g->b_select = b_alt ? b_select : nullptr;
-    if (b_alt && (rc = make_map(&g->b_alt, b_alt->data, b_alt->ld, b_alt->rows, b_alt->cols, 2, bf16, 128, b_box, what))) return rc;
+    if (b_alt && (rc = make_map(&g->b_alt, *b_alt, bf16, b_box, what))) return rc;
     g->e = e;
-    // results leave through tensor maps where their rows start on 16-byte boundaries
-    auto mappable = [](const void* p, long long ld, int bytes, long long rows) {
-        return p && ((uintptr_t)p & 15) == 0 && (rows <= 1 || ld * bytes % 16 == 0);
-    };
-    g->e.map_out = g->e.map_pre = 0;
-    if (e.acc_out) {
-        // the rows behind a piece are the next piece's: only whole groups of 32 rows leave that way (gemm_kernel)
-        if (mappable(e.acc_out, e.ldacc, 4, 2) && (long long)plan.splits * m <= INT32_MAX) {
-            g->e.map_out = 1;
-            rc = make_map(&g->out, e.acc_out, e.ldacc, (long long)plan.splits * m, e.ldacc, 4, bf16, 128, 32, what);
-        }
-    } else if (mappable(e.out, e.ldo, 2, m)) {
-        g->e.map_out = 1;
-        rc = make_map(&g->out, e.out, e.ldo, m, n, 2, bf16, 64, 32, what);
-    }
-    if (rc) return rc;
-    if (mappable(e.preact, e.ldp, 2, m)) {
-        g->e.map_pre = 1;
-        if ((rc = make_map(&g->pre, e.preact, e.ldp, m, n, 2, bf16, 64, 32, what))) return rc;
-    }
+    auto vec = [](const void* p, long long ld, int rows) { return ((uintptr_t)p & 15) == 0 && (rows <= 1 || (ld & 7) == 0); };
+    g->e.vec_out = vec(e.out, e.ldo, m);
+    g->e.vec_pre = vec(e.preact, e.ldp, m);
+    g->e.vec_res = vec(e.residual, e.ldr, e.residual_rows);
     g->m = m;
     g->n = n;
     g->bn = plan.bn;
@@ -211,7 +193,7 @@ __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ par
             if (e.preact) reinterpret_cast<T*>(e.preact)[row * e.ldp + col + i] = Elem<T>::from_float(z);
             v[i] = z;
         }
-        act_value4(v, e.act);
+        act_values<4>(v, e.act);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             if (col + i >= n) break;

@@ -4,8 +4,8 @@
 //   warp 1      issues the products of a stage (64 contracted elements) into one of two TMEM accumulators,
 //   warps 4-11  two groups of four; each group reads its own accumulator, 32 columns at a time (thread = row), and
 //               runs the epilogue of every other tile, so that the epilogues of two tiles overlap each other's latency
-//               and the products of the tiles behind them. Results pass through shared memory (32 columns of a warp's
-//               32 rows) and leave as tensor-map stores.
+//               and the products of the tiles behind them. Results cross over in shared memory from
+//               threads that hold rows to lanes that write whole pieces of rows.
 // CG = 2: two CTAs (a cluster) work on one tile of 256 rows; each holds its 128 rows of A and half of the B tile, so a
 // tile of 256 columns takes 128 bytes of operands per SM and clock at the full rate of the tensor cores instead of 192.
 // Either operand may have the contracted axis contiguous (K-major) or the other one (MN-major): the backward products
@@ -44,8 +44,7 @@ struct EpiArgs {
     void* preact;             // LINEAR: T[m][ldp] or null
     long long ldp;
     int act;
-    int vec_res;              // 1: the residual's rows start on 16-byte boundaries
-    int map_out, map_pre;     // 1: out / preact (acc_out) have tensor maps (GemmArgs)
+    int vec_out, vec_res, vec_pre;   // 1: the rows of that array start on 16-byte boundaries
     // STORE: value = acc + acc_in; to acc_out (fp32) if that is set, else scale * value to out.
     const float* acc_in;
     float* acc_out;
@@ -67,7 +66,6 @@ struct EpiArgs {
 
 struct GemmArgs {
     CUtensorMap a, b, b_alt;   // b_alt replaces b when *b_select is not 0
-    CUtensorMap out, pre;      // of the results, 32 rows x 32 columns (where e.map_out, e.map_pre)
     const int* b_select;
     int m, n;
     int bn;                    // columns of a tile
@@ -145,117 +143,118 @@ __device__ __forceinline__ float2 gelu_slope2(float2 z) {
 }
 __device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + exp2_fast(z * -1.4426950408889634f)); }
 
-// Four values at a time, so that the branch on the activation is taken once for them.
-__device__ __forceinline__ void act_value4(float* v, int act) {
+// N values at a time: one branch on the activation, and N independent chains of operations behind it.
+template <int N>
+__device__ __forceinline__ void act_values(float* v, int act) {
     if (act == ACT_RELU) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = v[i] < 0.0f ? 0.0f : v[i];   // NaN stays
+        for (int i = 0; i < N; i++) v[i] = v[i] < 0.0f ? 0.0f : v[i];   // NaN stays
     } else if (act == ACT_GELU) {
 #pragma unroll
-        for (int i = 0; i < 4; i += 2) {
+        for (int i = 0; i < N; i += 2) {
             const float2 r = gelu2(make_float2(v[i], v[i + 1]));
             v[i] = r.x;
             v[i + 1] = r.y;
         }
     } else if (act == ACT_SILU) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] *= sigmoid(v[i]);
+        for (int i = 0; i < N; i++) v[i] *= sigmoid(v[i]);
     }
 }
-__device__ __forceinline__ void act_slope4(float* v, int act) {   // z -> slope
+template <int N>
+__device__ __forceinline__ void act_slopes(float* v, int act) {   // z -> slope
     if (act == ACT_RELU) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = v[i] > 0.0f ? 1.0f : v[i] <= 0.0f ? 0.0f : v[i];   // NaN stays
+        for (int i = 0; i < N; i++) v[i] = v[i] > 0.0f ? 1.0f : v[i] <= 0.0f ? 0.0f : v[i];   // NaN stays
     } else if (act == ACT_GELU) {
 #pragma unroll
-        for (int i = 0; i < 4; i += 2) {
+        for (int i = 0; i < N; i += 2) {
             const float2 r = gelu_slope2(make_float2(v[i], v[i + 1]));
             v[i] = r.x;
             v[i + 1] = r.y;
         }
     } else if (act == ACT_SILU) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < N; i++) {
             const float g = sigmoid(v[i]);
             v[i] = g * fmaf(v[i], 1.0f - g, 1.0f);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = 1.0f;
-    }
-}
-
-// Adds columns [col, col + 32) of one row to v, `count` of them inside the matrix.
-template <typename T>
-__device__ __forceinline__ void add32(const T* row, int col, int count, bool vec, float (&v)[32]) {
-#pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-        if (vec && i + 8 <= count) {
-            const uint4 w = __ldg(reinterpret_cast<const uint4*>(row + col + i));
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float2 f = Elem<T>::unpack(u[j]);
-                v[i + 2 * j] += f.x;
-                v[i + 2 * j + 1] += f.y;
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (i + j < count) v[i + j] += Elem<T>::to_float(row[col + i + j]);
-        }
+        for (int i = 0; i < N; i++) v[i] = 1.0f;
     }
 }
 
 // ---- results through shared memory -----------------------------------------------------------------------
-// A warp's 32 rows x 32 columns lie in shared memory line by line in the swizzle of a tensor-map store: threads write their
-// own line without bank conflicts, and the store reads the block as it lies. Element type: lines of 64 bytes, two areas
-// that take turns (16-byte piece j of line r at place j ^ (r / 2 & 3)); fp32: lines of 128 bytes, one area (j ^ (r & 7)).
+// Threads hold rows; memory wants whole pieces of rows. A warp's 32 rows x 32 columns cross over in its staging area: each
+// thread writes its own line, then 16-byte pieces are read back so that neighbouring lanes hold neighbouring pieces of a row.
+// Pieces are permuted within a line so that neither side has bank conflicts. Element type: lines of 64 bytes (piece j of
+// line r at place j ^ (r / 2 & 3)), a row takes 4 lanes; fp32: lines of 128 bytes (j ^ (r & 7)), a row takes 8 lanes.
 __device__ __forceinline__ uint32_t staged16(uint32_t area, int line, int piece) { return area + line * 64 + ((piece ^ (line >> 1 & 3)) << 4); }
 __device__ __forceinline__ uint32_t staged32(uint32_t area, int line, int piece) { return area + line * 128 + ((piece ^ (line & 7)) << 4); }
-__device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+__device__ __forceinline__ void st_shared16(uint32_t addr, const uint4& w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
 }
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
+    uint4 w;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(addr) : "memory");
+    return w;
+}
+// Writes the strip v (a row a thread) to rows [row0, row0 + rows) and columns [col, col + cols) of out.
 template <typename T>
-__device__ __forceinline__ void stage32(uint32_t area, int lane, const float (&v)[32]) {
+__device__ __forceinline__ void leave16(uint32_t area, const float (&v)[32], T* out, long long ld, bool vec, int col, int cols, int row0, int rows,
+                                        int lane) {
 #pragma unroll
     for (int i = 0; i < 4; i++)
-        st_shared16(staged16(area, lane, i), Elem<T>::pack(v[8 * i], v[8 * i + 1]), Elem<T>::pack(v[8 * i + 2], v[8 * i + 3]),
-                    Elem<T>::pack(v[8 * i + 4], v[8 * i + 5]), Elem<T>::pack(v[8 * i + 6], v[8 * i + 7]));
+        st_shared16(staged16(area, lane, i), make_uint4(Elem<T>::pack(v[8 * i], v[8 * i + 1]), Elem<T>::pack(v[8 * i + 2], v[8 * i + 3]),
+                                                        Elem<T>::pack(v[8 * i + 4], v[8 * i + 5]), Elem<T>::pack(v[8 * i + 6], v[8 * i + 7])));
+    __syncwarp();
+    rows = min(rows, 32);
+    if (vec && (cols & 7) == 0) {
+        const int piece = lane & 3;
+        T* o = out + (long long)(row0 + (lane >> 2)) * ld + col + piece * 8;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = (lane >> 2) + 8 * i;
+            const uint4 w = ld_shared16(staged16(area, r, piece));
+            if (r < rows && piece * 8 < cols) *reinterpret_cast<uint4*>(o) = w;
+            o += 8 * ld;
+        }
+    } else {   // odd boundaries: a row at a time, an element a lane
+#pragma unroll 4
+        for (int r = 0; r < rows; r++) {
+            uint16_t w;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(staged16(area, r, lane >> 3) + (lane & 7) * 2) : "memory");
+            if (lane < cols) reinterpret_cast<uint16_t*>(out + (long long)(row0 + r) * ld + col)[lane] = w;
+        }
+    }
 }
-template <>
-__device__ __forceinline__ void stage32<float>(uint32_t area, int lane, const float (&v)[32]) {
+// The same in fp32, added to `in` if that is set. cols counts the padding of the rows: a multiple of 4.
+__device__ __forceinline__ void leave32(uint32_t area, const float (&v)[32], float* out, const float* in, long long ld, int cols, int rows, int lane) {
+    __syncwarp();   // the whole area is used: the strip before has been read
 #pragma unroll
     for (int i = 0; i < 8; i++)
-        st_shared16(staged32(area, lane, i), __float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
-                    __float_as_uint(v[4 * i + 3]));
-}
-// All but the last N stores have read their area.
-template <int N>
-__device__ __forceinline__ void stage_wait(int lane) {
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+        st_shared16(staged32(area, lane, i), make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                                                        __float_as_uint(v[4 * i + 3])));
     __syncwarp();
-}
-__device__ __forceinline__ void stage_flush(uint32_t area, const CUtensorMap* map, int col, int row, int lane) {
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncwarp();
-    if (lane == 0) {
-        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(col), "r"(row), "r"(area)
-                     : "memory");
-        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    const int piece = lane & 7;
+    const long long at = (lane >> 3) * ld + piece * 4;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int r = (lane >> 3) + 4 * i;
+        const uint4 w = ld_shared16(staged32(area, r, piece));
+        if (r < rows && piece * 4 < cols) {
+            float4 f = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+            if (in) {
+                const float4 s = *reinterpret_cast<const float4*>(in + at + 4 * i * ld);
+                f.x += s.x;
+                f.y += s.y;
+                f.z += s.z;
+                f.w += s.w;
+            }
+            *reinterpret_cast<float4*>(out + at + 4 * i * ld) = f;
+        }
     }
-}
-// The same for rows that no tensor map can describe: a warp writes one row's columns at a time.
-template <typename T>
-__device__ __forceinline__ void stage_copy(uint32_t area, T* out, long long ld, int col, int cols, int row, int rows, int lane) {
-    __syncwarp();
-#pragma unroll 4
-    for (int r = 0; r < rows; r++) {
-        uint16_t w;
-        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(staged16(area, r, lane >> 3) + (lane & 7) * 2) : "memory");
-        if (lane < cols) reinterpret_cast<uint16_t*>(out + (long long)(row + r) * ld + col)[lane] = w;
-    }
-    __syncwarp();
 }
 
 // Running maximum and sum of exp(z - maximum) of one row. A maximum of -inf (every class masked so far) is replaced by
@@ -287,7 +286,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     __shared__ int gave_up_s;
     __shared__ __align__(16) T bias_s[kEpiWarps][2][32];
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = CG == 2 ? tc::cta_rank() : 0;
     const uint32_t smem0 = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t bar0 = tc::smem_u32(bars);
@@ -340,7 +339,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     const int bn_cta = g.bn / CG;
 
     if (warp == 0) {
-        if (lane == 0) {
+        if (tc::elect_one()) {
             const CUtensorMap* map_b = (g.b_select && *g.b_select) ? &g.b_alt : &g.b;
             int s = 0;
             uint32_t phase = 0;
@@ -394,7 +393,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0 && tc::elect_one()) {
             int s = 0, buf = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true, issued = false;
@@ -440,7 +439,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         const uint32_t acc = tmem + group * kTileNMax + ((uint32_t)(quarter * 32) << 16);
         const int in_tile = (int)rank * kTileM + quarter * 32;
         uint32_t acc_phase = 0;
-        int turn = 0;   // which of the staging areas is next
         float scale = 1.0f;
         if constexpr (EPI == EPI_STORE) scale = g.e.scale.value();
         for (long long t = first + group * step; t < tiles; t += 2 * step) {
@@ -451,7 +449,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             const int n0 = nb * g.bn, n1 = min(n0 + g.bn, g.n);
 
             // what does not depend on the products is fetched before the wait for them
-            int label = -1, res_row = 0;
+            int label = -1;
             bool counted = false;
             float cmax = 0.0f, cscale = 0.0f, inv_sum = 0.0f, zsum = 0.0f;
             RunningSoftmax run = {-INFINITY, 0.0f};
@@ -468,8 +466,35 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     cscale = (g.e.coef ? g.e.coef[row] : 1.0f) * 32768.0f;
                 }
             }
+            // the residual's strip is fetched ahead, too: lane l takes piece l % 4 of the rows l / 4 + 8 i
+            uint4 res_next[4] = {};
+            long long res_at[4];
+            auto fetch_residual = [&](int c) {
+                const int col = n0 + c + (lane & 3) * 8, count = n1 - col;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (res_at[i] < 0 || count <= 0) continue;
+                    const T* p = reinterpret_cast<const T*>(g.e.residual) + res_at[i] + col;
+                    if (g.e.vec_res && count >= 8) {
+                        res_next[i] = __ldg(reinterpret_cast<const uint4*>(p));
+                    } else {
+                        uint32_t w[4] = {};
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            if (j < count) w[j >> 1] |= (uint32_t) reinterpret_cast<const uint16_t*>(p)[j] << (16 * (j & 1));
+                        res_next[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            };
             if constexpr (EPI == EPI_LINEAR) {
-                if (g.e.residual && row_ok) res_row = row % g.e.residual_rows;
+                if (g.e.residual) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int r = row0 + (lane >> 2) + 8 * i;
+                        res_at[i] = r < g.m ? (long long)(r % g.e.residual_rows) * g.e.ldr : -1;
+                    }
+                    fetch_residual(0);
+                }
             }
             // the bias of 32 columns, one lane each, is fetched a strip ahead and passed around in shared memory
             auto fetch_bias = [&](int c) {
@@ -491,7 +516,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     bias_next = fetch_bias(c + 32);
                     __syncwarp();
                 }
-                if (count <= 0) return;
+                if (count <= 0 || row0 >= g.m) return;
                 float v[32];
 #pragma unroll
                 for (int i = 0; i < 32; i++) v[i] = __uint_as_float(raw[i]);
@@ -508,56 +533,59 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                         }
                     }
                 }
-                auto leave = [&](const CUtensorMap* map, bool mapped, void* out, long long ld) {
-                    if (row0 >= g.m) return;
-                    const uint32_t half = area + turn * (kStageBytes / 2);
-                    turn ^= 1;
-                    stage_wait<1>(lane);
-                    stage32<T>(half, lane, v);
-                    if (mapped)
-                        stage_flush(half, map, col, row0, lane);
-                    else
-                        stage_copy(half, reinterpret_cast<T*>(out), ld, col, min(32, count), row0, min(32, g.m - row0), lane);
+                const uint32_t half = area + (c >> 5 & 1) * (kStageBytes / 2);   // strips take turns
+                auto leave = [&](void* out, long long ld, bool vec) {
+                    leave16<T>(half, v, reinterpret_cast<T*>(out), ld, vec, col, min(32, count), row0, g.m - row0, lane);
                 };
                 if constexpr (EPI == EPI_LINEAR) {
-                    if (g.e.preact) leave(&g.pre, g.e.map_pre, g.e.preact, g.e.ldp);
-                    if (g.e.act != ACT_NONE) {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) act_value4(v + i, g.e.act);
+                    if (g.e.preact) {
+                        leave(g.e.preact, g.e.ldp, g.e.vec_pre);
+                        __syncwarp();
                     }
-                    if (g.e.residual && row_ok)
-                        add32(reinterpret_cast<const T*>(g.e.residual) + (long long)res_row * g.e.ldr, col, count, g.e.vec_res, v);
-                    leave(&g.out, g.e.map_out, g.e.out, g.e.ldo);
-                }
-                if constexpr (EPI == EPI_STORE) {
-                    if (g.e.acc_in && row_ok) {
-                        const float* p = g.e.acc_in + (long long)row * g.e.ldacc + col;   // ldacc is a multiple of 4
+                    if (g.e.act != ACT_NONE) act_values<32>(v, g.e.act);
+                    if (g.e.residual) {   // the other way round: whole pieces of rows in, a row a thread out
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            if (i < count) {
-                                const float4 f = *reinterpret_cast<const float4*>(p + i);
-                                v[i] += f.x;
-                                v[i + 1] += f.y;
-                                v[i + 2] += f.z;
-                                v[i + 3] += f.w;
+                        for (int i = 0; i < 4; i++) st_shared16(staged16(half, (lane >> 2) + 8 * i, lane & 3), res_next[i]);
+                        fetch_residual(c + 32);
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const uint4 w = ld_shared16(staged16(half, lane, i));
+                            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                const float2 s = add2(make_float2(v[8 * i + 2 * j], v[8 * i + 2 * j + 1]), Elem<T>::unpack(u[j]));
+                                v[8 * i + 2 * j] = s.x;
+                                v[8 * i + 2 * j + 1] = s.y;
                             }
                         }
                     }
-                    if (g.e.acc_out) {   // pieces of a split product lie behind one another as rows of one matrix
-                        if (g.e.map_out && row0 + 32 <= g.m) {
-                            stage_wait<0>(lane);
-                            stage32<float>(area, lane, v);
-                            stage_flush(area, &g.out, col, sp * g.m + row0, lane);
-                        } else if (row_ok) {
-                            float* o = g.e.acc_out + (long long)sp * g.e.acc_split_stride + (long long)row * g.e.ldacc + col;
-#pragma unroll
-                            for (int i = 0; i < 32; i += 4)   // a row's padding takes the rest
-                                if (i < count) *reinterpret_cast<float4*>(o + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                        }
+                    leave(g.e.out, g.e.ldo, g.e.vec_out);
+                }
+                if constexpr (EPI == EPI_STORE) {
+                    // 32-bit sums: rows and columns of this strip, the padding of the rows included
+                    const long long at = (long long)row0 * g.e.ldacc + col;
+                    const int wide = min(32, (int)g.e.ldacc - col);
+                    if (g.e.acc_out) {
+                        leave32(area, v, g.e.acc_out + (long long)sp * g.e.acc_split_stride + at, g.e.acc_in ? g.e.acc_in + at : nullptr, g.e.ldacc,
+                                wide, g.m - row0, lane);
                     } else {
+                        if (g.e.acc_in && row_ok) {
+                            const float* p = g.e.acc_in + (long long)row * g.e.ldacc + col;
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4) {
+                                if (i < wide) {
+                                    const float4 f = *reinterpret_cast<const float4*>(p + i);
+                                    v[i] += f.x;
+                                    v[i + 1] += f.y;
+                                    v[i + 2] += f.z;
+                                    v[i + 3] += f.w;
+                                }
+                            }
+                        }
 #pragma unroll
                         for (int i = 0; i < 32; i++) v[i] *= scale;
-                        leave(&g.out, g.e.map_out, g.e.out, g.e.ldo);
+                        leave(g.e.out, g.e.ldo, g.e.vec_out);
                     }
                 }
                 if constexpr (EPI == EPI_CE_STATS) {
@@ -608,7 +636,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     }
 #pragma unroll
                     for (int i = 0; i < 32; i++) v[i] = counted ? v[i] * cscale : 0.0f;
-                    leave(&g.out, true, nullptr, 0);
+                    // the rows are padded to whole pieces, which nothing reads
+                    leave16<T>(half, v, reinterpret_cast<T*>(g.e.out), g.e.ldo, true, col, min(32, (count + 7) & ~7), row0, g.m - row0, lane);
                 }
             };
             uint32_t even[32], odd[32];   // the strip at work and the one on its way
@@ -624,7 +653,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 }
             }
             tc::fence_before();
-            __syncwarp();
+            __syncwarp();   // (also: the staging area and the bias strips are free for the next tile)
             if (lane == 0) tc::bar_arrive_cluster(CG == 2 ? tc::map_to_rank(acc_empty(group), 0) : acc_empty(group));
             if constexpr (EPI == EPI_CE_STATS) {
                 if (row_ok) {
@@ -635,7 +664,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 }
             }
         }
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the results are out before the CTA ends
         __syncwarp();
     }
     tc::fence_before();
@@ -664,9 +692,8 @@ struct DeviceInfo {
     int* status;              // the library-wide status word
 };
 int device_info(DeviceInfo* out);   // of the current device; 0 or an error code
-// A map of boxes box_bytes wide (128 or 64, the swizzle's width too); bytes: of an element, 2 or 4 (fp32).
-int make_map(CUtensorMap* map, const void* data, long long ld, long long rows, long long cols, int bytes, bool bf16, int box_bytes, int box_rows,
-             const char* what);
+// A map of an operand's 64 x box_rows boxes in the 128-byte swizzle.
+int make_map(CUtensorMap* map, const Operand& o, bool bf16, int box_rows, const char* what);
 // Rows on 16-byte boundaries, as a tensor-map copy needs them.
 static inline bool map_ready(const Operand& o) {
     return ((uintptr_t)o.data & 15) == 0 && (o.rows <= 1 || (o.ld & 7) == 0);

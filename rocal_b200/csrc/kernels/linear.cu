@@ -60,8 +60,7 @@ __global__ void __launch_bounds__(256) rows_kernel(RowsArgs a) {
                 if (a.preact) {
                     float z[8];
                     load8(reinterpret_cast<const T*>(a.preact) + row * a.ldp + col, count, a.vec_pre, z);
-                    act_slope4(z, a.act);
-                    act_slope4(z + 4, a.act);
+                    act_slopes<8>(z, a.act);
 #pragma unroll
                     for (int i = 0; i < 8; i++) v[i] *= z[i];
                 }
@@ -232,7 +231,6 @@ static int linear_run(const rb200_linear_params* p, void* stream_v, GemmWait wai
     e.preact = p->preact;
     e.ldp = p->ldp;
     e.act = p->activation;
-    e.vec_res = map_ready(operand(p->residual, p->ldr, p->residual_rows, p->out_features, false));
     wait.status = p->status;
     if (l.gemm.splits > 1) {
         EpiArgs part = {};
