@@ -508,7 +508,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             acc_phase ^= 1;
             tc::fence_after();
 
-            auto body = [&](const uint32_t (&raw)[32], int c) {
+            uint32_t raw[32];   // the strip on its way
+            tc::tmem_load32(acc, raw);
+            for (int c = 0; c < g.bn; c += 32) {
                 const int col = n0 + c, count = n1 - col;   // columns of this strip inside the matrix (may be <= 0)
                 T* bias = bias_s[ew][c >> 5 & 1];
                 if constexpr (EPI != EPI_STORE) {
@@ -516,10 +518,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     bias_next = fetch_bias(c + 32);
                     __syncwarp();
                 }
-                if (count <= 0 || row0 >= g.m) return;
+                tc::tmem_wait();
                 float v[32];
 #pragma unroll
                 for (int i = 0; i < 32; i++) v[i] = __uint_as_float(raw[i]);
+                if (c + 32 < g.bn) {
+                    tc::tmem_load32(acc + c + 32, raw);
+                } else {   // the accumulator is in registers: the products of the next tile but one may begin
+                    tc::fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::bar_arrive_relaxed(CG == 2 ? tc::map_to_rank(acc_empty(group), 0) : acc_empty(group));
+                }
+                if (count <= 0 || row0 >= g.m) continue;
                 if constexpr (EPI != EPI_STORE) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {
@@ -639,22 +649,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     // the rows are padded to whole pieces, which nothing reads
                     leave16<T>(half, v, reinterpret_cast<T*>(g.e.out), g.e.ldo, true, col, min(32, (count + 7) & ~7), row0, g.m - row0, lane);
                 }
-            };
-            uint32_t even[32], odd[32];   // the strip at work and the one on its way
-            tc::tmem_load32(acc, even);
-            for (int c = 0; c < g.bn; c += 64) {
-                tc::tmem_wait();
-                if (c + 32 < g.bn) tc::tmem_load32(acc + c + 32, odd);
-                body(even, c);
-                if (c + 32 < g.bn) {
-                    tc::tmem_wait();
-                    if (c + 64 < g.bn) tc::tmem_load32(acc + c + 64, even);
-                    body(odd, c + 32);
-                }
             }
-            tc::fence_before();
-            __syncwarp();   // (also: the staging area and the bias strips are free for the next tile)
-            if (lane == 0) tc::bar_arrive_cluster(CG == 2 ? tc::map_to_rank(acc_empty(group), 0) : acc_empty(group));
+            __syncwarp();   // the staging area and the bias strips are free for the next tile
             if constexpr (EPI == EPI_CE_STATS) {
                 if (row_ok) {
                     const long long plane = (long long)g.e.parts * g.m, at = (long long)nb * g.m + row;

@@ -42,9 +42,10 @@ __device__ __forceinline__ void bar_init_fence() { asm volatile("fence.mbarrier_
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// bar: an address of the cluster's shared window (a local one is its own).
-__device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+// bar: an address of the cluster's shared window (a local one is its own). Relaxed: it orders no memory accesses (a release
+// would wait for the thread's global stores); for accumulators that have been read into registers.
+__device__ __forceinline__ void bar_arrive_relaxed(uint32_t bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
