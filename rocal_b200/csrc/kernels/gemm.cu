@@ -156,24 +156,46 @@ int gemm_store(int kind, bool bf16, const Operand& a, const Operand& b, const Op
 }
 
 // ---- joining split products -----------------------------------------------------------------------------
-// Pieces are added in their order, so the result does not depend on which CTA finished first.
-template <typename T>
+// Pieces are added in an order of their own, so the result does not depend on which CTA finished first. SUBS threads
+// share the pieces of four columns: one where there are few pieces, eight where there are many (few outputs then).
+template <typename T, int SUBS>
 __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ part, int splits, long long stride, long long ldacc, int m, int n,
                                                    EpiArgs e) {
+    constexpr int OUT = 256 / SUBS;
+    __shared__ float4 sums[SUBS][OUT];
     const long long groups = (n + 3) / 4, total = groups * m;
     const float alpha = e.scale.value();
-    for (long long t = blockIdx.x * 256ll + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
+    const int lane = threadIdx.x % OUT, sub = threadIdx.x / OUT;
+    for (long long t0 = (long long)blockIdx.x * OUT; t0 < total; t0 += (long long)gridDim.x * OUT) {
+        const long long t = t0 + lane;
         const int row = (int)(t / groups), col = (int)(t - row * groups) * 4;
-        const float* p = part + row * ldacc + col;
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s = 0; s < splits; s++) {
-            const float4 f = *reinterpret_cast<const float4*>(p + s * stride);
-            v[0] += f.x;
-            v[1] += f.y;
-            v[2] += f.z;
-            v[3] += f.w;
-        }
         const long long at = row * ldacc + col;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (t < total) {
+#pragma unroll 4
+            for (int s = sub; s < splits; s += SUBS) {
+                const float4 f = *reinterpret_cast<const float4*>(part + at + s * stride);
+                v[0] += f.x;
+                v[1] += f.y;
+                v[2] += f.z;
+                v[3] += f.w;
+            }
+        }
+        if (SUBS > 1) {
+            __syncthreads();
+            sums[sub][lane] = make_float4(v[0], v[1], v[2], v[3]);
+            __syncthreads();
+            if (sub) continue;
+#pragma unroll
+            for (int s = 1; s < SUBS; s++) {
+                const float4 f = sums[s][lane];
+                v[0] += f.x;
+                v[1] += f.y;
+                v[2] += f.z;
+                v[3] += f.w;
+            }
+        }
+        if (t >= total) continue;
         if (e.acc_in) {
             const float4 f = *reinterpret_cast<const float4*>(e.acc_in + at);
             v[0] += f.x;
@@ -208,14 +230,22 @@ size_t gemm_partial_bytes(const GemmPlan& plan, int m, int n) {
     return plan.splits > 1 ? (size_t)plan.splits * m * round_up(n, 4) * sizeof(float) : 0;
 }
 
-int gemm_join(bool bf16, const float* partials, int splits, int m, int n, const EpiArgs& e, cudaStream_t stream, const char* what) {
+template <typename T>
+static void join_launch(const float* partials, int splits, int m, int n, const EpiArgs& e, cudaStream_t stream) {
     const long long ldacc = round_up(n, 4), total = ldacc / 4 * m;
-    const long long blocks = (total + 255) / 256;
+    const int out = splits >= 16 ? 32 : 256;
+    const long long blocks = (total + out - 1) / out;
     const unsigned grid = (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16);
-    if (bf16)
-        join_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(partials, splits, ldacc * m, ldacc, m, n, e);
+    if (splits >= 16)
+        join_kernel<T, 8><<<grid, 256, 0, stream>>>(partials, splits, ldacc * m, ldacc, m, n, e);
     else
-        join_kernel<__half><<<grid, 256, 0, stream>>>(partials, splits, ldacc * m, ldacc, m, n, e);
+        join_kernel<T, 1><<<grid, 256, 0, stream>>>(partials, splits, ldacc * m, ldacc, m, n, e);
+}
+int gemm_join(bool bf16, const float* partials, int splits, int m, int n, const EpiArgs& e, cudaStream_t stream, const char* what) {
+    if (bf16)
+        join_launch<__nv_bfloat16>(partials, splits, m, n, e, stream);
+    else
+        join_launch<__half>(partials, splits, m, n, e, stream);
     RB200_CHECK_LAUNCH(what);
     return RB200_OK;
 }

@@ -771,7 +771,8 @@ int gemm_join(bool bf16, const float* partials, int splits, int m, int n, const 
 // dst[rows][ldd] = src, for operands whose rows no tensor map can describe.
 int pack_rows(const Operand& src, void* dst, long long ldd, cudaStream_t stream, const char* what);
 
-// Column sums of a matrix (linear.cu): chunks planes of ldpart partial sums, joined (with other planes) by sum_chunks.
+// Column sums of a matrix in a workspace, its rows padded to 8 elements (linear.cu): chunks planes of ldpart partial sums,
+// joined (with other planes) by sum_chunks.
 struct ColumnSums {
     int chunks;
     long long ldpart;

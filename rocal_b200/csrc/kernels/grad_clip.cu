@@ -140,26 +140,69 @@ __global__ void __launch_bounds__(kClipThreads) clip_norm_kernel(const __grid_co
 }
 
 // ---- multiplication -----------------------------------------------------------------------------------------
+// Sixteen bytes that start SHIFT words and `bits` bits into two neighbouring aligned vectors.
+template <int SHIFT>
+__device__ __forceinline__ uint4 window(const uint4& a, const uint4& b, int bits) {
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    return make_uint4(__funnelshift_r(w[SHIFT], w[SHIFT + 1], bits), __funnelshift_r(w[SHIFT + 1], w[SHIFT + 2], bits),
+                      __funnelshift_r(w[SHIFT + 2], w[SHIFT + 3], bits), __funnelshift_r(w[SHIFT + 3], w[(SHIFT + 4) & 7], bits));
+}
+template <typename T, typename O>
+__device__ __forceinline__ void scale_vector(const uint4& w, O* o, int i, float factor) {
+    constexpr int N = Values<T>::N, M = Values<O>::N;
+    float v[N];
+    Values<T>::get(w, v);
+#pragma unroll
+    for (int j = 0; j < N; j++) v[j] *= factor;
+#pragma unroll
+    for (int j = 0; j < N; j += M) reinterpret_cast<uint4*>(o)[i * (N / M) + j / M] = Values<O>::put(v + j);
+}
+// SHIFT < 0: the gradients have the output's boundaries. Four vectors in flight a thread.
+template <typename T, typename O, int SHIFT>
+__device__ __forceinline__ void scale_vectors(const T* g, O* o, int vectors, float factor) {
+    constexpr int U = 4;
+    const uint4* q = reinterpret_cast<const uint4*>((uintptr_t)g & ~(uintptr_t)15);
+    const int bits = (int)((uintptr_t)g & 3) * 8;
+    auto fetch = [&](int i) {   // the second vector is one that the sixteen bytes reach into
+        if constexpr (SHIFT < 0)
+            return q[i];
+        else
+            return window<SHIFT>(q[i], q[i + 1], bits);
+    };
+    int i = threadIdx.x;
+    for (; i + (U - 1) * kClipThreads < vectors; i += U * kClipThreads) {
+        uint4 w[U];
+#pragma unroll
+        for (int k = 0; k < U; k++) w[k] = fetch(i + k * kClipThreads);
+#pragma unroll
+        for (int k = 0; k < U; k++) scale_vector<T>(w[k], o, i + k * kClipThreads, factor);
+    }
+    for (; i < vectors; i += kClipThreads) scale_vector<T>(fetch(i), o, i, factor);
+}
+// Whole vectors are written where the output has its 16-byte boundaries; the gradients that belong there are cut out of
+// the aligned vectors that hold them.
 template <typename T, typename O>
 __device__ __forceinline__ void scale_chunk(const T* g, O* o, int count, float factor) {
     constexpr int N = Values<T>::N;
-    if ((((uintptr_t)g | (uintptr_t)o) & 15) == 0) {
-        const int vectors = count / N;
-#pragma unroll 4
-        for (int i = threadIdx.x; i < vectors; i += kClipThreads) {
-            float v[N];
-            Values<T>::get(reinterpret_cast<const uint4*>(g)[i], v);
-#pragma unroll
-            for (int j = 0; j < N; j++) v[j] *= factor;
-#pragma unroll
-            for (int j = 0; j < N; j += Values<O>::N) reinterpret_cast<uint4*>(o)[i * (N / Values<O>::N) + j / Values<O>::N] = Values<O>::put(v + j);
+    const int head = min(count, (int)(((16 - ((uintptr_t)o & 15)) & 15) / sizeof(O)));
+    if ((int)threadIdx.x < head) o[threadIdx.x] = Values<O>::from_float(Values<T>::to_float(g[threadIdx.x]) * factor);
+    g += head;
+    o += head;
+    count -= head;
+    const int vectors = count / N;
+    const int offset = (int)((uintptr_t)g & 15);
+    if (offset == 0) {
+        scale_vectors<T, O, -1>(g, o, vectors, factor);
+    } else {
+        switch (offset >> 2) {
+            case 0: scale_vectors<T, O, 0>(g, o, vectors, factor); break;
+            case 1: scale_vectors<T, O, 1>(g, o, vectors, factor); break;
+            case 2: scale_vectors<T, O, 2>(g, o, vectors, factor); break;
+            default: scale_vectors<T, O, 3>(g, o, vectors, factor); break;
         }
-        g += vectors * N;
-        o += vectors * N;
-        count -= vectors * N;
     }
-#pragma unroll 8
-    for (int i = threadIdx.x; i < count; i += kClipThreads) o[i] = Values<O>::from_float(Values<T>::to_float(g[i]) * factor);
+    const int tail = vectors * N + threadIdx.x;
+    if (tail < count) o[tail] = Values<O>::from_float(Values<T>::to_float(g[tail]) * factor);
 }
 
 template <int CAP>
@@ -300,9 +343,9 @@ static int clip_run(const rb200_grad_tensor* tensors, int n, float max_norm, flo
     int rc = device_info(&dev);
     if (rc) return rc;
     const int most = std::min(dev.sms * kClipBlocksPerSm, kClipMaxBlocks);
-    // chunks: enough of them for every block, between 2048 elements (a block's vectors once) and 32768
-    long long chunk = round_up((total + most - 1) / most, 2048);
-    chunk = std::min(chunk, 32768ll);
+    // chunks: about four for every block, so that the ends of tensors even out; between 2048 elements and 16384
+    long long chunk = round_up((total + 4 * most - 1) / (4 * most), 2048);
+    chunk = std::min(chunk, 16384ll);
     while (total / chunk > (1ll << 30)) chunk *= 2;
     double* partial = (double*)ws;
     int partials = 0;

@@ -8,9 +8,9 @@ namespace rb200 {
 // ---- sweeps over a gradient matrix ------------------------------------------------------------------------
 // Rows j, j + period, j + 2 period, ... of `src` are summed into partial sums [chunk][j][column] in 32 bits; with
 // `preact` the elements are first multiplied by the activation's slope, and with `dst` what was read (multiplied) is
-// written, in the element type. A block takes 256 columns (a warp reads 512 contiguous bytes of a row) and a chunk of
-// the repeats, 8 rows at a time; its 8 row sums meet in shared memory, chunks meet in sum_chunks_kernel, always in the
-// same order.
+// written, in the element type. A block takes up to 256 columns (8 a thread, as many threads side by side as the columns
+// need, the others on further rows) and a chunk of the repeats; a thread has four rows in flight. The row sums meet in
+// shared memory, chunks meet in sum_chunks_kernel, always in the same order. Bound by memory.
 struct RowsArgs {
     const void* src;
     long long lds;
@@ -20,100 +20,155 @@ struct RowsArgs {
     long long ldd;
     float* part;              // [chunks][period][ldpart] or null
     long long ldpart;
+    void* out;                // one chunk only: the sums in the element type, [period][ldo], or null
+    long long ldo;
     int rows, cols, period, chunks, per_chunk;   // per_chunk: repeats of a chunk
+    int readable;             // columns that may be read: cols, or more where the rows are padded
+    int across;               // threads side by side: a power of two up to 32
     int act, vec_src, vec_pre;
 };
 
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int count, bool vec, float (&v)[8]) {
-    if (vec && count >= 8) {
-        const uint4 w = *reinterpret_cast<const uint4*>(p);
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+__device__ __forceinline__ uint4 load8(const T* p, int count, bool vec) {
+    if (vec && count >= 8) return __ldg(reinterpret_cast<const uint4*>(p));
+    uint32_t w[4] = {};
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float2 f = Elem<T>::unpack(u[i]);
-            v[2 * i] = f.x;
-            v[2 * i + 1] = f.y;
-        }
-    } else {
+    for (int i = 0; i < 8; i++)
+        if (i < count) w[i >> 1] |= (uint32_t) reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& w, float (&v)[8]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = i < count ? Elem<T>::to_float(p[i]) : 0.0f;
+    for (int i = 0; i < 4; i++) {
+        const float2 f = Elem<T>::unpack(u[i]);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
     }
 }
 
-template <typename T>
+template <typename T, bool SLOPE>
 __global__ void __launch_bounds__(256) rows_kernel(RowsArgs a) {
-    __shared__ float sums[8][256 + 8];
-    const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
-    const int col = blockIdx.x * 256 + lane * 8, count = a.cols - col;
+    constexpr int U = 4;   // rows in flight
+    __shared__ float sums[256 * 8];
+    __shared__ float half[256];
+    const int lane = threadIdx.x & (a.across - 1), sub = threadIdx.x / a.across, subs = 256 / a.across, wide = a.across * 8;
+    const int col = blockIdx.x * wide + lane * 8, count = a.readable - col;
+    const int repeats = a.rows / a.period;
     const long long units = (long long)a.period * a.chunks;
     for (long long u = blockIdx.y; u < units; u += gridDim.y) {
         const int chunk = (int)(u / a.period), j = (int)(u - (long long)chunk * a.period);
-        const int repeats = a.rows / a.period;
         const int t_end = min(repeats, (chunk + 1) * a.per_chunk);
         float acc[8] = {};
-        if (count > 0) {
-            for (int t = chunk * a.per_chunk + sub; t < t_end; t += 8) {
+        auto fetch = [&](int t, uint4& w, uint4& z) {
+            const long long row = (long long)t * a.period + j;
+            w = load8(reinterpret_cast<const T*>(a.src) + row * a.lds + col, count, a.vec_src);
+            if (SLOPE) z = load8(reinterpret_cast<const T*>(a.preact) + row * a.ldp + col, count, a.vec_pre);
+        };
+        auto take = [&](int t, const uint4& w, const uint4& z) {
+            float v[8];
+            unpack8<T>(w, v);
+            if (SLOPE) {
+                float s[8];
+                unpack8<T>(z, s);
+                act_slopes<8>(s, a.act);
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[k] *= s[k];
+            }
+            if (a.dst) {   // the destination's rows are padded to whole vectors
                 const long long row = (long long)t * a.period + j;
-                float v[8];
-                load8(reinterpret_cast<const T*>(a.src) + row * a.lds + col, count, a.vec_src, v);
-                if (a.preact) {
-                    float z[8];
-                    load8(reinterpret_cast<const T*>(a.preact) + row * a.ldp + col, count, a.vec_pre, z);
-                    act_slopes<8>(z, a.act);
+                *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.dst) + row * a.ldd + col) =
+                    make_uint4(Elem<T>::pack(v[0], v[1]), Elem<T>::pack(v[2], v[3]), Elem<T>::pack(v[4], v[5]), Elem<T>::pack(v[6], v[7]));
+            }
 #pragma unroll
-                    for (int i = 0; i < 8; i++) v[i] *= z[i];
-                }
-                if (a.dst) {   // the destination's rows are padded to whole vectors
-                    *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.dst) + row * a.ldd + col) =
-                        make_uint4(Elem<T>::pack(v[0], v[1]), Elem<T>::pack(v[2], v[3]), Elem<T>::pack(v[4], v[5]), Elem<T>::pack(v[6], v[7]));
-                }
+            for (int k = 0; k < 8; k++) acc[k] += v[k];
+        };
+        if (count > 0) {
+            int t = chunk * a.per_chunk + sub;
+            uint4 w[U], z[U];
+            for (; t + (U - 1) * subs < t_end; t += U * subs) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) acc[i] += v[i];
+                for (int i = 0; i < U; i++) fetch(t + i * subs, w[i], z[i]);
+#pragma unroll
+                for (int i = 0; i < U; i++) take(t + i * subs, w[i], z[i]);
+            }
+            for (; t < t_end; t += subs) {
+                fetch(t, w[0], z[0]);
+                take(t, w[0], z[0]);
             }
         }
-        if (a.part) {
+        if (a.part || a.out) {
+            // 256 / wide threads a column, 8 row sums each, then the first `wide` threads
 #pragma unroll
-            for (int i = 0; i < 8; i++) sums[sub][lane * 8 + i] = acc[i];
+            for (int k = 0; k < 8; k++) sums[sub * wide + lane * 8 + k] = acc[k];
             __syncthreads();
+            const int c = threadIdx.x & (wide - 1), piece = threadIdx.x / wide;
             float s = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) s += sums[i][threadIdx.x];
-            const int c = blockIdx.x * 256 + threadIdx.x;
-            if (c < a.cols) a.part[u * a.ldpart + c] = s;
+            for (int k = 0; k < 8; k++) s += sums[(piece * 8 + k) * wide + c];
+            half[threadIdx.x] = s;
+            __syncthreads();
+            const int out_col = blockIdx.x * wide + c;
+            if (piece == 0 && out_col < a.cols) {
+                for (int k = 1; k < 256 / wide; k++) s += half[k * wide + c];
+                if (a.part) a.part[u * a.ldpart + out_col] = s;
+                if (a.out) reinterpret_cast<T*>(a.out)[j * a.ldo + out_col] = Elem<T>::from_float(s);
+            }
             __syncthreads();
         }
     }
 }
 
-// out[j][c] = scale * sum over planes of part[plane][j][c].
+// out[j][c] = scale * sum over planes of part[plane][j][c]: 8 columns a block, planes spread over 32 threads a column.
 template <typename T>
 __global__ void __launch_bounds__(256) sum_chunks_kernel(const float* __restrict__ part, long long ldpart, int planes, int rows, int cols, T* out,
                                                          long long ldo, Scale scale) {
-    __shared__ float sums[8][33];
-    const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+    __shared__ float sums[32][9];
+    const int lane = threadIdx.x & 7, sub = threadIdx.x >> 3, col = blockIdx.x * 8 + lane;
     const float factor = scale.value();
     for (int j = blockIdx.y; j < rows; j += gridDim.y) {
         float s = 0.0f;
-        if (col < cols)
-            for (int p = sub; p < planes; p += 8) s += part[((long long)p * rows + j) * ldpart + col];
+        if (col < cols) {
+#pragma unroll 4
+            for (int p = sub; p < planes; p += 32) s += part[((long long)p * rows + j) * ldpart + col];
+        }
         sums[sub][lane] = s;
         __syncthreads();
         if (sub == 0 && col < cols) {
 #pragma unroll
-            for (int i = 1; i < 8; i++) s += sums[i][lane];
+            for (int i = 1; i < 32; i++) s += sums[i][lane];
             out[j * ldo + col] = Elem<T>::from_float(s * factor);
         }
         __syncthreads();
     }
 }
 
-// How many pieces the repeats are cut into: about four blocks an SM, at least 32 repeats a piece.
+// The same for few planes: a thread takes one sum.
+template <typename T>
+__global__ void __launch_bounds__(256) sum_few_kernel(const float* __restrict__ part, long long ldpart, int planes, int rows, int cols, T* out,
+                                                      long long ldo, Scale scale) {
+    const float factor = scale.value();
+    const long long total = (long long)rows * cols;
+    for (long long t = blockIdx.x * 256ll + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
+        const long long j = t / cols;
+        const int col = (int)(t - j * cols);
+        float s = 0.0f;
+#pragma unroll 4
+        for (int p = 0; p < planes; p++) s += part[((long long)p * rows + j) * ldpart + col];
+        out[j * ldo + col] = Elem<T>::from_float(s * factor);
+    }
+}
+
+// How the block's threads lie and how many pieces the repeats are cut into: about eight blocks an SM, at least eight
+// repeats a thread.
 static void cut_rows(RowsArgs* a, int sms) {
-    const int repeats = a->rows / a->period;
-    const long long blocks = (long long)((a->cols + 255) / 256) * a->period;
-    long long chunks = (4ll * sms + blocks - 1) / blocks;
-    if (chunks > (repeats + 31) / 32) chunks = (repeats + 31) / 32;
+    a->across = 1;
+    while (a->across < 32 && a->across * 8 < a->cols) a->across *= 2;
+    const int repeats = a->rows / a->period, wide = a->across * 8, least = 256 / a->across * 8;
+    const long long blocks = (long long)((a->cols + wide - 1) / wide) * a->period;
+    long long chunks = 8ll * sms / blocks;
+    if (chunks > (repeats + least - 1) / least) chunks = (repeats + least - 1) / least;
     if (chunks < 1) chunks = 1;
     a->per_chunk = (int)((repeats + chunks - 1) / chunks);
     a->chunks = (repeats + a->per_chunk - 1) / a->per_chunk;
@@ -121,22 +176,40 @@ static void cut_rows(RowsArgs* a, int sms) {
 
 static int rows_launch(bool bf16, const RowsArgs& a, cudaStream_t stream, const char* what) {
     const long long units = (long long)a.period * a.chunks;
-    const dim3 grid((unsigned)((a.cols + 255) / 256), (unsigned)(units < 32768 ? units : 32768));
-    if (bf16)
-        rows_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(a);
-    else
-        rows_kernel<__half><<<grid, 256, 0, stream>>>(a);
+    const int wide = a.across * 8;
+    const dim3 grid((unsigned)((a.cols + wide - 1) / wide), (unsigned)(units < 32768 ? units : 32768));
+    if (bf16) {
+        if (a.preact)
+            rows_kernel<__nv_bfloat16, true><<<grid, 256, 0, stream>>>(a);
+        else
+            rows_kernel<__nv_bfloat16, false><<<grid, 256, 0, stream>>>(a);
+    } else {
+        if (a.preact)
+            rows_kernel<__half, true><<<grid, 256, 0, stream>>>(a);
+        else
+            rows_kernel<__half, false><<<grid, 256, 0, stream>>>(a);
+    }
     RB200_CHECK_LAUNCH(what);
     return RB200_OK;
 }
 
+template <typename T>
+static void sum_launch(const float* part, long long ldpart, int planes, int rows, int cols, T* out, long long ldo, const Scale& scale,
+                       cudaStream_t stream) {
+    if (planes < 32) {
+        const long long blocks = ((long long)rows * cols + 255) / 256;
+        sum_few_kernel<T><<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, stream>>>(part, ldpart, planes, rows, cols, out, ldo, scale);
+    } else {
+        const dim3 grid((unsigned)((cols + 7) / 8), (unsigned)(rows < 32768 ? rows : 32768));
+        sum_chunks_kernel<T><<<grid, 256, 0, stream>>>(part, ldpart, planes, rows, cols, out, ldo, scale);
+    }
+}
 int sum_chunks(bool bf16, const float* part, long long ldpart, int planes, int rows, int cols, void* out, long long ldo, const Scale& scale,
                cudaStream_t stream, const char* what) {
-    const dim3 grid((unsigned)((cols + 31) / 32), (unsigned)(rows < 32768 ? rows : 32768));
     if (bf16)
-        sum_chunks_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(part, ldpart, planes, rows, cols, (__nv_bfloat16*)out, ldo, scale);
+        sum_launch(part, ldpart, planes, rows, cols, (__nv_bfloat16*)out, ldo, scale, stream);
     else
-        sum_chunks_kernel<__half><<<grid, 256, 0, stream>>>(part, ldpart, planes, rows, cols, (__half*)out, ldo, scale);
+        sum_launch(part, ldpart, planes, rows, cols, (__half*)out, ldo, scale, stream);
     RB200_CHECK_LAUNCH(what);
     return RB200_OK;
 }
@@ -157,6 +230,7 @@ int column_partials(bool bf16, const Operand& src, float* part, int sms, cudaStr
     a.lds = src.ld;
     a.rows = src.rows;
     a.cols = src.cols;
+    a.readable = (int)round_up(src.cols, 8);
     a.period = 1;
     a.vec_src = map_ready(src);
     a.part = part;
@@ -279,14 +353,20 @@ static LinearBackwardPlan plan_backward(const rb200_linear_backward_params& p, c
     a.src = p.dout;
     a.lds = p.lddo;
     a.rows = n;
-    a.cols = m;
+    a.cols = a.readable = m;
     a.vec_src = map_ready(dout);
     a.ldpart = round_up(m, 4);
     if (p.dresidual) {
         l.res_rows = a;
         l.res_rows.period = (int)p.residual_rows;
         cut_rows(&l.res_rows, dev.sms);
-        l.res_rows.part = (float*)c.take((size_t)l.res_rows.chunks * l.res_rows.period * a.ldpart * sizeof(float));
+        // whole sums leave in the element type at once; 32-bit ones are kept for further sums
+        if (l.res_rows.chunks == 1) {
+            l.res_rows.out = p.dresidual;
+            l.res_rows.ldo = p.lddr;
+        }
+        if (l.res_rows.chunks > 1 || (p.dbias && p.activation == RB200_ACT_NONE))
+            l.res_rows.part = (float*)c.take((size_t)l.res_rows.chunks * l.res_rows.period * a.ldpart * sizeof(float));
     }
     // without an activation the column sums are the sums of the residual's sums: no second sweep
     l.sums = p.dbias && (p.activation != RB200_ACT_NONE || !p.dresidual);
@@ -346,7 +426,7 @@ static int backward_run(const rb200_linear_backward_params* p, void* stream_v) {
     if (p->dresidual) {
         const RowsArgs& r = l.res_rows;
         if ((rc = rows_launch(bf16, r, stream, what))) return rc;
-        if ((rc = sum_chunks(bf16, r.part, r.ldpart, r.chunks, r.period, (int)m, p->dresidual, p->lddr, Scale(), stream, what))) return rc;
+        if (!r.out && (rc = sum_chunks(bf16, r.part, r.ldpart, r.chunks, r.period, (int)m, p->dresidual, p->lddr, Scale(), stream, what))) return rc;
         if (p->dbias && !l.sums &&
             (rc = sum_chunks(bf16, r.part, r.ldpart, r.chunks * r.period, 1, (int)m, p->dbias, 0, Scale(), stream, what)))
             return rc;

@@ -36,93 +36,134 @@ __device__ __forceinline__ void join(RunningSoftmax& a, float m, float s) {
     a.m = top;
 }
 
+// A block takes 256 / SUBS rows at a time; SUBS threads share a row's parts.
+template <int SUBS>
 __global__ void __launch_bounds__(256) ce_merge_kernel(MergeArgs a) {
-    __shared__ float sm[8][33], ss[8][33], sz[8][33];
+    constexpr int ROWS = 256 / SUBS;
+    __shared__ float sm[SUBS][ROWS], ss[SUBS][ROWS], sz[SUBS][ROWS];
     __shared__ double sums[256];
-    __shared__ int last_block;
-    const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
-    const int row = blockIdx.x * 32 + lane;
+    __shared__ int counts[8], dirts[8], last_block;
+    const int lane = threadIdx.x % ROWS, sub = threadIdx.x / ROWS;
     const long long plane = (long long)a.parts * a.rows;
-    RunningSoftmax r = {-INFINITY, 0.0f};
-    float z = 0.0f;
-    if (row < a.rows) {
-        for (int p = sub; p < a.parts; p += 8) {
-            const long long at = (long long)p * a.rows + row;
-            join(r, a.part[at], a.part[plane + at]);
-            if (a.want_zsum) z += a.part[2 * plane + at];
-        }
-    }
-    sm[sub][lane] = r.m;
-    ss[sub][lane] = r.s;
-    sz[sub][lane] = z;
-    __syncthreads();
-    if (sub == 0) {
-        bool counted = false, dirty = false;
-        double mine = 0.0;
+    double mine = 0.0;
+    int counts_mine = 0, dirty_mine = 0;
+    for (long long row0 = (long long)blockIdx.x * ROWS; row0 < a.rows; row0 += (long long)gridDim.x * ROWS) {
+        const long long row = row0 + lane;
+        RunningSoftmax r = {-INFINITY, 0.0f};
+        float z = 0.0f;
         if (row < a.rows) {
-            for (int i = 1; i < 8; i++) {
+#pragma unroll 4
+            for (int p = sub; p < a.parts; p += SUBS) {
+                const long long at = (long long)p * a.rows + row;
+                join(r, a.part[at], a.part[plane + at]);
+                if (a.want_zsum) z += a.part[2 * plane + at];
+            }
+        }
+        if (SUBS > 1) {
+            __syncthreads();
+            sm[sub][lane] = r.m;
+            ss[sub][lane] = r.s;
+            sz[sub][lane] = z;
+            __syncthreads();
+            if (sub) continue;
+#pragma unroll
+            for (int i = 1; i < SUBS; i++) {
                 join(r, sm[i][lane], ss[i][lane]);
                 z += sz[i][lane];
             }
-            if (!a.first) {
-                join(r, a.stats[row], a.stats[a.rows + row]);
-                if (a.want_zsum) z += a.zsum[row];
-            }
-            if (!a.last) {
-                if (a.want_zsum) a.zsum[row] = z;
-            } else {
-                const int label = load_label(a.labels, a.label_bytes, row, a.ignore_index, a.classes, &counted);
-                float loss = 0.0f;
-                if (counted) {
-                    if (label < 0) {
-                        r.m = r.s = loss = nanf("");
-                    } else {
-                        const float lse = logf(r.s);   // above the maximum
-                        loss = (1.0f - a.smoothing) * (lse + (r.m - a.zlabel[row]));
-                        if (a.want_zsum) loss += a.smoothing * (lse + (r.m - z / (float)a.classes));
-                    }
-                } else {
-                    dirty = !(isfinite(r.m) && isfinite(r.s));
-                }
-                mine = loss;
-                if (a.reduction == RB200_REDUCE_NONE) a.loss[row] = loss;
-            }
-            a.stats[row] = r.m;
-            a.stats[a.rows + row] = r.s;
         }
-        if (a.last) {
-            const unsigned n = __popc(__ballot_sync(0xFFFFFFFFu, counted));
-            const bool any = __any_sync(0xFFFFFFFFu, dirty);
-#pragma unroll
-            for (int d = 16; d; d >>= 1) mine += __shfl_down_sync(0xFFFFFFFFu, mine, d);
-            if (lane == 0) {
-                if (n) atomicAdd(a.info, (int)n);
-                if (any) atomicOr(a.info + 1, 1);
-                if (a.reduction != RB200_REDUCE_NONE) {
-                    a.block_sums[blockIdx.x] = mine;
-                    __threadfence();
-                    last_block = atomicAdd(a.info + 2, 1) == (int)gridDim.x - 1;
+        if (row >= a.rows) continue;
+        if (!a.first) {
+            join(r, a.stats[row], a.stats[a.rows + row]);
+            if (a.want_zsum) z += a.zsum[row];
+        }
+        if (!a.last) {
+            if (a.want_zsum) a.zsum[row] = z;
+        } else {
+            bool counted;
+            const int label = load_label(a.labels, a.label_bytes, row, a.ignore_index, a.classes, &counted);
+            float loss = 0.0f;
+            if (counted) {
+                counts_mine++;
+                if (label < 0) {
+                    r.m = r.s = loss = nanf("");
+                } else {
+                    const float lse = logf(r.s);   // above the maximum
+                    loss = (1.0f - a.smoothing) * (lse + (r.m - a.zlabel[row]));
+                    if (a.want_zsum) loss += a.smoothing * (lse + (r.m - z / (float)a.classes));
                 }
+            } else {
+                dirty_mine |= !(isfinite(r.m) && isfinite(r.s));
             }
+            mine += loss;
+            if (a.reduction == RB200_REDUCE_NONE) a.loss[row] = loss;
+        }
+        a.stats[row] = r.m;
+        a.stats[a.rows + row] = r.s;
+    }
+    if (!a.last) return;
+    // the block's counts and sum, then one atomic each (whole numbers: their order does not matter)
+    const int warp_count = __reduce_add_sync(0xFFFFFFFFu, counts_mine), warp_dirt = __any_sync(0xFFFFFFFFu, dirty_mine);
+    if ((threadIdx.x & 31) == 0) {
+        counts[threadIdx.x >> 5] = warp_count;
+        dirts[threadIdx.x >> 5] = warp_dirt;
+    }
+    auto block_sum = [&](double s) {   // in thread 0; always in the same order
+        __syncthreads();
+        sums[threadIdx.x] = s;
+        __syncthreads();
+        for (int d = 128; d; d >>= 1) {
+            if (threadIdx.x < d) sums[threadIdx.x] += sums[threadIdx.x + d];
+            __syncthreads();
+        }
+        return sums[0];
+    };
+    const double block = a.reduction != RB200_REDUCE_NONE ? block_sum(mine) : 0.0;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int n = 0, any = 0;
+        for (int i = 0; i < 8; i++) {
+            n += counts[i];
+            any |= dirts[i];
+        }
+        if (n) atomicAdd(a.info, n);
+        if (any) atomicOr(a.info + 1, 1);
+        if (a.reduction != RB200_REDUCE_NONE) {
+            a.block_sums[blockIdx.x] = block;
+            __threadfence();
+            last_block = atomicAdd(a.info + 2, 1) == (int)gridDim.x - 1;
         }
     }
-    if (!a.last || a.reduction == RB200_REDUCE_NONE) return;
+    if (a.reduction == RB200_REDUCE_NONE) return;
     __syncthreads();
     if (!last_block) return;
-    // the block that finished last adds the others' sums, always in the same order
+    // the block that finished last adds the others' sums
     __threadfence();
     double s = 0.0;
     for (unsigned b = threadIdx.x; b < gridDim.x; b += 256) s += __ldcg(a.block_sums + b);
-    sums[threadIdx.x] = s;
-    __syncthreads();
-    for (int d = 128; d; d >>= 1) {
-        if (threadIdx.x < d) sums[threadIdx.x] += sums[threadIdx.x + d];
-        __syncthreads();
-    }
+    s = block_sum(s);
     if (threadIdx.x == 0) {
         const int count = atomicAdd(a.info, 0);
-        *a.loss = (float)(a.reduction == RB200_REDUCE_MEAN ? sums[0] / (double)max(1, count) : sums[0]);
+        *a.loss = (float)(a.reduction == RB200_REDUCE_MEAN ? s / (double)max(1, count) : s);
     }
+}
+
+constexpr int kMergeBlocks = 148 * 8;
+static int merge_launch(const MergeArgs& m, cudaStream_t stream, const char* what) {
+    // as many threads a row as there are parts for them to share, while the rows alone do not fill the GPU
+    const int subs = m.parts >= 8 ? 8 : m.parts >= 4 ? 4 : m.parts >= 2 && m.rows < 148 * 256 ? 2 : 1;
+    const long long blocks = ((long long)m.rows + 256 / subs - 1) / (256 / subs);
+    const unsigned grid = (unsigned)(blocks < kMergeBlocks ? blocks : kMergeBlocks);
+    if (subs == 8)
+        ce_merge_kernel<8><<<grid, 256, 0, stream>>>(m);
+    else if (subs == 4)
+        ce_merge_kernel<4><<<grid, 256, 0, stream>>>(m);
+    else if (subs == 2)
+        ce_merge_kernel<2><<<grid, 256, 0, stream>>>(m);
+    else
+        ce_merge_kernel<1><<<grid, 256, 0, stream>>>(m);
+    RB200_CHECK_LAUNCH(what);
+    return RB200_OK;
 }
 
 // ---- backward: per-row factors --------------------------------------------------------------------------------
@@ -254,7 +295,7 @@ static StatsPlan plan_stats(const rb200_linear_ce_params& p, const DeviceInfo& d
     s.part = (float*)c.take(s.part_bytes);
     s.zlabel = (float*)c.take((size_t)p.rows * sizeof(float));
     s.zsum = (float*)c.take((size_t)p.rows * sizeof(float));
-    s.block_sums = (double*)c.take((size_t)((p.rows + 31) / 32) * sizeof(double));
+    s.block_sums = (double*)c.take(kMergeBlocks * sizeof(double));
     s.bytes = c.used;
     return s;
 }
@@ -316,8 +357,7 @@ static int ce_forward(const rb200_linear_ce_params* p, cudaStream_t stream) {
         m.loss = p->loss;
         m.info = p->info;
         m.block_sums = s.block_sums;
-        ce_merge_kernel<<<(unsigned)((p->rows + 31) / 32), 256, 0, stream>>>(m);
-        RB200_CHECK_LAUNCH(what);
+        if ((rc = merge_launch(m, stream, what))) return rc;
     }
     return RB200_OK;
 }
