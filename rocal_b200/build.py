@@ -1,4 +1,5 @@
-"""Builds librocal_b200.so (CUDA kernels + C-ABI + host pipeline) in-tree for sm_100a.
+"""Builds librocal_b200.so (CUDA kernels + C-ABI + host pipeline) in-tree for sm_100a, and _head.so (the torch binding of the
+head operators, g++ against the installed torch).
 
     python -m rocal_b200.build [--force] [--verbose] [--debug-bounds]
 
@@ -37,6 +38,35 @@ def headers():
             glob.glob(os.path.join(ROOT, "include", "*.h")))
 
 
+HEAD_SRC = os.path.join(CSRC, "torch", "head.cpp")
+HEAD_LIB = os.path.join(PKG, "_head.so")
+
+
+def head_command():
+    """The compiler call that makes _head.so, the torch binding of the head operators. It calls the library through
+    addresses it is given at import, so it does not link to it."""
+    import sysconfig
+
+    import torch
+    root = os.path.join(os.path.dirname(torch.__file__))
+    cuda = os.path.dirname(os.path.dirname(NVCC))
+    includes = [os.path.join(ROOT, "include"), os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    libs = os.path.join(root, "lib")
+    return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-w", "-DTORCH_EXTENSION_NAME=_head",
+             "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)] + ["-isystem" + i for i in includes[1:]] +
+            ["-I" + includes[0], HEAD_SRC, "-o", HEAD_LIB, "-L" + libs, "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda",
+             "-Wl,-rpath," + libs])
+
+
+def build_head(force=False):
+    """Starts the build of _head.so where it is out of date; returns the process to wait for, or None."""
+    newest = max(os.path.getmtime(f) for f in (HEAD_SRC, os.path.join(ROOT, "include", "rb200_kernels.h"), __file__))
+    if not force and os.path.exists(HEAD_LIB) and os.path.getmtime(HEAD_LIB) > newest:
+        return None
+    return subprocess.Popen(head_command(), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+
+
 LIB_BOUNDS = os.path.join(PKG, "librocal_b200_bounds.so")
 
 
@@ -47,6 +77,7 @@ def build(force=False, verbose=False, debug_bounds=False):
     os.makedirs(obj_dir, exist_ok=True)
     hdr_time = max([os.path.getmtime(h) for h in headers()] + [os.path.getmtime(__file__)])
     objs, procs = [], []
+    head = None if debug_bounds else build_head(force)
     for src in sources():
         obj = os.path.join(obj_dir, os.path.basename(src) + ".o")
         objs.append(obj)
@@ -63,6 +94,11 @@ def build(force=False, verbose=False, debug_bounds=False):
         if p.returncode != 0:
             failed = True
             sys.stderr.write("nvcc failed for %s\n" % src)
+    if head is not None:
+        out, _ = head.communicate()
+        if head.returncode != 0:
+            failed = True
+            sys.stderr.write(out + "g++ failed for %s\n" % HEAD_SRC)
     if failed:
         raise RuntimeError("rocal_b200: nvcc build failed")
     if procs or force or not os.path.exists(lib):

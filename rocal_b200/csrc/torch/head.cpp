@@ -1,0 +1,508 @@
+// The head operators on torch tensors: argument checks, outputs and workspaces from torch's allocator, and the autograd
+// functions. Every computation is a call into librocal_b200 through the addresses that bind() gets, so that one
+// binding serves whichever build of the library the process has loaded. In C++ because a step of a small head is
+// shorter than the interpreter's work on its arguments, and because the backward pass then runs on autograd's threads
+// without the interpreter.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <array>
+#include <cstring>
+#include <optional>
+#include <stdexcept>
+#include <string>
+#include <vector>
+
+#include "rb200_kernels.h"
+
+namespace {
+
+using at::Tensor;
+using MaybeTensor = std::optional<Tensor>;
+
+// ---- the library ------------------------------------------------------------------------------------------
+struct Api {
+    decltype(&rb200k_linear_workspace_bytes) linear_bytes;
+    decltype(&rb200k_linear) linear;
+    decltype(&rb200k_linear_probe) linear_probe;
+    decltype(&rb200k_linear_backward_workspace_bytes) linear_backward_bytes;
+    decltype(&rb200k_linear_backward) linear_backward;
+    decltype(&rb200k_linear_ce_workspace_bytes) ce_bytes;
+    decltype(&rb200k_linear_ce) ce;
+    decltype(&rb200k_linear_ce_backward_workspace_bytes) ce_backward_bytes;
+    decltype(&rb200k_linear_ce_backward) ce_backward;
+    decltype(&rb200k_grad_clip_workspace_bytes) clip_bytes;
+    decltype(&rb200k_grad_clip) clip;
+    decltype(&rb200k_last_error) last_error;
+} api;
+
+// A library call that failed; Python sees it as rocal_b200.Rb200Error.
+struct LibraryError : std::runtime_error {
+    using std::runtime_error::runtime_error;
+};
+PyObject* library_error = nullptr;
+
+void bind(const std::vector<uintptr_t>& a, pybind11::object error) {
+    TORCH_CHECK(a.size() * sizeof(uintptr_t) == sizeof(Api), "the binding and the library do not go together");
+    memcpy(&api, a.data(), sizeof(Api));
+    library_error = error.release().ptr();
+}
+
+void check(int rc, const char* what) {
+    if (rc) throw LibraryError(c10::str(what, " failed (", rc, "): ", api.last_error()));
+}
+
+// ---- arguments ----------------------------------------------------------------------------------------------
+int head_dtype(const Tensor& x) {
+    TORCH_CHECK_VALUE(x.is_cuda(), "x is on ", x.device(), ": the head operators run on a GPU");
+    TORCH_CHECK_VALUE(x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16, "x is ", x.scalar_type(),
+                      ": the head operators take float16 and bfloat16");
+    return x.scalar_type() == at::kHalf ? RB200_FP16 : RB200_BF16;
+}
+
+void same_kind(const Tensor& t, const char* name, const Tensor& like) {
+    TORCH_CHECK_VALUE(t.scalar_type() == like.scalar_type() && t.device() == like.device(), name, " is ", t.scalar_type(), " on ", t.device(),
+                      ", the input is ", like.scalar_type(), " on ", like.device());
+}
+
+// Rows contiguous and not overlapping.
+bool has_rows(const Tensor& t) {
+    return (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));
+}
+int64_t pitch(const Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
+
+// A matrix of the input's type and device, its rows contiguous (copied if need be).
+Tensor matrix(const Tensor& t, const char* name, const Tensor& like, int64_t rows, int64_t cols) {
+    TORCH_CHECK_VALUE(t.dim() == 2, name, " has ", t.dim(), " dimensions, a matrix is needed");
+    same_kind(t, name, like);
+    TORCH_CHECK_VALUE(cols < 0 || t.size(1) == cols, name, " has ", t.size(1), " columns, ", cols, " are needed");
+    TORCH_CHECK_VALUE(rows < 0 || t.size(0) == rows, name, " has ", t.size(0), " rows, ", rows, " are needed");
+    return has_rows(t) ? t : t.contiguous();
+}
+Tensor vector(const Tensor& t, const char* name, const Tensor& like, int64_t n) {
+    TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == n, name, " has shape ", t.sizes(), ", (", n, ",) is needed");
+    same_kind(t, name, like);
+    return t.contiguous();
+}
+bool given(const MaybeTensor& t) { return t.has_value() && t->defined(); }
+Tensor or_undefined(const MaybeTensor& t) { return given(t) ? *t : Tensor(); }
+MaybeTensor or_absent(const Tensor& t) { return t.defined() ? MaybeTensor(t) : std::nullopt; }
+
+Tensor workspace(uint64_t bytes, const Tensor& like) {
+    return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
+}
+void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+int32_t* status_word(const MaybeTensor& status, const Tensor& like) {
+    if (!given(status)) return nullptr;
+    TORCH_CHECK_VALUE(status->scalar_type() == at::kInt && status->device() == like.device() && status->numel() >= 1, "status has to be an int32 tensor on ",
+                      like.device());
+    return status->data_ptr<int32_t>();
+}
+void* stream_of(const Tensor& x) { return c10::cuda::getCurrentCUDAStream(x.device().index()).stream(); }
+
+int activation(const std::string& name) {
+    if (name == "none") return RB200_ACT_NONE;
+    if (name == "relu") return RB200_ACT_RELU;
+    if (name == "gelu") return RB200_ACT_GELU;
+    if (name == "silu") return RB200_ACT_SILU;
+    TORCH_CHECK_VALUE(false, "activation '", name, "': one of none, relu, gelu, silu is needed");
+}
+int reduction(const std::string& name) {
+    if (name == "none") return RB200_REDUCE_NONE;
+    if (name == "mean") return RB200_REDUCE_MEAN;
+    if (name == "sum") return RB200_REDUCE_SUM;
+    TORCH_CHECK_VALUE(false, "reduction '", name, "': one of none, mean, sum is needed");
+}
+
+// ---- linear -----------------------------------------------------------------------------------------------
+// x, weight and residual are matrices, bias a vector.
+Tensor linear_run(const Tensor& x_, const Tensor& weight_, const Tensor& bias_, const Tensor& residual_, int act, Tensor out, Tensor* preact,
+                  const MaybeTensor& status, std::optional<std::pair<uint64_t, int>> probe) {
+    rb200_linear_params p = {};
+    p.dtype = head_dtype(x_);
+    c10::cuda::CUDAGuard guard(x_.device());
+    const Tensor x = matrix(x_, "x", x_, -1, -1), weight = matrix(weight_, "weight", x, -1, x.size(1));
+    const int64_t n = x.size(0), m = weight.size(0);
+    p.activation = act;
+    p.rows = n;
+    p.in_features = x.size(1);
+    p.out_features = m;
+    p.x = x.data_ptr();
+    p.ldx = pitch(x);
+    p.weight = weight.data_ptr();
+    p.ldw = pitch(weight);
+    Tensor bias, residual;
+    if (bias_.defined()) {
+        bias = vector(bias_, "bias", x, m);
+        p.bias = bias.data_ptr();
+    }
+    if (residual_.defined()) {
+        residual = matrix(residual_, "residual", x, -1, m);
+        const int64_t r = residual.size(0);
+        TORCH_CHECK_VALUE(r > 0 ? n % r == 0 : n == 0, "residual has ", r, " rows, which do not divide the ", n, " rows of x");
+        p.residual = residual.data_ptr();
+        p.ldr = pitch(residual);
+        p.residual_rows = r;
+    }
+    if (out.defined()) {
+        TORCH_CHECK_VALUE(out.dim() == 2 && out.size(0) == n && out.size(1) == m && has_rows(out), "out has shape ", out.sizes(), ", strides ",
+                          out.strides(), "; (", n, ", ", m, ") with contiguous rows is needed");
+        same_kind(out, "out", x);
+    } else {
+        out = at::empty({n, m}, x.options());
+    }
+    p.out = out.data_ptr();
+    p.ldo = pitch(out);
+    if (preact) {
+        *preact = at::empty({n, m}, x.options());
+        p.preact = preact->data_ptr();
+        p.ldp = m;
+    }
+    if (n == 0) return out;
+    p.status = status_word(status, x);
+    const uint64_t need = api.linear_bytes(&p);
+    const Tensor ws = workspace(need, x);
+    p.workspace = data(ws);
+    p.workspace_bytes = need;
+    if (probe)
+        check(api.linear_probe(&p, stream_of(x), probe->first, probe->second), "rb200k_linear_probe");
+    else
+        check(api.linear(&p, stream_of(x)), "rb200k_linear");
+    return out;
+}
+
+std::vector<Tensor> linear_backward_run(const Tensor& dout_, const Tensor& x_, const Tensor& weight_, const Tensor& preact_, int act,
+                                        int64_t residual_rows, std::array<bool, 4> need, const MaybeTensor& status) {
+    rb200_linear_backward_params p = {};
+    p.dtype = head_dtype(x_);
+    c10::cuda::CUDAGuard guard(x_.device());
+    const Tensor x = matrix(x_, "x", x_, -1, -1), weight = matrix(weight_, "weight", x, -1, x.size(1));
+    const int64_t n = x.size(0), k = x.size(1), m = weight.size(0);
+    const Tensor dout = matrix(dout_, "dout", x, n, m);
+    p.activation = act;
+    p.rows = n;
+    p.in_features = k;
+    p.out_features = m;
+    p.dout = dout.data_ptr();
+    p.lddo = pitch(dout);
+    p.x = x.data_ptr();
+    p.ldx = pitch(x);
+    p.weight = weight.data_ptr();
+    p.ldw = pitch(weight);
+    Tensor preact;
+    if (act != RB200_ACT_NONE && (need[0] || need[1] || need[2])) {
+        TORCH_CHECK_VALUE(preact_.defined(), "the backward pass of an activation needs preact");
+        preact = matrix(preact_, "preact", x, n, m);
+        p.preact = preact.data_ptr();
+        p.ldp = pitch(preact);
+    }
+    std::vector<Tensor> g(4);
+    if (need[0]) p.dx = (g[0] = at::empty({n, k}, x.options())).data_ptr();
+    if (need[1]) p.dweight = (g[1] = at::empty({m, k}, x.options())).data_ptr();
+    if (need[2]) p.dbias = (g[2] = at::empty({m}, x.options())).data_ptr();
+    if (need[3]) {
+        TORCH_CHECK_VALUE(residual_rows > 0 && n % residual_rows == 0, "residual_rows ", residual_rows, " does not divide the ", n, " rows");
+        p.residual_rows = residual_rows;
+        p.dresidual = (g[3] = at::empty({residual_rows, m}, x.options())).data_ptr();
+    }
+    p.lddx = p.lddw = k;
+    p.lddr = m;
+    p.status = status_word(status, x);
+    const uint64_t bytes = api.linear_backward_bytes(&p);
+    const Tensor ws = workspace(bytes, x);
+    p.workspace = data(ws);
+    p.workspace_bytes = bytes;
+    check(api.linear_backward(&p, stream_of(x)), "rb200k_linear_backward");
+    return g;
+}
+
+constexpr const char* kOnce = " is differentiable once: create_graph is not supported";
+
+struct Linear : torch::autograd::Function<Linear> {
+    // Absent tensors are empty optionals here: autograd numbers the inputs that are there.
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight, const MaybeTensor& bias_,
+                          const MaybeTensor& residual_, int64_t act) {
+        Tensor preact, bias = or_undefined(bias_), residual = or_undefined(residual_);
+        const Tensor y = linear_run(x, weight, bias, residual, (int)act, Tensor(), act != RB200_ACT_NONE ? &preact : nullptr, {}, {});
+        ctx->save_for_backward({x, weight, preact});
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["rows"] = residual.defined() ? residual.size(0) : (int64_t)0;
+        ctx->saved_data["bias"] = bias.defined();
+        return y;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "linear", kOnce);
+        const auto saved = ctx->get_saved_variables();
+        const Tensor& dout = grads[0];
+        const int64_t rows = ctx->saved_data["rows"].toInt();
+        if (!dout.defined()) return torch::autograd::variable_list(5);
+        const bool has_bias = ctx->saved_data["bias"].toBool();
+        std::array<bool, 4> need = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), has_bias && ctx->needs_input_grad(2),
+                                    rows > 0 && ctx->needs_input_grad(has_bias ? 3 : 2)};
+        const bool whole = need[3] && rows == saved[0].size(0);   // nothing is summed: the gradient goes through as it is
+        if (whole) need[3] = false;
+        std::vector<Tensor> g(4);
+        if (need[0] || need[1] || need[2] || need[3])
+            g = linear_backward_run(dout, saved[0], saved[1], saved[2], (int)ctx->saved_data["act"].toInt(), rows, need, {});
+        return {g[0], g[1], g[2], whole ? dout : g[3], Tensor()};
+    }
+};
+
+bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+Tensor linear(const Tensor& x, const Tensor& weight, const MaybeTensor& bias_, const MaybeTensor& residual_, const std::string& act_name) {
+    const int act = activation(act_name);
+    TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1), "x ", x.sizes(), " does not go with weight ", weight.sizes());
+    const Tensor bias = or_undefined(bias_);
+    Tensor residual = or_undefined(residual_);
+    const int64_t m = weight.size(0);
+    std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = m;
+    if (residual.defined()) {
+        const int64_t d = residual.dim();
+        const bool tail = d >= 1 && d <= (int64_t)shape.size() && std::equal(residual.sizes().begin(), residual.sizes().end(), shape.end() - d);
+        TORCH_CHECK_VALUE(tail || (d == 2 && x.dim() == 2 && residual.size(1) == m), "residual ", residual.sizes(),
+                          " is not a tail of the result's shape ", at::IntArrayRef(shape));
+        if (d != 2) residual = residual.reshape({-1, m});
+    }
+    const bool flat = x.dim() == 2;
+    const Tensor x2 = flat ? x : x.reshape({-1, x.size(-1)});
+    Tensor y;
+    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias) || wants_grad(residual)))
+        y = Linear::apply(x2, weight, or_absent(bias), or_absent(residual), (int64_t)act);
+    else
+        y = linear_run(x2, weight, bias, residual, act, Tensor(), nullptr, {}, {});
+    return flat ? y : y.reshape(shape);
+}
+
+// ---- linear cross entropy -----------------------------------------------------------------------------------
+struct CeArgs {
+    rb200_linear_ce_params p = {};
+    Tensor x, weight, labels, bias;   // what the parameters point into
+};
+CeArgs ce_args(const Tensor& x, const Tensor& weight, const Tensor& labels, const Tensor& bias, int64_t ignore_index, double smoothing, int reduce) {
+    CeArgs a;
+    a.p.dtype = head_dtype(x);
+    a.x = matrix(x, "x", x, -1, -1);
+    a.weight = matrix(weight, "weight", x, -1, a.x.size(1));
+    a.p.reduction = reduce;
+    a.p.rows = a.x.size(0);
+    a.p.features = a.x.size(1);
+    a.p.classes = a.weight.size(0);
+    TORCH_CHECK_VALUE(labels.dim() == 1 && labels.size(0) == a.p.rows && labels.device() == x.device() &&
+                          (labels.scalar_type() == at::kInt || labels.scalar_type() == at::kLong),
+                      "labels are ", labels.scalar_type(), " ", labels.sizes(), " on ", labels.device(), ", needed: int32 or int64 of shape (",
+                      a.p.rows, ",) on ", x.device());
+    TORCH_CHECK_VALUE(smoothing >= 0.0 && smoothing <= 1.0, "label_smoothing ", smoothing, " outside [0, 1]");
+    a.labels = labels.contiguous();
+    a.p.x = a.x.data_ptr();
+    a.p.ldx = pitch(a.x);
+    a.p.weight = a.weight.data_ptr();
+    a.p.ldw = pitch(a.weight);
+    if (bias.defined()) {
+        a.bias = vector(bias, "bias", x, a.p.classes);
+        a.p.bias = a.bias.data_ptr();
+    }
+    a.p.labels = a.labels.data_ptr();
+    a.p.label_bytes = labels.scalar_type() == at::kInt ? 4 : 8;
+    a.p.label_smoothing = (float)smoothing;
+    a.p.ignore_index = ignore_index;
+    return a;
+}
+
+// (loss, stats, info)
+std::array<Tensor, 3> ce_run(const Tensor& x, const Tensor& weight, const Tensor& labels, const Tensor& bias, int64_t ignore_index, double smoothing,
+                             int reduce, const MaybeTensor& status) {
+    head_dtype(x);
+    c10::cuda::CUDAGuard guard(x.device());
+    CeArgs a = ce_args(x, weight, labels, bias, ignore_index, smoothing, reduce);
+    const auto fp32 = x.options().dtype(at::kFloat);
+    const Tensor loss = reduce == RB200_REDUCE_NONE ? at::empty({a.p.rows}, fp32) : at::empty({}, fp32);
+    const Tensor stats = at::empty({2, a.p.rows}, fp32), info = at::empty({4}, x.options().dtype(at::kInt));
+    a.p.loss = loss.data_ptr<float>();
+    a.p.stats = stats.data_ptr<float>();
+    a.p.info = info.data_ptr<int32_t>();
+    a.p.status = status_word(status, x);
+    const uint64_t bytes = api.ce_bytes(&a.p);
+    const Tensor ws = workspace(bytes, x);
+    a.p.workspace = data(ws);
+    a.p.workspace_bytes = bytes;
+    check(api.ce(&a.p, stream_of(x)), "rb200k_linear_ce");
+    return {loss, stats, info};
+}
+
+std::vector<Tensor> ce_backward_run(const Tensor& dloss_, const Tensor& x, const Tensor& weight, const Tensor& labels, const Tensor& stats,
+                                    const Tensor& info, const Tensor& bias, int64_t ignore_index, double smoothing, int reduce,
+                                    std::array<bool, 3> need, const MaybeTensor& status) {
+    head_dtype(x);
+    c10::cuda::CUDAGuard guard(x.device());
+    CeArgs a = ce_args(x, weight, labels, bias, ignore_index, smoothing, reduce);
+    const int64_t n = a.p.rows, k = a.p.features, v = a.p.classes;
+    TORCH_CHECK_VALUE(dloss_.scalar_type() == at::kFloat && dloss_.device() == x.device() &&
+                          (reduce == RB200_REDUCE_NONE ? dloss_.dim() == 1 && dloss_.size(0) == n : dloss_.dim() == 0),
+                      "dloss is ", dloss_.scalar_type(), " ", dloss_.sizes(), " on ", dloss_.device(), ", it has to be like the loss");
+    TORCH_CHECK_VALUE(stats.dim() == 2 && stats.size(0) == 2 && stats.size(1) == n && stats.scalar_type() == at::kFloat && stats.is_contiguous() &&
+                          stats.device() == x.device() && info.dim() == 1 && info.size(0) == 4 && info.scalar_type() == at::kInt &&
+                          info.is_contiguous() && info.device() == x.device(),
+                      "stats and info are not those of this forward pass");
+    const Tensor dloss = dloss_.contiguous();
+    std::vector<Tensor> g(3);
+    if (need[0]) a.p.dx = (g[0] = at::empty({n, k}, x.options())).data_ptr();
+    if (need[1]) a.p.dweight = (g[1] = at::empty({v, k}, x.options())).data_ptr();
+    if (need[2]) a.p.dbias = (g[2] = at::empty({v}, x.options())).data_ptr();
+    a.p.lddx = a.p.lddw = k;
+    a.p.dloss = dloss.data_ptr<float>();
+    a.p.stats = stats.data_ptr<float>();
+    a.p.info = info.data_ptr<int32_t>();
+    a.p.status = status_word(status, x);
+    const uint64_t bytes = api.ce_backward_bytes(&a.p);
+    const Tensor ws = workspace(bytes, x);
+    a.p.workspace = data(ws);
+    a.p.workspace_bytes = bytes;
+    check(api.ce_backward(&a.p, stream_of(x)), "rb200k_linear_ce_backward");
+    return g;
+}
+
+struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& labels,
+                          const MaybeTensor& bias_, int64_t ignore_index, double smoothing, int64_t reduce) {
+        const Tensor bias = or_undefined(bias_);
+        const auto r = ce_run(x, weight, labels, bias, ignore_index, smoothing, (int)reduce, {});
+        ctx->save_for_backward({x, weight, labels, bias, r[1], r[2]});
+        ctx->saved_data["ignore"] = ignore_index;
+        ctx->saved_data["smoothing"] = smoothing;
+        ctx->saved_data["reduce"] = reduce;
+        return r[0];
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "linear_cross_entropy", kOnce);
+        if (!grads[0].defined()) return torch::autograd::variable_list(7);
+        const auto s = ctx->get_saved_variables();
+        const auto g = ce_backward_run(grads[0], s[0], s[1], s[2], s[4], s[5], s[3], ctx->saved_data["ignore"].toInt(),
+                                       ctx->saved_data["smoothing"].toDouble(), (int)ctx->saved_data["reduce"].toInt(),
+                                       {ctx->needs_input_grad(0), ctx->needs_input_grad(1), s[3].defined() && ctx->needs_input_grad(3)}, {});
+        return {g[0], g[1], Tensor(), g[2], Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor& labels, const MaybeTensor& bias_, int64_t ignore_index,
+                            double smoothing, const std::string& reduce_name) {
+    const int reduce = reduction(reduce_name);
+    TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1) && labels.dim() == x.dim() - 1 &&
+                          std::equal(labels.sizes().begin(), labels.sizes().end(), x.sizes().begin()),
+                      "x ", x.sizes(), ", weight ", weight.sizes(), " and labels ", labels.sizes(), " do not go together");
+    const Tensor bias = or_undefined(bias_);
+    const bool flat = x.dim() == 2;
+    const Tensor x2 = flat ? x : x.reshape({-1, x.size(-1)}), l1 = flat ? labels : labels.reshape({-1});
+    Tensor loss;
+    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias)))
+        loss = LinearCrossEntropy::apply(x2, weight, l1, or_absent(bias), ignore_index, smoothing, (int64_t)reduce);
+    else
+        loss = ce_run(x2, weight, l1, bias, ignore_index, smoothing, reduce, {})[0];
+    return flat || reduce != RB200_REDUCE_NONE ? loss : loss.reshape(labels.sizes());
+}
+
+// ---- gradient norm and clipping -------------------------------------------------------------------------------
+int grad_dtype(const Tensor& t, const Tensor& first) {
+    TORCH_CHECK_VALUE(t.layout() == at::kStrided && t.device() == first.device(), "a gradient is ", t.layout(), " on ", t.device(),
+                      "; strided tensors on ", first.device(), " are needed");
+    switch (t.scalar_type()) {
+        case at::kFloat: return RB200_FP32;
+        case at::kHalf: return RB200_FP16;
+        case at::kBFloat16: return RB200_BF16;
+        default: TORCH_CHECK_VALUE(false, "a gradient is ", t.scalar_type(), "; float32, float16 or bfloat16 is needed");
+    }
+}
+
+Tensor grad_clip(const std::vector<Tensor>& grads, double max_norm, const std::optional<std::vector<Tensor>>& out, double inv_scale) {
+    TORCH_CHECK_VALUE(!grads.empty(), "no gradients");
+    TORCH_CHECK_VALUE(grads[0].is_cuda(), "the gradients are on ", grads[0].device(), ": the head operators run on a GPU");
+    TORCH_CHECK_VALUE(!out || out->size() == grads.size(), out ? out->size() : 0, " outputs for ", grads.size(), " gradients");
+    TORCH_CHECK_VALUE(max_norm >= 0 && inv_scale > 0, "max_norm ", max_norm, ", inv_scale ", inv_scale);
+    at::NoGradGuard no_grad;
+    c10::cuda::CUDAGuard guard(grads[0].device());
+    const size_t n = grads.size();
+    std::vector<rb200_grad_tensor> table(n);
+    std::vector<Tensor> held;                              // dense copies of tensors with gaps
+    std::vector<std::pair<Tensor, Tensor>> back;           // (the tensor with gaps, its dense result)
+    for (size_t i = 0; i < n; i++) {
+        const Tensor& g = grads[i];
+        const Tensor& o = out ? (*out)[i] : g;
+        rb200_grad_tensor& t = table[i];
+        t.grad_dtype = grad_dtype(g, grads[0]);
+        t.out_dtype = out ? grad_dtype(o, grads[0]) : t.grad_dtype;
+        t.count = g.numel();
+        TORCH_CHECK_VALUE(o.numel() == t.count, "an output has ", o.numel(), " elements for a gradient of ", t.count);
+        TORCH_CHECK_VALUE(t.out_dtype == t.grad_dtype || t.out_dtype == RB200_FP32, "an output is ", o.scalar_type(), " for a gradient ", g.scalar_type());
+        const bool plain = g.is_contiguous() && (!out || o.is_contiguous());
+        if (plain || (g.is_non_overlapping_and_dense() && (!out || (o.sizes() == g.sizes() && o.strides() == g.strides())))) {
+            t.grad = g.data_ptr();
+            t.out = o.data_ptr();
+            continue;
+        }
+        TORCH_CHECK_VALUE(o.sizes() == g.sizes(), "an output has shape ", o.sizes(), " for a gradient ", g.sizes());
+        Tensor dense = g.contiguous(), result = !out ? dense : o.is_contiguous() ? o : at::empty(o.sizes(), o.options());
+        if (!result.is_same(o)) back.emplace_back(o, result);
+        t.grad = dense.data_ptr();
+        t.out = result.data_ptr();
+        held.push_back(std::move(dense));
+    }
+    const Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+    const uint64_t bytes = api.clip_bytes((int)n);
+    const Tensor ws = workspace(bytes, grads[0]);
+    check(api.clip(table.data(), (int)n, (float)max_norm, (float)inv_scale, norm.data_ptr<float>(), data(ws), bytes, stream_of(grads[0])),
+          "rb200k_grad_clip");
+    for (auto& b : back) b.first.copy_(b.second);
+    return norm;
+}
+
+// ---- single launches (rocal_b200.kernels) -----------------------------------------------------------------------
+std::pair<Tensor, MaybeTensor> linear_raw(const Tensor& x, const Tensor& weight, const MaybeTensor& bias, const MaybeTensor& residual,
+                                          const std::string& act, const MaybeTensor& out, bool want_preact, const MaybeTensor& status,
+                                          std::optional<std::pair<uint64_t, int>> probe) {
+    Tensor preact;
+    Tensor y = linear_run(x, weight, or_undefined(bias), or_undefined(residual), activation(act), or_undefined(out), want_preact ? &preact : nullptr,
+                          status, probe);
+    return {y, want_preact ? MaybeTensor(preact) : std::nullopt};
+}
+template <typename G>
+std::vector<MaybeTensor> listed(const G& g) {
+    std::vector<MaybeTensor> r;
+    for (const Tensor& t : g) r.push_back(t.defined() ? MaybeTensor(t) : std::nullopt);
+    return r;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_head, m) {
+    namespace py = pybind11;
+    py::register_local_exception_translator([](std::exception_ptr p) {
+        try {
+            if (p) std::rethrow_exception(p);
+        } catch (const LibraryError& e) {
+            PyErr_SetString(library_error ? library_error : PyExc_RuntimeError, e.what());
+        }
+    });
+    m.def("bind", &bind);
+    m.def("linear", &linear);
+    m.def("linear_cross_entropy", &linear_cross_entropy);
+    m.def("grad_clip", &grad_clip);
+    m.def("linear_raw", &linear_raw);
+    m.def("linear_backward_raw", [](const Tensor& dout, const Tensor& x, const Tensor& weight, const MaybeTensor& preact, const std::string& act,
+                                    int64_t residual_rows, std::array<bool, 4> need, const MaybeTensor& status) {
+        return listed(linear_backward_run(dout, x, weight, or_undefined(preact), activation(act), residual_rows, need, status));
+    });
+    m.def("linear_ce_raw", [](const Tensor& x, const Tensor& weight, const Tensor& labels, const MaybeTensor& bias, int64_t ignore_index,
+                              double smoothing, const std::string& reduce, const MaybeTensor& status) {
+        return listed(ce_run(x, weight, labels, or_undefined(bias), ignore_index, smoothing, reduction(reduce), status));
+    });
+    m.def("linear_ce_backward_raw", [](const Tensor& dloss, const Tensor& x, const Tensor& weight, const Tensor& labels, const Tensor& stats,
+                                       const Tensor& info, const MaybeTensor& bias, int64_t ignore_index, double smoothing,
+                                       const std::string& reduce, std::array<bool, 3> need, const MaybeTensor& status) {
+        return listed(ce_backward_run(dloss, x, weight, labels, stats, info, or_undefined(bias), ignore_index, smoothing, reduction(reduce), need,
+                                      status));
+    });
+}

@@ -10,9 +10,7 @@ import numpy as np
 import torch
 
 from . import tables as T
-from ._lib import (BoxEncoderParams, BoxMatcherParams, LinearBackwardParams, LinearCeParams,
-                   LinearParams, NormalizeParams, PointwiseParams,
-                   ResampleParams, WarpParams, check, lib)
+from ._lib import (BoxEncoderParams, BoxMatcherParams, NormalizeParams, PointwiseParams, ResampleParams, WarpParams, check, lib)
 
 _TORCH_DTYPE = {T.FP32: torch.float32, T.FP16: torch.float16, T.UINT8: torch.uint8}
 
@@ -241,297 +239,67 @@ def transpose(arena, samples, perm, out_dims, out=None, d_samples=None, stream=N
 
 
 # ---- head operators -----------------------------------------------------------------------------
-# Tensors may live on any device; the call runs there, on `stream` or that device's current stream, and takes its
-# workspace from torch's allocator on that stream.
-_HEAD_DTYPE = {torch.float16: T.FP16, torch.bfloat16: T.BF16}
+# Tensors may live on any device; a call runs there, on `stream` or that device's current stream, and takes its workspace from
+# torch's allocator on that stream. Arguments are checked in the binding (ValueError); a failed library call is Rb200Error.
 
 
 class _on:
-    """The device and stream of a head operator's launch."""
+    """The stream of a head operator's launch."""
 
-    def __init__(self, device, stream):
-        self.device, self.stream = device, stream
-        self.away = device.index != torch.cuda.current_device()
+    def __init__(self, stream, x):
+        if stream is not None and stream.device != x.device:
+            raise ValueError("the stream is on %s, the tensors are on %s" % (stream.device, x.device))
+        self.guard = torch.cuda.stream(stream)
 
     def __enter__(self):
-        self.guards = []
-        if self.away:
-            self.guards.append(torch.cuda.device(self.device))
-        if self.stream is not None:
-            if self.stream.device != self.device:
-                raise ValueError("the stream is on %s, the tensors are on %s" % (self.stream.device, self.device))
-            self.guards.append(torch.cuda.stream(self.stream))
-        for g in self.guards:
-            g.__enter__()
-        s = self.stream if self.stream is not None else torch.cuda.current_stream(self.device)
-        return s.cuda_stream
+        self.guard.__enter__()
 
     def __exit__(self, *exc):
-        for g in reversed(self.guards):
-            g.__exit__(*exc)
-        return False
-
-
-def _matrix(t, name, like, cols=None):
-    """A 2-d tensor on the device and of the type of `like`, its rows contiguous and not overlapping (copied if need be)."""
-    if t.dim() != 2:
-        raise ValueError("%s has %d dimensions, a matrix is needed" % (name, t.dim()))
-    if t.dtype != like.dtype or t.device != like.device:
-        raise ValueError("%s is %s on %s, the input is %s on %s" % (name, t.dtype, t.device, like.dtype, like.device))
-    if cols is not None and t.shape[1] != cols:
-        raise ValueError("%s has %d columns, %d are needed" % (name, t.shape[1], cols))
-    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
-    return t
-
-
-def _vector(t, name, like, n):
-    if t.dim() != 1 or t.shape[0] != n:
-        raise ValueError("%s has shape %s, (%d,) is needed" % (name, tuple(t.shape), n))
-    if t.dtype != like.dtype or t.device != like.device:
-        raise ValueError("%s is %s on %s, the input is %s on %s" % (name, t.dtype, t.device, like.dtype, like.device))
-    return t.contiguous()
-
-
-def _head_input(x, weight):
-    """Element type of a head operator and its (x, weight) as matrices."""
-    if not x.is_cuda:
-        raise ValueError("x is on %s: the head operators run on a GPU" % x.device)
-    if x.dtype not in _HEAD_DTYPE:
-        raise ValueError("x is %s: the head operators take float16 and bfloat16" % x.dtype)
-    x = _matrix(x, "x", x)
-    return _HEAD_DTYPE[x.dtype], x, _matrix(weight, "weight", x, x.shape[1])
-
-
-def _output(out, name, shape, like):
-    if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
-    if tuple(out.shape) != tuple(shape) or out.dtype != like.dtype or out.device != like.device:
-        raise ValueError("%s is %s %s on %s, needed: %s %s on %s" % (name, tuple(out.shape), out.dtype, out.device, tuple(shape),
-                                                                    like.dtype, like.device))
-    if out.dim() == 2 and ((out.stride(1) != 1 and out.shape[1] > 1) or (out.shape[0] > 1 and out.stride(0) < out.shape[1])):
-        raise ValueError("%s needs contiguous rows that do not overlap" % name)
-    return out
-
-
-def _workspace(p, sizer, device):
-    need = sizer(ctypes.byref(p))
-    if not need:
-        return None
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
-    p.workspace, p.workspace_bytes = ws.data_ptr(), need
-    return ws
-
-
-def _activation(name):
-    if name not in T.ACTIVATIONS:
-        raise ValueError("activation %r: one of %s is needed" % (name, ", ".join(T.ACTIVATIONS)))
-    return T.ACTIVATIONS[name]
+        self.guard.__exit__(*exc)
 
 
 def linear(x, weight, bias=None, residual=None, activation="none", out=None, want_preact=False, stream=None, status=None, probe=None):
     """rb200k_linear: act(x weight^T + bias) + residual for x [n, k], weight [m, k], bias [m], residual [r, m] with r a
     divisor of n (row i takes residual row i % r), all float16 or all bfloat16. Returns [n, m], with want_preact also
     the value before the activation. probe=(wait_cycles, skip_block) launches through rb200k_linear_probe."""
-    dtype, x, weight = _head_input(x, weight)
-    n, k = x.shape
-    m = weight.shape[0]
-    act = _activation(activation)
-    if bias is not None:
-        bias = _vector(bias, "bias", x, m)
-    if residual is not None:
-        residual = _matrix(residual, "residual", x, m)
-        if residual.shape[0] == 0 and n or residual.shape[0] and n % residual.shape[0]:
-            raise ValueError("residual has %d rows, which do not divide the %d rows of x" % (residual.shape[0], n))
-    with _on(x.device, stream) as s:
-        out = _output(out, "out", (n, m), x)
-        pre = torch.empty((n, m), dtype=x.dtype, device=x.device) if want_preact else None
-        if n:
-            p = LinearParams(dtype, act, n, k, m, x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0))
-            p.out, p.ldo = out.data_ptr(), out.stride(0)
-            if bias is not None:
-                p.bias = bias.data_ptr()
-            if residual is not None:
-                p.residual, p.ldr, p.residual_rows = residual.data_ptr(), residual.stride(0), residual.shape[0]
-            if pre is not None:
-                p.preact, p.ldp = pre.data_ptr(), m
-            if status is not None:
-                p.status = status.data_ptr()
-            ws = _workspace(p, lib.rb200k_linear_workspace_bytes, x.device)  # noqa: F841  (alive until the launch)
-            if probe is not None:
-                check(lib.rb200k_linear_probe(ctypes.byref(p), s, int(probe[0]), int(probe[1])), "rb200k_linear_probe")
-            else:
-                check(lib.rb200k_linear(ctypes.byref(p), s), "rb200k_linear")
-    return (out, pre) if want_preact else out
+    from ._torch import head
+    with _on(stream, x):
+        y, preact = head.linear_raw(x, weight, bias, residual, activation, out, want_preact, status, probe)
+    return (y, preact) if want_preact else y
 
 
 def linear_backward(dout, x, weight, preact=None, activation="none", residual_rows=0, need=(True, True, True, True), stream=None,
                     status=None):
     """rb200k_linear_backward: (dx, dweight, dbias, dresidual), None where `need` is false. dresidual takes residual_rows."""
-    dtype, x, weight = _head_input(x, weight)
-    n, k = x.shape
-    m = weight.shape[0]
-    act = _activation(activation)
-    dout = _matrix(dout, "dout", x, m)
-    if dout.shape[0] != n:
-        raise ValueError("dout has %d rows, x has %d" % (dout.shape[0], n))
-    if act and (need[0] or need[1] or need[2]):
-        if preact is None:
-            raise ValueError("the backward pass of an activation needs preact")
-        preact = _matrix(preact, "preact", x, m)
-        if preact.shape[0] != n:
-            raise ValueError("preact has %d rows, x has %d" % (preact.shape[0], n))
-    if need[3] and (residual_rows < 1 or n % residual_rows):
-        raise ValueError("residual_rows %d does not divide the %d rows" % (residual_rows, n))
-    shapes = ((n, k), (m, k), (m,), (residual_rows, m))
-    with _on(x.device, stream) as s:
-        grads = [torch.empty(shape, dtype=x.dtype, device=x.device) if want else None for shape, want in zip(shapes, need)]
-        dx, dw, db, dr = grads
-        p = LinearBackwardParams(dtype, act, n, k, m, dout.data_ptr(), dout.stride(0), x.data_ptr(), x.stride(0), weight.data_ptr(),
-                                 weight.stride(0))
-        if act and preact is not None:
-            p.preact, p.ldp = preact.data_ptr(), preact.stride(0)
-        if dx is not None:
-            p.dx, p.lddx = dx.data_ptr(), k
-        if dw is not None:
-            p.dweight, p.lddw = dw.data_ptr(), k
-        if db is not None:
-            p.dbias = db.data_ptr()
-        if dr is not None:
-            p.dresidual, p.lddr, p.residual_rows = dr.data_ptr(), m, residual_rows
-        if status is not None:
-            p.status = status.data_ptr()
-        ws = _workspace(p, lib.rb200k_linear_backward_workspace_bytes, x.device)  # noqa: F841
-        check(lib.rb200k_linear_backward(ctypes.byref(p), s), "rb200k_linear_backward")
-    return tuple(grads)
-
-
-def _ce_params(x, weight, labels, bias, ignore_index, label_smoothing, reduction):
-    """(parameter block, tensors that it points into) of a linear cross entropy."""
-    dtype, x, weight = _head_input(x, weight)
-    n, k = x.shape
-    v = weight.shape[0]
-    if reduction not in T.REDUCTIONS:
-        raise ValueError("reduction %r: one of %s is needed" % (reduction, ", ".join(T.REDUCTIONS)))
-    if labels.dim() != 1 or labels.shape[0] != n or labels.device != x.device or labels.dtype not in (torch.int32, torch.int64):
-        raise ValueError("labels are %s %s on %s, needed: int32 or int64 of shape (%d,) on %s"
-                         % (labels.dtype, tuple(labels.shape), labels.device, n, x.device))
-    labels = labels.contiguous()
-    if not 0.0 <= label_smoothing <= 1.0:
-        raise ValueError("label_smoothing %r outside [0, 1]" % (label_smoothing,))
-    p = LinearCeParams(dtype, T.REDUCTIONS[reduction], n, k, v, x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0))
-    if bias is not None:
-        bias = _vector(bias, "bias", x, v)
-        p.bias = bias.data_ptr()
-    p.labels, p.label_bytes, p.label_smoothing, p.ignore_index = labels.data_ptr(), labels.element_size(), label_smoothing, ignore_index
-    return p, (x, weight, labels, bias)
+    from ._torch import head
+    with _on(stream, x):
+        return tuple(head.linear_backward_raw(dout, x, weight, preact, activation, residual_rows, need, status))
 
 
 def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, label_smoothing=0.0, reduction="mean", stream=None, status=None):
     """rb200k_linear_ce: the cross entropy of the scores x weight^T + bias for x [n, k], weight [v, k], labels [n] (int32 or
     int64), without making the [n, v] scores. Returns (loss, stats, info): the loss is fp32, [n] or a scalar; stats and info
     go to linear_cross_entropy_backward."""
-    p, held = _ce_params(x, weight, labels, bias, ignore_index, label_smoothing, reduction)
-    x, n = held[0], p.rows
-    with _on(x.device, stream) as s:
-        loss = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=x.device)
-        stats = torch.empty((2, n), dtype=torch.float32, device=x.device)
-        info = torch.empty((4,), dtype=torch.int32, device=x.device)
-        p.loss, p.stats, p.info = loss.data_ptr(), stats.data_ptr(), info.data_ptr()
-        if status is not None:
-            p.status = status.data_ptr()
-        ws = _workspace(p, lib.rb200k_linear_ce_workspace_bytes, x.device)  # noqa: F841
-        check(lib.rb200k_linear_ce(ctypes.byref(p), s), "rb200k_linear_ce")
-    return loss, stats, info
+    from ._torch import head
+    with _on(stream, x):
+        return tuple(head.linear_ce_raw(x, weight, labels, bias, ignore_index, label_smoothing, reduction, status))
 
 
 def linear_cross_entropy_backward(dloss, x, weight, labels, stats, info, bias=None, ignore_index=-100, label_smoothing=0.0,
                                   reduction="mean", need=(True, True, True), stream=None, status=None):
     """rb200k_linear_ce_backward: (dx, dweight, dbias), None where `need` is false. dloss: fp32, of the loss's shape."""
-    p, held = _ce_params(x, weight, labels, bias, ignore_index, label_smoothing, reduction)
-    x, n, k, v = held[0], p.rows, p.features, p.classes
-    if dloss.dtype != torch.float32 or dloss.device != x.device or tuple(dloss.shape) != ((n,) if reduction == "none" else ()):
-        raise ValueError("dloss is %s %s on %s, it has to be like the loss" % (dloss.dtype, tuple(dloss.shape), dloss.device))
-    if tuple(stats.shape) != (2, n) or stats.dtype != torch.float32 or tuple(info.shape) != (4,) or info.dtype != torch.int32 or \
-            stats.device != x.device or info.device != x.device or not stats.is_contiguous() or not info.is_contiguous():
-        raise ValueError("stats and info are not those of this forward pass")
-    dloss = dloss.contiguous()
-    with _on(x.device, stream) as s:
-        grads = [torch.empty(shape, dtype=x.dtype, device=x.device) if want else None for shape, want in zip(((n, k), (v, k), (v,)), need)]
-        dx, dw, db = grads
-        p.dloss, p.stats, p.info = dloss.data_ptr(), stats.data_ptr(), info.data_ptr()
-        if dx is not None:
-            p.dx, p.lddx = dx.data_ptr(), k
-        if dw is not None:
-            p.dweight, p.lddw = dw.data_ptr(), k
-        if db is not None:
-            p.dbias = db.data_ptr()
-        if status is not None:
-            p.status = status.data_ptr()
-        ws = _workspace(p, lib.rb200k_linear_ce_backward_workspace_bytes, x.device)  # noqa: F841
-        check(lib.rb200k_linear_ce_backward(ctypes.byref(p), s), "rb200k_linear_ce_backward")
-    return tuple(grads)
-
-
-_GRAD_DTYPE = {torch.float32: T.FP32, torch.float16: T.FP16, torch.bfloat16: T.BF16}
-
-
-def _dense(t):
-    """Whether the elements fill a contiguous stretch of memory, in whatever order of the dimensions."""
-    order = sorted(range(t.dim()), key=lambda d: -t.stride(d))
-    return t.is_contiguous() or t.permute(order).is_contiguous()
+    from ._torch import head
+    with _on(stream, x):
+        return tuple(head.linear_ce_backward_raw(dloss, x, weight, labels, stats, info, bias, ignore_index, label_smoothing, reduction,
+                                                 need, status))
 
 
 def grad_clip(grads, max_norm, out=None, inv_scale=1.0, stream=None):
     """rb200k_grad_clip: the norm (fp32 scalar tensor) of inv_scale * all of `grads`, and each of them times inv_scale * min(1,
     max_norm / (norm + 1e-6)) - in place, or written to the tensors of `out` (the gradients' types or float32)."""
+    from ._torch import head
     grads = list(grads)
-    targets = grads if out is None else list(out)
     if not grads:
         raise ValueError("no gradients")
-    device = grads[0].device
-    if not grads[0].is_cuda:
-        raise ValueError("the gradients are on %s: the head operators run on a GPU" % device)
-    if len(targets) != len(grads):
-        raise ValueError("%d outputs for %d gradients" % (len(targets), len(grads)))
-    copies = []                        # (view with gaps, the dense tensor that stands for it)
-    types = _GRAD_DTYPE
-    for both in ((grads,) if out is None else (grads, targets)):
-        for t in both:
-            if t.dtype not in types or t.device != device or t.layout != torch.strided:
-                raise ValueError("a tensor is %s %s on %s; float32, float16 or bfloat16 on %s are needed" % (t.layout, t.dtype, t.device, device))
-    with _on(device, stream) as s:
-        if out is None:
-            if not all(map(torch.Tensor.is_contiguous, grads)):
-                dense = [t if _dense(t) else t.contiguous() for t in grads]
-                copies = [(t, d) for t, d in zip(grads, dense) if d is not t]
-                grads = targets = dense
-        else:
-            for g, o in zip(grads, targets):
-                if g.shape != o.shape or (o.dtype != g.dtype and o.dtype != torch.float32):
-                    raise ValueError("an output is %s %s for a gradient %s %s" % (tuple(o.shape), o.dtype, tuple(g.shape), g.dtype))
-            if not (all(map(torch.Tensor.is_contiguous, grads)) and all(map(torch.Tensor.is_contiguous, targets))):
-                pairs = []
-                for g, o in zip(grads, targets):
-                    if g.is_contiguous() and o.is_contiguous() or g.stride() == o.stride() and _dense(g):
-                        pairs.append((g, o))
-                        continue
-                    d = o if o.is_contiguous() else torch.empty(o.shape, dtype=o.dtype, device=device)
-                    if d is not o:
-                        copies.append((o, d))
-                    pairs.append((g.contiguous(), d))
-                grads, targets = [g for g, _ in pairs], [o for _, o in pairs]
-        n = len(grads)
-        table = np.empty(n, dtype=T.GRAD_TENSOR)
-        table["grad"] = list(map(torch.Tensor.data_ptr, grads))
-        table["out"] = table["grad"] if targets is grads else list(map(torch.Tensor.data_ptr, targets))
-        table["count"] = list(map(torch.Tensor.numel, grads))
-        table["grad_dtype"] = [types[t.dtype] for t in grads]
-        table["out_dtype"] = table["grad_dtype"] if targets is grads else [types[t.dtype] for t in targets]
-        norm = torch.empty((), dtype=torch.float32, device=device)
-        need = lib.rb200k_grad_clip_workspace_bytes(n)
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
-        check(lib.rb200k_grad_clip(table.ctypes.data, n, max_norm, inv_scale, norm.data_ptr(), ws.data_ptr(), need, s), "rb200k_grad_clip")
-        for view, dense in copies:
-            view.copy_(dense)
-    return norm
+    with _on(stream, grads[0]):
+        return head.grad_clip(grads, max_norm, out, inv_scale)

@@ -79,32 +79,17 @@ class ROCALClassificationIterator(ROCALGenericIterator):
 
 
 # ---- the head of a training or serving step, on the batches above -----------------------------------
-# Differentiable by torch.autograd, once. Float16 and bfloat16 CUDA tensors; everything runs on the tensors' device, on
-# its current stream.
+# Float16 and bfloat16 CUDA tensors; differentiable by torch.autograd, once (create_graph is refused). Everything runs on the
+# tensors' device, on its current stream.
+_head = None
 
 
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, activation):
-        from .. import kernels
-        act = activation != "none"
-        y = kernels.linear(x, weight, bias, residual, activation, want_preact=act)
-        y, pre = y if act else (y, None)
-        ctx.save_for_backward(x, weight, pre)
-        ctx.activation = activation
-        ctx.residual_rows = 0 if residual is None else residual.shape[0]
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
-        from .. import kernels
-        x, weight, pre = ctx.saved_tensors
-        need = list(ctx.needs_input_grad[:4])
-        whole = need[3] and ctx.residual_rows == x.shape[0]      # nothing is summed: the gradient goes through as it is
-        need[3] = need[3] and not whole
-        grads = kernels.linear_backward(dout, x, weight, pre, ctx.activation, ctx.residual_rows, need) if any(need) else (None,) * 4
-        return grads[0], grads[1], grads[2], dout if whole else grads[3], None
+def _binding():
+    global _head
+    if _head is None:
+        from .._torch import head
+        _head = head
+    return _head
 
 
 def linear(x, weight, bias=None, residual=None, activation="none"):
@@ -112,43 +97,10 @@ def linear(x, weight, bias=None, residual=None, activation="none"):
     patches with their position table, a hidden layer or the scores of a classifier.
 
     x [..., k]; weight [m, k]; bias [m]; residual: the trailing dimensions of the result, repeated over the leading ones
-    (a position table [196, m] for x [images, 196, k]); activation "none", "relu", "gelu" (with the error function) or
-    "silu". All float16 or all bfloat16; sums in 32 bits, one rounding at the end. Returns [..., m]."""
-    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
-        raise ValueError("x %s does not go with weight %s" % (tuple(x.shape), tuple(weight.shape)))
-    shape = tuple(x.shape[:-1]) + (weight.shape[0],)
-    if residual is not None:
-        if residual.dim() < 1 or residual.dim() > len(shape) or tuple(residual.shape) != shape[len(shape) - residual.dim():]:
-            if not (residual.dim() == 2 and x.dim() == 2 and residual.shape[1] == shape[1]):
-                raise ValueError("residual %s is not a tail of the result's shape %s" % (tuple(residual.shape), shape))
-        residual = residual.reshape(-1, shape[-1])
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
-        y = _Linear.apply(x2, weight, bias, residual, activation)
-    else:
-        from .. import kernels
-        y = kernels.linear(x2, weight, bias, residual, activation)
-    return y if x.dim() == 2 else y.reshape(shape)
-
-
-class _LinearCrossEntropy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, labels, bias, ignore_index, label_smoothing, reduction):
-        from .. import kernels
-        loss, stats, info = kernels.linear_cross_entropy(x, weight, labels, bias, ignore_index, label_smoothing, reduction)
-        ctx.save_for_backward(x, weight, labels, bias, stats, info)
-        ctx.how = (ignore_index, label_smoothing, reduction)
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dloss):
-        from .. import kernels
-        x, weight, labels, bias, stats, info = ctx.saved_tensors
-        need = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3])
-        dx, dw, db = kernels.linear_cross_entropy_backward(dloss, x, weight, labels, stats, info, bias, *ctx.how, need)
-        return dx, dw, None, db, None, None, None
+    (a position table [196, m] for x [images, 196, k]), or for a matrix x a matrix whose row count divides that of x;
+    activation "none", "relu", "gelu" (with the error function) or "silu". All float16 or all bfloat16; sums in 32 bits, one
+    rounding at the end. Returns [..., m]."""
+    return (_head or _binding()).linear(x, weight, bias, residual, activation)
 
 
 def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
@@ -161,27 +113,17 @@ def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, label_
     gradient, whatever their features hold; any other label outside 0 .. v-1 makes the row's loss NaN. A class is masked by
     a bias of -inf or of the type's lowest value. reduction "mean" (over the rows that count; 0 if none does), "sum" or
     "none" (the shape of labels). The loss is float32."""
-    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or tuple(labels.shape) != tuple(x.shape[:-1]):
-        raise ValueError("x %s, weight %s and labels %s do not go together" % (tuple(x.shape), tuple(weight.shape), tuple(labels.shape)))
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    flat = labels if labels.dim() == 1 else labels.reshape(-1)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
-        loss = _LinearCrossEntropy.apply(x2, weight, flat, bias, ignore_index, label_smoothing, reduction)
-    else:
-        from .. import kernels
-        loss = kernels.linear_cross_entropy(x2, weight, flat, bias, ignore_index, label_smoothing, reduction)[0]
-    return loss.reshape(labels.shape) if reduction == "none" else loss
+    return (_head or _binding()).linear_cross_entropy(x, weight, labels, bias, ignore_index, label_smoothing, reduction)
 
 
 def clip_grad_norm(grads, max_norm, out=None, inv_scale=1.0):
     """The norm over all tensors of `grads` (times inv_scale, the inverse of a loss scale), and the clipping to it: every
     tensor is multiplied by inv_scale * min(1, max_norm / (norm + 1e-6)), in place or into the tensors of `out` (of the
-    gradients' types, or float32 copies for a 32-bit optimiser). Float32, float16 and bfloat16 CUDA tensors of any
-    shapes, mixed, on one device. Returns the norm, a float32 scalar on the device; nothing is read back.
-    A gradient with inf gives the norm inf and the factor 0, one with NaN gives NaN, as torch.nn.utils.clip_grad_norm_."""
-    from .. import kernels
-    with torch.no_grad():
-        return kernels.grad_clip(grads, max_norm, out, inv_scale)
+    gradients' types, or float32 copies for a 32-bit optimiser; contiguous ones need only the same number of elements).
+    Float32, float16 and bfloat16 CUDA tensors of any shapes, mixed, on one device. Returns the norm, a float32 scalar on
+    the device; nothing is read back. A gradient with inf gives the norm inf and the factor 0, one with NaN gives NaN, as
+    torch.nn.utils.clip_grad_norm_. No output may overlap another output or another tensor's gradients."""
+    return (_head or _binding()).grad_clip(grads if isinstance(grads, list) else list(grads), max_norm, out, inv_scale)
 
 
 def clip_grad_norm_(parameters, max_norm, inv_scale=1.0):
