@@ -116,6 +116,10 @@ GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed
 int gemm_args(GemmArgs* g, const DeviceInfo& dev, bool bf16, const Operand& a, const Operand& b, const Operand* b_alt, const int* b_select,
               const GemmPlan& plan, const EpiArgs& e, const GemmWait& wait, const char* what) {
     const int m = a.outer(), n = b.outer();
+    if ((double)plan.tiles_m * plan.tiles_n * plan.splits > 2e9) {
+        set_error("%s: a product of %d x %d has more than 2e9 tiles", what, m, n);
+        return RB200_E_LIMIT;
+    }
     g->a_box_rows = kTileM;
     if (!a.transposed && m < kTileM) g->a_box_rows = (int)round_up(m, 8);
     const int bn_cta = plan.bn / plan.cg, b_box = b.transposed ? kTileK : bn_cta;

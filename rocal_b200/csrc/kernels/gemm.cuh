@@ -323,18 +323,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     if (EPI == EPI_CE_STATS && g.e.clear && blockIdx.x == 0 && threadIdx.x < 4) g.e.clear[threadIdx.x] = 0;
     const tc::Patience patience = {&gave_up_s, g.status, g.wait_cycles};
 
-    const long long tiles = (long long)g.tiles_m * g.tiles_n * g.splits;
-    const long long first = blockIdx.x / CG, step = gridDim.x / CG;
+    const uint32_t tiles = (uint32_t)g.tiles_m * g.tiles_n * g.splits;   // below 2^31 (gemm_args)
+    const uint32_t first = blockIdx.x / CG, step = gridDim.x / CG;
     // Tiles in bands of 8 tile rows, row fastest: the tiles in flight share their operands in L2.
-    auto place = [&](long long t, int& mb, int& nb, int& sp) {
-        const long long per = (long long)g.tiles_m * g.tiles_n;
-        sp = (int)(t / per);
-        const long long r = t - sp * per;
-        const long long band = r / (8ll * g.tiles_n);
-        const int rows = min(8, g.tiles_m - (int)band * 8);
-        const int q = (int)(r - band * 8 * g.tiles_n);
-        nb = q / rows;
-        mb = (int)band * 8 + q - nb * rows;
+    auto place = [&](uint32_t t, int& mb, int& nb, int& sp) {
+        const uint32_t per = (uint32_t)g.tiles_m * g.tiles_n;
+        sp = g.splits == 1 ? 0 : (int)(t / per);
+        const uint32_t r = t - sp * per, whole = 8u * g.tiles_n, band = r / whole, q = r - band * whole;
+        const uint32_t rows = min(8u, g.tiles_m - band * 8u);
+        const uint32_t col = rows == 8 ? q >> 3 : q / rows;
+        nb = (int)col;
+        mb = (int)(band * 8 + q - col * rows);
     };
     const int bn_cta = g.bn / CG;
 
@@ -345,7 +344,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             uint32_t phase = 0;
             long long filled = 0;
             bool ok = true;
-            for (long long t = first; t < tiles && ok; t += step) {
+            for (uint32_t t = first; t < tiles && ok; t += step) {
                 int mb, nb, sp;
                 place(t, mb, nb, sp);
                 const int m0 = mb * (kTileM * CG) + (int)rank * kTileM, n0 = nb * g.bn + (int)rank * bn_cta;
@@ -397,7 +396,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             int s = 0, buf = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true, issued = false;
-            for (long long t = first; t < tiles && ok; t += step) {
+            for (uint32_t t = first; t < tiles && ok; t += step) {
                 int mb, nb, sp;
                 place(t, mb, nb, sp);
                 const int k_begin = sp * g.kblocks_per_split, k_end = min(g.kblocks, (sp + 1) * g.kblocks_per_split);
@@ -441,7 +440,33 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         uint32_t acc_phase = 0;
         float scale = 1.0f;
         if constexpr (EPI == EPI_STORE) scale = g.e.scale.value();
-        for (long long t = first + group * step; t < tiles; t += 2 * step) {
+        // a row's label and statistics, fetched a tile ahead
+        struct RowData {
+            int label;
+            bool counted;
+            float top, sum, coef;
+        };
+        auto fetch_row = [&](uint32_t t) {
+            RowData d = {-1, false, 0.0f, 1.0f, 1.0f};
+            if constexpr (EPI == EPI_CE_STATS || EPI == EPI_CE_GRAD) {
+                if (t < tiles) {
+                    int mb, nb, sp;
+                    place(t, mb, nb, sp);
+                    const int row = mb * (kTileM * CG) + in_tile + lane;
+                    if (row < g.m) {
+                        d.label = load_label(g.e.labels, g.e.label_bytes, row, g.e.ignore_index, g.e.classes, &d.counted);
+                        if constexpr (EPI == EPI_CE_GRAD) {
+                            d.top = g.e.stats[row];
+                            d.sum = g.e.stats[g.e.stats_stride + row];
+                            if (g.e.coef) d.coef = g.e.coef[row];
+                        }
+                    }
+                }
+            }
+            return d;
+        };
+        RowData ahead = fetch_row(first + group * step);
+        for (uint32_t t = first + group * step; t < tiles; t += 2 * step) {
             int mb, nb, sp;
             place(t, mb, nb, sp);
             const int row0 = mb * (kTileM * CG) + in_tile, row = row0 + lane;
@@ -449,21 +474,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             const int n0 = nb * g.bn, n1 = min(n0 + g.bn, g.n);
 
             // what does not depend on the products is fetched before the wait for them
-            int label = -1;
-            bool counted = false;
+            const RowData own = ahead;
+            const int label = own.label < g.e.class0 ? -1 : own.label - g.e.class0;
+            const bool counted = own.counted;
             float cmax = 0.0f, cscale = 0.0f, inv_sum = 0.0f, zsum = 0.0f;
             RunningSoftmax run = {-INFINITY, 0.0f};
-            if constexpr (EPI == EPI_CE_STATS || EPI == EPI_CE_GRAD) {
-                if (row_ok) {
-                    label = load_label(g.e.labels, g.e.label_bytes, row, g.e.ignore_index, g.e.classes, &counted);
-                    label = label < g.e.class0 ? -1 : label - g.e.class0;
-                }
-            }
             if constexpr (EPI == EPI_CE_GRAD) {
                 if (counted) {
-                    cmax = finite_max(g.e.stats[row]);
-                    inv_sum = 1.0f / g.e.stats[g.e.stats_stride + row];
-                    cscale = (g.e.coef ? g.e.coef[row] : 1.0f) * 32768.0f;
+                    cmax = finite_max(own.top);
+                    inv_sum = 1.0f / own.sum;
+                    cscale = own.coef * 32768.0f;
                 }
             }
             // the residual's strip is fetched ahead, too: lane l takes piece l % 4 of the rows l / 4 + 8 i
@@ -507,6 +527,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             if (!__all_sync(0xFFFFFFFFu, tc::bar_wait(acc_full(group), acc_phase, patience))) break;
             acc_phase ^= 1;
             tc::fence_after();
+            ahead = fetch_row(t + 2 * step);
 
             uint32_t raw[32];   // the strip on its way
             tc::tmem_load32(acc, raw);
