@@ -476,8 +476,8 @@ typedef struct rb200_linear_ce_params {
     float label_smoothing;       /* 0 .. 1 */
     int64_t ignore_index;
     float* loss;                 /* NONE: [rows], else one value (forward only) */
-    float* stats;                /* [2][rows]: each row's largest score and sum of exp(z - that) - written by the
-                                    forward pass, read by the backward pass */
+    float* stats;                /* [3][rows]: each row's largest score, sum of exp(z - that), and its label's score -
+                                    written by the forward pass, read by the backward pass */
     int32_t* info;               /* [4]: rows that count, 1 if a row that does not count holds inf or NaN, two reserved
                                     words - written by the forward pass, read by the backward pass */
     /* backward pass only: */

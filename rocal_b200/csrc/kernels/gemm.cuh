@@ -2,10 +2,12 @@
 // tensor cores, and what is done with the accumulators before they leave the chip (EPI_*). One persistent kernel:
 //   warp 0      copies operand tiles (128-byte swizzle) into a ring of shared-memory stages,
 //   warp 1      issues the products of a stage (64 contracted elements) into one of two TMEM accumulators,
-//   warps 4-11  two groups of four; each group reads its own accumulator, 32 columns at a time (thread = row), and
-//               runs the epilogue of every other tile, so that the epilogues of two tiles overlap each other's latency
-//               and the products of the tiles behind them. Results cross over in shared memory from
-//               threads that hold rows to lanes that write whole pieces of rows.
+//   warps 4-19  two groups of eight; each group reads its own accumulator, 32 columns at a time (thread = row, two
+//               warps share a row's strips), and runs the epilogue of every other tile, so that the epilogues of two tiles
+//               overlap each other's latency and the products of the tiles behind them. Results cross over in shared
+//               memory from threads that hold rows to lanes that write whole pieces of rows.
+//               An epilogue strip is some 150 to 400 instructions of a warp, mostly in chains: with 8 warps instead of 16
+//               it took 900 to 2500 clocks and bounded products of up to 1024 contracted elements.
 // CG = 2: two CTAs (a cluster) work on one tile of 256 rows; each holds its 128 rows of A and half of the B tile, so a
 // tile of 256 columns takes 128 bytes of operands per SM and clock at the full rate of the tensor cores instead of 192.
 // Either operand may have the contracted axis contiguous (K-major) or the other one (MN-major): the backward products
@@ -17,8 +19,8 @@
 namespace rb200 {
 
 constexpr int kTileM = 128, kTileK = 64, kTileNMax = 256;
-constexpr int kGemmThreads = 384, kEpiWarps = 8;
-constexpr int kStageBytes = 4096;            // of an epilogue warp: 32 lines of 128 bytes
+constexpr int kEpiWarps = 16, kGemmThreads = 128 + 32 * kEpiWarps;
+constexpr int kStageBytes = 2048;            // of an epilogue warp: 32 lines of 64 bytes
 constexpr int kRingBytes = 196608;           // of the 227 KB: operand stages
 
 enum { EPI_LINEAR = 0, EPI_STORE = 1, EPI_CE_STATS = 2, EPI_CE_GRAD = 3 };
@@ -55,11 +57,12 @@ struct EpiArgs {
     int label_bytes, classes, class0;
     long long ignore_index;
     float smooth_on, smooth_off;   // 1 - smoothing, smoothing / classes
-    float* part;              // STATS: [parts][m] maxima, then [parts][m] sums, then (smoothing) [parts][m] sums of z
+    float* part;              // STATS: [parts][m] maxima, then [parts][m] sums, then (smoothing) [parts][m] sums of z;
+                              // two parts a tile
     int parts, want_zsum;
     float* zlabel;            // STATS: [m] the label's z
     int* clear;               // STATS: four words to be zeroed, or null
-    const float* stats;       // GRAD: maxima, and stats_stride further the sums
+    const float* stats;       // GRAD: maxima; stats_stride further the sums, twice that the labels' z
     long long stats_stride;
     const float* coef;        // GRAD: [m] per-row factor or null (= 1)
 };
@@ -104,6 +107,27 @@ struct Elem<__nv_bfloat16> {
         return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
     }
 };
+
+// Eight elements, `count` of them there (the others are zeros).
+template <typename T>
+__device__ __forceinline__ uint4 load8(const T* p, int count, bool vec) {
+    if (vec && count >= 8) return __ldg(reinterpret_cast<const uint4*>(p));
+    uint32_t w[4] = {};
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (i < count) w[i >> 1] |= (uint32_t) reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& w, float (&v)[8]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = Elem<T>::unpack(u[i]);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
 
 // Upper tail of the normal distribution over its density shape: R(a) = Q(a) exp(a^2 / 2) for a in [0, 6], a polynomial
 // of degree 12 in a / 3 - 1 fitted for the least relative error (2.3e-6 evaluated in fp32). Beyond 6, where z Q(z) is
@@ -186,12 +210,10 @@ __device__ __forceinline__ void act_slopes(float* v, int act) {   // z -> slope
 }
 
 // ---- results through shared memory -----------------------------------------------------------------------
-// Threads hold rows; memory wants whole pieces of rows. A warp's 32 rows x 32 columns cross over in its staging area: each
-// thread writes its own line, then 16-byte pieces are read back so that neighbouring lanes hold neighbouring pieces of a row.
-// Pieces are permuted within a line so that neither side has bank conflicts. Element type: lines of 64 bytes (piece j of
-// line r at place j ^ (r / 2 & 3)), a row takes 4 lanes; fp32: lines of 128 bytes (j ^ (r & 7)), a row takes 8 lanes.
-__device__ __forceinline__ uint32_t staged16(uint32_t area, int line, int piece) { return area + line * 64 + ((piece ^ (line >> 1 & 3)) << 4); }
-__device__ __forceinline__ uint32_t staged32(uint32_t area, int line, int piece) { return area + line * 128 + ((piece ^ (line & 7)) << 4); }
+// Threads hold rows; memory wants whole pieces of rows. A warp's strip crosses over in its staging area, 32 lines of 64
+// bytes: each thread writes its own line, then 16-byte pieces are read back so that four neighbouring lanes hold the pieces of a
+// line. Piece j of line r lies at place j ^ (r / 2 & 3), so that neither side has bank conflicts.
+__device__ __forceinline__ uint32_t staged(uint32_t area, int line, int piece) { return area + line * 64 + ((piece ^ (line >> 1 & 3)) << 4); }
 __device__ __forceinline__ void st_shared16(uint32_t addr, const uint4& w) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
 }
@@ -200,15 +222,13 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(addr) : "memory");
     return w;
 }
-// Writes the strip v (a row a thread) to rows [row0, row0 + rows) and columns [col, col + cols) of out.
 template <typename T>
-__device__ __forceinline__ void leave16(uint32_t area, const float (&v)[32], T* out, long long ld, bool vec, int col, int cols, int row0, int rows,
-                                        int lane) {
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        st_shared16(staged16(area, lane, i), make_uint4(Elem<T>::pack(v[8 * i], v[8 * i + 1]), Elem<T>::pack(v[8 * i + 2], v[8 * i + 3]),
-                                                        Elem<T>::pack(v[8 * i + 4], v[8 * i + 5]), Elem<T>::pack(v[8 * i + 6], v[8 * i + 7])));
-    __syncwarp();
+__device__ __forceinline__ uint4 pack8(const float* v) {
+    return make_uint4(Elem<T>::pack(v[0], v[1]), Elem<T>::pack(v[2], v[3]), Elem<T>::pack(v[4], v[5]), Elem<T>::pack(v[6], v[7]));
+}
+// The staged strip to rows [row0, row0 + rows) and columns [col, col + cols) of out.
+template <typename T>
+__device__ __forceinline__ void copy_strip(uint32_t area, T* out, long long ld, bool vec, int col, int cols, int row0, int rows, int lane) {
     rows = min(rows, 32);
     if (vec && (cols & 7) == 0) {
         const int piece = lane & 3;
@@ -216,7 +236,7 @@ __device__ __forceinline__ void leave16(uint32_t area, const float (&v)[32], T* 
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int r = (lane >> 2) + 8 * i;
-            const uint4 w = ld_shared16(staged16(area, r, piece));
+            const uint4 w = ld_shared16(staged(area, r, piece));
             if (r < rows && piece * 8 < cols) *reinterpret_cast<uint4*>(o) = w;
             o += 8 * ld;
         }
@@ -224,35 +244,41 @@ __device__ __forceinline__ void leave16(uint32_t area, const float (&v)[32], T* 
 #pragma unroll 4
         for (int r = 0; r < rows; r++) {
             uint16_t w;
-            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(staged16(area, r, lane >> 3) + (lane & 7) * 2) : "memory");
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(staged(area, r, lane >> 3) + (lane & 7) * 2) : "memory");
             if (lane < cols) reinterpret_cast<uint16_t*>(out + (long long)(row0 + r) * ld + col)[lane] = w;
         }
     }
 }
-// The same in fp32, added to `in` if that is set. cols counts the padding of the rows: a multiple of 4.
-__device__ __forceinline__ void leave32(uint32_t area, const float (&v)[32], float* out, const float* in, long long ld, int cols, int rows, int lane) {
-    __syncwarp();   // the whole area is used: the strip before has been read
+// 32-bit sums: the strip in two halves of 16 columns, added to `in` if that is set. out and in point at the strip's first
+// element, cols counts the padding of the rows (a multiple of 4).
+__device__ __forceinline__ void leave_sums(uint32_t area, const float (&v)[32], float* out, const float* in, long long ld, int cols, int rows,
+                                           int lane) {
+    const int piece = lane & 3;
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-        st_shared16(staged32(area, lane, i), make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
-                                                        __float_as_uint(v[4 * i + 3])));
-    __syncwarp();
-    const int piece = lane & 7;
-    const long long at = (lane >> 3) * ld + piece * 4;
+    for (int h = 0; h < 2; h++) {
+        __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int r = (lane >> 3) + 4 * i;
-        const uint4 w = ld_shared16(staged32(area, r, piece));
-        if (r < rows && piece * 4 < cols) {
-            float4 f = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
-            if (in) {
-                const float4 s = *reinterpret_cast<const float4*>(in + at + 4 * i * ld);
-                f.x += s.x;
-                f.y += s.y;
-                f.z += s.z;
-                f.w += s.w;
+        for (int i = 0; i < 4; i++) {
+            const float* q = v + 16 * h + 4 * i;
+            st_shared16(staged(area, lane, i), make_uint4(__float_as_uint(q[0]), __float_as_uint(q[1]), __float_as_uint(q[2]), __float_as_uint(q[3])));
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = (lane >> 2) + 8 * i;
+            const long long at = r * ld + 16 * h + piece * 4;
+            const uint4 w = ld_shared16(staged(area, r, piece));
+            if (r < rows && 16 * h + piece * 4 < cols) {
+                float4 f = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+                if (in) {
+                    const float4 s = *reinterpret_cast<const float4*>(in + at);
+                    f.x += s.x;
+                    f.y += s.y;
+                    f.z += s.z;
+                    f.w += s.w;
+                }
+                *reinterpret_cast<float4*>(out + at) = f;
             }
-            *reinterpret_cast<float4*>(out + at + 4 * i * ld) = f;
         }
     }
 }
@@ -284,7 +310,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     __shared__ __align__(8) uint64_t bars[2 * 16 + 2 * 2 + 1];
     __shared__ uint32_t tmem_addr_s;
     __shared__ int gave_up_s;
-    __shared__ __align__(16) T bias_s[kEpiWarps][2][32];
 
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = CG == 2 ? tc::cta_rank() : 0;
@@ -433,161 +458,122 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         }
         __syncwarp();
     } else if (warp >= 4) {
-        const int ew = warp - 4, quarter = warp & 3, group = ew >> 2;   // group 0: even tiles and accumulator 0
+        // group 0: even tiles and accumulator 0; share 0: even strips
+        const int ew = warp - 4, quarter = warp & 3, group = ew >> 3, share = ew >> 2 & 1;
         const uint32_t area = smem0 + kRingBytes + ew * kStageBytes;
         const uint32_t acc = tmem + group * kTileNMax + ((uint32_t)(quarter * 32) << 16);
-        const int in_tile = (int)rank * kTileM + quarter * 32;
         uint32_t acc_phase = 0;
         float scale = 1.0f;
         if constexpr (EPI == EPI_STORE) scale = g.e.scale.value();
-        // a row's label and statistics, fetched a tile ahead
-        struct RowData {
-            int label;
-            bool counted;
-            float top, sum, coef;
-        };
-        auto fetch_row = [&](uint32_t t) {
-            RowData d = {-1, false, 0.0f, 1.0f, 1.0f};
-            if constexpr (EPI == EPI_CE_STATS || EPI == EPI_CE_GRAD) {
-                if (t < tiles) {
-                    int mb, nb, sp;
-                    place(t, mb, nb, sp);
-                    const int row = mb * (kTileM * CG) + in_tile + lane;
-                    if (row < g.m) {
-                        d.label = load_label(g.e.labels, g.e.label_bytes, row, g.e.ignore_index, g.e.classes, &d.counted);
-                        if constexpr (EPI == EPI_CE_GRAD) {
-                            d.top = g.e.stats[row];
-                            d.sum = g.e.stats[g.e.stats_stride + row];
-                            if (g.e.coef) d.coef = g.e.coef[row];
-                        }
-                    }
-                }
-            }
-            return d;
-        };
-        RowData ahead = fetch_row(first + group * step);
         for (uint32_t t = first + group * step; t < tiles; t += 2 * step) {
             int mb, nb, sp;
             place(t, mb, nb, sp);
-            const int row0 = mb * (kTileM * CG) + in_tile, row = row0 + lane;
+            const int row0 = mb * (kTileM * CG) + (int)rank * kTileM + quarter * 32, row = row0 + lane;
             const bool row_ok = row < g.m;
             const int n0 = nb * g.bn, n1 = min(n0 + g.bn, g.n);
 
             // what does not depend on the products is fetched before the wait for them
-            const RowData own = ahead;
-            const int label = own.label < g.e.class0 ? -1 : own.label - g.e.class0;
-            const bool counted = own.counted;
-            float cmax = 0.0f, cscale = 0.0f, inv_sum = 0.0f, zsum = 0.0f;
+            int label = -1;
+            bool counted = false;
+            float top = 0.0f, zsum = 0.0f, mul = 0.0f, add = 0.0f, at_label = 0.0f;
             RunningSoftmax run = {-INFINITY, 0.0f};
+            if constexpr (EPI == EPI_CE_STATS || EPI == EPI_CE_GRAD) {
+                if (row_ok) {
+                    label = load_label(g.e.labels, g.e.label_bytes, row, g.e.ignore_index, g.e.classes, &counted);
+                    label = label < g.e.class0 ? -1 : label - g.e.class0;
+                }
+            }
             if constexpr (EPI == EPI_CE_GRAD) {
-                if (counted) {
-                    cmax = finite_max(own.top);
-                    inv_sum = 1.0f / own.sum;
-                    cscale = own.coef * 32768.0f;
+                if (counted) {   // (softmax - target) * factor = exp(z - top) * mul + add, and at the label
+                    const float zl = g.e.stats[2 * g.e.stats_stride + row], factor = (g.e.coef ? g.e.coef[row] : 1.0f) * 32768.0f;
+                    top = finite_max(g.e.stats[row]);
+                    mul = factor / g.e.stats[g.e.stats_stride + row];
+                    add = -g.e.smooth_off * factor;
+                    at_label = exp_diff(zl - top) * mul + add - g.e.smooth_on * factor;
+                } else {
+                    label = -1;
                 }
             }
-            // the residual's strip is fetched ahead, too: lane l takes piece l % 4 of the rows l / 4 + 8 i
-            uint4 res_next[4] = {};
-            long long res_at[4];
-            auto fetch_residual = [&](int c) {
-                const int col = n0 + c + (lane & 3) * 8, count = n1 - col;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    if (res_at[i] < 0 || count <= 0) continue;
-                    const T* p = reinterpret_cast<const T*>(g.e.residual) + res_at[i] + col;
-                    if (g.e.vec_res && count >= 8) {
-                        res_next[i] = __ldg(reinterpret_cast<const uint4*>(p));
-                    } else {
-                        uint32_t w[4] = {};
-#pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            if (j < count) w[j >> 1] |= (uint32_t) reinterpret_cast<const uint16_t*>(p)[j] << (16 * (j & 1));
-                        res_next[i] = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                }
-            };
-            if constexpr (EPI == EPI_LINEAR) {
-                if (g.e.residual) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int r = row0 + (lane >> 2) + 8 * i;
-                        res_at[i] = r < g.m ? (long long)(r % g.e.residual_rows) * g.e.ldr : -1;
-                    }
-                    fetch_residual(0);
-                }
-            }
-            // the bias of 32 columns, one lane each, is fetched a strip ahead and passed around in shared memory
-            auto fetch_bias = [&](int c) {
-                return EPI != EPI_STORE && g.e.bias && n0 + c + lane < n1 ? reinterpret_cast<const T*>(g.e.bias)[n0 + c + lane]
-                                                                          : Elem<T>::from_float(0.0f);
-            };
-            T bias_next = fetch_bias(0);
 
             // the lanes leave together: what follows needs whole warps
             if (!__all_sync(0xFFFFFFFFu, tc::bar_wait(acc_full(group), acc_phase, patience))) break;
             acc_phase ^= 1;
             tc::fence_after();
-            ahead = fetch_row(t + 2 * step);
 
-            uint32_t raw[32];   // the strip on its way
-            tc::tmem_load32(acc, raw);
-            for (int c = 0; c < g.bn; c += 32) {
+            for (int c = share * 32; c < g.bn; c += 64) {
                 const int col = n0 + c, count = n1 - col;   // columns of this strip inside the matrix (may be <= 0)
-                T* bias = bias_s[ew][c >> 5 & 1];
+                const bool work = count > 0 && row0 < g.m;
+                uint32_t raw[32];
+                if (work) tc::tmem_load32(acc + c, raw);
+                float own_bias = 0.0f;   // of column `lane`
                 if constexpr (EPI != EPI_STORE) {
-                    bias[lane] = bias_next;
-                    bias_next = fetch_bias(c + 32);
-                    __syncwarp();
+                    if (work && g.e.bias && lane < count) own_bias = Elem<T>::to_float(reinterpret_cast<const T*>(g.e.bias)[col + lane]);
                 }
                 tc::tmem_wait();
-                float v[32];
-#pragma unroll
-                for (int i = 0; i < 32; i++) v[i] = __uint_as_float(raw[i]);
-                if (c + 32 < g.bn) {
-                    tc::tmem_load32(acc + c + 32, raw);
-                } else {   // the accumulator is in registers: the products of the next tile but one may begin
+                if (c + 64 >= g.bn) {   // this warp's part of the accumulator is in registers
                     tc::fence_before();
                     __syncwarp();
                     if (lane == 0) tc::bar_arrive_relaxed(CG == 2 ? tc::map_to_rank(acc_empty(group), 0) : acc_empty(group));
                 }
-                if (count <= 0 || row0 >= g.m) continue;
+                if (!work) continue;
+                float v[32];
+#pragma unroll
+                for (int i = 0; i < 32; i++) v[i] = __uint_as_float(raw[i]);
+                __syncwarp();   // the staging area is free: the strip before has been read
                 if constexpr (EPI != EPI_STORE) {
+                    if (g.e.bias) {
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(area + lane * 4), "f"(own_bias) : "memory");
+                        __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        const uint4 w = *reinterpret_cast<const uint4*>(bias + i);
-                        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const float2 s = add2(make_float2(v[i + 2 * j], v[i + 2 * j + 1]), Elem<T>::unpack(u[j]));
-                            v[i + 2 * j] = s.x;
-                            v[i + 2 * j + 1] = s.y;
+                        for (int i = 0; i < 32; i += 4) {
+                            const uint4 w = ld_shared16(area + i * 4);
+                            const float2 s = add2(make_float2(v[i], v[i + 1]), make_float2(__uint_as_float(w.x), __uint_as_float(w.y)));
+                            const float2 u = add2(make_float2(v[i + 2], v[i + 3]), make_float2(__uint_as_float(w.z), __uint_as_float(w.w)));
+                            v[i] = s.x;
+                            v[i + 1] = s.y;
+                            v[i + 2] = u.x;
+                            v[i + 3] = u.y;
                         }
+                        __syncwarp();
                     }
                 }
-                const uint32_t half = area + (c >> 5 & 1) * (kStageBytes / 2);   // strips take turns
                 auto leave = [&](void* out, long long ld, bool vec) {
-                    leave16<T>(half, v, reinterpret_cast<T*>(out), ld, vec, col, min(32, count), row0, g.m - row0, lane);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) st_shared16(staged(area, lane, i), pack8<T>(v + 8 * i));
+                    __syncwarp();
+                    copy_strip(area, reinterpret_cast<T*>(out), ld, vec, col, min(32, count), row0, g.m - row0, lane);
                 };
                 if constexpr (EPI == EPI_LINEAR) {
                     if (g.e.preact) {
                         leave(g.e.preact, g.e.ldp, g.e.vec_pre);
                         __syncwarp();
                     }
-                    if (g.e.act != ACT_NONE) act_values<32>(v, g.e.act);
+                    if (g.e.act != ACT_NONE) {
+                        act_values<16>(v, g.e.act);
+                        act_values<16>(v + 16, g.e.act);
+                    }
                     if (g.e.residual) {   // the other way round: whole pieces of rows in, a row a thread out
+                        const int piece = lane & 3, left = count - piece * 8;
 #pragma unroll
-                        for (int i = 0; i < 4; i++) st_shared16(staged16(half, (lane >> 2) + 8 * i, lane & 3), res_next[i]);
-                        fetch_residual(c + 32);
+                        for (int i = 0; i < 4; i++) {
+                            const int r = (lane >> 2) + 8 * i;
+                            uint4 w = make_uint4(0, 0, 0, 0);
+                            if (row0 + r < g.m && left > 0)
+                                w = load8(reinterpret_cast<const T*>(g.e.residual) + (long long)((row0 + r) % g.e.residual_rows) * g.e.ldr + col +
+                                              piece * 8,
+                                          left, g.e.vec_res);
+                            st_shared16(staged(area, r, piece), w);
+                        }
                         __syncwarp();
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            const uint4 w = ld_shared16(staged16(half, lane, i));
-                            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+                            float r[8];
+                            unpack8<T>(ld_shared16(staged(area, lane, i)), r);
 #pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                const float2 s = add2(make_float2(v[8 * i + 2 * j], v[8 * i + 2 * j + 1]), Elem<T>::unpack(u[j]));
-                                v[8 * i + 2 * j] = s.x;
-                                v[8 * i + 2 * j + 1] = s.y;
+                            for (int j = 0; j < 8; j += 2) {
+                                const float2 s = add2(make_float2(v[8 * i + j], v[8 * i + j + 1]), make_float2(r[j], r[j + 1]));
+                                v[8 * i + j] = s.x;
+                                v[8 * i + j + 1] = s.y;
                             }
                         }
                     }
@@ -598,8 +584,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     const long long at = (long long)row0 * g.e.ldacc + col;
                     const int wide = min(32, (int)g.e.ldacc - col);
                     if (g.e.acc_out) {
-                        leave32(area, v, g.e.acc_out + (long long)sp * g.e.acc_split_stride + at, g.e.acc_in ? g.e.acc_in + at : nullptr, g.e.ldacc,
-                                wide, g.m - row0, lane);
+                        leave_sums(area, v, g.e.acc_out + (long long)sp * g.e.acc_split_stride + at, g.e.acc_in ? g.e.acc_in + at : nullptr,
+                                   g.e.ldacc, wide, g.m - row0, lane);
                     } else {
                         if (g.e.acc_in && row_ok) {
                             const float* p = g.e.acc_in + (long long)row * g.e.ldacc + col;
@@ -615,15 +601,25 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                             }
                         }
 #pragma unroll
-                        for (int i = 0; i < 32; i++) v[i] *= scale;
+                        for (int i = 0; i < 32; i += 2) {
+                            const float2 s = mul2(make_float2(v[i], v[i + 1]), make_float2(scale, scale));
+                            v[i] = s.x;
+                            v[i + 1] = s.y;
+                        }
                         leave(g.e.out, g.e.ldo, g.e.vec_out);
                     }
                 }
                 if constexpr (EPI == EPI_CE_STATS) {
-                    if (row_ok && label >= col && label < col + 32 && label < g.n) {
+                    const int l = label - col;
+                    if (l >= 0 && l < 32) {   // element l of the strip, by its bits
+                        float a[16];
 #pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            if (label == col + i) g.e.zlabel[row] = v[i];
+                        for (int i = 0; i < 16; i++) a[i] = l & 16 ? v[i + 16] : v[i];
+#pragma unroll
+                        for (int w = 8; w; w >>= 1)
+#pragma unroll
+                            for (int i = 0; i < w; i++) a[i] = l & w ? a[i + w] : a[i];
+                        if (label < g.n) g.e.zlabel[row] = a[0];
                     }
                     if (g.e.want_zsum) {
 #pragma unroll
@@ -635,46 +631,58 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                         for (int i = 0; i < 32; i++)
                             if (i >= count) v[i] = -INFINITY;
                     }
-                    float top = run.m;
+                    float m[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                    for (int i = 0; i < 32; i++) top = fmaxf(top, v[i]);
-                    const float base = finite_max(top);
+                    for (int i = 4; i < 32; i += 4)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) m[j] = fmaxf(m[j], v[i + j]);
+                    const float strip = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), now = fmaxf(run.m, strip), base = finite_max(now);
                     run.s *= exp_diff(run.m - base);
-                    run.m = top;
-                    float2 sum = make_float2(0.0f, 0.0f);
+                    run.m = now;
+                    float2 sum[2] = {};
                     const float2 off = make_float2(-base, -base), unit = make_float2(kLog2e, kLog2e);
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
                         const float2 d = mul2(add2(make_float2(v[i], v[i + 1]), off), unit);
-                        sum = add2(sum, make_float2(exp2_fast(d.x), exp2_fast(d.y)));
+                        sum[i >> 1 & 1] = add2(sum[i >> 1 & 1], make_float2(exp2_fast(d.x), exp2_fast(d.y)));
                     }
-                    run.s += sum.x + sum.y;
+                    run.s += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 }
                 if constexpr (EPI == EPI_CE_GRAD) {
-                    const float2 off = make_float2(-cmax, -cmax), unit = make_float2(kLog2e, kLog2e);
-                    const float2 inv = make_float2(inv_sum, inv_sum), smooth = make_float2(-g.e.smooth_off, -g.e.smooth_off);
+                    const float2 off = make_float2(-top, -top), unit = make_float2(kLog2e, kLog2e);
+                    const float2 mul_v = make_float2(mul, mul), add_v = make_float2(add, add);
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
                         const float2 d = mul2(add2(make_float2(v[i], v[i + 1]), off), unit);
-                        const float2 p = fma2(make_float2(exp2_fast(d.x), exp2_fast(d.y)), inv, smooth);
+                        const float2 p = fma2(make_float2(exp2_fast(d.x), exp2_fast(d.y)), mul_v, add_v);
                         v[i] = p.x;
                         v[i + 1] = p.y;
                     }
-                    if (label >= col && label < col + 32) {
 #pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            if (label == col + i) v[i] -= g.e.smooth_on;
+                    for (int i = 0; i < 4; i++) {
+                        uint4 w = pack8<T>(v + 8 * i);
+                        if (!counted) w = make_uint4(0, 0, 0, 0);   // whatever the row held
+                        st_shared16(staged(area, lane, i), w);
                     }
-#pragma unroll
-                    for (int i = 0; i < 32; i++) v[i] = counted ? v[i] * cscale : 0.0f;
+                    const int l = label - col;
+                    if (l >= 0 && l < 32) {
+                        const T e = Elem<T>::from_float(at_label);
+                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(staged(area, lane, l >> 3) + (l & 7) * 2),
+                                     "h"(*reinterpret_cast<const uint16_t*>(&e))
+                                     : "memory");
+                    }
+                    __syncwarp();
                     // the rows are padded to whole pieces, which nothing reads
-                    leave16<T>(half, v, reinterpret_cast<T*>(g.e.out), g.e.ldo, true, col, min(32, (count + 7) & ~7), row0, g.m - row0, lane);
+                    copy_strip(area, reinterpret_cast<T*>(g.e.out), g.e.ldo, true, col, min(32, (count + 7) & ~7), row0, g.m - row0, lane);
                 }
             }
-            __syncwarp();   // the staging area and the bias strips are free for the next tile
+            if (g.bn <= share * 32) {   // a tile of one strip: the other warps have nothing to read
+                __syncwarp();
+                if (lane == 0) tc::bar_arrive_relaxed(CG == 2 ? tc::map_to_rank(acc_empty(group), 0) : acc_empty(group));
+            }
             if constexpr (EPI == EPI_CE_STATS) {
                 if (row_ok) {
-                    const long long plane = (long long)g.e.parts * g.m, at = (long long)nb * g.m + row;
+                    const long long plane = (long long)g.e.parts * g.m, at = (long long)(2 * nb + share) * g.m + row;
                     g.e.part[at] = run.m;
                     g.e.part[plane + at] = run.s;
                     if (g.e.want_zsum) g.e.part[2 * plane + at] = zsum;

@@ -28,26 +28,6 @@ struct RowsArgs {
     int act, vec_src, vec_pre;
 };
 
-template <typename T>
-__device__ __forceinline__ uint4 load8(const T* p, int count, bool vec) {
-    if (vec && count >= 8) return __ldg(reinterpret_cast<const uint4*>(p));
-    uint32_t w[4] = {};
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-        if (i < count) w[i >> 1] |= (uint32_t) reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& w, float (&v)[8]) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float2 f = Elem<T>::unpack(u[i]);
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-    }
-}
-
 template <typename T, bool SLOPE>
 __global__ void __launch_bounds__(256) rows_kernel(RowsArgs a) {
     constexpr int U = 4;   // rows in flight

@@ -17,13 +17,12 @@ constexpr size_t kPieceBytes = 256u << 20;   // scores' gradients of one piece
 struct MergeArgs {
     const float* part;      // [parts][rows] maxima, sums, sums of z
     int parts, want_zsum;
-    const float* zlabel;
     const void* labels;
     int label_bytes, classes, rows, reduction;
     long long ignore_index;
     float smoothing;
     int first, last;        // piece of the classes: the first starts the statistics, the last makes the loss
-    float* stats;           // [2][rows]
+    float* stats;           // [3][rows]: maximum, sum, the label's z
     float* zsum;            // [rows], between pieces
     float* loss;
     int* info;
@@ -89,7 +88,7 @@ __global__ void __launch_bounds__(256) ce_merge_kernel(MergeArgs a) {
                     r.m = r.s = loss = nanf("");
                 } else {
                     const float lse = logf(r.s);   // above the maximum
-                    loss = (1.0f - a.smoothing) * (lse + (r.m - a.zlabel[row]));
+                    loss = (1.0f - a.smoothing) * (lse + (r.m - a.stats[2ll * a.rows + row]));
                     if (a.want_zsum) loss += a.smoothing * (lse + (r.m - z / (float)a.classes));
                 }
             } else {
@@ -271,7 +270,7 @@ struct StatsPlan {
     Packed x, w;
     int piece;              // classes of one launch
     size_t part_bytes;
-    float *part, *zlabel, *zsum;
+    float *part, *zsum;
     double* block_sums;
     size_t bytes;
 };
@@ -283,17 +282,16 @@ static StatsPlan plan_stats(const rb200_linear_ce_params& p, const DeviceInfo& d
     Carver c(ws);
     s.x = plan_pack(operand(p.x, p.ldx, p.rows, p.features, false), &c);
     s.w = plan_pack(operand(p.weight, p.ldw, p.classes, p.features, false), &c);
-    // a tile has 32 columns at least
+    // a tile has 32 columns at least, and two parts
     const size_t per_part = (size_t)p.rows * 3 * sizeof(float);
     long long parts = (long long)(kStatBytes / per_part);
-    long long piece = parts * 32 / kTileNMax * kTileNMax;
+    long long piece = parts / 2 * 32 / kTileNMax * kTileNMax;
     if (piece < kTileNMax) piece = kTileNMax;
     s.piece = (int)(piece < p.classes ? piece : p.classes);
-    const long long most = stats_gemm(p, dev, s.piece).tiles_n;
-    const long long rest = p.classes % s.piece ? stats_gemm(p, dev, (int)(p.classes % s.piece)).tiles_n : 0;
+    const long long most = 2ll * stats_gemm(p, dev, s.piece).tiles_n;
+    const long long rest = p.classes % s.piece ? 2ll * stats_gemm(p, dev, (int)(p.classes % s.piece)).tiles_n : 0;
     s.part_bytes = (size_t)(most > rest ? most : rest) * per_part;
     s.part = (float*)c.take(s.part_bytes);
-    s.zlabel = (float*)c.take((size_t)p.rows * sizeof(float));
     s.zsum = (float*)c.take((size_t)p.rows * sizeof(float));
     s.block_sums = (double*)c.take(kMergeBlocks * sizeof(double));
     s.bytes = c.used;
@@ -332,9 +330,9 @@ static int ce_forward(const rb200_linear_ce_params* p, cudaStream_t stream) {
         e.bias = p->bias ? at_row(p->bias, 1, c0) : nullptr;
         e.class0 = (int)c0;
         e.part = s.part;
-        e.parts = plan.tiles_n;
+        e.parts = 2 * plan.tiles_n;
         e.want_zsum = p->label_smoothing > 0.0f;
-        e.zlabel = s.zlabel;
+        e.zlabel = p->stats + 2 * p->rows;
         e.clear = p->info;
         const Operand w = operand(at_row(s.w.use.data, s.w.use.ld, c0), s.w.use.ld, classes, p->features, false);
         if ((rc = gemm_launch<EPI_CE_STATS, false, false>(bf16, s.x.use, w, nullptr, nullptr, plan, e, wait, stream, what))) return rc;
@@ -342,7 +340,6 @@ static int ce_forward(const rb200_linear_ce_params* p, cudaStream_t stream) {
         m.part = s.part;
         m.parts = e.parts;
         m.want_zsum = e.want_zsum;
-        m.zlabel = s.zlabel;
         m.labels = p->labels;
         m.label_bytes = p->label_bytes;
         m.classes = (int)p->classes;

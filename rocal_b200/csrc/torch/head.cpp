@@ -321,7 +321,7 @@ std::array<Tensor, 3> ce_run(const Tensor& x, const Tensor& weight, const Tensor
     CeArgs a = ce_args(x, weight, labels, bias, ignore_index, smoothing, reduce);
     const auto fp32 = x.options().dtype(at::kFloat);
     const Tensor loss = reduce == RB200_REDUCE_NONE ? at::empty({a.p.rows}, fp32) : at::empty({}, fp32);
-    const Tensor stats = at::empty({2, a.p.rows}, fp32), info = at::empty({4}, x.options().dtype(at::kInt));
+    const Tensor stats = at::empty({3, a.p.rows}, fp32), info = at::empty({4}, x.options().dtype(at::kInt));
     a.p.loss = loss.data_ptr<float>();
     a.p.stats = stats.data_ptr<float>();
     a.p.info = info.data_ptr<int32_t>();
@@ -344,7 +344,7 @@ std::vector<Tensor> ce_backward_run(const Tensor& dloss_, const Tensor& x, const
     TORCH_CHECK_VALUE(dloss_.scalar_type() == at::kFloat && dloss_.device() == x.device() &&
                           (reduce == RB200_REDUCE_NONE ? dloss_.dim() == 1 && dloss_.size(0) == n : dloss_.dim() == 0),
                       "dloss is ", dloss_.scalar_type(), " ", dloss_.sizes(), " on ", dloss_.device(), ", it has to be like the loss");
-    TORCH_CHECK_VALUE(stats.dim() == 2 && stats.size(0) == 2 && stats.size(1) == n && stats.scalar_type() == at::kFloat && stats.is_contiguous() &&
+    TORCH_CHECK_VALUE(stats.dim() == 2 && stats.size(0) == 3 && stats.size(1) == n && stats.scalar_type() == at::kFloat && stats.is_contiguous() &&
                           stats.device() == x.device() && info.dim() == 1 && info.size(0) == 4 && info.scalar_type() == at::kInt &&
                           info.is_contiguous() && info.device() == x.device(),
                       "stats and info are not those of this forward pass");
