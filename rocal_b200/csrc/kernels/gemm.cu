@@ -166,6 +166,8 @@ template <typename T, int SUBS>
 __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ part, int splits, long long stride, long long ldacc, int m, int n,
                                                    EpiArgs e) {
     constexpr int OUT = 256 / SUBS;
+    pdl_launch_dependents();
+    pdl_wait();
     __shared__ float4 sums[SUBS][OUT];
     const long long groups = (n + 3) / 4, total = groups * m;
     const float alpha = e.scale.value();
@@ -235,22 +237,19 @@ size_t gemm_partial_bytes(const GemmPlan& plan, int m, int n) {
 }
 
 template <typename T>
-static void join_launch(const float* partials, int splits, int m, int n, const EpiArgs& e, cudaStream_t stream) {
+static cudaError_t join_launch(const float* partials, int splits, int m, int n, const EpiArgs& e, cudaStream_t stream) {
     const long long ldacc = round_up(n, 4), total = ldacc / 4 * m;
     const int out = splits >= 16 ? 32 : 256;
     const long long blocks = (total + out - 1) / out;
-    const unsigned grid = (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16);
-    if (splits >= 16)
-        join_kernel<T, 8><<<grid, 256, 0, stream>>>(partials, splits, ldacc * m, ldacc, m, n, e);
-    else
-        join_kernel<T, 1><<<grid, 256, 0, stream>>>(partials, splits, ldacc * m, ldacc, m, n, e);
+    const dim3 grid((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16));
+    return launch_overlapped(splits >= 16 ? join_kernel<T, 8> : join_kernel<T, 1>, grid, dim3(256), 0, stream, partials, splits, ldacc * m, ldacc, m,
+                             n, e);
 }
 int gemm_join(bool bf16, const float* partials, int splits, int m, int n, const EpiArgs& e, cudaStream_t stream, const char* what) {
-    if (bf16)
-        join_launch<__nv_bfloat16>(partials, splits, m, n, e, stream);
-    else
-        join_launch<__half>(partials, splits, m, n, e, stream);
-    RB200_CHECK_LAUNCH(what);
+    int rc = check_cuda(bf16 ? join_launch<__nv_bfloat16>(partials, splits, m, n, e, stream) : join_launch<__half>(partials, splits, m, n, e, stream),
+                        what);
+    if (rc) return rc;
+    count_launch();
     return RB200_OK;
 }
 
@@ -268,26 +267,44 @@ int gemm_store_joined(int kind, bool bf16, const Operand& a, const Operand& b, c
 }
 
 // ---- packing --------------------------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) pack_kernel(const uint16_t* __restrict__ src, long long lds, int rows, int cols, uint16_t* __restrict__ dst,
-                                                   long long ldd) {
-    const long long groups = (cols + 7) / 8, total = groups * rows;
-    for (long long t = blockIdx.x * 256ll + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
+struct PackArgs {
+    const uint16_t* src[2];
+    uint16_t* dst[2];
+    long long lds[2], ldd[2], total[2];   // total: pieces of 8 elements
+    int cols[2];
+};
+__global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int w = blockIdx.y, cols = a.cols[w];
+    const long long groups = (cols + 7) / 8;
+    for (long long t = blockIdx.x * 256ll + threadIdx.x; t < a.total[w]; t += (long long)gridDim.x * 256) {
         const long long row = t / groups;
         const int col = (int)(t - row * groups) * 8;
-        const uint16_t* p = src + row * lds + col;
-        uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (col + i < cols) w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
-        *reinterpret_cast<uint4*>(dst + row * ldd + col) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(a.dst[w] + row * a.ldd[w] + col) = load8(a.src[w] + row * a.lds[w] + col, cols - col, false);
     }
 }
 
-int pack_rows(const Operand& src, void* dst, long long ldd, cudaStream_t stream, const char* what) {
-    const long long total = (long long)((src.cols + 7) / 8) * src.rows, blocks = (total + 255) / 256;
-    pack_kernel<<<(unsigned)(blocks < 148 * 32 ? blocks : 148 * 32), 256, 0, stream>>>((const uint16_t*)src.data, src.ld, src.rows, src.cols,
-                                                                                     (uint16_t*)dst, ldd);
-    RB200_CHECK_LAUNCH(what);
+int pack_operands(const Packed* a, const Packed* b, cudaStream_t stream, const char* what) {
+    PackArgs p = {};
+    int n = 0;
+    long long most = 0;
+    for (const Packed* o : {a, b}) {
+        if (!o || !o->copy) continue;
+        p.src[n] = (const uint16_t*)o->src.data;
+        p.lds[n] = o->src.ld;
+        p.cols[n] = o->src.cols;
+        p.dst[n] = (uint16_t*)const_cast<void*>(o->use.data);
+        p.ldd[n] = o->use.ld;
+        p.total[n] = (long long)((o->src.cols + 7) / 8) * o->src.rows;
+        if (p.total[n] > most) most = p.total[n];
+        n++;
+    }
+    if (n == 0) return RB200_OK;
+    const long long blocks = (most + 255) / 256;
+    int rc = check_cuda(launch_overlapped(pack_kernel, dim3((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), n), dim3(256), 0, stream, p), what);
+    if (rc) return rc;
+    count_launch();
     return RB200_OK;
 }
 

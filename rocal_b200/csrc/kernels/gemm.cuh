@@ -345,6 +345,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         __syncthreads();
     tc::fence_after();
     const uint32_t tmem = tmem_addr_s;
+    pdl_launch_dependents();
+    pdl_wait();   // everything above touches this CTA's own state only
     if (EPI == EPI_CE_STATS && g.e.clear && blockIdx.x == 0 && threadIdx.x < 4) g.e.clear[threadIdx.x] = 0;
     const tc::Patience patience = {&gave_up_s, g.status, g.wait_cycles};
 
@@ -509,6 +511,21 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 if constexpr (EPI != EPI_STORE) {
                     if (work && g.e.bias && lane < count) own_bias = Elem<T>::to_float(reinterpret_cast<const T*>(g.e.bias)[col + lane]);
                 }
+                uint4 res[4];   // the residual's strip: lane l takes piece l % 4 of the rows l / 4 + 8 i
+                if constexpr (EPI == EPI_LINEAR) {
+                    if (work && g.e.residual) {
+                        const int left = count - (lane & 3) * 8;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int r = row0 + (lane >> 2) + 8 * i;
+                            res[i] = make_uint4(0, 0, 0, 0);
+                            if (r < g.m && left > 0)
+                                res[i] = load8(reinterpret_cast<const T*>(g.e.residual) + (long long)(r % g.e.residual_rows) * g.e.ldr + col +
+                                                   (lane & 3) * 8,
+                                               left, g.e.vec_res);
+                        }
+                    }
+                }
                 tc::tmem_wait();
                 if (c + 64 >= g.bn) {   // this warp's part of the accumulator is in registers
                     tc::fence_before();
@@ -553,17 +570,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                         act_values<16>(v + 16, g.e.act);
                     }
                     if (g.e.residual) {   // the other way round: whole pieces of rows in, a row a thread out
-                        const int piece = lane & 3, left = count - piece * 8;
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int r = (lane >> 2) + 8 * i;
-                            uint4 w = make_uint4(0, 0, 0, 0);
-                            if (row0 + r < g.m && left > 0)
-                                w = load8(reinterpret_cast<const T*>(g.e.residual) + (long long)((row0 + r) % g.e.residual_rows) * g.e.ldr + col +
-                                              piece * 8,
-                                          left, g.e.vec_res);
-                            st_shared16(staged(area, r, piece), w);
-                        }
+                        for (int i = 0; i < 4; i++) st_shared16(staged(area, (lane >> 2) + 8 * i, lane & 3), res[i]);
                         __syncwarp();
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
@@ -747,13 +755,15 @@ int gemm_launch_as(const GemmArgs& g, const DeviceInfo& dev, cudaStream_t stream
     cfg.blockDim = dim3(kGemmThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CG;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = CG;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = CG == 2 ? 1 : 0;
+    cfg.numAttrs = CG == 2 ? 2 : 1;
     rc = check_cuda(cudaLaunchKernelEx(&cfg, kernel, g), what);
     if (rc) return rc;
     count_launch();
@@ -797,17 +807,23 @@ int gemm_store_joined(int kind, bool bf16, const Operand& a, const Operand& b, c
                       EpiArgs e, void* partials, const GemmWait& wait, cudaStream_t stream, const char* what);
 // Joins the pieces: sum over splits (and acc_in), to acc_out, or scaled with bias, activation and residual to out.
 int gemm_join(bool bf16, const float* partials, int splits, int m, int n, const EpiArgs& e, cudaStream_t stream, const char* what);
-// dst[rows][ldd] = src, for operands whose rows no tensor map can describe.
-int pack_rows(const Operand& src, void* dst, long long ldd, cudaStream_t stream, const char* what);
+// An operand as a product reads it: in place, or from a copy in the workspace (operands whose rows no tensor map can
+// describe). pack_operands makes the copies of up to two operands in one launch.
+struct Packed {
+    Operand src, use;
+    bool copy;
+};
+int pack_operands(const Packed* a, const Packed* b, cudaStream_t stream, const char* what);
 
 // Column sums of a matrix in a workspace, its rows padded to 8 elements (linear.cu): chunks planes of ldpart partial sums,
-// joined (with other planes) by sum_chunks.
+// joined (with other planes) by sum_chunks; of few rows the sums themselves (chunks = 0: no planes are needed).
 struct ColumnSums {
     int chunks;
     long long ldpart;
 };
-ColumnSums plan_column_sums(int rows, int cols, int sms);
-int column_partials(bool bf16, const Operand& src, float* part, int sms, cudaStream_t stream, const char* what);
+ColumnSums plan_column_sums(int rows, int cols, int sms, bool whole);
+int column_partials(bool bf16, const Operand& src, bool whole, float* part, void* out, const Scale& scale, int sms, cudaStream_t stream,
+                    const char* what);
 int sum_chunks(bool bf16, const float* part, long long ldpart, int planes, int rows, int cols, void* out, long long ldo, const Scale& scale,
                cudaStream_t stream, const char* what);
 

@@ -1,7 +1,7 @@
 // rb200k_grad_clip: norm over many tensors and clipping. Two sweeps, both bound by memory: the first adds the squares,
 // the second multiplies. The tensors' table travels in the launch's own parameters (no copy, nothing to keep alive, and
 // a captured graph holds it). Tensors are cut into chunks of one size, which blocks take in turn; the second sweep walks
-// the chunks backwards, so that what the first one read last is still in L2.
+// the chunks backwards, so that what the first one read last is still in L2. Few elements take one launch.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -94,19 +94,33 @@ __device__ __forceinline__ double square_sum(const T* p, int count) {
     count -= head;
     const uint4* q = reinterpret_cast<const uint4*>(p);
     const int vectors = count / N;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < vectors; i += kClipThreads) {
+    auto add = [&](const uint4& w) {
         float v[N];
-        Values<T>::get(__ldg(q + i), v);
+        Values<T>::get(w, v);
 #pragma unroll
         for (int j = 0; j < N; j++) s += (double)v[j] * (double)v[j];
+    };
+    int i = threadIdx.x;
+    for (; i + 3 * kClipThreads < vectors; i += 4 * kClipThreads) {   // four vectors in flight
+        uint4 w[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) w[k] = __ldg(q + i + k * kClipThreads);
+#pragma unroll
+        for (int k = 0; k < 4; k++) add(w[k]);
     }
+    for (; i < vectors; i += kClipThreads) add(__ldg(q + i));
     const int tail = vectors * N + threadIdx.x;
     if (tail < count) {
         const double v = Values<T>::to_float(p[tail]);
         s += v * v;
     }
     return s;
+}
+
+__device__ __forceinline__ double square_piece(const ClipEntry& e, long long begin, int count) {
+    if (e.grad_dtype == RB200_FP32) return square_sum(reinterpret_cast<const float*>(e.grad) + begin, count);
+    if (e.grad_dtype == RB200_FP16) return square_sum(reinterpret_cast<const __half*>(e.grad) + begin, count);
+    return square_sum(reinterpret_cast<const __nv_bfloat16*>(e.grad) + begin, count);
 }
 
 // The block's sum, in thread 0.
@@ -123,86 +137,145 @@ __device__ __forceinline__ double block_sum(double s, double* shared) {
 template <int CAP>
 __global__ void __launch_bounds__(kClipThreads) clip_norm_kernel(const __grid_constant__ ClipTable<CAP> t, double* partial) {
     __shared__ double shared[kClipThreads / 32];
+    pdl_launch_dependents();
+    pdl_wait();
     double s = 0.0;
     for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
         const ClipEntry& e = t.e[find_tensor(t, c)];
         const long long begin = (long long)(c - e.chunk0) * t.chunk;
         const int count = (int)min((long long)t.chunk, e.count - begin);
-        if (e.grad_dtype == RB200_FP32)
-            s += square_sum(reinterpret_cast<const float*>(e.grad) + begin, count);
-        else if (e.grad_dtype == RB200_FP16)
-            s += square_sum(reinterpret_cast<const __half*>(e.grad) + begin, count);
-        else
-            s += square_sum(reinterpret_cast<const __nv_bfloat16*>(e.grad) + begin, count);
+        s += square_piece(e, begin, count);
     }
     s = block_sum(s, shared);
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 
 // ---- multiplication -----------------------------------------------------------------------------------------
-// Sixteen bytes that start SHIFT words and `bits` bits into two neighbouring aligned vectors.
-template <int SHIFT>
-__device__ __forceinline__ uint4 window(const uint4& a, const uint4& b, int bits) {
-    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    return make_uint4(__funnelshift_r(w[SHIFT], w[SHIFT + 1], bits), __funnelshift_r(w[SHIFT + 1], w[SHIFT + 2], bits),
-                      __funnelshift_r(w[SHIFT + 2], w[SHIFT + 3], bits), __funnelshift_r(w[SHIFT + 3], w[(SHIFT + 4) & 7], bits));
+// W words (the gradients of one 16-byte vector of the output) that start SHIFT words and `bits` bits into two neighbouring
+// aligned vectors of W words.
+template <int W, int SHIFT>
+__device__ __forceinline__ void window(const uint32_t (&w)[2 * W], uint32_t (&out)[W], int bits) {
+#pragma unroll
+    for (int k = 0; k < W; k++) out[k] = __funnelshift_r(w[SHIFT + k], w[(SHIFT + k + 1) % (2 * W)], bits);
 }
+template <int W>
+__device__ __forceinline__ void load_words(const uint32_t* p, uint32_t* w) {
+    if constexpr (W == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        w[0] = v.x;
+        w[1] = v.y;
+        w[2] = v.z;
+        w[3] = v.w;
+    } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x;
+        w[1] = v.y;
+    }
+}
+// One output vector: as many gradients as sixteen bytes of the output hold, so that a warp's stores are whole lines.
 template <typename T, typename O>
-__device__ __forceinline__ void scale_vector(const uint4& w, O* o, int i, float factor) {
-    constexpr int N = Values<T>::N, M = Values<O>::N;
+__device__ __forceinline__ uint4 scale_words(const uint32_t* w, float factor) {
+    constexpr int N = Values<O>::N;
     float v[N];
-    Values<T>::get(w, v);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < N; j++) v[j] = __uint_as_float(w[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+            const float2 f = Elem<T>::unpack(w[j / 2]);
+            v[j] = f.x;
+            v[j + 1] = f.y;
+        }
+    }
 #pragma unroll
     for (int j = 0; j < N; j++) v[j] *= factor;
-#pragma unroll
-    for (int j = 0; j < N; j += M) reinterpret_cast<uint4*>(o)[i * (N / M) + j / M] = Values<O>::put(v + j);
+    return Values<O>::put(v);
 }
-// SHIFT < 0: the gradients have the output's boundaries. Four vectors in flight a thread.
+// SHIFT < 0: the gradients have boundaries of their own words where the output has its 16-byte ones.
 template <typename T, typename O, int SHIFT>
 __device__ __forceinline__ void scale_vectors(const T* g, O* o, int vectors, float factor) {
-    constexpr int U = 4;
-    const uint4* q = reinterpret_cast<const uint4*>((uintptr_t)g & ~(uintptr_t)15);
+    constexpr int W = Values<O>::N * (int)sizeof(T) / 4, U = 16 / W;   // U vectors in flight
+    const uint32_t* q = reinterpret_cast<const uint32_t*>((uintptr_t)g & ~(uintptr_t)(4 * W - 1));
     const int bits = (int)((uintptr_t)g & 3) * 8;
-    auto fetch = [&](int i) {   // the second vector is one that the sixteen bytes reach into
-        if constexpr (SHIFT < 0)
-            return q[i];
-        else
-            return window<SHIFT>(q[i], q[i + 1], bits);
+    uint4* out = reinterpret_cast<uint4*>(o);
+    auto fetch = [&](int i, uint32_t (&w)[W]) {   // the second vector is one that the window reaches into
+        if constexpr (SHIFT < 0) {
+            load_words<W>(q + i * W, w);
+        } else {
+            uint32_t both[2 * W];
+            load_words<W>(q + i * W, both);
+            load_words<W>(q + (i + 1) * W, both + W);
+            window<W, SHIFT>(both, w, bits);
+        }
     };
     int i = threadIdx.x;
     for (; i + (U - 1) * kClipThreads < vectors; i += U * kClipThreads) {
-        uint4 w[U];
+        uint32_t w[U][W];
 #pragma unroll
-        for (int k = 0; k < U; k++) w[k] = fetch(i + k * kClipThreads);
+        for (int k = 0; k < U; k++) fetch(i + k * kClipThreads, w[k]);
 #pragma unroll
-        for (int k = 0; k < U; k++) scale_vector<T>(w[k], o, i + k * kClipThreads, factor);
+        for (int k = 0; k < U; k++) out[i + k * kClipThreads] = scale_words<T, O>(w[k], factor);
     }
-    for (; i < vectors; i += kClipThreads) scale_vector<T>(fetch(i), o, i, factor);
+    for (; i < vectors; i += kClipThreads) {
+        uint32_t w[W];
+        fetch(i, w);
+        out[i] = scale_words<T, O>(w, factor);
+    }
 }
 // Whole vectors are written where the output has its 16-byte boundaries; the gradients that belong there are cut out of
 // the aligned vectors that hold them.
 template <typename T, typename O>
 __device__ __forceinline__ void scale_chunk(const T* g, O* o, int count, float factor) {
-    constexpr int N = Values<T>::N;
+    constexpr int N = Values<O>::N, W = N * (int)sizeof(T) / 4;
     const int head = min(count, (int)(((16 - ((uintptr_t)o & 15)) & 15) / sizeof(O)));
     if ((int)threadIdx.x < head) o[threadIdx.x] = Values<O>::from_float(Values<T>::to_float(g[threadIdx.x]) * factor);
     g += head;
     o += head;
     count -= head;
-    const int vectors = count / N;
-    const int offset = (int)((uintptr_t)g & 15);
+    const int vectors = count / N, offset = (int)((uintptr_t)g & (4 * W - 1));
     if (offset == 0) {
         scale_vectors<T, O, -1>(g, o, vectors, factor);
+    } else if (W == 2) {
+        if (offset < 4)
+            scale_vectors<T, O, 0>(g, o, vectors, factor);
+        else
+            scale_vectors<T, O, 1>(g, o, vectors, factor);
     } else {
         switch (offset >> 2) {
             case 0: scale_vectors<T, O, 0>(g, o, vectors, factor); break;
             case 1: scale_vectors<T, O, 1>(g, o, vectors, factor); break;
-            case 2: scale_vectors<T, O, 2>(g, o, vectors, factor); break;
-            default: scale_vectors<T, O, 3>(g, o, vectors, factor); break;
+            case 2: scale_vectors<T, O, W == 2 ? 0 : 2>(g, o, vectors, factor); break;
+            default: scale_vectors<T, O, W == 2 ? 1 : 3>(g, o, vectors, factor); break;
         }
     }
     const int tail = vectors * N + threadIdx.x;
     if (tail < count) o[tail] = Values<O>::from_float(Values<T>::to_float(g[tail]) * factor);
+}
+__device__ __forceinline__ void scale_piece(const ClipEntry& e, long long begin, int count, float factor) {
+    if (factor == 1.0f && e.out == e.grad) return;
+    if (e.grad_dtype == RB200_FP32) {
+        scale_chunk(reinterpret_cast<const float*>(e.grad) + begin, reinterpret_cast<float*>(e.out) + begin, count, factor);
+    } else if (e.grad_dtype == RB200_FP16) {
+        const __half* g = reinterpret_cast<const __half*>(e.grad) + begin;
+        if (e.out_dtype == RB200_FP32)
+            scale_chunk(g, reinterpret_cast<float*>(e.out) + begin, count, factor);
+        else
+            scale_chunk(g, reinterpret_cast<__half*>(e.out) + begin, count, factor);
+    } else {
+        const __nv_bfloat16* g = reinterpret_cast<const __nv_bfloat16*>(e.grad) + begin;
+        if (e.out_dtype == RB200_FP32)
+            scale_chunk(g, reinterpret_cast<float*>(e.out) + begin, count, factor);
+        else
+            scale_chunk(g, reinterpret_cast<__nv_bfloat16*>(e.out) + begin, count, factor);
+    }
+}
+// The norm and the factor of a sum of squares.
+__device__ __forceinline__ float clip_factor(double sum, float max_norm, float inv_scale, float* norm) {
+    const float n = (float)(sqrt(sum) * (double)inv_scale);
+    const float c = max_norm / (n + 1e-6f);
+    if (norm) *norm = n;
+    return (c > 1.0f ? 1.0f : c) * inv_scale;   // NaN stays
 }
 
 template <int CAP>
@@ -210,57 +283,84 @@ __global__ void __launch_bounds__(kClipThreads) clip_scale_kernel(const __grid_c
                                                                   int partials, float max_norm, float inv_scale, float* norm) {
     __shared__ double shared[kClipThreads / 32];
     __shared__ float factor_s;
+    pdl_launch_dependents();
+    pdl_wait();
     double s = 0.0;
     for (int i = threadIdx.x; i < partials; i += kClipThreads) s += partial[i];
     s = block_sum(s, shared);
-    if (threadIdx.x == 0) {
-        const float n = (float)(sqrt(s) * (double)inv_scale);
-        const float c = max_norm / (n + 1e-6f);
-        factor_s = (c > 1.0f ? 1.0f : c) * inv_scale;   // NaN stays
-        if (norm && blockIdx.x == 0) *norm = n;
-    }
+    if (threadIdx.x == 0) factor_s = clip_factor(s, max_norm, inv_scale, blockIdx.x == 0 ? norm : nullptr);
     __syncthreads();
     const float factor = factor_s;
     for (int i = blockIdx.x; i < t.chunks; i += gridDim.x) {
         const int c = t.chunks - 1 - i;
         const ClipEntry& e = t.e[find_tensor(t, c)];
         const long long begin = (long long)(c - e.chunk0) * t.chunk;
-        const int count = (int)min((long long)t.chunk, e.count - begin);
-        if (factor == 1.0f && e.out == e.grad) continue;
-        if (e.grad_dtype == RB200_FP32) {
-            scale_chunk(reinterpret_cast<const float*>(e.grad) + begin, reinterpret_cast<float*>(e.out) + begin, count, factor);
-        } else if (e.grad_dtype == RB200_FP16) {
-            const __half* g = reinterpret_cast<const __half*>(e.grad) + begin;
-            if (e.out_dtype == RB200_FP32)
-                scale_chunk(g, reinterpret_cast<float*>(e.out) + begin, count, factor);
-            else
-                scale_chunk(g, reinterpret_cast<__half*>(e.out) + begin, count, factor);
-        } else {
-            const __nv_bfloat16* g = reinterpret_cast<const __nv_bfloat16*>(e.grad) + begin;
-            if (e.out_dtype == RB200_FP32)
-                scale_chunk(g, reinterpret_cast<float*>(e.out) + begin, count, factor);
-            else
-                scale_chunk(g, reinterpret_cast<__nv_bfloat16*>(e.out) + begin, count, factor);
-        }
+        scale_piece(e, begin, (int)min((long long)t.chunk, e.count - begin), factor);
+    }
+}
+
+// ---- both sweeps in one launch ----------------------------------------------------------------------------------
+// Few elements: one cluster of eight blocks, which exchange their sums through distributed shared memory. Sums are added in
+// rank order by every block, so all of them have the same factor.
+constexpr int kClipCluster = 8;
+constexpr long long kClipFew = 131072;
+template <int CAP>
+__global__ void __launch_bounds__(kClipThreads) __cluster_dims__(kClipCluster, 1, 1)
+    clip_few_kernel(const __grid_constant__ ClipTable<CAP> t, float max_norm, float inv_scale, float* norm) {
+    __shared__ double shared[kClipThreads / 32];
+    __shared__ double sums[kClipCluster];
+    __shared__ float factor_s;
+    pdl_launch_dependents();
+    pdl_wait();
+    double s = 0.0;
+    for (int c = blockIdx.x; c < t.chunks; c += kClipCluster) {
+        const ClipEntry& e = t.e[find_tensor(t, c)];
+        const long long begin = (long long)(c - e.chunk0) * t.chunk;
+        s += square_piece(e, begin, (int)min((long long)t.chunk, e.count - begin));
+    }
+    s = block_sum(s, shared);
+    if (threadIdx.x == 0) {
+        const uint32_t mine = tc::smem_u32(&sums[tc::cta_rank()]);
+#pragma unroll
+        for (int r = 0; r < kClipCluster; r++)
+            asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(tc::map_to_rank(mine, r)), "d"(s) : "memory");
+    }
+    __syncwarp();
+    tc::cluster_sync();
+    if (threadIdx.x == 0) {
+        s = 0.0;
+        for (int r = 0; r < kClipCluster; r++) s += sums[r];
+        factor_s = clip_factor(s, max_norm, inv_scale, blockIdx.x == 0 ? norm : nullptr);
+    }
+    __syncthreads();
+    const float factor = factor_s;
+    for (int c = blockIdx.x; c < t.chunks; c += kClipCluster) {
+        const ClipEntry& e = t.e[find_tensor(t, c)];
+        const long long begin = (long long)(c - e.chunk0) * t.chunk;
+        scale_piece(e, begin, (int)min((long long)t.chunk, e.count - begin), factor);
     }
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------
 constexpr int kClipSmall = 16, kClipMedium = 192, kClipLarge = 960;   // 960 entries: 30 KB of launch parameters
 
+enum { CLIP_NORM, CLIP_SCALE, CLIP_FEW };
 template <int CAP>
-static int clip_table_launch(const ClipEntry* entries, int n, int chunks, int chunk, bool scale, double* partial, int partials, float max_norm,
+static int clip_table_launch(const ClipEntry* entries, int n, int chunks, int chunk, int sweep, double* partial, int partials, float max_norm,
                              float inv_scale, float* norm, int blocks, cudaStream_t stream) {
     ClipTable<CAP> t;
     for (int i = 0; i < n; i++) t.e[i] = entries[i];
     t.n = n;
     t.chunks = chunks;
     t.chunk = chunk;
-    if (scale)
-        clip_scale_kernel<CAP><<<blocks, kClipThreads, 0, stream>>>(t, partial, partials, max_norm, inv_scale, norm);
-    else
-        clip_norm_kernel<CAP><<<blocks, kClipThreads, 0, stream>>>(t, partial);
-    RB200_CHECK_LAUNCH("rb200k_grad_clip");
+    const dim3 grid(blocks), block(kClipThreads);
+    int rc = check_cuda(sweep == CLIP_NORM    ? launch_overlapped(clip_norm_kernel<CAP>, grid, block, 0, stream, t, partial)
+                        : sweep == CLIP_SCALE ? launch_overlapped(clip_scale_kernel<CAP>, grid, block, 0, stream, t, (const double*)partial, partials,
+                                                                  max_norm, inv_scale, norm)
+                                              : launch_overlapped(clip_few_kernel<CAP>, grid, block, 0, stream, t, max_norm, inv_scale, norm),
+                        "rb200k_grad_clip");
+    if (rc) return rc;
+    count_launch();
     return RB200_OK;
 }
 
@@ -347,9 +447,11 @@ static int clip_run(const rb200_grad_tensor* tensors, int n, float max_norm, flo
     long long chunk = round_up((total + 4 * most - 1) / (4 * most), 2048);
     chunk = std::min(chunk, 16384ll);
     while (total / chunk > (1ll << 30)) chunk *= 2;
+    const bool few = total <= kClipFew && v.size() <= kClipMedium;
+    if (few) chunk = round_up((total + kClipCluster - 1) / kClipCluster, 2048);
     double* partial = (double*)ws;
     int partials = 0;
-    for (int pass = 0; pass < 2; pass++) {
+    for (int pass = 0; pass < (few ? 1 : 2); pass++) {
         const size_t tables = (v.size() + kClipLarge - 1) / kClipLarge;
         for (size_t k = 0; k < tables; k++) {
             const size_t b = pass ? tables - 1 - k : k;   // the second sweep starts with the last table
@@ -360,10 +462,10 @@ static int clip_run(const rb200_grad_tensor* tensors, int n, float max_norm, flo
                 first[i].chunk0 = chunks;
                 chunks += (int)((first[i].count + chunk - 1) / chunk);
             }
-            const int blocks = std::min(chunks, most);
+            const int blocks = few ? kClipCluster : std::min(chunks, most);
             auto* launch = count <= kClipSmall ? clip_table_launch<kClipSmall>
                                                : count <= kClipMedium ? clip_table_launch<kClipMedium> : clip_table_launch<kClipLarge>;
-            rc = launch(first, count, chunks, (int)chunk, pass == 1, pass ? partial : partial + partials, partials, max_norm, inv_scale,
+            rc = launch(first, count, chunks, (int)chunk, few ? CLIP_FEW : pass ? CLIP_SCALE : CLIP_NORM, pass ? partial : partial + partials, partials, max_norm, inv_scale,
                         k == 0 ? norm : nullptr, blocks, stream);
             if (rc) return rc;
             if (pass == 0) partials += blocks;

@@ -9,7 +9,7 @@ namespace rb200 {
 // Rows j, j + period, j + 2 period, ... of `src` are summed into partial sums [chunk][j][column] in 32 bits; with
 // `preact` the elements are first multiplied by the activation's slope, and with `dst` what was read (multiplied) is
 // written, in the element type. A block takes up to 256 columns (8 a thread, as many threads side by side as the columns
-// need, the others on further rows) and a chunk of the repeats; a thread has four rows in flight. The row sums meet in
+// need, the others on further rows) and a chunk of the repeats; a thread has two or four rows in flight. The row sums meet in
 // shared memory, chunks meet in sum_chunks_kernel, always in the same order. Bound by memory.
 struct RowsArgs {
     const void* src;
@@ -22,6 +22,7 @@ struct RowsArgs {
     long long ldpart;
     void* out;                // one chunk only: the sums in the element type, [period][ldo], or null
     long long ldo;
+    Scale scale;              // of what goes to out
     int rows, cols, period, chunks, per_chunk;   // per_chunk: repeats of a chunk
     int readable;             // columns that may be read: cols, or more where the rows are padded
     int across;               // threads side by side: a power of two up to 32
@@ -29,8 +30,10 @@ struct RowsArgs {
 };
 
 template <typename T, bool SLOPE>
-__global__ void __launch_bounds__(256) rows_kernel(RowsArgs a) {
-    constexpr int U = 4;   // rows in flight
+__global__ void __launch_bounds__(256, 4) rows_kernel(RowsArgs a) {
+    constexpr int U = SLOPE ? 2 : 4;   // rows in flight
+    pdl_launch_dependents();
+    pdl_wait();
     __shared__ float sums[256 * 8];
     __shared__ float half[256];
     const int lane = threadIdx.x & (a.across - 1), sub = threadIdx.x / a.across, subs = 256 / a.across, wide = a.across * 8;
@@ -52,7 +55,8 @@ __global__ void __launch_bounds__(256) rows_kernel(RowsArgs a) {
             if (SLOPE) {
                 float s[8];
                 unpack8<T>(z, s);
-                act_slopes<8>(s, a.act);
+                act_slopes<4>(s, a.act);
+                act_slopes<4>(s + 4, a.act);
 #pragma unroll
                 for (int k = 0; k < 8; k++) v[k] *= s[k];
             }
@@ -93,7 +97,7 @@ __global__ void __launch_bounds__(256) rows_kernel(RowsArgs a) {
             if (piece == 0 && out_col < a.cols) {
                 for (int k = 1; k < 256 / wide; k++) s += half[k * wide + c];
                 if (a.part) a.part[u * a.ldpart + out_col] = s;
-                if (a.out) reinterpret_cast<T*>(a.out)[j * a.ldo + out_col] = Elem<T>::from_float(s);
+                if (a.out) reinterpret_cast<T*>(a.out)[j * a.ldo + out_col] = Elem<T>::from_float(s * a.scale.value());
             }
             __syncthreads();
         }
@@ -105,6 +109,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) sum_chunks_kernel(const float* __restrict__ part, long long ldpart, int planes, int rows, int cols, T* out,
                                                          long long ldo, Scale scale) {
     __shared__ float sums[32][9];
+    pdl_launch_dependents();
+    pdl_wait();
     const int lane = threadIdx.x & 7, sub = threadIdx.x >> 3, col = blockIdx.x * 8 + lane;
     const float factor = scale.value();
     for (int j = blockIdx.y; j < rows; j += gridDim.y) {
@@ -128,6 +134,8 @@ __global__ void __launch_bounds__(256) sum_chunks_kernel(const float* __restrict
 template <typename T>
 __global__ void __launch_bounds__(256) sum_few_kernel(const float* __restrict__ part, long long ldpart, int planes, int rows, int cols, T* out,
                                                       long long ldo, Scale scale) {
+    pdl_launch_dependents();
+    pdl_wait();
     const float factor = scale.value();
     const long long total = (long long)rows * cols;
     for (long long t = blockIdx.x * 256ll + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
@@ -158,64 +166,67 @@ static int rows_launch(bool bf16, const RowsArgs& a, cudaStream_t stream, const 
     const long long units = (long long)a.period * a.chunks;
     const int wide = a.across * 8;
     const dim3 grid((unsigned)((a.cols + wide - 1) / wide), (unsigned)(units < 32768 ? units : 32768));
-    if (bf16) {
-        if (a.preact)
-            rows_kernel<__nv_bfloat16, true><<<grid, 256, 0, stream>>>(a);
-        else
-            rows_kernel<__nv_bfloat16, false><<<grid, 256, 0, stream>>>(a);
-    } else {
-        if (a.preact)
-            rows_kernel<__half, true><<<grid, 256, 0, stream>>>(a);
-        else
-            rows_kernel<__half, false><<<grid, 256, 0, stream>>>(a);
-    }
-    RB200_CHECK_LAUNCH(what);
+    auto* kernel = bf16 ? (a.preact ? rows_kernel<__nv_bfloat16, true> : rows_kernel<__nv_bfloat16, false>)
+                        : (a.preact ? rows_kernel<__half, true> : rows_kernel<__half, false>);
+    int rc = check_cuda(launch_overlapped(kernel, grid, dim3(256), 0, stream, a), what);
+    if (rc) return rc;
+    count_launch();
     return RB200_OK;
 }
 
 template <typename T>
-static void sum_launch(const float* part, long long ldpart, int planes, int rows, int cols, T* out, long long ldo, const Scale& scale,
-                       cudaStream_t stream) {
-    if (planes < 32) {
-        const long long blocks = ((long long)rows * cols + 255) / 256;
-        sum_few_kernel<T><<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, stream>>>(part, ldpart, planes, rows, cols, out, ldo, scale);
-    } else {
-        const dim3 grid((unsigned)((cols + 7) / 8), (unsigned)(rows < 32768 ? rows : 32768));
-        sum_chunks_kernel<T><<<grid, 256, 0, stream>>>(part, ldpart, planes, rows, cols, out, ldo, scale);
-    }
+static cudaError_t sum_launch(const float* part, long long ldpart, int planes, int rows, int cols, T* out, long long ldo, const Scale& scale,
+                              cudaStream_t stream) {
+    const long long blocks = ((long long)rows * cols + 255) / 256;
+    const dim3 grid = planes < 32 ? dim3((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16))
+                                  : dim3((unsigned)((cols + 7) / 8), (unsigned)(rows < 32768 ? rows : 32768));
+    return launch_overlapped(planes < 32 ? sum_few_kernel<T> : sum_chunks_kernel<T>, grid, dim3(256), 0, stream, part, ldpart, planes, rows, cols,
+                             out, ldo, scale);
 }
 int sum_chunks(bool bf16, const float* part, long long ldpart, int planes, int rows, int cols, void* out, long long ldo, const Scale& scale,
                cudaStream_t stream, const char* what) {
-    if (bf16)
-        sum_launch(part, ldpart, planes, rows, cols, (__nv_bfloat16*)out, ldo, scale, stream);
-    else
-        sum_launch(part, ldpart, planes, rows, cols, (__half*)out, ldo, scale, stream);
-    RB200_CHECK_LAUNCH(what);
+    int rc = check_cuda(bf16 ? sum_launch(part, ldpart, planes, rows, cols, (__nv_bfloat16*)out, ldo, scale, stream)
+                             : sum_launch(part, ldpart, planes, rows, cols, (__half*)out, ldo, scale, stream),
+                        what);
+    if (rc) return rc;
+    count_launch();
     return RB200_OK;
 }
 
-ColumnSums plan_column_sums(int rows, int cols, int sms) {
+// Few rows: one chunk, 64 columns a block, and the sums leave at once - one launch (5 us for 1024 x 1000) instead of
+// two (3 + 3 us and a launch).
+constexpr int kFewRows = 2048;
+static RowsArgs column_args(int rows, int cols, int sms, bool whole) {
     RowsArgs a = {};
     a.rows = rows;
     a.cols = cols;
     a.period = 1;
     cut_rows(&a, sms);
-    ColumnSums c = {a.chunks, round_up(cols, 4)};
+    if (whole && rows <= kFewRows) {
+        if (a.across > 8) a.across = 8;
+        a.chunks = 1;
+        a.per_chunk = rows;
+    }
+    return a;
+}
+ColumnSums plan_column_sums(int rows, int cols, int sms, bool whole) {
+    ColumnSums c = {whole && rows <= kFewRows ? 0 : column_args(rows, cols, sms, whole).chunks, round_up(cols, 4)};
     return c;
 }
-
-int column_partials(bool bf16, const Operand& src, float* part, int sms, cudaStream_t stream, const char* what) {
-    RowsArgs a = {};
+int column_partials(bool bf16, const Operand& src, bool whole, float* part, void* out, const Scale& scale, int sms, cudaStream_t stream,
+                    const char* what) {
+    RowsArgs a = column_args(src.rows, src.cols, sms, whole);
     a.src = src.data;
     a.lds = src.ld;
-    a.rows = src.rows;
-    a.cols = src.cols;
     a.readable = (int)round_up(src.cols, 8);
-    a.period = 1;
     a.vec_src = map_ready(src);
-    a.part = part;
-    a.ldpart = round_up(src.cols, 4);
-    cut_rows(&a, sms);
+    if (whole && src.rows <= kFewRows) {
+        a.out = out;
+        a.scale = scale;
+    } else {
+        a.part = part;
+        a.ldpart = round_up(src.cols, 4);
+    }
     return rows_launch(bf16, a, stream, what);
 }
 
@@ -274,7 +285,7 @@ static int linear_run(const rb200_linear_params* p, void* stream_v, GemmWait wai
     if ((rc = check_workspace(what, p->workspace, p->workspace_bytes, l.bytes))) return rc;
     cudaStream_t stream = (cudaStream_t)stream_v;
     const bool bf16 = p->dtype == RB200_BF16;
-    if ((rc = do_pack(l.x, stream, what)) || (rc = do_pack(l.w, stream, what))) return rc;
+    if ((rc = pack_operands(&l.x, &l.w, stream, what))) return rc;
     EpiArgs e = {};
     e.out = p->out;
     e.ldo = p->ldo;
@@ -417,15 +428,14 @@ static int backward_run(const rb200_linear_backward_params* p, void* stream_v) {
         if (l.sums && (rc = sum_chunks(bf16, r.part, r.ldpart, r.chunks, 1, (int)m, p->dbias, 0, Scale(), stream, what))) return rc;
     }
     const GemmWait wait = {p->status, 0, -1};
+    if ((rc = pack_operands(p->dx ? &l.w : nullptr, p->dweight ? &l.x : nullptr, stream, what))) return rc;
     EpiArgs e = {};
     if (p->dx) {
-        if ((rc = do_pack(l.w, stream, what))) return rc;
         e.out = p->dx;
         e.ldo = p->lddx;
             if ((rc = gemm_store_joined(GEMM_KN, bf16, l.dz, l.w.use, nullptr, nullptr, l.gx, e, l.px, wait, stream, what))) return rc;
     }
     if (p->dweight) {
-        if ((rc = do_pack(l.x, stream, what))) return rc;
         e.out = p->dweight;
         e.ldo = p->lddw;
             Operand dzt = l.dz;

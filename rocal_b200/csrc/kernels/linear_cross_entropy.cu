@@ -42,6 +42,8 @@ __global__ void __launch_bounds__(256) ce_merge_kernel(MergeArgs a) {
     __shared__ float sm[SUBS][ROWS], ss[SUBS][ROWS], sz[SUBS][ROWS];
     __shared__ double sums[256];
     __shared__ int counts[8], dirts[8], last_block;
+    pdl_launch_dependents();
+    pdl_wait();
     const int lane = threadIdx.x % ROWS, sub = threadIdx.x / ROWS;
     const long long plane = (long long)a.parts * a.rows;
     double mine = 0.0;
@@ -153,15 +155,10 @@ static int merge_launch(const MergeArgs& m, cudaStream_t stream, const char* wha
     const int subs = m.parts >= 8 ? 8 : m.parts >= 4 ? 4 : m.parts >= 2 && m.rows < 148 * 256 ? 2 : 1;
     const long long blocks = ((long long)m.rows + 256 / subs - 1) / (256 / subs);
     const unsigned grid = (unsigned)(blocks < kMergeBlocks ? blocks : kMergeBlocks);
-    if (subs == 8)
-        ce_merge_kernel<8><<<grid, 256, 0, stream>>>(m);
-    else if (subs == 4)
-        ce_merge_kernel<4><<<grid, 256, 0, stream>>>(m);
-    else if (subs == 2)
-        ce_merge_kernel<2><<<grid, 256, 0, stream>>>(m);
-    else
-        ce_merge_kernel<1><<<grid, 256, 0, stream>>>(m);
-    RB200_CHECK_LAUNCH(what);
+    auto* kernel = subs == 8 ? ce_merge_kernel<8> : subs == 4 ? ce_merge_kernel<4> : subs == 2 ? ce_merge_kernel<2> : ce_merge_kernel<1>;
+    int rc = check_cuda(launch_overlapped(kernel, dim3(grid), dim3(256), 0, stream, m), what);
+    if (rc) return rc;
+    count_launch();
     return RB200_OK;
 }
 
@@ -172,6 +169,8 @@ __global__ void __launch_bounds__(1024) ce_factors_kernel(const float* __restric
                                                           long long ignore_index, int rows, float* coef, float* factor) {
     __shared__ float tops[32];
     __shared__ float inv_s;
+    pdl_launch_dependents();
+    pdl_wait();
     float top = 0.0f;
     for (int i = threadIdx.x; i < rows; i += 1024) {
         bool counted;
@@ -201,6 +200,8 @@ __global__ void __launch_bounds__(1024) ce_factors_kernel(const float* __restric
 __global__ void __launch_bounds__(256) ce_clean_kernel(const int* info, const uint16_t* __restrict__ x, long long ldx, int rows, int cols,
                                                        const void* labels, int label_bytes, int classes, long long ignore_index,
                                                        uint16_t* __restrict__ out, long long ldo) {
+    pdl_launch_dependents();
+    pdl_wait();
     if (info[1] == 0) return;
     const long long groups = ldo / 8, total = groups * rows;
     for (long long t = blockIdx.x * 256ll + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
@@ -321,7 +322,7 @@ static int ce_forward(const rb200_linear_ce_params* p, cudaStream_t stream) {
     const StatsPlan s = plan_stats(*p, dev, p->workspace);
     if ((rc = check_workspace(what, p->workspace, p->workspace_bytes, s.bytes))) return rc;
     const bool bf16 = p->dtype == RB200_BF16;
-    if ((rc = do_pack(s.x, stream, what)) || (rc = do_pack(s.w, stream, what))) return rc;
+    if ((rc = pack_operands(&s.x, &s.w, stream, what))) return rc;
     const GemmWait wait = {p->status, 0, -1};
     for (long long c0 = 0; c0 < p->classes; c0 += s.piece) {
         const int classes = (int)(p->classes - c0 < s.piece ? p->classes - c0 : s.piece);
@@ -421,14 +422,14 @@ static GradPlan plan_grad(const rb200_linear_ce_params& p, const DeviceInfo& dev
         const size_t bw = gemm_partial_bytes(gemm_plan(dev, classes, k, rows, true, true), classes, k);
         if (bx > px) px = bx;
         if (bw > pw) pw = bw;
-        const ColumnSums cs = plan_column_sums(rows, classes, dev.sms);
+        const ColumnSums cs = plan_column_sums(rows, classes, dev.sms, !g.by_rows || g.pieces == 1);
         if (cs.chunks > g.col_chunks) g.col_chunks = cs.chunks;   // a smaller piece may be cut into more chunks
         if (cs.chunks * (size_t)cs.ldpart > pc) pc = cs.chunks * (size_t)cs.ldpart;
     }
     if (p.dx) g.px = c.take(px);
     if (p.dweight) g.pw = c.take(pw);
     // pieces of the rows keep theirs until the last one, packed behind one another
-    if (p.dbias) g.col_part = (float*)c.take((g.by_rows ? (size_t)g.col_chunks * g.pieces * round_up(p.classes, 4) : pc) * sizeof(float));
+    if (p.dbias && (pc || (g.by_rows && g.col_chunks))) g.col_part = (float*)c.take((g.by_rows ? (size_t)g.col_chunks * g.pieces * round_up(p.classes, 4) : pc) * sizeof(float));
     g.bytes = c.used;
     return g;
 }
@@ -462,18 +463,24 @@ static int ce_backward(const rb200_linear_ce_params* p, cudaStream_t stream) {
     if ((rc = check_workspace(what, p->workspace, p->workspace_bytes, g.bytes))) return rc;
     const bool bf16 = p->dtype == RB200_BF16;
     const GemmWait wait = {p->status, 0, -1};
-    if ((rc = do_pack(g.x, stream, what)) || (rc = do_pack(g.w, stream, what))) return rc;
+    if ((rc = pack_operands(&g.x, &g.w, stream, what))) return rc;
     const bool none = p->reduction == RB200_REDUCE_NONE;
     if (none) {
-        ce_factors_kernel<<<1, 1024, 0, stream>>>(p->dloss, p->labels, p->label_bytes, (int)v, p->ignore_index, (int)n, g.coef, g.factor);
-        RB200_CHECK_LAUNCH(what);
+        if ((rc = check_cuda(launch_overlapped(ce_factors_kernel, dim3(1), dim3(1024), 0, stream, p->dloss, p->labels, p->label_bytes, (int)v,
+                                               (long long)p->ignore_index, (int)n, g.coef, g.factor),
+                             what)))
+            return rc;
+        count_launch();
     }
     if (p->dweight) {
         const long long blocks = (g.clean.ld / 8 * n + 255) / 256;
-        ce_clean_kernel<<<(unsigned)(blocks < 8 * dev.sms ? blocks : 8 * dev.sms), 256, 0, stream>>>(
-            p->info, (const uint16_t*)p->x, p->ldx, (int)n, (int)k, p->labels, p->label_bytes, (int)v, p->ignore_index,
-            (uint16_t*)const_cast<void*>(g.clean.data), g.clean.ld);
-        RB200_CHECK_LAUNCH(what);
+        const dim3 grid((unsigned)(blocks < 8 * dev.sms ? blocks : 8 * dev.sms));
+        if ((rc = check_cuda(launch_overlapped(ce_clean_kernel, grid, dim3(256), 0, stream, (const int*)p->info, (const uint16_t*)p->x,
+                                               (long long)p->ldx, (int)n, (int)k, p->labels, p->label_bytes, (int)v, (long long)p->ignore_index,
+                                               (uint16_t*)const_cast<void*>(g.clean.data), g.clean.ld),
+                             what)))
+            return rc;
+        count_launch();
     }
     const Scale scale(1.0f / 32768.0f, none ? g.factor : p->dloss, p->reduction == RB200_REDUCE_MEAN ? p->info : nullptr);
     int planes = 0;   // of partial column sums so far
@@ -536,14 +543,13 @@ static int ce_backward(const rb200_linear_ce_params* p, cudaStream_t stream) {
                 return rc;
         }
         if (p->dbias) {
-            const ColumnSums cs = plan_column_sums(rows, classes, dev.sms);
+            const ColumnSums cs = plan_column_sums(rows, classes, dev.sms, !g.by_rows || g.pieces == 1);
             if (!g.by_rows) planes = 0;
-            if ((rc = column_partials(bf16, dz, g.col_part + planes * cs.ldpart, dev.sms, stream, what))) return rc;
+            void* db = const_cast<uint8_t*>(at_row(p->dbias, 1, c0));
+            if ((rc = column_partials(bf16, dz, !g.by_rows || g.pieces == 1, g.col_part + planes * cs.ldpart, db, scale, dev.sms, stream, what))) return rc;
             planes += cs.chunks;
-            if (!g.by_rows || last) {
-                if ((rc = sum_chunks(bf16, g.col_part, cs.ldpart, planes, 1, classes, const_cast<uint8_t*>(at_row(p->dbias, 1, c0)), 0, scale,
-                                     stream, what)))
-                    return rc;
+            if (cs.chunks && (!g.by_rows || last)) {
+                if ((rc = sum_chunks(bf16, g.col_part, cs.ldpart, planes, 1, classes, db, 0, scale, stream, what))) return rc;
             }
         }
     }

@@ -63,11 +63,6 @@ static inline Operand operand(const void* data, long long ld, long long rows, lo
     return o;
 }
 
-// An operand as the product reads it: in place, or from a packed copy in the workspace.
-struct Packed {
-    Operand src, use;
-    bool copy;
-};
 static inline Packed plan_pack(const Operand& o, Carver* c) {
     Packed p = {o, o, !map_ready(o)};
     if (p.copy) {
@@ -76,10 +71,6 @@ static inline Packed plan_pack(const Operand& o, Carver* c) {
     }
     return p;
 }
-static inline int do_pack(const Packed& p, cudaStream_t stream, const char* what) {
-    return p.copy ? pack_rows(p.src, const_cast<void*>(p.use.data), p.use.ld, stream, what) : RB200_OK;
-}
-
 // Zeroes a matrix of 16-bit elements.
 static inline int clear_matrix(void* data, long long ld, long long rows, long long cols, cudaStream_t stream, const char* what) {
     return check_cuda(cudaMemset2DAsync(data, (size_t)(rows > 1 ? ld : cols) * 2, 0, (size_t)cols * 2, (size_t)rows, stream), what);
