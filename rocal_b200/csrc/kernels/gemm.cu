@@ -136,6 +136,7 @@ int gemm_args(GemmArgs* g, const DeviceInfo& dev, bool bf16, const Operand& a, c
     g->e.vec_res = vec(e.residual, e.ldr, e.residual_rows);
     g->m = m;
     g->n = n;
+    g->k = a.inner();
     g->bn = plan.bn;
     g->tiles_m = plan.tiles_m;
     g->tiles_n = plan.tiles_n;

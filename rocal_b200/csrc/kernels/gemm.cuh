@@ -1,6 +1,7 @@
 // Matrix products C[m][n] = sum_k A[m][k] B[n][k] of 16-bit operands with fp32 accumulation on the fifth-generation
 // tensor cores, and what is done with the accumulators before they leave the chip (EPI_*). One persistent kernel:
 //   warp 0      copies operand tiles (128-byte swizzle) into a ring of shared-memory stages,
+//   warp 3      idle but for one rare task (EpiArgs::dirty); warp 2 allocates TMEM,
 //   warp 1      issues the products of a stage (64 contracted elements) into one of two TMEM accumulators,
 //   warps 4-19  two groups of eight; each group reads its own accumulator, 32 columns at a time (thread = row, two
 //               warps share a row's strips), and runs the epilogue of every other tile, so that the epilogues of two tiles
@@ -65,12 +66,18 @@ struct EpiArgs {
     const float* stats;       // GRAD: maxima; stats_stride further the sums, twice that the labels' z
     long long stats_stride;
     const float* coef;        // GRAD: [m] per-row factor or null (= 1)
+    // GRAD: if *dirty, clean[clean_rows][k] = clean_src with the rows that do not count zeroed, made on the side; or null.
+    const int* dirty;
+    const void* clean_src;
+    void* clean;
+    long long ldsrc, ldclean, clean_rows;
+    const void* clean_labels;
 };
 
 struct GemmArgs {
     CUtensorMap a, b, b_alt;   // b_alt replaces b when *b_select is not 0
     const int* b_select;
-    int m, n;
+    int m, n, k;
     int bn;                    // columns of a tile
     int tiles_m, tiles_n, splits;
     int kblocks, kblocks_per_split;
@@ -459,6 +466,20 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             }
         }
         __syncwarp();
+    } else if (warp == 3) {
+        if constexpr (EPI == EPI_CE_GRAD) {
+            if (g.e.dirty && *g.e.dirty) {
+                const int cols = g.k;
+                for (long long r = blockIdx.x; r < g.e.clean_rows; r += gridDim.x) {
+                    bool counted;
+                    load_label(g.e.clean_labels, g.e.label_bytes, r, g.e.ignore_index, g.e.classes, &counted);
+                    const T* src = reinterpret_cast<const T*>(g.e.clean_src) + r * g.e.ldsrc;
+                    T* dst = reinterpret_cast<T*>(g.e.clean) + r * g.e.ldclean;   // rows padded to whole pieces
+                    for (int c = lane * 8; c < cols; c += 256)
+                        *reinterpret_cast<uint4*>(dst + c) = counted ? load8(src + c, cols - c, false) : make_uint4(0, 0, 0, 0);
+                }
+            }
+        }
     } else if (warp >= 4) {
         // group 0: even tiles and accumulator 0; share 0: even strips
         const int ew = warp - 4, quarter = warp & 3, group = ew >> 3, share = ew >> 2 & 1;
@@ -497,6 +518,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 }
             }
 
+            int res_row[4];   // the residual's rows of this lane (below), -1: none
+            if constexpr (EPI == EPI_LINEAR) {
+                if (g.e.residual) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int r = row0 + (lane >> 2) + 8 * i;
+                        res_row[i] = r < g.m ? r % g.e.residual_rows : -1;
+                    }
+                }
+            }
+
             // the lanes leave together: what follows needs whole warps
             if (!__all_sync(0xFFFFFFFFu, tc::bar_wait(acc_full(group), acc_phase, patience))) break;
             acc_phase ^= 1;
@@ -517,12 +549,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                         const int left = count - (lane & 3) * 8;
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            const int r = row0 + (lane >> 2) + 8 * i;
                             res[i] = make_uint4(0, 0, 0, 0);
-                            if (r < g.m && left > 0)
-                                res[i] = load8(reinterpret_cast<const T*>(g.e.residual) + (long long)(r % g.e.residual_rows) * g.e.ldr + col +
-                                                   (lane & 3) * 8,
-                                               left, g.e.vec_res);
+                            if (res_row[i] >= 0 && left > 0)
+                                res[i] = load8(reinterpret_cast<const T*>(g.e.residual) + res_row[i] * g.e.ldr + col + (lane & 3) * 8, left,
+                                               g.e.vec_res);
                         }
                     }
                 }

@@ -192,7 +192,8 @@ __device__ __forceinline__ uint4 scale_words(const uint32_t* w, float factor) {
     for (int j = 0; j < N; j++) v[j] *= factor;
     return Values<O>::put(v);
 }
-// SHIFT < 0: the gradients have boundaries of their own words where the output has its 16-byte ones.
+// SHIFT < 0: the gradients have boundaries of their own words where the output has its 16-byte ones. Outputs are written
+// past L2, where gradients still wait for their second read.
 template <typename T, typename O, int SHIFT>
 __device__ __forceinline__ void scale_vectors(const T* g, O* o, int vectors, float factor) {
     constexpr int W = Values<O>::N * (int)sizeof(T) / 4, U = 16 / W;   // U vectors in flight
@@ -215,12 +216,12 @@ __device__ __forceinline__ void scale_vectors(const T* g, O* o, int vectors, flo
 #pragma unroll
         for (int k = 0; k < U; k++) fetch(i + k * kClipThreads, w[k]);
 #pragma unroll
-        for (int k = 0; k < U; k++) out[i + k * kClipThreads] = scale_words<T, O>(w[k], factor);
+        for (int k = 0; k < U; k++) __stcs(out + i + k * kClipThreads, scale_words<T, O>(w[k], factor));
     }
     for (; i < vectors; i += kClipThreads) {
         uint32_t w[W];
         fetch(i, w);
-        out[i] = scale_words<T, O>(w, factor);
+        __stcs(out + i, scale_words<T, O>(w, factor));
     }
 }
 // Whole vectors are written where the output has its 16-byte boundaries; the gradients that belong there are cut out of

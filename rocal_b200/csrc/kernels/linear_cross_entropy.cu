@@ -152,10 +152,10 @@ __global__ void __launch_bounds__(256) ce_merge_kernel(MergeArgs a) {
 constexpr int kMergeBlocks = 148 * 8;
 static int merge_launch(const MergeArgs& m, cudaStream_t stream, const char* what) {
     // as many threads a row as there are parts for them to share, while the rows alone do not fill the GPU
-    const int subs = m.parts >= 8 ? 8 : m.parts >= 4 ? 4 : m.parts >= 2 && m.rows < 148 * 256 ? 2 : 1;
+    const int subs = m.parts >= 32 && m.rows <= 4096 ? 32 : m.parts >= 8 ? 8 : m.parts >= 4 ? 4 : m.parts >= 2 && m.rows < 148 * 256 ? 2 : 1;
     const long long blocks = ((long long)m.rows + 256 / subs - 1) / (256 / subs);
     const unsigned grid = (unsigned)(blocks < kMergeBlocks ? blocks : kMergeBlocks);
-    auto* kernel = subs == 8 ? ce_merge_kernel<8> : subs == 4 ? ce_merge_kernel<4> : subs == 2 ? ce_merge_kernel<2> : ce_merge_kernel<1>;
+    auto* kernel = subs == 32 ? ce_merge_kernel<32> : subs == 8 ? ce_merge_kernel<8> : subs == 4 ? ce_merge_kernel<4> : subs == 2 ? ce_merge_kernel<2> : ce_merge_kernel<1>;
     int rc = check_cuda(launch_overlapped(kernel, dim3(grid), dim3(256), 0, stream, m), what);
     if (rc) return rc;
     count_launch();
@@ -193,30 +193,6 @@ __global__ void __launch_bounds__(1024) ce_factors_kernel(const float* __restric
     __syncthreads();
     const float inv = inv_s;
     for (int i = threadIdx.x; i < rows; i += 1024) coef[i] = dloss[i] * inv;
-}
-
-// Rows that do not count but hold inf or NaN would reach dweight as 0 * NaN: a copy of x with those rows zeroed, made
-// only if the forward pass found any.
-__global__ void __launch_bounds__(256) ce_clean_kernel(const int* info, const uint16_t* __restrict__ x, long long ldx, int rows, int cols,
-                                                       const void* labels, int label_bytes, int classes, long long ignore_index,
-                                                       uint16_t* __restrict__ out, long long ldo) {
-    pdl_launch_dependents();
-    pdl_wait();
-    if (info[1] == 0) return;
-    const long long groups = ldo / 8, total = groups * rows;
-    for (long long t = blockIdx.x * 256ll + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
-        const long long row = t / groups;
-        const int col = (int)(t - row * groups) * 8;
-        bool counted;
-        load_label(labels, label_bytes, row, ignore_index, classes, &counted);
-        uint32_t w[4] = {0, 0, 0, 0};
-        if (counted) {
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (col + i < cols) w[i >> 1] |= (uint32_t)x[row * ldx + col + i] << (16 * (i & 1));
-        }
-        *reinterpret_cast<uint4*>(out + row * ldo + col) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
 }
 
 // ---- argument checks --------------------------------------------------------------------------------------------
@@ -472,16 +448,6 @@ static int ce_backward(const rb200_linear_ce_params* p, cudaStream_t stream) {
             return rc;
         count_launch();
     }
-    if (p->dweight) {
-        const long long blocks = (g.clean.ld / 8 * n + 255) / 256;
-        const dim3 grid((unsigned)(blocks < 8 * dev.sms ? blocks : 8 * dev.sms));
-        if ((rc = check_cuda(launch_overlapped(ce_clean_kernel, grid, dim3(256), 0, stream, (const int*)p->info, (const uint16_t*)p->x,
-                                               (long long)p->ldx, (int)n, (int)k, p->labels, p->label_bytes, (int)v, (long long)p->ignore_index,
-                                               (uint16_t*)const_cast<void*>(g.clean.data), g.clean.ld),
-                             what)))
-            return rc;
-        count_launch();
-    }
     const Scale scale(1.0f / 32768.0f, none ? g.factor : p->dloss, p->reduction == RB200_REDUCE_MEAN ? p->info : nullptr);
     int planes = 0;   // of partial column sums so far
     for (int i = 0; i < g.pieces; i++) {
@@ -499,6 +465,17 @@ static int ce_backward(const rb200_linear_ce_params* p, cudaStream_t stream) {
         e.coef = none ? g.coef + r0 : nullptr;
         e.out = g.dz;
         e.ldo = g.ldd;
+        // Rows that do not count but hold inf or NaN would reach dweight as 0 * NaN: if the forward pass found any, the
+        // first launch also makes a copy of x with those rows zeroed.
+        if (p->dweight && i == 0) {
+            e.clean = const_cast<void*>(g.clean.data);
+            e.ldclean = g.clean.ld;
+            e.clean_src = p->x;
+            e.ldsrc = p->ldx;
+            e.clean_rows = n;
+            e.clean_labels = p->labels;
+            e.dirty = p->info + 1;
+        }
         const GemmPlan plan = gemm_plan(dev, rows, classes, (int)k, false, false);
         if ((rc = gemm_launch<EPI_CE_GRAD, false, false>(bf16, x, w, nullptr, nullptr, plan, e, wait, stream, what))) return rc;
         const bool first = i == 0, last = i == g.pieces - 1;
