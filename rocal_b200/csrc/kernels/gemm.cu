@@ -143,6 +143,11 @@ int gemm_args(GemmArgs* g, const DeviceInfo& dev, bool bf16, const Operand& a, c
     g->splits = plan.splits;
     g->kblocks = plan.kblocks;
     g->kblocks_per_split = plan.kblocks_per_split;
+    // several accumulators where a tile's columns leave room (gemm.cuh)
+    int sums = kTileNMax / plan.bn;
+    if (sums > plan.kblocks_per_split / 8) sums = plan.kblocks_per_split / 8;
+    if (sums < 1) sums = 1;
+    g->kblocks_per_sum = (plan.kblocks_per_split + sums - 1) / sums;
     g->idesc = tc::instr_desc(bf16, a.transposed, b.transposed, kTileM * plan.cg, plan.bn);
     g->stage_bytes = (uint32_t)(kTileM + bn_cta) * kTileK * 2;
     g->stages = kRingBytes / g->stage_bytes;

@@ -11,6 +11,9 @@
 //               it took 900 to 2500 clocks and bounded products of up to 1024 contracted elements.
 // CG = 2: two CTAs (a cluster) work on one tile of 256 rows; each holds its 128 rows of A and half of the B tile, so a
 // tile of 256 columns takes 128 bytes of operands per SM and clock at the full rate of the tensor cores instead of 192.
+// The tensor cores cut the sums they add to where they do not fit 32 bits, always to the same side, so a long sum drifts (measured:
+// 3e-6 relative after 4096 products). Tiles of up to 128 columns leave TMEM columns free: they spread the contracted
+// axis over several accumulators, 512 elements at least in each, which the epilogue adds with correct rounding.
 // Either operand may have the contracted axis contiguous (K-major) or the other one (MN-major): the backward products
 // need no transposed copies. Rows and columns beyond the matrices arrive as zeros and are not stored.
 #pragma once
@@ -66,6 +69,8 @@ struct EpiArgs {
     const float* stats;       // GRAD: maxima; stats_stride further the sums, twice that the labels' z
     long long stats_stride;
     const float* coef;        // GRAD: [m] per-row factor or null (= 1)
+    float* col_part;          // GRAD: [m / 32][ldcol] sums over 32 rows of what is written, before its rounding, or null
+    long long ldcol;
     // GRAD: if *dirty, clean[clean_rows][k] = clean_src with the rows that do not count zeroed, made on the side; or null.
     const int* dirty;
     const void* clean_src;
@@ -81,6 +86,7 @@ struct GemmArgs {
     int bn;                    // columns of a tile
     int tiles_m, tiles_n, splits;
     int kblocks, kblocks_per_split;
+    int kblocks_per_sum;       // contracted blocks that go into one accumulator of a tile
     int a_box_rows;            // rows of a K-major A copy
     uint32_t idesc, stage_bytes, stages;
     int* status;
@@ -137,8 +143,8 @@ __device__ __forceinline__ void unpack8(const uint4& w, float (&v)[8]) {
 }
 
 // Upper tail of the normal distribution over its density shape: R(a) = Q(a) exp(a^2 / 2) for a in [0, 6], a polynomial
-// of degree 12 in a / 3 - 1 fitted for the least relative error (2.3e-6 evaluated in fp32). Beyond 6, where z Q(z) is
-// below 6e-9, R(6) stands in. Two values at a time.
+// of degree 12 in a / 3 - 1 fitted for the least relative error (2.3e-6 evaluated in fp32). Beyond 6, where Q is below
+// 1e-9, R(6) stands in. Two values at a time.
 __device__ __forceinline__ float2 tail_ratio(float2 a) {
     constexpr float c[13] = {0.121513851f,   -0.103198029f, 0.0824128985f,  -0.0624807179f,   0.0450092852f,  -0.0303888023f, 0.020790372f,
                              -0.0161429029f, 0.00893525127f, -0.000628449256f, 0.00143634493f, -0.00477083307f, 0.0022911916f};
@@ -153,16 +159,16 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// z Phi(z) = max(z, 0) - |z| Q(|z|): one exponential and no division, accurate in the negative tail as well.
-// |z| is held at 40, where the exponential is 0, so that infinities give 0 and inf; NaN passes through the maximum.
+// z Phi(z) = max(z, 0) - |z| Q(|z|): one exponential and no division, accurate in the negative tail as well: beyond 6,
+// |z| R(|z|) is within 2% of what it is at 6. Infinities give 0 and inf (the exponential is 0 there), NaN stays.
 __device__ __forceinline__ float2 gelu2(float2 z) {
-    const float2 a = make_float2(fminf(fabsf(z.x), 40.0f), fminf(fabsf(z.y), 40.0f));
-    const float2 h = mul2(a, mul2(a, make_float2(-0.72134752f, -0.72134752f)));
+    const float2 a = make_float2(fminf(fabsf(z.x), 6.0f), fminf(fabsf(z.y), 6.0f));
+    const float2 h = mul2(z, mul2(z, make_float2(-0.72134752f, -0.72134752f)));
     const float2 e = make_float2(exp2_fast(h.x), exp2_fast(h.y));
     const float2 q = mul2(mul2(a, e), tail_ratio(a));
     return make_float2((z.x < 0.0f ? 0.0f : z.x) - q.x, (z.y < 0.0f ? 0.0f : z.y) - q.y);
 }
-// Phi(z) + z phi(z)
+// Phi(z) + z phi(z). |z| is held at 40, where the exponential is 0, so that infinities give 0 and 1.
 __device__ __forceinline__ float2 gelu_slope2(float2 z) {
     const float2 a = make_float2(fminf(fabsf(z.x), 40.0f), fminf(fabsf(z.y), 40.0f));
     const float2 h = mul2(a, mul2(a, make_float2(-0.72134752f, -0.72134752f)));
@@ -437,8 +443,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 ok = tc::bar_wait(acc_empty(buf), acc_phase ^ 1, patience);
                 if (!ok) break;
                 tc::fence_after();
-                const uint32_t d = tmem + buf * kTileNMax;
+                uint32_t d = tmem + buf * kTileNMax - g.bn;
+                int left = 0;   // blocks that still go into accumulator d
                 for (int kb = k_begin; kb < k_end; kb++) {
+                    const bool fresh = left == 0;
+                    if (fresh) {
+                        d += g.bn;
+                        left = g.kblocks_per_sum;
+                    }
+                    left--;
                     ok = tc::bar_wait(full(s), phase, patience);
                     if (!ok) break;
                     tc::fence_after();
@@ -447,7 +460,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
 #pragma unroll
                     for (int k = 0; k < kTileK / 16; k++)
                         tc::mma_f16<CG>(d, da + k * (A_MN ? 2048 >> 4 : 32 >> 4), db + k * (B_MN ? 2048 >> 4 : 32 >> 4), g.idesc,
-                                        (kb > k_begin || k > 0) ? 1u : 0u);
+                                        (!fresh || k > 0) ? 1u : 0u);
                     issued = true;
                     tc::mma_commit<CG>(empty(s));
                     if (++s == S) {
@@ -534,6 +547,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             acc_phase ^= 1;
             tc::fence_after();
 
+            const int in_sum = min(g.kblocks, (sp + 1) * g.kblocks_per_split) - sp * g.kblocks_per_split;
+            const int sums = (in_sum + g.kblocks_per_sum - 1) / g.kblocks_per_sum;
+            auto release = [&] {   // this warp's part of the accumulator is in registers
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) tc::bar_arrive_relaxed(CG == 2 ? tc::map_to_rank(acc_empty(group), 0) : acc_empty(group));
+            };
             for (int c = share * 32; c < g.bn; c += 64) {
                 const int col = n0 + c, count = n1 - col;   // columns of this strip inside the matrix (may be <= 0)
                 const bool work = count > 0 && row0 < g.m;
@@ -557,15 +577,24 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     }
                 }
                 tc::tmem_wait();
-                if (c + 64 >= g.bn) {   // this warp's part of the accumulator is in registers
-                    tc::fence_before();
-                    __syncwarp();
-                    if (lane == 0) tc::bar_arrive_relaxed(CG == 2 ? tc::map_to_rank(acc_empty(group), 0) : acc_empty(group));
+                if (!work) {
+                    if (c + 64 >= g.bn) release();
+                    continue;
                 }
-                if (!work) continue;
                 float v[32];
 #pragma unroll
                 for (int i = 0; i < 32; i++) v[i] = __uint_as_float(raw[i]);
+                for (int s = 1; s < sums; s++) {   // the tile's other accumulators
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        uint32_t more[8];
+                        tc::tmem_load8(acc + s * g.bn + c + i, more);
+                        tc::tmem_wait();
+#pragma unroll
+                        for (int j = 0; j < 8; j++) v[i + j] += __uint_as_float(more[j]);
+                    }
+                }
+                if (c + 64 >= g.bn) release();
                 __syncwarp();   // the staging area is free: the strip before has been read
                 if constexpr (EPI != EPI_STORE) {
                     if (g.e.bias) {
@@ -696,28 +725,35 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                         v[i] = p.x;
                         v[i + 1] = p.y;
                     }
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        uint4 w = pack8<T>(v + 8 * i);
-                        if (!counted) w = make_uint4(0, 0, 0, 0);   // whatever the row held
-                        st_shared16(staged(area, lane, i), w);
-                    }
                     const int l = label - col;
                     if (l >= 0 && l < 32) {
-                        const T e = Elem<T>::from_float(at_label);
-                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(staged(area, lane, l >> 3) + (l & 7) * 2),
-                                     "h"(*reinterpret_cast<const uint16_t*>(&e))
-                                     : "memory");
+#pragma unroll
+                        for (int i = 0; i < 32; i++) v[i] = i == l ? at_label : v[i];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[i] = counted ? v[i] : 0.0f;   // whatever the row held
+#pragma unroll
+                    for (int i = 0; i < 4; i++) st_shared16(staged(area, lane, i), pack8<T>(v + 8 * i));
+                    if (g.e.col_part) {
+                        // Column sums over the warp's rows: at every step a lane keeps the half of its columns that its own
+                        // number's next bit names and hands the other half to its partner. Lane l ends with column l.
+#pragma unroll
+                        for (int w = 16; w; w >>= 1) {
+                            const bool upper = lane & w;
+#pragma unroll
+                            for (int i = 0; i < w; i++) {
+                                const float keep = upper ? v[i + w] : v[i], send = upper ? v[i] : v[i + w];
+                                v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, send, w);
+                            }
+                        }
+                        if (lane < count) g.e.col_part[(long long)(row0 >> 5) * g.e.ldcol + col + lane] = v[0];
                     }
                     __syncwarp();
                     // the rows are padded to whole pieces, which nothing reads
                     copy_strip(area, reinterpret_cast<T*>(g.e.out), g.e.ldo, true, col, min(32, (count + 7) & ~7), row0, g.m - row0, lane);
                 }
             }
-            if (g.bn <= share * 32) {   // a tile of one strip: the other warps have nothing to read
-                __syncwarp();
-                if (lane == 0) tc::bar_arrive_relaxed(CG == 2 ? tc::map_to_rank(acc_empty(group), 0) : acc_empty(group));
-            }
+            if (g.bn <= share * 32) release();   // a tile of one strip: the other warps have nothing to read
             if constexpr (EPI == EPI_CE_STATS) {
                 if (row_ok) {
                     const long long plane = (long long)g.e.parts * g.m, at = (long long)(2 * nb + share) * g.m + row;
@@ -845,17 +881,9 @@ struct Packed {
 };
 int pack_operands(const Packed* a, const Packed* b, cudaStream_t stream, const char* what);
 
-// Column sums of a matrix in a workspace, its rows padded to 8 elements (linear.cu): chunks planes of ldpart partial sums,
-// joined (with other planes) by sum_chunks; of few rows the sums themselves (chunks = 0: no planes are needed).
-struct ColumnSums {
-    int chunks;
-    long long ldpart;
-};
-ColumnSums plan_column_sums(int rows, int cols, int sms, bool whole);
-int column_partials(bool bf16, const Operand& src, bool whole, float* part, void* out, const Scale& scale, int sms, cudaStream_t stream,
-                    const char* what);
-int sum_chunks(bool bf16, const float* part, long long ldpart, int planes, int rows, int cols, void* out, long long ldo, const Scale& scale,
-               cudaStream_t stream, const char* what);
+// out[c] = scale * sum over planes of part[plane * ldpart + c] (linear.cu). Many planes are first summed in groups, which take
+// the place of the first planes.
+int sum_planes(bool bf16, float* part, long long ldpart, int planes, int cols, void* out, const Scale& scale, cudaStream_t stream, const char* what);
 
 static inline long long round_up(long long v, long long to) { return (v + to - 1) / to * to; }
 

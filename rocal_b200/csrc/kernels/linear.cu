@@ -22,9 +22,7 @@ struct RowsArgs {
     long long ldpart;
     void* out;                // one chunk only: the sums in the element type, [period][ldo], or null
     long long ldo;
-    Scale scale;              // of what goes to out
     int rows, cols, period, chunks, per_chunk;   // per_chunk: repeats of a chunk
-    int readable;             // columns that may be read: cols, or more where the rows are padded
     int across;               // threads side by side: a power of two up to 32
     int act, vec_src, vec_pre;
 };
@@ -37,7 +35,7 @@ __global__ void __launch_bounds__(256, 4) rows_kernel(RowsArgs a) {
     __shared__ float sums[256 * 8];
     __shared__ float half[256];
     const int lane = threadIdx.x & (a.across - 1), sub = threadIdx.x / a.across, subs = 256 / a.across, wide = a.across * 8;
-    const int col = blockIdx.x * wide + lane * 8, count = a.readable - col;
+    const int col = blockIdx.x * wide + lane * 8, count = a.cols - col;
     const int repeats = a.rows / a.period;
     const long long units = (long long)a.period * a.chunks;
     for (long long u = blockIdx.y; u < units; u += gridDim.y) {
@@ -97,7 +95,7 @@ __global__ void __launch_bounds__(256, 4) rows_kernel(RowsArgs a) {
             if (piece == 0 && out_col < a.cols) {
                 for (int k = 1; k < 256 / wide; k++) s += half[k * wide + c];
                 if (a.part) a.part[u * a.ldpart + out_col] = s;
-                if (a.out) reinterpret_cast<T*>(a.out)[j * a.ldo + out_col] = Elem<T>::from_float(s * a.scale.value());
+                if (a.out) reinterpret_cast<T*>(a.out)[j * a.ldo + out_col] = Elem<T>::from_float(s);
             }
             __syncthreads();
         }
@@ -183,7 +181,7 @@ static cudaError_t sum_launch(const float* part, long long ldpart, int planes, i
     return launch_overlapped(planes < 32 ? sum_few_kernel<T> : sum_chunks_kernel<T>, grid, dim3(256), 0, stream, part, ldpart, planes, rows, cols,
                              out, ldo, scale);
 }
-int sum_chunks(bool bf16, const float* part, long long ldpart, int planes, int rows, int cols, void* out, long long ldo, const Scale& scale,
+static int sum_chunks(bool bf16, const float* part, long long ldpart, int planes, int rows, int cols, void* out, long long ldo, const Scale& scale,
                cudaStream_t stream, const char* what) {
     int rc = check_cuda(bf16 ? sum_launch(part, ldpart, planes, rows, cols, (__nv_bfloat16*)out, ldo, scale, stream)
                              : sum_launch(part, ldpart, planes, rows, cols, (__half*)out, ldo, scale, stream),
@@ -193,41 +191,30 @@ int sum_chunks(bool bf16, const float* part, long long ldpart, int planes, int r
     return RB200_OK;
 }
 
-// Few rows: one chunk, 64 columns a block, and the sums leave at once - one launch (5 us for 1024 x 1000) instead of
-// two (3 + 3 us and a launch).
-constexpr int kFewRows = 2048;
-static RowsArgs column_args(int rows, int cols, int sms, bool whole) {
-    RowsArgs a = {};
-    a.rows = rows;
-    a.cols = cols;
-    a.period = 1;
-    cut_rows(&a, sms);
-    if (whole && rows <= kFewRows) {
-        if (a.across > 8) a.across = 8;
-        a.chunks = 1;
-        a.per_chunk = rows;
-    }
-    return a;
+// part[g] = sum of the planes g, g + groups, g + 2 groups, ...: a thread takes one column of one group, in place (the planes
+// of a group are read by the one thread that writes the group's).
+__global__ void __launch_bounds__(256) group_planes_kernel(float* part, long long ldpart, int planes, int cols, int groups) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int col = blockIdx.x * 32 + (threadIdx.x & 31);
+    const int g = blockIdx.y * 8 + (threadIdx.x >> 5);
+    if (col >= cols || g >= groups) return;
+    float s = 0.0f;
+#pragma unroll 8
+    for (int p = g; p < planes; p += groups) s += part[p * ldpart + col];
+    part[g * ldpart + col] = s;
 }
-ColumnSums plan_column_sums(int rows, int cols, int sms, bool whole) {
-    ColumnSums c = {whole && rows <= kFewRows ? 0 : column_args(rows, cols, sms, whole).chunks, round_up(cols, 4)};
-    return c;
-}
-int column_partials(bool bf16, const Operand& src, bool whole, float* part, void* out, const Scale& scale, int sms, cudaStream_t stream,
-                    const char* what) {
-    RowsArgs a = column_args(src.rows, src.cols, sms, whole);
-    a.src = src.data;
-    a.lds = src.ld;
-    a.readable = (int)round_up(src.cols, 8);
-    a.vec_src = map_ready(src);
-    if (whole && src.rows <= kFewRows) {
-        a.out = out;
-        a.scale = scale;
-    } else {
-        a.part = part;
-        a.ldpart = round_up(src.cols, 4);
+
+int sum_planes(bool bf16, float* part, long long ldpart, int planes, int cols, void* out, const Scale& scale, cudaStream_t stream, const char* what) {
+    constexpr int kGroups = 256;
+    if (planes > 2 * kGroups) {
+        const dim3 grid((unsigned)((cols + 31) / 32), kGroups / 8);
+        int rc = check_cuda(launch_overlapped(group_planes_kernel, grid, dim3(256), 0, stream, part, ldpart, planes, cols, kGroups), what);
+        if (rc) return rc;
+        count_launch();
+        planes = kGroups;
     }
-    return rows_launch(bf16, a, stream, what);
+    return sum_chunks(bf16, part, ldpart, planes, 1, cols, out, 0, scale, stream, what);
 }
 
 static int check_shape(const char* what, int dtype, int act, long long rows, long long in, long long out) {
@@ -344,7 +331,7 @@ static LinearBackwardPlan plan_backward(const rb200_linear_backward_params& p, c
     a.src = p.dout;
     a.lds = p.lddo;
     a.rows = n;
-    a.cols = a.readable = m;
+    a.cols = m;
     a.vec_src = map_ready(dout);
     a.ldpart = round_up(m, 4);
     if (p.dresidual) {

@@ -348,8 +348,8 @@ struct GradPlan {
     float* sum;                 // 32-bit sums over pieces: dx (pieces of classes) or dweight (pieces of rows)
     long long ldsum;
     void *px, *pw;              // partial products
-    int col_chunks;             // partial sums that a piece makes at most
-    float* col_part;
+    float* col_part;            // [rows / 32][ldcol] column sums
+    long long ldcol;
     size_t bytes;
 };
 static int piece_rows(const rb200_linear_ce_params& p, const GradPlan& g, int i) {
@@ -391,21 +391,18 @@ static GradPlan plan_grad(const rb200_linear_ce_params& p, const DeviceInfo& dev
     g.ldsum = round_up(k, 4);
     if (g.pieces > 1 && (g.by_rows ? p.dweight : p.dx)) g.sum = (float*)c.take((size_t)shorter * g.ldsum * sizeof(float));
     // the last piece is the only one of another size
-    size_t px = 0, pw = 0, pc = 0;
+    size_t px = 0, pw = 0;
     for (int i = 0; i < g.pieces; i += g.pieces > 1 ? g.pieces - 1 : 1) {
         const int rows = piece_rows(p, g, i), classes = piece_classes(p, g, i);
         const size_t bx = gemm_partial_bytes(gemm_plan(dev, rows, k, classes, true, true), rows, k);
         const size_t bw = gemm_partial_bytes(gemm_plan(dev, classes, k, rows, true, true), classes, k);
         if (bx > px) px = bx;
         if (bw > pw) pw = bw;
-        const ColumnSums cs = plan_column_sums(rows, classes, dev.sms, !g.by_rows || g.pieces == 1);
-        if (cs.chunks > g.col_chunks) g.col_chunks = cs.chunks;   // a smaller piece may be cut into more chunks
-        if (cs.chunks * (size_t)cs.ldpart > pc) pc = cs.chunks * (size_t)cs.ldpart;
     }
     if (p.dx) g.px = c.take(px);
     if (p.dweight) g.pw = c.take(pw);
-    // pieces of the rows keep theirs until the last one, packed behind one another
-    if (p.dbias && (pc || (g.by_rows && g.col_chunks))) g.col_part = (float*)c.take((g.by_rows ? (size_t)g.col_chunks * g.pieces * round_up(p.classes, 4) : pc) * sizeof(float));
+    g.ldcol = round_up(piece_classes(p, g, 0), 32);
+    if (p.dbias) g.col_part = (float*)c.take((size_t)((p.rows + 31) / 32) * g.ldcol * sizeof(float));
     g.bytes = c.used;
     return g;
 }
@@ -449,7 +446,6 @@ static int ce_backward(const rb200_linear_ce_params* p, cudaStream_t stream) {
         count_launch();
     }
     const Scale scale(1.0f / 32768.0f, none ? g.factor : p->dloss, p->reduction == RB200_REDUCE_MEAN ? p->info : nullptr);
-    int planes = 0;   // of partial column sums so far
     for (int i = 0; i < g.pieces; i++) {
         const int rows = piece_rows(*p, g, i), classes = piece_classes(*p, g, i);
         const long long r0 = g.by_rows ? (long long)i * g.piece : 0, c0 = g.by_rows ? 0 : (long long)i * g.piece;
@@ -463,6 +459,10 @@ static int ce_backward(const rb200_linear_ce_params* p, cudaStream_t stream) {
         e.stats = p->stats + r0;
         e.stats_stride = n;
         e.coef = none ? g.coef + r0 : nullptr;
+        if (p->dbias) {   // pieces of the rows keep their sums until the last one
+            e.col_part = g.col_part + (r0 >> 5) * g.ldcol;
+            e.ldcol = g.ldcol;
+        }
         e.out = g.dz;
         e.ldo = g.ldd;
         // Rows that do not count but hold inf or NaN would reach dweight as 0 * NaN: if the forward pass found any, the
@@ -519,15 +519,10 @@ static int ce_backward(const rb200_linear_ce_params* p, cudaStream_t stream) {
                                         wait, stream, what)))
                 return rc;
         }
-        if (p->dbias) {
-            const ColumnSums cs = plan_column_sums(rows, classes, dev.sms, !g.by_rows || g.pieces == 1);
-            if (!g.by_rows) planes = 0;
-            void* db = const_cast<uint8_t*>(at_row(p->dbias, 1, c0));
-            if ((rc = column_partials(bf16, dz, !g.by_rows || g.pieces == 1, g.col_part + planes * cs.ldpart, db, scale, dev.sms, stream, what))) return rc;
-            planes += cs.chunks;
-            if (cs.chunks && (!g.by_rows || last)) {
-                if ((rc = sum_chunks(bf16, g.col_part, cs.ldpart, planes, 1, classes, db, 0, scale, stream, what))) return rc;
-            }
+        if (p->dbias && (!g.by_rows || last)) {
+            const int planes = (int)((r0 + rows + 31) / 32);   // a piece of the rows starts on a multiple of 256
+            if ((rc = sum_planes(bf16, g.col_part, g.ldcol, planes, classes, const_cast<uint8_t*>(at_row(p->dbias, 1, c0)), scale, stream, what)))
+                return rc;
         }
     }
     return RB200_OK;

@@ -156,6 +156,12 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&v)[32]) {
         : "r"(addr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_load8(uint32_t addr, uint32_t (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(addr)
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // ---- operand descriptors --------------------------------------------------------------------------------

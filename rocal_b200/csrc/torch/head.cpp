@@ -6,7 +6,9 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <array>
@@ -253,6 +255,22 @@ struct Linear : torch::autograd::Function<Linear> {
 
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
+// A leaf's gradient node lives as long as any graph that holds it, and belongs to the stream that was current when it was
+// made. In a capture, autograd would make the legacy default stream wait for the capturing one if an eager graph of
+// the same leaf were still alive there: CUDA does not allow that, and the error ends the process. Refused here, before anything is
+// captured.
+void refuse_stale_leaves(std::initializer_list<const Tensor*> tensors) {
+    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+    for (const Tensor* t : tensors) {
+        if (!wants_grad(*t) || !t->is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (!node || !node->stream()) continue;
+        TORCH_CHECK(*node->stream() != c10::cuda::getDefaultCUDAStream(t->device().index()).unwrap(),
+                    "capture with gradients: a graph of the same leaf, made on the default stream, is still alive; drop it "
+                    "(its outputs and losses) before the capture, or make it on another stream");
+    }
+}
+
 Tensor linear(const Tensor& x, const Tensor& weight, const MaybeTensor& bias_, const MaybeTensor& residual_, const std::string& act_name) {
     const int act = activation(act_name);
     TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1), "x ", x.sizes(), " does not go with weight ", weight.sizes());
@@ -271,10 +289,12 @@ Tensor linear(const Tensor& x, const Tensor& weight, const MaybeTensor& bias_, c
     const bool flat = x.dim() == 2;
     const Tensor x2 = flat ? x : x.reshape({-1, x.size(-1)});
     Tensor y;
-    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias) || wants_grad(residual)))
+    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias) || wants_grad(residual))) {
+        refuse_stale_leaves({&x, &weight, &bias, &residual});
         y = Linear::apply(x2, weight, or_absent(bias), or_absent(residual), (int64_t)act);
-    else
+    } else {
         y = linear_run(x2, weight, bias, residual, act, Tensor(), nullptr, {}, {});
+    }
     return flat ? y : y.reshape(shape);
 }
 
@@ -398,10 +418,12 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
     const bool flat = x.dim() == 2;
     const Tensor x2 = flat ? x : x.reshape({-1, x.size(-1)}), l1 = flat ? labels : labels.reshape({-1});
     Tensor loss;
-    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias)))
+    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias))) {
+        refuse_stale_leaves({&x, &weight, &bias});
         loss = LinearCrossEntropy::apply(x2, weight, l1, or_absent(bias), ignore_index, smoothing, (int64_t)reduce);
-    else
+    } else {
         loss = ce_run(x2, weight, l1, bias, ignore_index, smoothing, reduce, {})[0];
+    }
     return flat || reduce != RB200_REDUCE_NONE ? loss : loss.reshape(labels.sizes());
 }
 
@@ -419,8 +441,8 @@ int grad_dtype(const Tensor& t, const Tensor& first) {
 
 Tensor grad_clip(const std::vector<Tensor>& grads, double max_norm, const std::optional<std::vector<Tensor>>& out, double inv_scale) {
     TORCH_CHECK_VALUE(!grads.empty(), "no gradients");
-    TORCH_CHECK_VALUE(grads[0].is_cuda(), "the gradients are on ", grads[0].device(), ": the head operators run on a GPU");
     TORCH_CHECK_VALUE(!out || out->size() == grads.size(), out ? out->size() : 0, " outputs for ", grads.size(), " gradients");
+    TORCH_CHECK_VALUE(grads[0].is_cuda(), "the gradients are on ", grads[0].device(), ": the head operators run on a GPU");
     TORCH_CHECK_VALUE(max_norm >= 0 && inv_scale > 0, "max_norm ", max_norm, ", inv_scale ", inv_scale);
     at::NoGradGuard no_grad;
     c10::cuda::CUDAGuard guard(grads[0].device());
