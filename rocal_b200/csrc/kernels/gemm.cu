@@ -71,10 +71,13 @@ int make_map(CUtensorMap* map, const Operand& o, bool bf16, int box_rows, const 
 }
 
 // A model of the kernel's time in clocks, good enough to order the ways of cutting a product:
-//   a k-block of a tile takes the longer of the tensor cores' time (bn clocks: 128 rows per SM and 8192 products a
-//   clock) and the copies' (about 100 bytes of operands per SM and clock);
-//   a tile also keeps the epilogue warps busy (about 10 clocks a column), which counts where it is the longest;
-//   the last tile's epilogue is not hidden, and pieces of the contracted axis have to be joined by another launch.
+//   a k-block of a tile takes the longer of the tensor cores' time (2 bn clocks: 128 rows per SM and 4096 products a
+//   clock, but 290 at least: they read all 128 rows of A however few the columns are) and the copies' (about 48 bytes of
+//   operands per SM and clock while all SMs copy);
+//   a tile also keeps its group of epilogue warps busy (about 16 clocks a column; two groups take turns);
+//   the last tile's epilogue is not hidden, and pieces of the contracted axis have to be joined by another launch (about 8000,
+//   half of it on the host). Clusters whose CTAs join their pieces through distributed shared memory were tried instead: 14 us against
+//   9 us for one row of 2048 x 1000, because clusters of full-size CTAs do not fill the GPU.
 GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed, bool may_split) {
     GemmPlan best = {};
     double best_cost = 0;
@@ -87,7 +90,8 @@ GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed
             const int tiles_n = (n + bn - 1) / bn;
             if (bn > unit && (n + bn - unit - 1) / (bn - unit) == tiles_n && bn - unit >= n) continue;   // wider than the matrix
             const long long tiles = (long long)tiles_m * tiles_n;
-            const double copies = (kTileM + bn / cg) * 128 / 100.0, block = copies > bn ? copies : bn, epilogue = 10.0 * bn + 500;
+            const double copies = (kTileM + bn / cg) * 128 / 48.0, products = 2.0 * bn > 290 ? 2.0 * bn : 290;
+            const double block = copies > products ? copies : products, epilogue = 16.0 * bn + 500;
             // one piece, or as many as the free SMs take in one or two rounds
             long long choices[3] = {1, 1, 1};
             if (may_split && kblocks >= 16) {
@@ -102,7 +106,7 @@ GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed
                 const long long waves = (tiles * splits + slots - 1) / slots;
                 const double work = per * block + 300;
                 double cost = waves * (work > epilogue / 2 ? work : epilogue / 2) + epilogue + 1000;
-                if (splits > 1) cost += 6000 + 8.0 * splits * m * n / 2500;   // partial sums: about 2500 bytes a clock
+                if (splits > 1) cost += 8000 + 8.0 * splits * m * n / 2500;   // partial sums: about 2500 bytes a clock
                 if (best_cost == 0 || cost < best_cost * 0.99) {
                     best_cost = cost;
                     best = {bn, cg, splits, tiles_m, tiles_n, kblocks, per};
@@ -113,7 +117,7 @@ GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed
     return best;
 }
 
-int gemm_args(GemmArgs* g, const DeviceInfo& dev, bool bf16, const Operand& a, const Operand& b, const Operand* b_alt, const int* b_select,
+int gemm_args(GemmArgs* g, const DeviceInfo& dev, int epi, bool bf16, const Operand& a, const Operand& b, const Operand* b_alt, const int* b_select,
               const GemmPlan& plan, const EpiArgs& e, const GemmWait& wait, const char* what) {
     const int m = a.outer(), n = b.outer();
     if ((double)plan.tiles_m * plan.tiles_n * plan.splits > 2e9) {
@@ -143,14 +147,15 @@ int gemm_args(GemmArgs* g, const DeviceInfo& dev, bool bf16, const Operand& a, c
     g->splits = plan.splits;
     g->kblocks = plan.kblocks;
     g->kblocks_per_split = plan.kblocks_per_split;
-    // several accumulators where a tile's columns leave room (gemm.cuh)
-    int sums = kTileNMax / plan.bn;
+    // several accumulators where the sums are kept in 32 bits and a tile's columns leave room (gemm.cuh)
+    int sums = epi == EPI_CE_STATS ? kTileNMax / plan.bn : 1;
     if (sums > plan.kblocks_per_split / 8) sums = plan.kblocks_per_split / 8;
     if (sums < 1) sums = 1;
     g->kblocks_per_sum = (plan.kblocks_per_split + sums - 1) / sums;
     g->idesc = tc::instr_desc(bf16, a.transposed, b.transposed, kTileM * plan.cg, plan.bn);
-    g->stage_bytes = (uint32_t)(kTileM + bn_cta) * kTileK * 2;
-    g->stages = kRingBytes / g->stage_bytes;
+    g->block_bytes = (uint32_t)(kTileM + bn_cta) * kTileK * 2;
+    g->stage_blocks = 8 * g->block_bytes <= kRingBytes ? 2 : 1;   // two while four stages remain
+    g->stages = kRingBytes / (g->stage_blocks * g->block_bytes);
     if (g->stages > 12) g->stages = 12;
     g->status = wait.status ? wait.status : dev.status;
     g->wait_cycles = wait.cycles ? wait.cycles : kDefaultWaitCycles;

@@ -1,8 +1,9 @@
 // Matrix products C[m][n] = sum_k A[m][k] B[n][k] of 16-bit operands with fp32 accumulation on the fifth-generation
 // tensor cores, and what is done with the accumulators before they leave the chip (EPI_*). One persistent kernel:
-//   warp 0      copies operand tiles (128-byte swizzle) into a ring of shared-memory stages,
-//   warp 3      idle but for one rare task (EpiArgs::dirty); warp 2 allocates TMEM,
-//   warp 1      issues the products of a stage (64 contracted elements) into one of two TMEM accumulators,
+//   warps 0, 3  copy the tiles of A and of B (128-byte swizzle) into a ring of shared-memory stages,
+//   warp 2      allocates TMEM (and has one rare task, EpiArgs::dirty),
+//   warp 1      issues the products of a stage (64 contracted elements, 128 of small tiles: the handshakes of a stage cost
+//               some 300 clocks, 234 on this side, which is more than a small tile's products) into one of two TMEM accumulators,
 //   warps 4-19  two groups of eight; each group reads its own accumulator, 32 columns at a time (thread = row, two
 //               warps share a row's strips), and runs the epilogue of every other tile, so that the epilogues of two tiles
 //               overlap each other's latency and the products of the tiles behind them. Results cross over in shared
@@ -12,8 +13,9 @@
 // CG = 2: two CTAs (a cluster) work on one tile of 256 rows; each holds its 128 rows of A and half of the B tile, so a
 // tile of 256 columns takes 128 bytes of operands per SM and clock at the full rate of the tensor cores instead of 192.
 // The tensor cores cut the sums they add to where they do not fit 32 bits, always to the same side, so a long sum drifts (measured:
-// 3e-6 relative after 4096 products). Tiles of up to 128 columns leave TMEM columns free: they spread the contracted
-// axis over several accumulators, 512 elements at least in each, which the epilogue adds with correct rounding.
+// 3e-6 relative after 4096 products). That is far below a 16-bit result's rounding, but not below an fp32 loss': where that is
+// made, tiles of up to 128 columns, which leave TMEM columns free, spread the contracted axis over several accumulators,
+// 512 elements at least in each, and the epilogue adds them with correct rounding.
 // Either operand may have the contracted axis contiguous (K-major) or the other one (MN-major): the backward products
 // need no transposed copies. Rows and columns beyond the matrices arrive as zeros and are not stored.
 #pragma once
@@ -88,7 +90,8 @@ struct GemmArgs {
     int kblocks, kblocks_per_split;
     int kblocks_per_sum;       // contracted blocks that go into one accumulator of a tile
     int a_box_rows;            // rows of a K-major A copy
-    uint32_t idesc, stage_bytes, stages;
+    int stage_blocks;          // contracted blocks of a stage
+    uint32_t idesc, block_bytes, stages;
     int* status;
     unsigned long long wait_cycles;
     int skip_block;            // copies of the k-blocks from this one on are left out (-1: none)
@@ -338,7 +341,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     if (threadIdx.x == 0) {
         gave_up_s = 0;
         for (int s = 0; s < S; s++) {
-            tc::bar_init(full(s), 1);
+            tc::bar_init(full(s), 2);   // what A and what B have to bring
             tc::bar_init(empty(s), 1);
         }
         for (int b = 0; b < 2; b++) {
@@ -377,9 +380,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     };
     const int bn_cta = g.bn / CG;
 
-    if (warp == 0) {
+    if (warp == 0 || warp == 3) {
+        const bool loads_a = warp == 0;
         if (tc::elect_one()) {
-            const CUtensorMap* map_b = (g.b_select && *g.b_select) ? &g.b_alt : &g.b;
+            const CUtensorMap* map_b = (!loads_a && g.b_select && *g.b_select) ? &g.b_alt : &g.b;
+            const uint32_t block_bytes = loads_a ? (A_MN ? kTileM : g.a_box_rows) * kTileK * 2 : bn_cta * kTileK * 2;
             int s = 0;
             uint32_t phase = 0;
             long long filled = 0;
@@ -389,27 +394,30 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 place(t, mb, nb, sp);
                 const int m0 = mb * (kTileM * CG) + (int)rank * kTileM, n0 = nb * g.bn + (int)rank * bn_cta;
                 const int k_end = min(g.kblocks, (sp + 1) * g.kblocks_per_split);
-                for (int kb = sp * g.kblocks_per_split; kb < k_end; kb++) {
+                for (int k0 = sp * g.kblocks_per_split; k0 < k_end; k0 += g.stage_blocks) {
                     ok = tc::bar_wait(empty(s), phase ^ 1, patience);
                     if (!ok) break;
-                    const uint32_t sa = smem0 + s * g.stage_bytes, sb = sa + kTileM * kTileK * 2;
+                    const int blocks = min(g.stage_blocks, k_end - k0);
                     uint32_t bar = full(s);
                     if constexpr (CG == 2) bar = tc::map_to_rank(bar, 0);
-                    if (rank == 0) {
-                        const uint32_t a_bytes = A_MN ? kTileM * kTileK * 2 : g.a_box_rows * kTileK * 2;
-                        tc::bar_expect(full(s), CG * (a_bytes + bn_cta * kTileK * 2));
-                    }
-                    if (g.skip_block < 0 || kb < g.skip_block) {
-                        if constexpr (A_MN) {
-                            tc::tma_load<CG>(sa, &g.a, m0, kb * kTileK, bar);
-                            tc::tma_load<CG>(sa + 64 * kTileK * 2, &g.a, m0 + 64, kb * kTileK, bar);
+                    if (rank == 0) tc::bar_expect(full(s), CG * blocks * block_bytes);
+                    for (int i = 0; i < blocks; i++) {
+                        const int kb = k0 + i;
+                        if (g.skip_block >= 0 && kb >= g.skip_block) break;
+                        const uint32_t sa = smem0 + (s * g.stage_blocks + i) * g.block_bytes, sb = sa + kTileM * kTileK * 2;
+                        if (loads_a) {
+                            if constexpr (A_MN) {
+                                tc::tma_load<CG>(sa, &g.a, m0, kb * kTileK, bar);
+                                tc::tma_load<CG>(sa + 64 * kTileK * 2, &g.a, m0 + 64, kb * kTileK, bar);
+                            } else {
+                                tc::tma_load<CG>(sa, &g.a, kb * kTileK, m0, bar);
+                            }
                         } else {
-                            tc::tma_load<CG>(sa, &g.a, kb * kTileK, m0, bar);
-                        }
-                        if constexpr (B_MN) {
-                            for (int j = 0; j < bn_cta; j += 64) tc::tma_load<CG>(sb + j * kTileK * 2, map_b, n0 + j, kb * kTileK, bar);
-                        } else {
-                            tc::tma_load<CG>(sb, map_b, kb * kTileK, n0, bar);
+                            if constexpr (B_MN) {
+                                for (int j = 0; j < bn_cta; j += 64) tc::tma_load<CG>(sb + j * kTileK * 2, map_b, n0 + j, kb * kTileK, bar);
+                            } else {
+                                tc::tma_load<CG>(sb, map_b, kb * kTileK, n0, bar);
+                            }
                         }
                     }
                     filled++;
@@ -445,22 +453,24 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 tc::fence_after();
                 uint32_t d = tmem + buf * kTileNMax - g.bn;
                 int left = 0;   // blocks that still go into accumulator d
-                for (int kb = k_begin; kb < k_end; kb++) {
-                    const bool fresh = left == 0;
-                    if (fresh) {
-                        d += g.bn;
-                        left = g.kblocks_per_sum;
-                    }
-                    left--;
+                for (int k0 = k_begin; k0 < k_end; k0 += g.stage_blocks) {
                     ok = tc::bar_wait(full(s), phase, patience);
                     if (!ok) break;
                     tc::fence_after();
-                    const uint32_t sa = smem0 + s * g.stage_bytes, sb = sa + kTileM * kTileK * 2;
-                    const uint64_t da = tc::operand_desc(sa, A_MN, 64 * kTileK * 2), db = tc::operand_desc(sb, B_MN, 64 * kTileK * 2);
+                    for (int i = 0; i < g.stage_blocks && k0 + i < k_end; i++) {
+                        const bool fresh = left == 0;
+                        if (fresh) {
+                            d += g.bn;
+                            left = g.kblocks_per_sum;
+                        }
+                        left--;
+                        const uint32_t sa = smem0 + (s * g.stage_blocks + i) * g.block_bytes, sb = sa + kTileM * kTileK * 2;
+                        const uint64_t da = tc::operand_desc(sa, A_MN, 64 * kTileK * 2), db = tc::operand_desc(sb, B_MN, 64 * kTileK * 2);
 #pragma unroll
-                    for (int k = 0; k < kTileK / 16; k++)
-                        tc::mma_f16<CG>(d, da + k * (A_MN ? 2048 >> 4 : 32 >> 4), db + k * (B_MN ? 2048 >> 4 : 32 >> 4), g.idesc,
-                                        (!fresh || k > 0) ? 1u : 0u);
+                        for (int k = 0; k < kTileK / 16; k++)
+                            tc::mma_f16<CG>(d, da + k * (A_MN ? 2048 >> 4 : 32 >> 4), db + k * (B_MN ? 2048 >> 4 : 32 >> 4), g.idesc,
+                                            (!fresh || k > 0) ? 1u : 0u);
+                    }
                     issued = true;
                     tc::mma_commit<CG>(empty(s));
                     if (++s == S) {
@@ -479,7 +489,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             }
         }
         __syncwarp();
-    } else if (warp == 3) {
+    } else if (warp == 2) {
         if constexpr (EPI == EPI_CE_GRAD) {
             if (g.e.dirty && *g.e.dirty) {
                 const int cols = g.k;
@@ -584,7 +594,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 float v[32];
 #pragma unroll
                 for (int i = 0; i < 32; i++) v[i] = __uint_as_float(raw[i]);
-                for (int s = 1; s < sums; s++) {   // the tile's other accumulators
+                for (int s = 1; EPI == EPI_CE_STATS && s < sums; s++) {   // the tile's other accumulators
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {
                         uint32_t more[8];
@@ -844,7 +854,7 @@ struct GemmWait {
 };
 
 // Fills the launch block. Both operands are map_ready.
-int gemm_args(GemmArgs* g, const DeviceInfo& dev, bool bf16, const Operand& a, const Operand& b, const Operand* b_alt, const int* b_select, const GemmPlan& plan,
+int gemm_args(GemmArgs* g, const DeviceInfo& dev, int epi, bool bf16, const Operand& a, const Operand& b, const Operand* b_alt, const int* b_select, const GemmPlan& plan,
               const EpiArgs& e, const GemmWait& wait, const char* what);
 
 template <int EPI, bool A_MN, bool B_MN>
@@ -854,7 +864,7 @@ int gemm_launch(bool bf16, const Operand& a, const Operand& b, const Operand* b_
     DeviceInfo dev;
     int rc = device_info(&dev);
     if (rc) return rc;
-    rc = gemm_args(&g, dev, bf16, a, b, b_alt, b_select, plan, e, wait, what);
+    rc = gemm_args(&g, dev, EPI, bf16, a, b, b_alt, b_select, plan, e, wait, what);
     if (rc) return rc;
     if (plan.cg == 2)
         return bf16 ? gemm_launch_as<__nv_bfloat16, A_MN, B_MN, EPI, 2>(g, dev, stream, what)
