@@ -73,7 +73,7 @@ int make_map(CUtensorMap* map, const Operand& o, bool bf16, int box_rows, const 
 // A model of the kernel's time in clocks, good enough to order the ways of cutting a product:
 //   a k-block of a tile takes the longer of the tensor cores' time (2 bn clocks: 128 rows per SM and 4096 products a
 //   clock, but 290 at least: they read all 128 rows of A however few the columns are) and the copies' (about 48 bytes of
-//   operands per SM and clock while all SMs copy);
+//   operands per SM and clock while most SMs copy, up to twice that while few do);
 //   a tile also keeps its group of epilogue warps busy (about 16 clocks a column; two groups take turns);
 //   the last tile's epilogue is not hidden, and pieces of the contracted axis have to be joined by another launch (about 8000,
 //   half of it on the host). Clusters whose CTAs join their pieces through distributed shared memory were tried instead: 14 us against
@@ -81,7 +81,7 @@ int make_map(CUtensorMap* map, const Operand& o, bool bf16, int box_rows, const 
 GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed, bool may_split) {
     GemmPlan best = {};
     double best_cost = 0;
-    const int kblocks = (k + kTileK - 1) / kTileK;
+    const int kblocks = (k + kTileK - 1) / kTileK, a_rows = m < kTileM ? m : kTileM;
     for (int cg = 2; cg >= 1; cg--) {
         if (cg == 2 && m <= kTileM) continue;
         const int unit = (b_transposed ? 64 : 32) * cg, slots = dev.sms / cg;
@@ -90,8 +90,7 @@ GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed
             const int tiles_n = (n + bn - 1) / bn;
             if (bn > unit && (n + bn - unit - 1) / (bn - unit) == tiles_n && bn - unit >= n) continue;   // wider than the matrix
             const long long tiles = (long long)tiles_m * tiles_n;
-            const double copies = (kTileM + bn / cg) * 128 / 48.0, products = 2.0 * bn > 290 ? 2.0 * bn : 290;
-            const double block = copies > products ? copies : products, epilogue = 16.0 * bn + 500;
+            const double products = 2.0 * bn > 290 ? 2.0 * bn : 290, epilogue = 16.0 * bn + 500;
             // one piece, or as many as the free SMs take in one or two rounds
             long long choices[3] = {1, 1, 1};
             if (may_split && kblocks >= 16) {
@@ -103,8 +102,9 @@ GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed
             }
             for (long long s : choices) {
                 const int per = (int)((kblocks + s - 1) / s), splits = (kblocks + per - 1) / per;   // none of them empty
-                const long long waves = (tiles * splits + slots - 1) / slots;
-                const double work = per * block + 300;
+                const long long units = tiles * splits, waves = (units + slots - 1) / slots;
+                const double rate = units * 2 >= slots ? 48.0 : 96.0 - 96.0 * units / slots;
+                const double copies = (a_rows + bn / cg) * 128 / rate, block = copies > products ? copies : products, work = per * block + 300;
                 double cost = waves * (work > epilogue / 2 ? work : epilogue / 2) + epilogue + 1000;
                 if (splits > 1) cost += 8000 + 8.0 * splits * m * n / 2500;   // partial sums: about 2500 bytes a clock
                 if (best_cost == 0 || cost < best_cost * 0.99) {
@@ -284,15 +284,47 @@ struct PackArgs {
     long long lds[2], ldd[2], total[2];   // total: pieces of 8 elements
     int cols[2];
 };
+// Eight elements at any address: cut out of the two aligned vectors that hold them (the second only if they reach into it;
+// neither leaves the 16-byte granules of the row's elements).
+__device__ __forceinline__ uint4 load8_anywhere(const uint16_t* p, int count) {
+    const int offset = (int)((uintptr_t)p & 15);
+    const uint4* q = reinterpret_cast<const uint4*>((uintptr_t)p - offset);
+    const uint4 a = __ldg(q);
+    const uint4 b = offset + 2 * min(count, 8) > 16 ? __ldg(q + 1) : make_uint4(0, 0, 0, 0);
+    const uint32_t both[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    uint32_t w[4];
+    const int bits = (offset & 3) * 8;
+    switch (offset >> 2) {
+        case 0: window<4, 0>(both, w, bits); break;
+        case 1: window<4, 1>(both, w, bits); break;
+        case 2: window<4, 2>(both, w, bits); break;
+        default: window<4, 3>(both, w, bits); break;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Rows are padded to whole pieces; what the padding holds does not matter, the tensor map ends before it.
 __global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
+    constexpr int U = 4;   // pieces in flight
     pdl_launch_dependents();
     pdl_wait();
     const int w = blockIdx.y, cols = a.cols[w];
-    const long long groups = (cols + 7) / 8;
-    for (long long t = blockIdx.x * 256ll + threadIdx.x; t < a.total[w]; t += (long long)gridDim.x * 256) {
-        const long long row = t / groups;
-        const int col = (int)(t - row * groups) * 8;
-        *reinterpret_cast<uint4*>(a.dst[w] + row * a.ldd[w] + col) = load8(a.src[w] + row * a.lds[w] + col, cols - col, false);
+    const long long groups = (cols + 7) / 8, stride = (long long)gridDim.x * 256;
+    for (long long t0 = blockIdx.x * 256ll + threadIdx.x; t0 < a.total[w]; t0 += U * stride) {
+        uint4 v[U];
+        long long at[U];
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const long long t = t0 + i * stride;
+            at[i] = -1;
+            if (t >= a.total[w]) continue;
+            const long long row = a.total[w] < (1ll << 31) ? (long long)((uint32_t)t / (uint32_t)groups) : t / groups;
+            const int col = (int)(t - row * groups) * 8;
+            v[i] = load8_anywhere(a.src[w] + row * a.lds[w] + col, cols - col);
+            at[i] = row * a.ldd[w] + col;
+        }
+#pragma unroll
+        for (int i = 0; i < U; i++)
+            if (at[i] >= 0) *reinterpret_cast<uint4*>(a.dst[w] + at[i]) = v[i];
     }
 }
 

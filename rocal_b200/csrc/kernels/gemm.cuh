@@ -29,7 +29,7 @@ constexpr int kEpiWarps = 16, kGemmThreads = 128 + 32 * kEpiWarps;
 constexpr int kStageBytes = 2048;            // of an epilogue warp: 32 lines of 64 bytes
 constexpr int kRingBytes = 196608;           // of the 227 KB: operand stages
 
-enum { EPI_LINEAR = 0, EPI_STORE = 1, EPI_CE_STATS = 2, EPI_CE_GRAD = 3 };
+enum { EPI_LINEAR = 0, EPI_STORE = 1, EPI_CE_STATS = 2, EPI_CE_GRAD = 3, EPI_LINEAR_ADD = 4 };   // ADD: with a residual
 enum { ACT_NONE = RB200_ACT_NONE, ACT_RELU = RB200_ACT_RELU, ACT_GELU = RB200_ACT_GELU, ACT_SILU = RB200_ACT_SILU };
 
 // A factor that is partly known on the device only: constant * *scalar / max(1, *count).
@@ -145,17 +145,32 @@ __device__ __forceinline__ void unpack8(const uint4& w, float (&v)[8]) {
     }
 }
 
+// W words that start SHIFT words and `bits` bits into two neighbouring vectors of W words.
+template <int W, int SHIFT>
+__device__ __forceinline__ void window(const uint32_t (&w)[2 * W], uint32_t (&out)[W], int bits) {
+#pragma unroll
+    for (int k = 0; k < W; k++) out[k] = __funnelshift_r(w[SHIFT + k], w[(SHIFT + k + 1) % (2 * W)], bits);
+}
+
 // Upper tail of the normal distribution over its density shape: R(a) = Q(a) exp(a^2 / 2) for a in [0, 6], a polynomial
 // of degree 12 in a / 3 - 1 fitted for the least relative error (2.3e-6 evaluated in fp32). Beyond 6, where Q is below
-// 1e-9, R(6) stands in. Two values at a time.
-__device__ __forceinline__ float2 tail_ratio(float2 a) {
-    constexpr float c[13] = {0.121513851f,   -0.103198029f, 0.0824128985f,  -0.0624807179f,   0.0450092852f,  -0.0303888023f, 0.020790372f,
-                             -0.0161429029f, 0.00893525127f, -0.000628449256f, 0.00143634493f, -0.00477083307f, 0.0022911916f};
-    const float2 t = fma2(make_float2(fminf(a.x, 6.0f), fminf(a.y, 6.0f)), make_float2(1.0f / 3.0f, 1.0f / 3.0f), make_float2(-1.0f, -1.0f));
-    float2 r = make_float2(c[12], c[12]);
-#pragma unroll
-    for (int i = 11; i >= 0; i--) r = fma2(r, t, make_float2(c[i], c[i]));
-    return r;
+// 1e-9, R(6) stands in. In single operations, not in packed pairs: a pair's coefficients would sit in 26 registers, which the
+// epilogues do not have (they spilled, and the spills took half of the L1's stores).
+__device__ __forceinline__ float tail_ratio(float a) {
+    const float t = fmaf(fminf(a, 6.0f), 1.0f / 3.0f, -1.0f);
+    float r = 0.0022911916f;
+    r = fmaf(r, t, -0.00477083307f);
+    r = fmaf(r, t, 0.00143634493f);
+    r = fmaf(r, t, -0.000628449256f);
+    r = fmaf(r, t, 0.00893525127f);
+    r = fmaf(r, t, -0.0161429029f);
+    r = fmaf(r, t, 0.020790372f);
+    r = fmaf(r, t, -0.0303888023f);
+    r = fmaf(r, t, 0.0450092852f);
+    r = fmaf(r, t, -0.0624807179f);
+    r = fmaf(r, t, 0.0824128985f);
+    r = fmaf(r, t, -0.103198029f);
+    return fmaf(r, t, 0.121513851f);
 }
 __device__ __forceinline__ float exp2_fast(float x) {
     float r;
@@ -164,22 +179,16 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 // z Phi(z) = max(z, 0) - |z| Q(|z|): one exponential and no division, accurate in the negative tail as well: beyond 6,
 // |z| R(|z|) is within 2% of what it is at 6. Infinities give 0 and inf (the exponential is 0 there), NaN stays.
-__device__ __forceinline__ float2 gelu2(float2 z) {
-    const float2 a = make_float2(fminf(fabsf(z.x), 6.0f), fminf(fabsf(z.y), 6.0f));
-    const float2 h = mul2(z, mul2(z, make_float2(-0.72134752f, -0.72134752f)));
-    const float2 e = make_float2(exp2_fast(h.x), exp2_fast(h.y));
-    const float2 q = mul2(mul2(a, e), tail_ratio(a));
-    return make_float2((z.x < 0.0f ? 0.0f : z.x) - q.x, (z.y < 0.0f ? 0.0f : z.y) - q.y);
+__device__ __forceinline__ float gelu(float z) {
+    const float a = fminf(fabsf(z), 6.0f), e = exp2_fast(z * (z * -0.72134752f));
+    return (z < 0.0f ? 0.0f : z) - a * e * tail_ratio(a);
 }
 // Phi(z) + z phi(z). |z| is held at 40, where the exponential is 0, so that infinities give 0 and 1.
-__device__ __forceinline__ float2 gelu_slope2(float2 z) {
-    const float2 a = make_float2(fminf(fabsf(z.x), 40.0f), fminf(fabsf(z.y), 40.0f));
-    const float2 h = mul2(a, mul2(a, make_float2(-0.72134752f, -0.72134752f)));
-    const float2 e = make_float2(exp2_fast(h.x), exp2_fast(h.y));
+__device__ __forceinline__ float gelu_slope(float z) {
+    const float a = fminf(fabsf(z), 40.0f), e = exp2_fast(a * (a * -0.72134752f));
     // |z| phi - Q, which the sign of z turns into the distance from 1 or from 0
-    const float2 r = tail_ratio(a);
-    const float2 d = mul2(e, fma2(a, make_float2(0.39894228f, 0.39894228f), make_float2(-r.x, -r.y)));
-    return make_float2(z.x < 0.0f ? -d.x : z.x >= 0.0f ? 1.0f + d.x : z.x, z.y < 0.0f ? -d.y : z.y >= 0.0f ? 1.0f + d.y : z.y);
+    const float d = e * fmaf(a, 0.39894228f, -tail_ratio(a));
+    return z < 0.0f ? -d : z >= 0.0f ? 1.0f + d : z;
 }
 __device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + exp2_fast(z * -1.4426950408889634f)); }
 
@@ -191,11 +200,7 @@ __device__ __forceinline__ void act_values(float* v, int act) {
         for (int i = 0; i < N; i++) v[i] = v[i] < 0.0f ? 0.0f : v[i];   // NaN stays
     } else if (act == ACT_GELU) {
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const float2 r = gelu2(make_float2(v[i], v[i + 1]));
-            v[i] = r.x;
-            v[i + 1] = r.y;
-        }
+        for (int i = 0; i < N; i++) v[i] = gelu(v[i]);
     } else if (act == ACT_SILU) {
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] *= sigmoid(v[i]);
@@ -208,11 +213,7 @@ __device__ __forceinline__ void act_slopes(float* v, int act) {   // z -> slope
         for (int i = 0; i < N; i++) v[i] = v[i] > 0.0f ? 1.0f : v[i] <= 0.0f ? 0.0f : v[i];   // NaN stays
     } else if (act == ACT_GELU) {
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const float2 r = gelu_slope2(make_float2(v[i], v[i + 1]));
-            v[i] = r.x;
-            v[i + 1] = r.y;
-        }
+        for (int i = 0; i < N; i++) v[i] = gelu_slope(v[i]);
     } else if (act == ACT_SILU) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
@@ -542,13 +543,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             }
 
             int res_row[4];   // the residual's rows of this lane (below), -1: none
-            if constexpr (EPI == EPI_LINEAR) {
-                if (g.e.residual) {
+            if constexpr (EPI == EPI_LINEAR_ADD) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int r = row0 + (lane >> 2) + 8 * i;
-                        res_row[i] = r < g.m ? r % g.e.residual_rows : -1;
-                    }
+                for (int i = 0; i < 4; i++) {
+                    const int r = row0 + (lane >> 2) + 8 * i;
+                    res_row[i] = r < g.m ? r % g.e.residual_rows : -1;
                 }
             }
 
@@ -573,19 +572,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 if constexpr (EPI != EPI_STORE) {
                     if (work && g.e.bias && lane < count) own_bias = Elem<T>::to_float(reinterpret_cast<const T*>(g.e.bias)[col + lane]);
                 }
-                uint4 res[4];   // the residual's strip: lane l takes piece l % 4 of the rows l / 4 + 8 i
-                if constexpr (EPI == EPI_LINEAR) {
-                    if (work && g.e.residual) {
-                        const int left = count - (lane & 3) * 8;
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            res[i] = make_uint4(0, 0, 0, 0);
-                            if (res_row[i] >= 0 && left > 0)
-                                res[i] = load8(reinterpret_cast<const T*>(g.e.residual) + res_row[i] * g.e.ldr + col + (lane & 3) * 8, left,
-                                               g.e.vec_res);
-                        }
-                    }
-                }
                 tc::tmem_wait();
                 if (!work) {
                     if (c + 64 >= g.bn) release();
@@ -602,6 +588,19 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                         tc::tmem_wait();
 #pragma unroll
                         for (int j = 0; j < 8; j++) v[i + j] += __uint_as_float(more[j]);
+                    }
+                }
+                uint4 res[4];   // the residual's strip: lane l takes piece l % 4 of the rows l / 4 + 8 i
+                if constexpr (EPI == EPI_LINEAR_ADD) {
+                    {
+                        const int left = count - (lane & 3) * 8;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            res[i] = make_uint4(0, 0, 0, 0);
+                            if (res_row[i] >= 0 && left > 0)
+                                res[i] = load8(reinterpret_cast<const T*>(g.e.residual) + res_row[i] * g.e.ldr + col + (lane & 3) * 8, left,
+                                               g.e.vec_res);
+                        }
                     }
                 }
                 if (c + 64 >= g.bn) release();
@@ -629,16 +628,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     __syncwarp();
                     copy_strip(area, reinterpret_cast<T*>(out), ld, vec, col, min(32, count), row0, g.m - row0, lane);
                 };
-                if constexpr (EPI == EPI_LINEAR) {
+                if constexpr (EPI == EPI_LINEAR || EPI == EPI_LINEAR_ADD) {
                     if (g.e.preact) {
                         leave(g.e.preact, g.e.ldp, g.e.vec_pre);
                         __syncwarp();
                     }
                     if (g.e.act != ACT_NONE) {
-                        act_values<16>(v, g.e.act);
-                        act_values<16>(v + 16, g.e.act);
+                        act_values<8>(v, g.e.act);
+                        act_values<8>(v + 8, g.e.act);
+                        act_values<8>(v + 16, g.e.act);
+                        act_values<8>(v + 24, g.e.act);
                     }
-                    if (g.e.residual) {   // the other way round: whole pieces of rows in, a row a thread out
+                    if constexpr (EPI == EPI_LINEAR_ADD) {   // the other way round: whole pieces of rows in, a row a thread out
 #pragma unroll
                         for (int i = 0; i < 4; i++) st_shared16(staged(area, (lane >> 2) + 8 * i, lane & 3), res[i]);
                         __syncwarp();

@@ -151,13 +151,6 @@ __global__ void __launch_bounds__(kClipThreads) clip_norm_kernel(const __grid_co
 }
 
 // ---- multiplication -----------------------------------------------------------------------------------------
-// W words (the gradients of one 16-byte vector of the output) that start SHIFT words and `bits` bits into two neighbouring
-// aligned vectors of W words.
-template <int W, int SHIFT>
-__device__ __forceinline__ void window(const uint32_t (&w)[2 * W], uint32_t (&out)[W], int bits) {
-#pragma unroll
-    for (int k = 0; k < W; k++) out[k] = __funnelshift_r(w[SHIFT + k], w[(SHIFT + k + 1) % (2 * W)], bits);
-}
 template <int W>
 __device__ __forceinline__ void load_words(const uint32_t* p, uint32_t* w) {
     if constexpr (W == 4) {
@@ -343,7 +336,7 @@ __global__ void __launch_bounds__(kClipThreads) __cluster_dims__(kClipCluster, 1
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------
-constexpr int kClipSmall = 16, kClipMedium = 192, kClipLarge = 960;   // 960 entries: 30 KB of launch parameters
+constexpr int kClipMedium = 192, kClipLarge = 960;   // 960 entries: 30 KB of launch parameters
 
 enum { CLIP_NORM, CLIP_SCALE, CLIP_FEW };
 template <int CAP>
@@ -367,23 +360,46 @@ static int clip_table_launch(const ClipEntry* entries, int n, int chunks, int ch
 
 static size_t clip_bytes(int dtype) { return dtype == RB200_FP32 ? 4 : 2; }
 
+struct ClipRange {
+    uintptr_t begin, end;
+    bool out;
+};
+// Ascending order of begin. Comparison sorts cost some 30 us for the 600 ranges of 300 tensors, mostly in mispredicted
+// branches; counting 11 bits at a time, over the bits in which the addresses differ, takes about 5.
+static void sort_ranges(std::vector<ClipRange>& r) {
+    uintptr_t low = ~(uintptr_t)0, high = 0;
+    bool sorted = true;
+    for (size_t i = 0; i < r.size(); i++) {
+        low = std::min(low, r[i].begin);
+        high = std::max(high, r[i].begin);
+        sorted &= i == 0 || r[i - 1].begin <= r[i].begin;
+    }
+    if (sorted) return;
+    if (r.size() < 64) {
+        std::sort(r.begin(), r.end(), [](const ClipRange& a, const ClipRange& b) { return a.begin < b.begin; });
+        return;
+    }
+    std::vector<ClipRange> other(r.size());
+    for (int shift = 0; (high - low) >> shift; shift += 11) {
+        uint32_t at[2049] = {};
+        for (const ClipRange& a : r) at[((a.begin - low) >> shift & 2047) + 1]++;
+        for (int i = 0; i < 2048; i++) at[i + 1] += at[i];
+        for (const ClipRange& a : r) other[at[(a.begin - low) >> shift & 2047]++] = a;
+        r.swap(other);
+    }
+}
 // No output meets another output or another tensor's gradients.
 static bool outputs_disjoint(const std::vector<ClipEntry>& v) {
-    struct Range {
-        uintptr_t begin, end;
-        bool out;
-        size_t owner;
-    };
-    std::vector<Range> r;
+    std::vector<ClipRange> r;
     r.reserve(2 * v.size());
-    for (size_t i = 0; i < v.size(); i++) {
-        const uintptr_t g = (uintptr_t)v[i].grad, o = (uintptr_t)v[i].out;
-        r.push_back({o, o + v[i].count * clip_bytes(v[i].out_dtype), true, i});
-        if (g != o) r.push_back({g, g + v[i].count * clip_bytes(v[i].grad_dtype), false, i});
+    for (const ClipEntry& e : v) {
+        const uintptr_t g = (uintptr_t)e.grad, o = (uintptr_t)e.out;
+        r.push_back({o, o + e.count * clip_bytes(e.out_dtype), true});
+        if (g != o) r.push_back({g, g + e.count * clip_bytes(e.grad_dtype), false});
     }
-    std::sort(r.begin(), r.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+    sort_ranges(r);
     uintptr_t out_end = 0, any_end = 0;   // of the ranges so far
-    for (const Range& a : r) {
+    for (const ClipRange& a : r) {
         if (a.begin < out_end || (a.out && a.begin < any_end)) return false;
         if (a.out) out_end = std::max(out_end, a.end);
         any_end = std::max(any_end, a.end);
@@ -464,8 +480,11 @@ static int clip_run(const rb200_grad_tensor* tensors, int n, float max_norm, flo
                 chunks += (int)((first[i].count + chunk - 1) / chunk);
             }
             const int blocks = few ? kClipCluster : std::min(chunks, most);
-            auto* launch = count <= kClipSmall ? clip_table_launch<kClipSmall>
-                                               : count <= kClipMedium ? clip_table_launch<kClipMedium> : clip_table_launch<kClipLarge>;
+            auto* launch = count <= 16            ? clip_table_launch<16>
+                           : count <= 64          ? clip_table_launch<64>
+                           : count <= kClipMedium ? clip_table_launch<kClipMedium>
+                           : count <= 448         ? clip_table_launch<448>
+                                                  : clip_table_launch<kClipLarge>;
             rc = launch(first, count, chunks, (int)chunk, few ? CLIP_FEW : pass ? CLIP_SCALE : CLIP_NORM, pass ? partial : partial + partials, partials, max_norm, inv_scale,
                         k == 0 ? norm : nullptr, blocks, stream);
             if (rc) return rc;

@@ -292,6 +292,7 @@ static int linear_run(const rb200_linear_params* p, void* stream_v, GemmWait wai
         if ((rc = gemm_store(GEMM_KK, bf16, l.x.use, l.w.use, nullptr, nullptr, l.gemm, part, wait, stream, what))) return rc;
         return gemm_join(bf16, (const float*)l.partials, l.gemm.splits, (int)p->rows, (int)p->out_features, e, stream, what);
     }
+    if (e.residual) return gemm_launch<EPI_LINEAR_ADD, false, false>(bf16, l.x.use, l.w.use, nullptr, nullptr, l.gemm, e, wait, stream, what);
     return gemm_launch<EPI_LINEAR, false, false>(bf16, l.x.use, l.w.use, nullptr, nullptr, l.gemm, e, wait, stream, what);
 }
 
