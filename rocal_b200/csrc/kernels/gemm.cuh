@@ -152,32 +152,27 @@ __device__ __forceinline__ void window(const uint32_t (&w)[2 * W], uint32_t (&ou
     for (int k = 0; k < W; k++) out[k] = __funnelshift_r(w[SHIFT + k], w[(SHIFT + k + 1) % (2 * W)], bits);
 }
 
-// Upper tail of the normal distribution over its density shape: R(a) = Q(a) exp(a^2 / 2) for a in [0, 6], a polynomial
-// of degree 12 in a / 3 - 1 fitted for the least relative error (2.3e-6 evaluated in fp32). Beyond 6, where Q is below
-// 1e-9, R(6) stands in. In single operations, not in packed pairs: a pair's coefficients would sit in 26 registers, which the
-// epilogues do not have (they spilled, and the spills took half of the L1's stores).
+// Upper tail of the normal distribution over its density shape: R(a) = Q(a) exp(a^2 / 2) for a in [0, 6]. Q falls like
+// 1 / a times the density, so R is smooth in t = 1 / (1 + p a): a polynomial t, ..., t^6, fitted here together with p for the least
+// relative error (1.0e-6 evaluated in fp32, and the reciprocal's 1e-7). Beyond 6, where Q is below 1e-9, R(6) stands in.
+// (A polynomial in a takes degree 12 for 2e-6, and in packed pairs its coefficients sit in 26 registers: the epilogues
+// spilled, and the spills took half of the L1's stores.)
 __device__ __forceinline__ float tail_ratio(float a) {
-    const float t = fmaf(fminf(a, 6.0f), 1.0f / 3.0f, -1.0f);
-    float r = 0.0022911916f;
-    r = fmaf(r, t, -0.00477083307f);
-    r = fmaf(r, t, 0.00143634493f);
-    r = fmaf(r, t, -0.000628449256f);
-    r = fmaf(r, t, 0.00893525127f);
-    r = fmaf(r, t, -0.0161429029f);
-    r = fmaf(r, t, 0.020790372f);
-    r = fmaf(r, t, -0.0303888023f);
-    r = fmaf(r, t, 0.0450092852f);
-    r = fmaf(r, t, -0.0624807179f);
-    r = fmaf(r, t, 0.0824128985f);
-    r = fmaf(r, t, -0.103198029f);
-    return fmaf(r, t, 0.121513851f);
+    float t;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(fminf(a, 6.0f), 0.294f, 1.0f)));
+    float r = fmaf(t, -0.0888040438f, 0.272132337f);
+    r = fmaf(r, t, -0.0816512033f);
+    r = fmaf(r, t, 0.177665651f);
+    r = fmaf(r, t, 0.102016911f);
+    r = fmaf(r, t, 0.118640058f);
+    return r * t;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// z Phi(z) = max(z, 0) - |z| Q(|z|): one exponential and no division, accurate in the negative tail as well: beyond 6,
+// z Phi(z) = max(z, 0) - |z| Q(|z|): one exponential and one reciprocal, accurate in the negative tail as well: beyond 6,
 // |z| R(|z|) is within 2% of what it is at 6. Infinities give 0 and inf (the exponential is 0 there), NaN stays.
 __device__ __forceinline__ float gelu(float z) {
     const float a = fminf(fabsf(z), 6.0f), e = exp2_fast(z * (z * -0.72134752f));

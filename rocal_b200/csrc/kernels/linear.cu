@@ -146,14 +146,14 @@ __global__ void __launch_bounds__(256) sum_few_kernel(const float* __restrict__ 
     }
 }
 
-// How the block's threads lie and how many pieces the repeats are cut into: about eight blocks an SM, at least eight
+// How the block's threads lie and how many pieces the repeats are cut into: four blocks an SM (as many as fit), at least eight
 // repeats a thread.
 static void cut_rows(RowsArgs* a, int sms) {
     a->across = 1;
     while (a->across < 32 && a->across * 8 < a->cols) a->across *= 2;
     const int repeats = a->rows / a->period, wide = a->across * 8, least = 256 / a->across * 8;
     const long long blocks = (long long)((a->cols + wide - 1) / wide) * a->period;
-    long long chunks = 8ll * sms / blocks;
+    long long chunks = 4ll * sms / blocks;
     if (chunks > (repeats + least - 1) / least) chunks = (repeats + least - 1) / least;
     if (chunks < 1) chunks = 1;
     a->per_chunk = (int)((repeats + chunks - 1) / chunks);
