@@ -388,7 +388,10 @@ RB200_API int rb200k_transpose(const uint8_t* arena, const rb200_pointwise_sampl
  * operand of a matrix product is first copied into the workspace. Workspaces hold nothing of value between calls and
  * need no initialisation; two calls that can run at the same time need two workspaces. Results do not depend on
  * timing: no floating-point atomics are used. Every wait inside these kernels is bounded (see "Bounded waits"); trouble
- * goes to `status` or, where that is NULL, to the library-wide status word. */
+ * goes to `status` or, where that is NULL, to the library-wide status word. Outputs overlap neither inputs nor one
+ * another (rb200k_grad_clip says where it allows that). The calls may be captured into a graph; make the first call on a device
+ * before any capture (it looks up the device's properties and the status word's address). Launches overlap the tail of
+ * the stream's preceding kernel and wait for its completion before they touch memory. */
 enum { RB200_BF16 = 16 };   /* element type of the head operators besides RB200_FP16 / RB200_FP32 (not a rocAL type) */
 enum { RB200_ACT_NONE = 0, RB200_ACT_RELU = 1, RB200_ACT_GELU = 2, RB200_ACT_SILU = 3 };
 

@@ -11,6 +11,14 @@ int device_info(DeviceInfo* out) {
         set_error("device %d: only devices 0..63 are supported", dev);
         return RB200_E_LIMIT;
     }
+    // A thread that has not used CUDA yet (autograd's, for one) has a current device but no context, which the driver's
+    // tensor-map call needs; setting the device makes its primary context current.
+    static thread_local int bound = -1;
+    if (bound != dev) {
+        rc = check_cuda(cudaSetDevice(dev), "cudaSetDevice");
+        if (rc) return rc;
+        bound = dev;
+    }
     // properties of the device; every writer writes the same values
     static int sms[64];
     static int* words[64];

@@ -300,7 +300,7 @@ static int linear_run(const rb200_linear_params* p, void* stream_v, GemmWait wai
 struct LinearBackwardPlan {
     Packed x, w;
     Operand dz;               // [rows][out]: dout itself, or the copy that rows_kernel writes
-    bool own_dz, sums;        // sums: rows_kernel makes the column sums
+    bool own_dz, sums, reuse; // sums: rows_kernel makes the column sums; reuse: they come from the residual's
     RowsArgs bias_rows, res_rows;
     GemmPlan gx, gw;
     void *px, *pw;
@@ -344,11 +344,12 @@ static LinearBackwardPlan plan_backward(const rb200_linear_backward_params& p, c
             l.res_rows.out = p.dresidual;
             l.res_rows.ldo = p.lddr;
         }
-        if (l.res_rows.chunks > 1 || (p.dbias && p.activation == RB200_ACT_NONE))
+        // without an activation the column sums are the sums of the residual's sums, if those are few: no second sweep
+        l.reuse = p.dbias && p.activation == RB200_ACT_NONE && (long long)l.res_rows.chunks * l.res_rows.period <= 1024;
+        if (l.res_rows.chunks > 1 || l.reuse)
             l.res_rows.part = (float*)c.take((size_t)l.res_rows.chunks * l.res_rows.period * a.ldpart * sizeof(float));
     }
-    // without an activation the column sums are the sums of the residual's sums: no second sweep
-    l.sums = p.dbias && (p.activation != RB200_ACT_NONE || !p.dresidual);
+    l.sums = p.dbias && !l.reuse;
     l.bias_rows = a;
     l.bias_rows.period = 1;
     cut_rows(&l.bias_rows, dev.sms);
@@ -406,7 +407,7 @@ static int backward_run(const rb200_linear_backward_params* p, void* stream_v) {
         const RowsArgs& r = l.res_rows;
         if ((rc = rows_launch(bf16, r, stream, what))) return rc;
         if (!r.out && (rc = sum_chunks(bf16, r.part, r.ldpart, r.chunks, r.period, (int)m, p->dresidual, p->lddr, Scale(), stream, what))) return rc;
-        if (p->dbias && !l.sums &&
+        if (l.reuse &&
             (rc = sum_chunks(bf16, r.part, r.ldpart, r.chunks * r.period, 1, (int)m, p->dbias, 0, Scale(), stream, what)))
             return rc;
     }

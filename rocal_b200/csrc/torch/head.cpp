@@ -103,6 +103,10 @@ int32_t* status_word(const MaybeTensor& status, const Tensor& like) {
                       like.device());
     return status->data_ptr<int32_t>();
 }
+// The library has written to a tensor of the caller's: autograd's version check has to know.
+void written(const Tensor& t) {
+    if (!t.is_inference()) torch::autograd::impl::bump_version(t);
+}
 void* stream_of(const Tensor& x) { return c10::cuda::getCurrentCUDAStream(x.device().index()).stream(); }
 
 int activation(const std::string& name) {
@@ -153,6 +157,7 @@ Tensor linear_run(const Tensor& x_, const Tensor& weight_, const Tensor& bias_, 
         TORCH_CHECK_VALUE(out.dim() == 2 && out.size(0) == n && out.size(1) == m && has_rows(out), "out has shape ", out.sizes(), ", strides ",
                           out.strides(), "; (", n, ", ", m, ") with contiguous rows is needed");
         same_kind(out, "out", x);
+        written(out);
     } else {
         out = at::empty({n, m}, x.options());
     }
@@ -477,6 +482,7 @@ Tensor grad_clip(const std::vector<Tensor>& grads, double max_norm, const std::o
     const Tensor ws = workspace(bytes, grads[0]);
     check(api.clip(table.data(), (int)n, (float)max_norm, (float)inv_scale, norm.data_ptr<float>(), data(ws), bytes, stream_of(grads[0])),
           "rb200k_grad_clip");
+    for (const Tensor& o : out ? *out : grads) written(o);
     for (auto& b : back) b.first.copy_(b.second);
     return norm;
 }

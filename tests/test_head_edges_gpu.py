@@ -1,6 +1,9 @@
 """The head operators where they can go wrong: masked classes and rows, infinities and NaN, odd strides and alignments,
 outputs inside larger buffers, other streams, captured graphs, threads, waits that run out."""
 import math
+import os
+import subprocess
+import sys
 import threading
 
 import pytest
@@ -13,6 +16,7 @@ from test_head_loss_gpu import _check, _close, _make, _reference
 
 pytestmark = pytest.mark.gpu
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 WAIT_CYCLES = 2_000_000      # about a millisecond of SM clock
 
 
@@ -411,6 +415,72 @@ def test_clip_refusals_and_parameters(cuda):
     assert float(P.clip_grad_norm_([torch.nn.Parameter(torch.zeros((1,), device=cuda))], 1.0)) == 0.0
 
 
+# ---- sizes beyond 32 bits, what autograd is told -----------------------------------------------------
+
+
+def test_offsets_beyond_32_bits(cuda):
+    """Rows of 40000 elements apart: the last rows lie beyond 2^31 elements; gradients of more than 2^31 elements."""
+    from rocal_b200 import kernels as K
+    from rocal_b200.plugin import pytorch as P
+    n, ld, k, m = 60000, 40000, 64, 40
+    whole = torch.zeros((n, ld), dtype=torch.float16, device=cuda)           # 4.8 GB
+    g = torch.Generator(device=cuda).manual_seed(4)
+    x = whole[:, 16:16 + k]
+    x.copy_(torch.randn((n, k), generator=g, device=cuda))
+    w, b = torch.randn((m, k), generator=g, device=cuda).half() / 8, torch.randn((m,), generator=g, device=cuda).half()
+    out = whole[:, 2000:2000 + m]
+    K.linear(x, w, b, activation="relu", out=out)
+    y64, _, tol, _ = _forward(x, w, b, None, "relu", "fp16")
+    _linear_close(out, y64, tol, "y")
+    odd = whole[:, 3001:3001 + k]                                             # not on 16-byte boundaries: packed
+    odd.copy_(x)
+    assert torch.equal(K.linear(odd, w, b, activation="relu"), out)
+    dy = out
+    _, dw, db, _ = K.linear_backward(dy, x, w, need=(False, True, True, False))
+    _, dw2, db2, _ = K.linear_backward(dy.contiguous(), x.contiguous(), w, need=(False, True, True, False))
+    assert torch.equal(dw, dw2) and torch.equal(db, db2)
+    labels = torch.randint(0, m, (n,), generator=g, device=cuda)
+    assert torch.equal(P.linear_cross_entropy(x, w, labels, b), P.linear_cross_entropy(x.contiguous(), w, labels, b))
+    del whole, x, out, odd, dy
+    big = torch.full(((1 << 31) + 77,), 2.0 ** -10, dtype=torch.bfloat16, device=cuda)
+    small = torch.ones((3,), device=cuda)
+    norm = P.clip_grad_norm([big, small], 1.0)
+    want = math.sqrt(((1 << 31) + 77) * 2.0 ** -20 + 3)
+    assert abs(float(norm) / want - 1) <= 2.0 ** -23
+    c = torch.tensor(2.0 ** -10 / want, device=cuda).bfloat16()
+    assert bool((big[:1000] == c).all()) and bool((big[-1000:] == c).all()) and bool((big[(1 << 30) - 500:(1 << 30) + 500] == c).all())
+
+
+def test_in_place_writes_are_known_to_autograd(cuda):
+    from rocal_b200 import kernels as K
+    from rocal_b200.plugin import pytorch as P
+    a = torch.ones((8,), device=cuda, requires_grad=True)
+    saved = torch.full((8,), 2.0, device=cuda)
+    y = (a * saved).sum()                       # saves `saved`
+    P.clip_grad_norm([saved], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    out = torch.zeros((4, 8), device=cuda, dtype=torch.float16)
+    before = out._version
+    K.linear(torch.ones((4, 16), device=cuda, dtype=torch.float16), torch.ones((8, 16), device=cuda, dtype=torch.float16), out=out)
+    assert out._version > before
+
+
+@pytest.mark.parametrize("period", [1, 2, 60, 1024, 1500, 3000])
+def test_residual_gradients_of_any_period(cuda, period):
+    """Few and many rows to a residual row, with and without the bias' sums."""
+    from rocal_b200 import kernels as K
+    n, k, m = 3000 // period * period, 24, 300
+    x, w, _, _, dy = _linear_make(period, n, k, m, "bf16", False, 0, cuda)
+    z = torch.zeros((n, m), dtype=torch.float64, device=cuda)
+    wants, tols = _backward(x, w, dy, z, z, "none", period, "bf16")
+    for need in ((False, False, False, True), (False, False, True, True), (True, True, True, True)):
+        got = K.linear_backward(dy, x, w, residual_rows=period, need=need)
+        for g, want, tol, name in zip(got, wants, tols, ("dx", "dweight", "dbias", "dresidual")):
+            if g is not None:
+                _linear_close(g, want, tol, name)
+
+
 # ---- streams, graphs, threads --------------------------------------------------------------------------
 
 
@@ -543,6 +613,27 @@ def test_concurrent_threads(cuda):
     for t in threads:
         t.join()
     assert not wrong
+
+
+def test_threads_that_have_not_used_cuda(cuda):
+    """The first CUDA work of a thread is the operator's: a backward pass in a fresh process (autograd's own thread), a new
+    thread of this one."""
+    code = ("import torch\n"
+            "from rocal_b200.plugin import pytorch as P\n"
+            "x, w = torch.ones(8, 128).half().cuda(), torch.ones(10, 128).half().cuda().requires_grad_(True)\n"
+            "loss = P.linear_cross_entropy(x, w, torch.arange(8, device='cuda'))\n"
+            "loss.backward()\n"
+            "print('gradient', float(w.grad.float().abs().sum()) > 0)\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "gradient True" in r.stdout, r.stderr[-2000:]
+    from rocal_b200 import kernels as K
+    x, w, b, _, _ = _linear_make(1, 20, 64, 30, "fp16", True, 0, cuda)
+    want, got = K.linear(x, w, b), []
+    thread = threading.Thread(target=lambda: got.append(K.linear(x, w, b)))
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert torch.equal(want, got[0])
 
 
 def test_loss_bound_is_not_vacuous(cuda):

@@ -31,6 +31,7 @@ def _reference(x, w, b, labels, smooth, reduction, g, dtype, ignore=-100):
     """loss, gradients and their tolerances; ignored rows of x are taken as zeros, which is what "takes no part" means."""
     u = torch.finfo(TYPES[dtype]).eps / 2
     keep = labels.long() != ignore
+    x, w, b = x.detach(), w.detach(), None if b is None else b.detach()
     x, w = torch.where(keep[:, None], x.double(), torch.zeros((), dtype=torch.float64, device=x.device)), w.double()
     v, k = w.shape
     z = x @ w.t()
