@@ -51,7 +51,13 @@ __global__ void __launch_bounds__(256) ce_merge_kernel(MergeArgs a) {
     for (long long row0 = (long long)blockIdx.x * ROWS; row0 < a.rows; row0 += (long long)gridDim.x * ROWS) {
         const long long row = row0 + lane;
         RunningSoftmax r = {-INFINITY, 0.0f};
-        float z = 0.0f;
+        float z = 0.0f, at_label = 0.0f;
+        int label = -1;
+        bool counted = false;
+        if (row < a.rows && sub == 0 && a.last) {   // on their way while the parts are joined
+            label = load_label(a.labels, a.label_bytes, row, a.ignore_index, a.classes, &counted);
+            at_label = a.stats[2ll * a.rows + row];
+        }
         if (row < a.rows) {
 #pragma unroll 4
             for (int p = sub; p < a.parts; p += SUBS) {
@@ -81,8 +87,6 @@ __global__ void __launch_bounds__(256) ce_merge_kernel(MergeArgs a) {
         if (!a.last) {
             if (a.want_zsum) a.zsum[row] = z;
         } else {
-            bool counted;
-            const int label = load_label(a.labels, a.label_bytes, row, a.ignore_index, a.classes, &counted);
             float loss = 0.0f;
             if (counted) {
                 counts_mine++;
@@ -90,7 +94,7 @@ __global__ void __launch_bounds__(256) ce_merge_kernel(MergeArgs a) {
                     r.m = r.s = loss = nanf("");
                 } else {
                     const float lse = logf(r.s);   // above the maximum
-                    loss = (1.0f - a.smoothing) * (lse + (r.m - a.stats[2ll * a.rows + row]));
+                    loss = (1.0f - a.smoothing) * (lse + (r.m - at_label));
                     if (a.want_zsum) loss += a.smoothing * (lse + (r.m - z / (float)a.classes));
                 }
             } else {
@@ -149,7 +153,7 @@ __global__ void __launch_bounds__(256) ce_merge_kernel(MergeArgs a) {
     }
 }
 
-constexpr int kMergeBlocks = 148 * 8;
+constexpr int kMergeBlocks = 148 * 2;   // every block ends with atomics on the same words
 static int merge_launch(const MergeArgs& m, cudaStream_t stream, const char* what) {
     // as many threads a row as there are parts for them to share, while the rows alone do not fill the GPU
     const int subs = m.parts >= 32 && m.rows <= 4096 ? 32 : m.parts >= 8 ? 8 : m.parts >= 4 ? 4 : m.parts >= 2 && m.rows < 148 * 256 ? 2 : 1;
