@@ -1,6 +1,6 @@
-// rb200k_linear: out = act(x W^T + b) + r, and its gradients. The products run on the tensor cores (gemm.cuh); the
-// passes over the gradient of the output that the products do not make (activation slope, column sums, sums over rows
-// that share a residual row) are memory-bound and made by rows_kernel in one sweep.
+// rb200k_linear: out = act(x W^T + b) + r, and its gradients. The products run on the tensor cores (gemm.cuh), those of a few
+// rows on the ordinary ones (few_rows_kernel). The passes over the gradient of the output that the products do not make
+// (activation slope, column sums, sums over rows that share a residual row) are memory-bound and made by rows_kernel in one sweep.
 #include "matrix_args.cuh"
 
 namespace rb200 {
@@ -227,8 +227,189 @@ static int check_shape(const char* what, int dtype, int act, long long rows, lon
     return check_extents(what, rows, "in_features", in, "out_features", out);
 }
 
+// ---- a few rows ------------------------------------------------------------------------------------------------
+// Up to kFewRows rows: every element of W is used so few times that the product is a read of W, which bounds it, and a tile of
+// the tensor cores would be nearly empty. A warp takes C columns and a slice of the contracted axis; a lane holds 8 elements
+// of each column (16 bytes) against the same 8 of every row, whose few KB come from L1, while its next reads of W are in flight. Sums
+// in 32 bits, in pairs of elements (fma.f32x2), joined across lanes and then across the block's slices in a fixed order. Rows that
+// are not on 16-byte boundaries are read by elements, without packing. Several rows share what a row costs in L1 reads and
+// conversions between two columns. 1 x 2048 -> 1000: 4.0 us (tensor cores 8.9), the call 6.6 us of host time (8.2: two tensor maps).
+struct FewArgs {
+    const void *x, *w;
+    long long ldx, ldw;
+    int rows, cols, k;
+    int slices, per_slice;    // a power of two up to 8; elements of a slice, a multiple of 256
+    EpiArgs e;
+};
+constexpr int kFewRows = 4;
+
+__device__ __forceinline__ unsigned long long pair_bits(float2 f) {
+    return (unsigned long long)__float_as_uint(f.y) << 32 | __float_as_uint(f.x);
+}
+__device__ __forceinline__ unsigned long long fma_pairs(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+template <typename T, int R, int C, bool VEC>
+__global__ void __launch_bounds__(256) few_rows_kernel(const FewArgs a) {
+    constexpr int N = R * C, LOG = N == 1 ? 0 : N == 4 ? 2 : 3;
+    static_assert(N == 1 << LOG, "sums of a warp");
+    __shared__ float part[8][N];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slice = warp & (a.slices - 1);
+    const long long col0 = ((long long)blockIdx.x * (8 / a.slices) + warp / a.slices) * C;
+    const int k0 = slice * a.per_slice, k1 = min(a.k, k0 + a.per_slice);
+    const T *x[R], *w[C];
+#pragma unroll
+    for (int r = 0; r < R; r++) x[r] = reinterpret_cast<const T*>(a.x) + min(r, a.rows - 1) * a.ldx;   // what is not there is read, not kept
+#pragma unroll
+    for (int c = 0; c < C; c++) w[c] = reinterpret_cast<const T*>(a.w) + min(col0 + c, (long long)a.cols - 1) * a.ldw;
+    float v[N];
+    if constexpr (VEC) {
+        unsigned long long acc[R][C] = {};
+        auto add = [&](const uint4* wv, const uint4* xv) {
+            unsigned long long p[C][4];
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                p[c][0] = pair_bits(Elem<T>::unpack(wv[c].x));
+                p[c][1] = pair_bits(Elem<T>::unpack(wv[c].y));
+                p[c][2] = pair_bits(Elem<T>::unpack(wv[c].z));
+                p[c][3] = pair_bits(Elem<T>::unpack(wv[c].w));
+            }
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const unsigned long long q[4] = {pair_bits(Elem<T>::unpack(xv[r].x)), pair_bits(Elem<T>::unpack(xv[r].y)),
+                                                 pair_bits(Elem<T>::unpack(xv[r].z)), pair_bits(Elem<T>::unpack(xv[r].w))};
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int c = 0; c < C; c++) acc[r][c] = fma_pairs(p[c][i], q[i], acc[r][c]);
+            }
+        };
+        int k = k0 + lane * 8;
+        constexpr int U = C == 1 ? 4 : 2;   // steps whose reads of W are in flight while the ones before are summed
+        uint4 next[U][C];
+        auto fetch = [&](int at) {
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int c = 0; c < C; c++) next[u][c] = __ldg(reinterpret_cast<const uint4*>(w[c] + at + 256 * u));
+        };
+        auto whole = [&](int at) { return at + 256 * (U - 1) + 8 <= k1; };
+        if (whole(k)) fetch(k);
+#pragma unroll 1
+        for (; whole(k); k += 256 * U) {
+            uint4 wv[U][C];
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int c = 0; c < C; c++) wv[u][c] = next[u][c];
+            if (whole(k + 256 * U)) fetch(k + 256 * U);
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                uint4 xv[R];
+#pragma unroll
+                for (int r = 0; r < R; r++) xv[r] = __ldg(reinterpret_cast<const uint4*>(x[r] + k + 256 * u));
+                add(wv[u], xv);
+            }
+        }
+#pragma unroll 1
+        for (; k < k1; k += 256) {
+            uint4 wv[C], xv[R];
+#pragma unroll
+            for (int c = 0; c < C; c++) wv[c] = load8(w[c] + k, k1 - k, true);
+#pragma unroll
+            for (int r = 0; r < R; r++) xv[r] = load8(x[r] + k, k1 - k, true);
+            add(wv, xv);
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int c = 0; c < C; c++) v[r * C + c] = __uint_as_float((uint32_t)acc[r][c]) + __uint_as_float((uint32_t)(acc[r][c] >> 32));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = 0.0f;
+#pragma unroll 4
+        for (int k = k0 + lane; k < k1; k += 32) {
+            float p[C];
+#pragma unroll
+            for (int c = 0; c < C; c++) p[c] = Elem<T>::to_float(w[c][k]);
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const float q = Elem<T>::to_float(x[r][k]);
+#pragma unroll
+                for (int c = 0; c < C; c++) v[r * C + c] = fmaf(p[c], q, v[r * C + c]);
+            }
+        }
+    }
+    // Halves of the lanes exchange halves of the sums, until each sum is in 32 >> LOG neighbouring lanes, then those lanes join theirs.
+#pragma unroll
+    for (int s = 0; s < 5; s++) {
+        const int d = 16 >> s;
+        if (s < LOG) {
+            const int h = N >> (s + 1);
+            const bool upper = lane & d;
+#pragma unroll
+            for (int i = 0; i < h; i++) {
+                const float give = upper ? v[i] : v[i + h], keep = upper ? v[i + h] : v[i];
+                v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, d);
+            }
+        } else {
+            v[0] += __shfl_xor_sync(0xFFFFFFFFu, v[0], d);
+        }
+    }
+    const int at = lane >> (5 - LOG);   // the sum that the lane holds
+    const bool owner = (lane & ((32 >> LOG) - 1)) == 0;
+    float z = v[0];
+    if (a.slices > 1) {
+        if (owner) part[warp][at] = z;
+        __syncthreads();
+        if (slice) return;
+        for (int s = 1; s < a.slices; s++) z += part[warp + s][at];
+    }
+    const int row = at / C;
+    const long long col = col0 + at % C;
+    if (!owner || row >= a.rows || col >= a.cols) return;
+    if (a.e.bias) z += Elem<T>::to_float(reinterpret_cast<const T*>(a.e.bias)[col]);
+    if (a.e.preact) reinterpret_cast<T*>(a.e.preact)[row * a.e.ldp + col] = Elem<T>::from_float(z);
+    act_values<1>(&z, a.e.act);
+    if (a.e.residual) z += Elem<T>::to_float(reinterpret_cast<const T*>(a.e.residual)[row % a.e.residual_rows * a.e.ldr + col]);
+    reinterpret_cast<T*>(a.e.out)[row * a.e.ldo + col] = Elem<T>::from_float(z);
+}
+
+// Rows on 16-byte boundaries: one or two rows read W at up to 5 TB/s whatever its size (1 x 4096 -> 4096: 9.6 us, tensor cores and
+// their joining launch 13.9; 8192 -> 8192: 28 against 31); three and four are as long as the tensor cores at 2^24 elements (12.0
+// against 13.9 us) and slower beyond (39 against 31). Other rows would have to be packed first: 4 x 8191 -> 8192 takes 73 us against
+// 121. A long contracted axis needs more slices than a block's eight (1 x 100000 -> 1024: 65 against 41 us).
+static bool few_vec(const rb200_linear_params& p) {
+    return map_ready(operand(p.x, p.ldx, p.rows, p.in_features, false)) && map_ready(operand(p.weight, p.ldw, p.out_features, p.in_features, false));
+}
+static bool few_rows(const rb200_linear_params& p) {
+    return p.rows <= kFewRows && p.in_features <= 16384 && (p.rows <= 2 || p.in_features * p.out_features <= (1 << 24) || !few_vec(p));
+}
+template <typename T>
+static int few_launch(FewArgs& a, bool vec, int sms, cudaStream_t stream, const char* what) {
+    const int columns = a.rows == 1 ? 1 : 2;
+    const long long warps = (a.cols + columns - 1) / columns;
+    a.slices = 1;
+    while (a.slices < 8 && warps * a.slices < 8ll * sms && a.k > 256 * a.slices) a.slices *= 2;
+    a.per_slice = (int)round_up((a.k + a.slices - 1) / a.slices, 256);
+    const dim3 grid((unsigned)((warps * a.slices + 7) / 8));
+    void (*kernel)(FewArgs) = a.rows == 1   ? (vec ? few_rows_kernel<T, 1, 1, true> : few_rows_kernel<T, 1, 1, false>)
+                              : a.rows == 2 ? (vec ? few_rows_kernel<T, 2, 2, true> : few_rows_kernel<T, 2, 2, false>)
+                                            : (vec ? few_rows_kernel<T, 4, 2, true> : few_rows_kernel<T, 4, 2, false>);
+    const int rc = check_cuda(launch_overlapped(kernel, grid, dim3(256), 0, stream, a), what);
+    if (rc) return rc;
+    count_launch();
+    return RB200_OK;
+}
+
 // ---- forward ------------------------------------------------------------------------------------------------
 struct LinearPlan {
+    bool few;
     Packed x, w;
     GemmPlan gemm;
     void* partials;
@@ -237,6 +418,9 @@ struct LinearPlan {
 static LinearPlan plan_linear(const rb200_linear_params& p, const DeviceInfo& dev, void* ws) {
     LinearPlan l;
     Carver c(ws);
+    l.few = few_rows(p);
+    l.bytes = 0;
+    if (l.few) return l;
     l.x = plan_pack(operand(p.x, p.ldx, p.rows, p.in_features, false), &c);
     l.w = plan_pack(operand(p.weight, p.ldw, p.out_features, p.in_features, false), &c);
     l.gemm = gemm_plan(dev, (int)p.rows, (int)p.out_features, (int)p.in_features, false, true);
@@ -272,7 +456,6 @@ static int linear_run(const rb200_linear_params* p, void* stream_v, GemmWait wai
     if ((rc = check_workspace(what, p->workspace, p->workspace_bytes, l.bytes))) return rc;
     cudaStream_t stream = (cudaStream_t)stream_v;
     const bool bf16 = p->dtype == RB200_BF16;
-    if ((rc = pack_operands(&l.x, &l.w, stream, what))) return rc;
     EpiArgs e = {};
     e.out = p->out;
     e.ldo = p->ldo;
@@ -283,6 +466,12 @@ static int linear_run(const rb200_linear_params* p, void* stream_v, GemmWait wai
     e.preact = p->preact;
     e.ldp = p->ldp;
     e.act = p->activation;
+    if (l.few) {
+        FewArgs a = {p->x, p->weight, p->ldx, p->ldw, (int)p->rows, (int)p->out_features, (int)p->in_features, 1, 0, e};
+        const bool vec = few_vec(*p);
+        return bf16 ? few_launch<__nv_bfloat16>(a, vec, dev.sms, stream, what) : few_launch<__half>(a, vec, dev.sms, stream, what);
+    }
+    if ((rc = pack_operands(&l.x, &l.w, stream, what))) return rc;
     wait.status = p->status;
     if (l.gemm.splits > 1) {
         EpiArgs part = {};
