@@ -6,11 +6,12 @@
 //             gradient that sums over pieces is accumulated in 32 bits.
 // Pieces hold (softmax - target) * c_i * 2^15 with |c_i| <= 1, so that a probability of 2^-29 is still a normal fp16;
 // the common factor (2^-15, the loss gradient, 1 / count) is applied to the 32-bit sums.
-#include "matrix_args.cuh"
+// Few classes and features take one sweep over x each way instead (narrow_loss.cuh).
+#include "narrow_loss.cuh"
 
 namespace rb200 {
 
-constexpr size_t kStatBytes = 64u << 20;     // partial maxima and sums of one launch
+constexpr size_t kStatBytes = 128u << 20;    // partial maxima and sums of one launch (about)
 constexpr size_t kPieceBytes = 256u << 20;   // scores' gradients of one piece
 
 // ---- forward: joining the partial statistics ----------------------------------------------------------------
@@ -168,35 +169,72 @@ static int merge_launch(const MergeArgs& m, cudaStream_t stream, const char* wha
 
 // ---- backward: per-row factors --------------------------------------------------------------------------------
 // NONE: c_i = g_i / G and the common factor G, the power of two above the largest finite |g_i| of a counted row (so
-// the division is exact). One block: rows are few next to the products' work.
-__global__ void __launch_bounds__(1024) ce_factors_kernel(const float* __restrict__ dloss, const void* labels, int label_bytes, int classes,
-                                                          long long ignore_index, int rows, float* coef, float* factor) {
-    __shared__ float tops[32];
-    __shared__ float inv_s;
-    pdl_launch_dependents();
-    pdl_wait();
+// the division is exact). Two launches where there are many rows: the blocks' largest (ce_tops_kernel), then the factors, for which
+// every block looks at all of those. (One block for all rows took 330 us for 279424 of them.)
+__device__ __forceinline__ float largest(float top) {   // of a block of 256 threads, in all of them
+    __shared__ float tops[8];
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+    for (int i = 0; i < 8; i++) top = fmaxf(top, tops[i]);
+    return top;
+}
+__device__ __forceinline__ float counted_top(const float* dloss, const void* labels, int label_bytes, int classes, long long ignore_index, int rows) {
     float top = 0.0f;
-    for (int i = threadIdx.x; i < rows; i += 1024) {
+#pragma unroll 4
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < rows; i += gridDim.x * 256) {
         bool counted;
         load_label(labels, label_bytes, i, ignore_index, classes, &counted);
         const float g = fabsf(dloss[i]);
         if (counted && g <= 3.4028235e38f) top = fmaxf(top, g);
     }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < 32; i++) top = fmaxf(top, tops[i]);
-        // both the factor and its inverse stay normal: exponents -100 .. 100
-        int e = top > 0.0f ? ilogbf(top) + 1 : 0;
-        e = max(-100, min(100, e));
-        *factor = ldexpf(1.0f, e);
-        inv_s = ldexpf(1.0f, -e);
+    return largest(top);
+}
+__global__ void __launch_bounds__(256) ce_tops_kernel(const float* __restrict__ dloss, const void* labels, int label_bytes, int classes,
+                                                      long long ignore_index, int rows, float* tops) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const float top = counted_top(dloss, labels, label_bytes, classes, ignore_index, rows);
+    if (threadIdx.x == 0) tops[blockIdx.x] = top;
+}
+// blocks: the entries of `tops`, or 0 if this one block finds the largest itself.
+__global__ void __launch_bounds__(256) ce_factors_kernel(const float* __restrict__ dloss, const void* labels, int label_bytes, int classes,
+                                                         long long ignore_index, int rows, const float* tops, int blocks, float* coef, float* factor) {
+    pdl_launch_dependents();
+    pdl_wait();
+    float top;
+    if (blocks) {
+        top = 0.0f;
+        for (int i = threadIdx.x; i < blocks; i += 256) top = fmaxf(top, tops[i]);
+        top = largest(top);
+    } else {
+        top = counted_top(dloss, labels, label_bytes, classes, ignore_index, rows);
     }
-    __syncthreads();
-    const float inv = inv_s;
-    for (int i = threadIdx.x; i < rows; i += 1024) coef[i] = dloss[i] * inv;
+    // both the factor and its inverse stay normal: exponents -100 .. 100
+    int e = top > 0.0f ? ilogbf(top) + 1 : 0;
+    e = max(-100, min(100, e));
+    if (blockIdx.x == 0 && threadIdx.x == 0) *factor = ldexpf(1.0f, e);
+    const float inv = ldexpf(1.0f, -e);
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < rows; i += gridDim.x * 256) coef[i] = dloss[i] * inv;
+}
+constexpr int kFactorBlocks = 296;
+static int factors_launch(const rb200_linear_ce_params& p, float* tops, float* coef, float* factor, cudaStream_t stream, const char* what) {
+    const int rows = (int)p.rows, wanted = (rows + 2047) / 2048, blocks = wanted < kFactorBlocks ? wanted : kFactorBlocks;
+    int rc;
+    if (blocks > 1) {
+        if ((rc = check_cuda(launch_overlapped(ce_tops_kernel, dim3(blocks), dim3(256), 0, stream, p.dloss, p.labels, p.label_bytes, (int)p.classes,
+                                               (long long)p.ignore_index, rows, tops),
+                             what)))
+            return rc;
+        count_launch();
+    }
+    if ((rc = check_cuda(launch_overlapped(ce_factors_kernel, dim3(blocks), dim3(256), 0, stream, p.dloss, p.labels, p.label_bytes, (int)p.classes,
+                                           (long long)p.ignore_index, rows, (const float*)tops, blocks > 1 ? blocks : 0, coef, factor),
+                         what)))
+        return rc;
+    count_launch();
+    return RB200_OK;
 }
 
 // ---- argument checks --------------------------------------------------------------------------------------------
@@ -244,11 +282,26 @@ static EpiArgs label_args(const rb200_linear_ce_params& p) {
     e.smooth_off = p.label_smoothing / (float)p.classes;
     return e;
 }
+static NarrowArgs narrow_args(const rb200_linear_ce_params& p) {
+    NarrowArgs g = {};
+    g.bias = p.bias;
+    g.labels = p.labels;
+    g.label_bytes = p.label_bytes;
+    g.ignore_index = p.ignore_index;
+    g.smoothing = p.label_smoothing;
+    g.smooth_on = 1.0f - p.label_smoothing;
+    g.smooth_off = p.label_smoothing / (float)p.classes;
+    g.stats = p.stats;
+    g.status = p.status;
+    return g;
+}
 static const uint8_t* at_row(const void* p, long long ld, long long row) { return (const uint8_t*)p + row * ld * 2; }
 
 // ---- forward ------------------------------------------------------------------------------------------------------
 struct StatsPlan {
     Packed x, w;
+    bool narrow;
+    int* counts;            // narrow, with block_sums
     int piece;              // classes of one launch
     size_t part_bytes;
     float *part, *zsum;
@@ -259,14 +312,22 @@ static GemmPlan stats_gemm(const rb200_linear_ce_params& p, const DeviceInfo& de
     return gemm_plan(dev, (int)p.rows, classes, (int)p.features, false, false);
 }
 static StatsPlan plan_stats(const rb200_linear_ce_params& p, const DeviceInfo& dev, void* ws) {
-    StatsPlan s;
+    StatsPlan s = {};
     Carver c(ws);
     s.x = plan_pack(operand(p.x, p.ldx, p.rows, p.features, false), &c);
     s.w = plan_pack(operand(p.weight, p.ldw, p.classes, p.features, false), &c);
-    // a tile has 32 columns at least, and two parts
+    s.narrow = narrow_fits(p.classes, p.features);
+    if (s.narrow) {
+        const int ctas = narrow_ctas(p.rows, dev.sms);
+        s.block_sums = (double*)c.take(ctas * sizeof(double));
+        s.counts = (int*)c.take(2 * ctas * sizeof(int));
+        s.bytes = c.used;
+        return s;
+    }
+    // two parts a tile, as wide as the tiles of the whole product (those of a piece may be cut anew)
     const size_t per_part = (size_t)p.rows * 3 * sizeof(float);
-    long long parts = (long long)(kStatBytes / per_part);
-    long long piece = parts / 2 * 32 / kTileNMax * kTileNMax;
+    const long long parts = (long long)(kStatBytes / per_part);
+    long long piece = parts / 2 * stats_gemm(p, dev, (int)p.classes).bn / kTileNMax * kTileNMax;
     if (piece < kTileNMax) piece = kTileNMax;
     s.piece = (int)(piece < p.classes ? piece : p.classes);
     const long long most = 2ll * stats_gemm(p, dev, s.piece).tiles_n;
@@ -303,6 +364,20 @@ static int ce_forward(const rb200_linear_ce_params* p, cudaStream_t stream) {
     if ((rc = check_workspace(what, p->workspace, p->workspace_bytes, s.bytes))) return rc;
     const bool bf16 = p->dtype == RB200_BF16;
     if ((rc = pack_operands(&s.x, &s.w, stream, what))) return rc;
+    if (s.narrow) {
+        NarrowArgs g = narrow_args(*p);
+        g.loss = p->loss;
+        g.none = p->reduction == RB200_REDUCE_NONE;
+        g.sums = s.block_sums;
+        g.counts = s.counts;
+        if ((rc = narrow_launch(g, false, bf16, s.x.use, s.w.use, dev, stream, what))) return rc;
+        rc = check_cuda(launch_overlapped(ce_total_kernel, dim3(1), dim3(256), 0, stream, (const double*)s.block_sums, (const int*)s.counts,
+                                          narrow_ctas(p->rows, dev.sms), p->reduction, p->loss, p->info),
+                        what);
+        if (rc) return rc;
+        count_launch();
+        return RB200_OK;
+    }
     const GemmWait wait = {p->status, 0, -1};
     for (long long c0 = 0; c0 < p->classes; c0 += s.piece) {
         const int classes = (int)(p->classes - c0 < s.piece ? p->classes - c0 : s.piece);
@@ -343,12 +418,15 @@ static int ce_forward(const rb200_linear_ce_params* p, cudaStream_t stream) {
 // ---- backward -----------------------------------------------------------------------------------------------------
 struct GradPlan {
     Packed x, w;
+    bool narrow;
+    float* dw_part;             // narrow: [CTAs][classes][ldpart]
+    long long ldpart;
     Operand clean;              // x without the rows that do not count
     bool by_rows;               // pieces are cut along the rows
     int piece, pieces;
     long long ldd;              // of the piece's gradients
     void* dz;
-    float *coef, *factor;
+    float *coef, *factor, *tops;
     float* sum;                 // 32-bit sums over pieces: dx (pieces of classes) or dweight (pieces of rows)
     long long ldsum;
     void *px, *pw;              // partial products
@@ -372,6 +450,18 @@ static GradPlan plan_grad(const rb200_linear_ce_params& p, const DeviceInfo& dev
     const int k = (int)p.features;
     g.x = plan_pack(operand(p.x, p.ldx, p.rows, k, false), &c);
     g.w = plan_pack(operand(p.weight, p.ldw, p.classes, k, false), &c);
+    if (p.reduction == RB200_REDUCE_NONE) {
+        g.coef = (float*)c.take((size_t)p.rows * sizeof(float));
+        g.factor = (float*)c.take(sizeof(float));
+        g.tops = (float*)c.take(kFactorBlocks * sizeof(float));
+    }
+    g.narrow = narrow_fits(p.classes, p.features);
+    if (g.narrow) {
+        g.ldpart = round_up(k + 1, 4);
+        if (p.dweight || p.dbias) g.dw_part = (float*)c.take((size_t)narrow_ctas(p.rows, dev.sms) * p.classes * g.ldpart * sizeof(float));
+        g.bytes = c.used;
+        return g;
+    }
     g.by_rows = p.rows > p.classes;
     const long long longer = g.by_rows ? p.rows : p.classes, shorter = g.by_rows ? p.classes : p.rows;
     long long piece = (long long)(kPieceBytes / 2) / shorter / kTileNMax * kTileNMax;
@@ -384,10 +474,6 @@ static GradPlan plan_grad(const rb200_linear_ce_params& p, const DeviceInfo& dev
     g.pieces = (int)((longer + g.piece - 1) / g.piece);
     g.ldd = round_up(piece_classes(p, g, 0), 8);
     g.dz = c.take((size_t)g.ldd * piece_rows(p, g, 0) * 2);
-    if (p.reduction == RB200_REDUCE_NONE) {
-        g.coef = (float*)c.take((size_t)p.rows * sizeof(float));
-        g.factor = (float*)c.take(sizeof(float));
-    }
     if (p.dweight) {
         g.clean = operand(nullptr, round_up(k, 8), p.rows, k, true);
         g.clean.data = c.take((size_t)g.clean.ld * p.rows * 2);
@@ -411,6 +497,17 @@ static GradPlan plan_grad(const rb200_linear_ce_params& p, const DeviceInfo& dev
     return g;
 }
 
+template <typename T>
+static int narrow_join(const NarrowArgs& a, const rb200_linear_ce_params& p, const DeviceInfo& dev, cudaStream_t stream, const char* what) {
+    const dim3 grid((unsigned)((a.features + (p.dbias ? 1 : 0) + 31) / 32), (unsigned)a.classes);
+    const int rc = check_cuda(launch_overlapped(narrow_join_kernel<T>, grid, dim3(256), 0, stream, (const float*)a.dw_part,
+                                                narrow_ctas(a.rows, dev.sms), a.classes, a.features, a.ldpart, (T*)p.dweight, (long long)p.lddw,
+                                                (T*)p.dbias, a.scale),
+                              what);
+    if (rc) return rc;
+    count_launch();
+    return RB200_OK;
+}
 static int ce_backward(const rb200_linear_ce_params* p, cudaStream_t stream) {
     const char* what = "rb200k_linear_ce_backward";
     if (!p) {
@@ -442,14 +539,23 @@ static int ce_backward(const rb200_linear_ce_params* p, cudaStream_t stream) {
     const GemmWait wait = {p->status, 0, -1};
     if ((rc = pack_operands(&g.x, &g.w, stream, what))) return rc;
     const bool none = p->reduction == RB200_REDUCE_NONE;
-    if (none) {
-        if ((rc = check_cuda(launch_overlapped(ce_factors_kernel, dim3(1), dim3(1024), 0, stream, p->dloss, p->labels, p->label_bytes, (int)v,
-                                               (long long)p->ignore_index, (int)n, g.coef, g.factor),
-                             what)))
-            return rc;
-        count_launch();
-    }
+    if (none && (rc = factors_launch(*p, g.tops, g.coef, g.factor, stream, what))) return rc;
     const Scale scale(1.0f / 32768.0f, none ? g.factor : p->dloss, p->reduction == RB200_REDUCE_MEAN ? p->info : nullptr);
+    if (g.narrow) {
+        NarrowArgs a = narrow_args(*p);
+        a.coef = none ? g.coef : nullptr;
+        a.dirty = p->info + 1;
+        a.dx = p->dx;
+        a.lddx = p->lddx;
+        a.vec_dx = ((uintptr_t)p->dx & 15) == 0 && (n == 1 || (p->lddx & 7) == 0);
+        a.scale = scale;
+        a.dw_part = g.dw_part;
+        a.ldpart = g.ldpart;
+        a.want_dw = p->dweight != nullptr;
+        a.want_db = p->dbias != nullptr;
+        if ((rc = narrow_launch(a, true, bf16, g.x.use, g.w.use, dev, stream, what)) || !g.dw_part) return rc;
+        return bf16 ? narrow_join<__nv_bfloat16>(a, *p, dev, stream, what) : narrow_join<__half>(a, *p, dev, stream, what);
+    }
     for (int i = 0; i < g.pieces; i++) {
         const int rows = piece_rows(*p, g, i), classes = piece_classes(*p, g, i);
         const long long r0 = g.by_rows ? (long long)i * g.piece : 0, c0 = g.by_rows ? 0 : (long long)i * g.piece;
