@@ -6,10 +6,13 @@
 //             tensor cores read it; then dx = dz W leaves at once, and W's gradient (transposed: features x classes) stays in
 //             TMEM over all of the CTA's tiles, with the same chunks of x as its other operand. CTAs' sums are joined by
 //             narrow_join_kernel in a fixed order, with the column sums for the bias.
-// Against the general way (scores' gradients through memory, x read for each product): 279424 x 256, 81 classes, bf16: forward
-// @@F us (@@F0), backward @@B us (@@B0). Bound by memory: 143 MB in, and 143 MB out backwards.
-// Warps: 0 copies, 1 issues products, 2 allocates TMEM, 4-7 softmax (backward) or, with 8-11, softmax of every other tile (forward),
-// 8-15 dx. Rows that do not count but hold inf or NaN (the forward pass found some) are zeroed in shared memory before W's gradient.
+// Against the general way (scores' gradients through memory, x read for each product), 279424 x 256, 81 classes, bf16: forward
+// 31 us (43), backward 81 us (156). Forward it is bound by the read of x (143 MB at 5 TB/s). Backwards a tile takes 7700 clocks, most
+// of them one after another, since shared memory has no room for a third tile of x: scores 1300, softmax 2600, the other two products
+// 2900 (128 clocks for 16 elements of the contracted axis: operands that are not contiguous along it), handshakes 900. Tried and
+// slower: sixteen softmax warps (91 us), the next scores ahead of dx with the softmax holding its results until dz is read (93 us).
+// Warps: 0 copies, 1 issues products, 2 allocates TMEM, 4-11 softmax (forward: two groups take turns; backward: two warps share a
+// row), 12-19 dx. Rows that do not count but hold inf or NaN (the forward pass found some) are zeroed in shared memory before W's gradient.
 #pragma once
 
 #include "matrix_args.cuh"
@@ -17,7 +20,8 @@
 namespace rb200 {
 
 constexpr int kNarrowClasses = 128, kNarrowFeatures = 256;
-constexpr int kNarrowThreads = 512, kNarrowSlots = 8;
+constexpr int kNarrowSlots = 8;
+constexpr int narrow_threads(bool grad) { return grad ? 640 : 384; }
 constexpr uint32_t kChunkBytes = kTileM * kTileK * 2;   // 128 rows x 64 features
 constexpr uint32_t kNarrowSmem = 232448 - 2048;         // 227 KB, without the kernel's own KB and what aligning the start may take
 enum { kNarrowDw = 128, kNarrowDx = 384 };              // TMEM columns: scores at 0 (forward: and at 128)
@@ -57,7 +61,7 @@ static __host__ __device__ inline uint32_t narrow_smem(int vb, int chunks, int s
 }
 
 template <typename T, bool GRAD>
-__global__ void __launch_bounds__(kNarrowThreads, 1) ce_narrow_kernel(const __grid_constant__ NarrowArgs g) {
+__global__ void __launch_bounds__(narrow_threads(GRAD), 1) ce_narrow_kernel(const __grid_constant__ NarrowArgs g) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[2 * kNarrowSlots + 9];
     __shared__ uint32_t tmem_addr_s;
@@ -86,7 +90,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ce_narrow_kernel(const __gr
         }
         tc::bar_init(s_full(0), 1);
         tc::bar_init(s_full(1), 1);
-        tc::bar_init(s_empty(0), 4);
+        tc::bar_init(s_empty(0), GRAD ? 8 : 4);
         tc::bar_init(s_empty(1), GRAD ? 1 : 4);
         tc::bar_init(dx_full, 1);
         tc::bar_init(dx_empty, 8);
@@ -200,8 +204,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ce_narrow_kernel(const __gr
                         tc::mma_commit<1>(dx_full);
                         return true;
                     };
-                    if (want_dx) ok = gradient_of_x(0);
-                    if (!ok) break;
+                    if (want_dx && !(ok = gradient_of_x(0))) break;
                     if (want_dw) {
                         const uint64_t b = tc::operand_desc(dz0, true, kChunkBytes);
                         for (int h = 0; h < halves; h++) {
@@ -211,12 +214,11 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ce_narrow_kernel(const __gr
                                 tc::mma_f16<1>(tmem + kNarrowDw + h * 128, a + k * 128, b + k * 128, g.idesc_w, it > 0 || k > 0);
                         }
                     }
-                    if (want_dx && halves > 1) ok = gradient_of_x(1);
-                    if (!ok) break;
                     for (int c = 0; c < g.chunks; c++) tc::mma_commit<1>(empty(first + c));
-                    tc::mma_commit<1>(dz_empty);
                     first = first + g.chunks == g.slots ? 0 : first + g.chunks;
-                    if (t + (int)gridDim.x < tiles) ok = scores(tmem, s_full(0));
+                    if (want_dx && halves > 1 && !(ok = gradient_of_x(1))) break;
+                    tc::mma_commit<1>(dz_empty);
+                    if (t + (int)gridDim.x < tiles) ok = scores(tmem, s_full(0));   // dz says that the scores before have been read
                 }
                 if (ok) tc::mma_commit<1>(done);
             }
@@ -226,41 +228,133 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ce_narrow_kernel(const __gr
             }
         }
         __syncwarp();
-    } else if (warp >= 4 && warp < (GRAD ? 8 : 12)) {
-        const int quarter = warp & 3, group = warp - 4 >> 2;   // forward: the group's tiles and scores
+    } else if (GRAD && warp >= 4 && warp < 12) {   // softmax - target; two warps share a row's classes
+        const int quarter = warp & 3, share = warp - 4 >> 2, half = g.vb / 2, line = quarter * 32 + lane;
+        const uint32_t acc = tmem + share * half + ((uint32_t)(quarter * 32) << 16);
+        constexpr int kStrips = kNarrowClasses / 32;   // of 16 classes
+        float cols[kStrips] = {};   // column sums, in both halves of the lanes
+        const bool dirty = *g.dirty, zero_rows = want_dw && dirty;
+        int it = 0, first = 0;
+        // what does not depend on the products is on its way a tile ahead
+        struct {
+            int label;
+            bool counted;
+            float m, s, zl, coef;
+        } next;
+        auto fetch = [&](int t) {
+            const int row = t * kTileM + line;
+            next.label = -1;
+            next.counted = false;
+            next.m = next.zl = 0.0f;
+            next.s = next.coef = 1.0f;
+            if (t < tiles && row < g.rows) {
+                next.label = load_label(g.labels, g.label_bytes, row, g.ignore_index, g.classes, &next.counted);
+                next.m = g.stats[row];
+                next.s = g.stats[(long long)g.rows + row];
+                next.zl = g.stats[2ll * g.rows + row];
+                if (g.coef) next.coef = g.coef[row];
+            }
+        };
+        fetch(blockIdx.x);
+        for (int t = blockIdx.x; t < tiles; t += gridDim.x, it++) {
+            const bool counted = next.counted;
+            const int label = counted ? next.label : -1;
+            // (softmax - target) * factor = exp(z - top) * mul + add, and at the label
+            // rows that do not count: exp(z - inf) * 0 + 0
+            const float factor = counted ? next.coef * 32768.0f : 0.0f, top = counted ? finite_max(next.m) : INFINITY;
+            const float mul = counted ? factor / next.s : 0.0f, add = -g.smooth_off * factor;
+            const float at_label = exp_diff(next.zl - top) * mul + add - g.smooth_on * factor;
+            fetch(t + gridDim.x);
+            // the lanes leave together: what follows needs whole warps
+            if (!__all_sync(0xFFFFFFFFu, tc::bar_wait(s_full(0), it & 1, patience) && tc::bar_wait(dz_empty, (it & 1) ^ 1, patience))) break;
+            tc::fence_after();
+            const float2 off = make_float2(-top, -top), unit = make_float2(kLog2e, kLog2e);
+            const float2 mul_v = make_float2(mul, mul), add_v = make_float2(add, add);
+#pragma unroll
+            for (int c = 0; c < kStrips; c++) {
+                if (c * 16 >= half) break;
+                const int col = share * half + c * 16, count = counted || !dirty ? g.classes - col : 0, l = label - col;
+                uint32_t raw[16];
+                tc::tmem_load16(acc + c * 16, raw);
+                tc::tmem_wait();
+                float v[16];
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const float4 b = *reinterpret_cast<const float4*>(bias_s + col + i);
+                    const float2 z[2] = {add2(make_float2(__uint_as_float(raw[i]), __uint_as_float(raw[i + 1])), make_float2(b.x, b.y)),
+                                         add2(make_float2(__uint_as_float(raw[i + 2]), __uint_as_float(raw[i + 3])), make_float2(b.z, b.w))};
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const float2 d = mul2(add2(z[j], off), unit);
+                        const float2 p = fma2(make_float2(exp2_fast(d.x), exp2_fast(d.y)), mul_v, add_v);
+                        v[i + 2 * j] = p.x;
+                        v[i + 2 * j + 1] = p.y;
+                    }
+                }
+                if (l >= 0 && l < 16) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) v[i] = i == l ? at_label : v[i];
+                }
+                if (count < 16) {   // beyond the classes; rows that do not count and may hold anything
+#pragma unroll
+                    for (int i = 0; i < 16; i++) v[i] = i < count ? v[i] : 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < 2; i++) {   // piece j of line r lies at j ^ (r % 8): the 128-byte swizzle
+                    const int piece = col / 8 + i;
+                    st_shared16(dz0 + (piece >> 3) * kChunkBytes + line * 128 + (((piece & 7) ^ (line & 7)) << 4), pack8<T>(v + 8 * i));
+                }
+                if (g.want_db) {
+                    // Column sums over the warp's rows: at every step a lane keeps the half of its columns that its own
+                    // number's next bit names and hands the other half to its partner. Lanes l and l + 16 end with column l.
+#pragma unroll
+                    for (int w = 8; w; w >>= 1) {
+                        const bool upper = lane & w;
+#pragma unroll
+                        for (int i = 0; i < w; i++) {
+                            const float keep = upper ? v[i + w] : v[i], send = upper ? v[i] : v[i + w];
+                            v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, send, w);
+                        }
+                    }
+                    cols[c] += v[0];
+                }
+            }
+            tc::fence_before();
+            if (zero_rows && !counted && share == 0) {
+                for (int c = 0; c < g.chunks; c++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) st_shared16(x0 + (first + c) * kChunkBytes + line * 128 + i * 16, make_uint4(0, 0, 0, 0));
+            }
+            first = first + g.chunks == g.slots ? 0 : first + g.chunks;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the tensor cores read what was written
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(dz_full) : "memory");
+        }
+        if (g.want_db && __all_sync(0xFFFFFFFFu, tc::bar_wait(done, 0, patience))) {   // nothing reads dz any more: [4][128] column sums
+#pragma unroll
+            for (int c = 0; c < kStrips; c++) {
+                const float s = cols[c] + __shfl_xor_sync(0xFFFFFFFFu, cols[c], 16);
+                if (c * 16 < half && lane < 16)
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(dz0 + (quarter * kNarrowClasses + share * half + c * 16 + lane) * 4), "f"(s) : "memory");
+            }
+        }
+    } else if (!GRAD && warp >= 4 && warp < 12) {   // a group of four takes every other tile
+        const int quarter = warp & 3, group = warp - 4 >> 2;
         const uint32_t acc = tmem + group * 128 + ((uint32_t)(quarter * 32) << 16);
         double mine = 0.0;
-        int counts = 0, dirts = 0;
-        float cols[kNarrowClasses / 32] = {};   // backward: column sums, lane l of strip c: column 32 c + l
-        const bool zero_rows = want_dw && *g.dirty;
-        int it = 0, first = 0;
+        int counts = 0, dirts = 0, it = 0;
         for (int t = blockIdx.x; t < tiles; t += gridDim.x, it++) {
-            if (!GRAD && (it & 1) != group) continue;
+            if ((it & 1) != group) continue;
             const int row = t * kTileM + quarter * 32 + lane;
             const bool row_ok = row < g.rows;
             bool counted = false;
             int label = -1;
-            float top = 0.0f, mul = 0.0f, add = 0.0f, at_label = 0.0f;
             if (row_ok) label = load_label(g.labels, g.label_bytes, row, g.ignore_index, g.classes, &counted);
-            if constexpr (GRAD) {
-                if (counted) {   // (softmax - target) * factor = exp(z - top) * mul + add, and at the label
-                    const float zl = g.stats[2ll * g.rows + row], factor = (g.coef ? g.coef[row] : 1.0f) * 32768.0f;
-                    top = finite_max(g.stats[row]);
-                    mul = factor / g.stats[(long long)g.rows + row];
-                    add = -g.smooth_off * factor;
-                    at_label = exp_diff(zl - top) * mul + add - g.smooth_on * factor;
-                } else {
-                    label = -1;
-                }
-                // the lanes leave together: what follows needs whole warps
-                if (!__all_sync(0xFFFFFFFFu, tc::bar_wait(s_full(0), it & 1, patience) && tc::bar_wait(dz_empty, (it & 1) ^ 1, patience))) break;
-            } else {
-                if (!__all_sync(0xFFFFFFFFu, tc::bar_wait(s_full(group), it >> 1 & 1, patience))) break;
-            }
+            // the lanes leave together: what follows needs whole warps
+            if (!__all_sync(0xFFFFFFFFu, tc::bar_wait(s_full(group), it >> 1 & 1, patience))) break;
             tc::fence_after();
             RunningSoftmax run = {-INFINITY, 0.0f};
             float z_label = 0.0f, zsum = 0.0f;
-            const int line = quarter * 32 + lane;
 #pragma unroll
             for (int c = 0; c < kNarrowClasses / 32; c++) {
                 const int count = g.classes - c * 32;
@@ -278,136 +372,79 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ce_narrow_kernel(const __gr
                     v[i + 3] = __uint_as_float(raw[i + 3]) + b.w;
                 }
                 const int l = label - c * 32;
-                if constexpr (!GRAD) {
-                    if (l >= 0 && l < 32) {   // element l of the strip, by its bits
-                        float a[16];
+                if (l >= 0 && l < 32) {   // element l of the strip, by its bits
+                    float a[16];
 #pragma unroll
-                        for (int i = 0; i < 16; i++) a[i] = l & 16 ? v[i + 16] : v[i];
+                    for (int i = 0; i < 16; i++) a[i] = l & 16 ? v[i + 16] : v[i];
 #pragma unroll
-                        for (int w = 8; w; w >>= 1)
+                    for (int w = 8; w; w >>= 1)
 #pragma unroll
-                            for (int i = 0; i < w; i++) a[i] = l & w ? a[i + w] : a[i];
-                        z_label = a[0];
-                    }
-                    if (g.smoothing > 0.0f) {
-#pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            if (i < count) zsum += v[i];
-                    }
-                    if (count < 32) {
-#pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            if (i >= count) v[i] = -INFINITY;
-                    }
-                    float m[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-                    for (int i = 4; i < 32; i += 4)
-#pragma unroll
-                        for (int j = 0; j < 4; j++) m[j] = fmaxf(m[j], v[i + j]);
-                    const float now = fmaxf(run.m, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))), base = finite_max(now);
-                    run.s *= exp_diff(run.m - base);
-                    run.m = now;
-                    float2 sum[2] = {};
-                    const float2 off = make_float2(-base, -base), unit = make_float2(kLog2e, kLog2e);
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float2 d = mul2(add2(make_float2(v[i], v[i + 1]), off), unit);
-                        sum[i >> 1 & 1] = add2(sum[i >> 1 & 1], make_float2(exp2_fast(d.x), exp2_fast(d.y)));
-                    }
-                    run.s += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-                } else {
-                    const float2 off = make_float2(-top, -top), unit = make_float2(kLog2e, kLog2e);
-                    const float2 mul_v = make_float2(mul, mul), add_v = make_float2(add, add);
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float2 d = mul2(add2(make_float2(v[i], v[i + 1]), off), unit);
-                        const float2 p = fma2(make_float2(exp2_fast(d.x), exp2_fast(d.y)), mul_v, add_v);
-                        v[i] = p.x;
-                        v[i + 1] = p.y;
-                    }
-                    if (l >= 0 && l < 32) {
-#pragma unroll
-                        for (int i = 0; i < 32; i++) v[i] = i == l ? at_label : v[i];
-                    }
-#pragma unroll
-                    for (int i = 0; i < 32; i++) v[i] = counted && i < count ? v[i] : 0.0f;   // whatever the row held; beyond the classes
-#pragma unroll
-                    for (int i = 0; i < 4; i++)   // piece j of line r lies at j ^ (r % 8): the 128-byte swizzle
-                        st_shared16(dz0 + (c >> 1) * kChunkBytes + line * 128 + ((((c & 1) * 4 + i) ^ (line & 7)) << 4), pack8<T>(v + 8 * i));
-                    if (g.want_db) {
-                        // Column sums over the warp's rows: at every step a lane keeps the half of its columns that its own
-                        // number's next bit names and hands the other half to its partner. Lane l ends with column l.
-#pragma unroll
-                        for (int w = 16; w; w >>= 1) {
-                            const bool upper = lane & w;
-#pragma unroll
-                            for (int i = 0; i < w; i++) {
-                                const float keep = upper ? v[i + w] : v[i], send = upper ? v[i] : v[i + w];
-                                v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, send, w);
-                            }
-                        }
-                        cols[c] += v[0];
-                    }
+                        for (int i = 0; i < w; i++) a[i] = l & w ? a[i + w] : a[i];
+                    z_label = a[0];
                 }
+                if (g.smoothing > 0.0f) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if (i < count) zsum += v[i];
+                }
+                if (count < 32) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if (i >= count) v[i] = -INFINITY;
+                }
+                float m[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+                for (int i = 4; i < 32; i += 4)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) m[j] = fmaxf(m[j], v[i + j]);
+                const float now = fmaxf(run.m, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))), base = finite_max(now);
+                run.s *= exp_diff(run.m - base);
+                run.m = now;
+                float2 sum[2] = {};
+                const float2 off = make_float2(-base, -base), unit = make_float2(kLog2e, kLog2e);
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 d = mul2(add2(make_float2(v[i], v[i + 1]), off), unit);
+                    sum[i >> 1 & 1] = add2(sum[i >> 1 & 1], make_float2(exp2_fast(d.x), exp2_fast(d.y)));
+                }
+                run.s += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             }
             tc::fence_before();
-            if constexpr (GRAD) {
-                if (zero_rows && !counted) {
-                    for (int c = 0; c < g.chunks; c++)
-#pragma unroll
-                        for (int i = 0; i < 8; i++)
-                            st_shared16(x0 + (first + c) * kChunkBytes + line * 128 + i * 16, make_uint4(0, 0, 0, 0));
-                }
-                first = first + g.chunks == g.slots ? 0 : first + g.chunks;
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the tensor cores read what was written
-                __syncwarp();
-                if (lane == 0) asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(dz_full) : "memory");
-            } else {
-                __syncwarp();
-                if (lane == 0) tc::bar_arrive_relaxed(s_empty(group));
-                if (row_ok) {
-                    float loss = 0.0f;
-                    if (counted) {
-                        counts++;
-                        if (label < 0) {
-                            run.m = run.s = loss = nanf("");
-                        } else {
-                            const float lse = logf(run.s);   // above the maximum
-                            loss = g.smooth_on * (lse + (run.m - z_label));
-                            if (g.smoothing > 0.0f) loss += g.smoothing * (lse + (run.m - zsum / (float)g.classes));
-                        }
+            __syncwarp();
+            if (lane == 0) tc::bar_arrive_relaxed(s_empty(group));
+            if (row_ok) {
+                float loss = 0.0f;
+                if (counted) {
+                    counts++;
+                    if (label < 0) {
+                        run.m = run.s = loss = nanf("");
                     } else {
-                        dirts |= !(isfinite(run.m) && isfinite(run.s));
+                        const float lse = logf(run.s);   // above the maximum
+                        loss = g.smooth_on * (lse + (run.m - z_label));
+                        if (g.smoothing > 0.0f) loss += g.smoothing * (lse + (run.m - zsum / (float)g.classes));
                     }
-                    mine += loss;
-                    if (g.none) g.loss[row] = loss;
-                    g.stats[row] = run.m;
-                    g.stats[(long long)g.rows + row] = run.s;
-                    g.stats[2ll * g.rows + row] = z_label;
+                } else {
+                    dirts |= !(isfinite(run.m) && isfinite(run.s));
                 }
+                mine += loss;
+                if (g.none) g.loss[row] = loss;
+                g.stats[row] = run.m;
+                g.stats[(long long)g.rows + row] = run.s;
+                g.stats[2ll * g.rows + row] = z_label;
             }
         }
-        if constexpr (GRAD) {
-            if (g.want_db && __all_sync(0xFFFFFFFFu, tc::bar_wait(done, 0, patience))) {   // nothing reads dz any more: [4][128] column sums
 #pragma unroll
-                for (int c = 0; c < kNarrowClasses / 32; c++)
-                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(dz0 + (quarter * kNarrowClasses + c * 32 + lane) * 4), "f"(cols[c]) : "memory");
-            }
-        } else {
-#pragma unroll
-            for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, d);
-            counts = __reduce_add_sync(0xFFFFFFFFu, counts);
-            dirts = __any_sync(0xFFFFFFFFu, dirts);
-            if (lane == 0) {
-                sums_s[warp - 4] = mine;
-                counts_s[0][warp - 4] = counts;
-                counts_s[1][warp - 4] = dirts;
-            }
+        for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, d);
+        counts = __reduce_add_sync(0xFFFFFFFFu, counts);
+        dirts = __any_sync(0xFFFFFFFFu, dirts);
+        if (lane == 0) {
+            sums_s[warp - 4] = mine;
+            counts_s[0][warp - 4] = counts;
+            counts_s[1][warp - 4] = dirts;
         }
-    } else if (GRAD && warp >= 8) {
-        const int quarter = warp & 3, share = warp - 8 >> 2;
-        const uint32_t area = stage0 + (warp - 8) * kStageBytes;
-        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    } else if (GRAD && warp >= 12) {
+        const int quarter = warp & 3, share = warp - 12 >> 2;   // 64 columns of a piece
+        const uint32_t area = stage0 + (warp - 12) * kStageBytes, lanes = (uint32_t)(quarter * 32) << 16;
         const float scale = g.scale.value();
         int pieces = 0;
         bool ok = true;
@@ -417,42 +454,44 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) ce_narrow_kernel(const __gr
                 ok = __all_sync(0xFFFFFFFFu, tc::bar_wait(dx_full, pieces & 1, patience));
                 if (!ok) break;
                 tc::fence_after();
-                uint32_t raw[2][32];
-                tc::tmem_load32(tmem + kNarrowDx + share * 64 + lanes, raw[0]);
-                tc::tmem_load32(tmem + kNarrowDx + share * 64 + 32 + lanes, raw[1]);
-                tc::tmem_wait();
-                tc::fence_before();
+                uint4 out[8];
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    uint32_t raw[16];
+                    tc::tmem_load16(tmem + kNarrowDx + share * 64 + q * 16 + lanes, raw);
+                    tc::tmem_wait();
+                    float v[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) v[i] = __uint_as_float(raw[i]) * scale;
+                    out[2 * q] = pack8<T>(v);
+                    out[2 * q + 1] = pack8<T>(v + 8);
+                }
+                tc::fence_before();   // the accumulator is in registers
                 __syncwarp();
                 if (lane == 0) tc::bar_arrive_relaxed(dx_empty);
 #pragma unroll
                 for (int s = 0; s < 2; s++) {
                     const int col = h * 128 + share * 64 + s * 32, count = g.features - col;
                     if (count <= 0 || row0 >= g.rows) continue;
-                    float v[32];
-#pragma unroll
-                    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(raw[s][i]) * scale;
                     __syncwarp();   // the staging area is free: the strip before has been read
 #pragma unroll
-                    for (int i = 0; i < 4; i++) st_shared16(staged(area, lane, i), pack8<T>(v + 8 * i));
+                    for (int i = 0; i < 4; i++) st_shared16(staged(area, lane, i), out[4 * s + i]);
                     __syncwarp();
                     copy_strip(area, reinterpret_cast<T*>(g.dx), g.lddx, g.vec_dx, col, min(32, count), row0, g.rows - row0, lane);
                 }
             }
         }
-        if (want_dw && ok && share < halves) {   // the CTA's sums: lanes are features, columns classes
-            ok = __all_sync(0xFFFFFFFFu, tc::bar_wait(done, 0, patience));
-            if (ok) {
-                tc::fence_after();
-                const int feature = share * 128 + quarter * 32 + lane;
-                for (int c = 0; c < g.classes; c += 32) {
-                    uint32_t raw[32];
-                    tc::tmem_load32(tmem + kNarrowDw + share * 128 + c + lanes, raw);
-                    tc::tmem_wait();
-                    float* out = g.dw_part + ((long long)blockIdx.x * g.classes + c) * g.ldpart + feature;
+        if (want_dw && ok && __all_sync(0xFFFFFFFFu, tc::bar_wait(done, 0, patience))) {   // the CTA's sums: lanes are features, columns classes
+            tc::fence_after();
+            const int feature = share * 128 + quarter * 32 + lane;
+            for (int c = 0; c < g.classes && share < halves; c += 16) {
+                uint32_t raw[16];
+                tc::tmem_load16(tmem + kNarrowDw + share * 128 + c + lanes, raw);
+                tc::tmem_wait();
+                float* out = g.dw_part + ((long long)blockIdx.x * g.classes + c) * g.ldpart + feature;
 #pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (c + i < g.classes && feature < g.features) out[i * g.ldpart] = __uint_as_float(raw[i]);
-                }
+                for (int i = 0; i < 16; i++)
+                    if (c + i < g.classes && feature < g.features) out[i * g.ldpart] = __uint_as_float(raw[i]);
             }
         }
         __syncwarp();
@@ -566,7 +605,7 @@ static int narrow_launch_as(const NarrowArgs& g, const DeviceInfo& dev, cudaStre
         if (rc) return rc;
         __atomic_fetch_or(&ready, 1ull << dev.index, __ATOMIC_RELAXED);
     }
-    rc = check_cuda(launch_overlapped(kernel, dim3(narrow_ctas(g.rows, dev.sms)), dim3(kNarrowThreads),
+    rc = check_cuda(launch_overlapped(kernel, dim3(narrow_ctas(g.rows, dev.sms)), dim3(narrow_threads(GRAD)),
                                       narrow_smem(g.vb, g.chunks, g.slots, GRAD) + 1024, stream, g),
                     what);
     if (rc) return rc;
