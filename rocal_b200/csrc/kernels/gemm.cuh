@@ -545,6 +545,21 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     res_row[i] = r < g.m ? r % g.e.residual_rows : -1;
                 }
             }
+            // A strip of the residual: lane l takes piece l % 4 of the rows l / 4 + 8 i. The tile's first one is on its way
+            // before the products are done, the others from the strip before (50176 x 768 -> 1024 with a residual of as many rows: 116 -> 104 us).
+            uint4 res[4];
+            auto fetch_residual = [&](int c) {
+                if constexpr (EPI == EPI_LINEAR_ADD) {
+                    const int col = n0 + c, left = n1 - col - (lane & 3) * 8;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        res[i] = make_uint4(0, 0, 0, 0);
+                        if (res_row[i] >= 0 && left > 0)
+                            res[i] = load8(reinterpret_cast<const T*>(g.e.residual) + res_row[i] * g.e.ldr + col + (lane & 3) * 8, left, g.e.vec_res);
+                    }
+                }
+            };
+            fetch_residual(share * 32);
 
             // the lanes leave together: what follows needs whole warps
             if (!__all_sync(0xFFFFFFFFu, tc::bar_wait(acc_full(group), acc_phase, patience))) break;
@@ -583,19 +598,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                         tc::tmem_wait();
 #pragma unroll
                         for (int j = 0; j < 8; j++) v[i + j] += __uint_as_float(more[j]);
-                    }
-                }
-                uint4 res[4];   // the residual's strip: lane l takes piece l % 4 of the rows l / 4 + 8 i
-                if constexpr (EPI == EPI_LINEAR_ADD) {
-                    {
-                        const int left = count - (lane & 3) * 8;
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            res[i] = make_uint4(0, 0, 0, 0);
-                            if (res_row[i] >= 0 && left > 0)
-                                res[i] = load8(reinterpret_cast<const T*>(g.e.residual) + res_row[i] * g.e.ldr + col + (lane & 3) * 8, left,
-                                               g.e.vec_res);
-                        }
                     }
                 }
                 if (c + 64 >= g.bn) release();
@@ -637,6 +639,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     if constexpr (EPI == EPI_LINEAR_ADD) {   // the other way round: whole pieces of rows in, a row a thread out
 #pragma unroll
                         for (int i = 0; i < 4; i++) st_shared16(staged(area, (lane >> 2) + 8 * i, lane & 3), res[i]);
+                        if (c + 64 < g.bn) fetch_residual(c + 64);
                         __syncwarp();
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
