@@ -697,10 +697,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                             for (int i = 0; i < w; i++) a[i] = l & w ? a[i + w] : a[i];
                         if (label < g.n) g.e.zlabel[row] = a[0];
                     }
-                    if (g.e.want_zsum) {
+                    if (g.e.want_zsum) {   // four sums, not one chain of 32
+                        float2 sum[2] = {};
+                        if (count >= 32) {
 #pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            if (i < count) zsum += v[i];
+                            for (int i = 0; i < 32; i += 2) sum[i >> 1 & 1] = add2(sum[i >> 1 & 1], make_float2(v[i], v[i + 1]));
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2)
+                                sum[i >> 1 & 1] = add2(sum[i >> 1 & 1], make_float2(i < count ? v[i] : 0.0f, i + 1 < count ? v[i + 1] : 0.0f));
+                        }
+                        zsum += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                     }
                     if (count < 32) {
 #pragma unroll
