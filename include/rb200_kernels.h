@@ -385,7 +385,7 @@ RB200_API int rb200k_transpose(const uint8_t* arena, const rb200_pointwise_sampl
  *
  * Matrices are row-major: element (i, j) at data[i * ld + j], ld in elements. All pointers are device pointers. Rows
  * that start on 16-byte boundaries (base address and ld * element size multiples of 16) are read in place; any other
- * operand of a matrix product is first copied into the workspace. Workspaces hold nothing of value between calls and
+ * operand of a matrix product is first copied into the workspace (not for up to four rows of rb200k_linear). Workspaces hold nothing of value between calls and
  * need no initialisation; two calls that can run at the same time need two workspaces. Results do not depend on
  * timing: no floating-point atomics are used. Every wait inside these kernels is bounded (see "Bounded waits"); trouble
  * goes to `status` or, where that is NULL, to the library-wide status word. Outputs overlap neither inputs nor one
@@ -424,7 +424,7 @@ typedef struct rb200_linear_params {
 RB200_API uint64_t rb200k_linear_workspace_bytes(const rb200_linear_params* params);
 RB200_API int rb200k_linear(const rb200_linear_params* params, void* stream);
 /* Self-test of the bounded waits, as rb200k_resample_probe: the copies of the contracted axis' blocks (64 elements)
- * from skip_block on are left out, and waits give up after wait_cycles. */
+ * from skip_block on are left out, and waits give up after wait_cycles. (Products of up to four rows may have no waits.) */
 RB200_API int rb200k_linear_probe(const rb200_linear_params* params, void* stream, uint64_t wait_cycles, int skip_block);
 
 /* The gradients, each of them only where its pointer is given: with dz = dout * act'(preact),

@@ -178,12 +178,29 @@ __device__ __forceinline__ float gelu(float z) {
     const float a = fminf(fabsf(z), 6.0f), e = exp2_fast(z * (z * -0.72134752f));
     return (z < 0.0f ? 0.0f : z) - a * e * tail_ratio(a);
 }
-// Phi(z) + z phi(z). |z| is held at 40, where the exponential is 0, so that infinities give 0 and 1.
-__device__ __forceinline__ float gelu_slope(float z) {
-    const float a = fminf(fabsf(z), 40.0f), e = exp2_fast(a * (a * -0.72134752f));
+// Phi(z) + z phi(z), two at a time (fma.f32x2: the sweep over a gradient that this is for is bound by issue as much as by memory;
+// 8192 x 4096 with gelu 47 -> 39 us). |z| is held at 40, where the exponential is 0, so that infinities give 0 and 1; NaN passes.
+__device__ __forceinline__ float2 gelu_slopes(float2 z) {
+    float2 a, t;
+    asm("min.NaN.f32 %0, %1, 0f42200000;" : "=f"(a.x) : "f"(fabsf(z.x)));
+    asm("min.NaN.f32 %0, %1, 0f42200000;" : "=f"(a.y) : "f"(fabsf(z.y)));
+    const float2 x = mul2(a, mul2(a, make_float2(-0.72134752f, -0.72134752f))), e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+    const float2 b = fma2(make_float2(fminf(a.x, 6.0f), fminf(a.y, 6.0f)), make_float2(0.294f, 0.294f), make_float2(1.0f, 1.0f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t.x) : "f"(b.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t.y) : "f"(b.y));
+    auto both = [](float c) { return make_float2(c, c); };
+    float2 r = fma2(t, both(0.0888040438f), both(-0.272132337f));   // -R: tail_ratio's polynomial
+    r = fma2(r, t, both(0.0816512033f));
+    r = fma2(r, t, both(-0.177665651f));
+    r = fma2(r, t, both(-0.102016911f));
+    r = fma2(r, t, both(-0.118640058f));
     // |z| phi - Q, which the sign of z turns into the distance from 1 or from 0
-    const float d = e * fmaf(a, 0.39894228f, -tail_ratio(a));
-    return z < 0.0f ? -d : z >= 0.0f ? 1.0f + d : z;
+    const float2 d = mul2(e, fma2(a, both(0.39894228f), mul2(r, t)));
+    auto turn = [](float v, float dist) {
+        const uint32_t sign = __float_as_uint(v) & 0x80000000u;
+        return (sign ? 0.0f : 1.0f) + __uint_as_float(__float_as_uint(dist) ^ sign);
+    };
+    return make_float2(turn(z.x, d.x), turn(z.y, d.y));
 }
 __device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + exp2_fast(z * -1.4426950408889634f)); }
 
@@ -208,7 +225,11 @@ __device__ __forceinline__ void act_slopes(float* v, int act) {   // z -> slope
         for (int i = 0; i < N; i++) v[i] = v[i] > 0.0f ? 1.0f : v[i] <= 0.0f ? 0.0f : v[i];   // NaN stays
     } else if (act == ACT_GELU) {
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = gelu_slope(v[i]);
+        for (int i = 0; i < N; i += 2) {
+            const float2 s = gelu_slopes(make_float2(v[i], v[i + 1]));
+            v[i] = s.x;
+            v[i + 1] = s.y;
+        }
     } else if (act == ACT_SILU) {
 #pragma unroll
         for (int i = 0; i < N; i++) {

@@ -53,8 +53,7 @@ __global__ void __launch_bounds__(256, 4) rows_kernel(RowsArgs a) {
             if (SLOPE) {
                 float s[8];
                 unpack8<T>(z, s);
-                act_slopes<4>(s, a.act);
-                act_slopes<4>(s + 4, a.act);
+                act_slopes<8>(s, a.act);
 #pragma unroll
                 for (int k = 0; k < 8; k++) v[k] *= s[k];
             }
