@@ -379,9 +379,9 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const FewArgs a) {
     reinterpret_cast<T*>(a.e.out)[row * a.e.ldo + col] = Elem<T>::from_float(z);
 }
 
-// Rows on 16-byte boundaries: one or two rows read W at up to 5 TB/s whatever its size (1 x 4096 -> 4096: 9.6 us, tensor cores and
+// Rows on 16-byte boundaries: one or two rows read W at up to 4.8 TB/s whatever its size (1 x 4096 -> 4096: 9.6 us, tensor cores and
 // their joining launch 13.9; 8192 -> 8192: 28 against 31); three and four are as long as the tensor cores at 2^24 elements (12.0
-// against 13.9 us) and slower beyond (39 against 31). Other rows would have to be packed first: 4 x 8191 -> 8192 takes 73 us against
+// against 13.9 us) and slower beyond (39 against 31). Other rows would have to be packed first: 4 x 8191 -> 8192 takes 58 us against
 // 121. A long contracted axis needs more slices than a block's eight (1 x 100000 -> 1024: 65 against 41 us).
 static bool few_vec(const rb200_linear_params& p) {
     return map_ready(operand(p.x, p.ldx, p.rows, p.in_features, false)) && map_ready(operand(p.weight, p.ldw, p.out_features, p.in_features, false));
@@ -394,7 +394,10 @@ static int few_launch(FewArgs& a, bool vec, int sms, cudaStream_t stream, const 
     const int columns = a.rows == 1 ? 1 : 2;
     const long long warps = (a.cols + columns - 1) / columns;
     a.slices = 1;
-    while (a.slices < 8 && warps * a.slices < 8ll * sms && a.k > 256 * a.slices) a.slices *= 2;
+    // eight warps an SM; single elements, of which a warp has less in flight, want more of them (2 x 8191 -> 8192: 64 us, then 45; whole
+    // vectors lose by it: 1 x 4096 -> 4096 9.6 us, then 11.8)
+    while (a.slices < 8 && a.k > 256 * a.slices && (warps * a.slices < 8ll * sms || (!vec && a.k >= 2048 * a.slices && warps * a.slices < 192ll * sms)))
+        a.slices *= 2;
     a.per_slice = (int)round_up((a.k + a.slices - 1) / a.slices, 256);
     const dim3 grid((unsigned)((warps * a.slices + 7) / 8));
     void (*kernel)(FewArgs) = a.rows == 1   ? (vec ? few_rows_kernel<T, 1, 1, true> : few_rows_kernel<T, 1, 1, false>)
