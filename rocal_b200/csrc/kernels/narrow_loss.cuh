@@ -12,7 +12,7 @@
 // 2900 (128 clocks for 16 elements of the contracted axis: operands that are not contiguous along it), handshakes 900. Tried and
 // slower: sixteen softmax warps (91 us), the next scores ahead of dx with the softmax holding its results until dz is read (93 us).
 // Warps: 0 copies, 1 issues products, 2 allocates TMEM, 4-11 softmax (forward: two groups take turns; backward: two warps share a
-// row), 12-19 dx. Rows that do not count but hold inf or NaN (the forward pass found some) are zeroed in shared memory before W's gradient.
+// row), 12-15 dx. Rows that do not count but hold inf or NaN (the forward pass found some) are zeroed in shared memory before W's gradient.
 #pragma once
 
 #include "matrix_args.cuh"
@@ -21,7 +21,7 @@ namespace rb200 {
 
 constexpr int kNarrowClasses = 128, kNarrowFeatures = 256;
 constexpr int kNarrowSlots = 8;
-constexpr int narrow_threads(bool grad) { return grad ? 640 : 384; }
+constexpr int narrow_threads(bool grad) { return grad ? 512 : 384; }
 constexpr uint32_t kChunkBytes = kTileM * kTileK * 2;   // 128 rows x 64 features
 constexpr uint32_t kNarrowSmem = 232448 - 2048;         // 227 KB, without the kernel's own KB and what aligning the start may take
 enum { kNarrowDw = 128, kNarrowDx = 384 };              // TMEM columns: scores at 0 (forward: and at 128)
@@ -57,7 +57,22 @@ struct NarrowArgs {
 };
 
 static __host__ __device__ inline uint32_t narrow_smem(int vb, int chunks, int slots, bool grad) {
-    return (uint32_t)chunks * vb * 128 + slots * kChunkBytes + (grad ? (vb + 63) / 64 * kChunkBytes + 8 * kStageBytes : 0);
+    return (uint32_t)chunks * vb * 128 + slots * kChunkBytes + (grad ? (vb + 63) / 64 * kChunkBytes + 4 * kStageBytes : 0);
+}
+
+// Sums of 16 columns over the warp's lanes: at every step a lane keeps the half of its columns that its own number's next bit names
+// and hands the other half to its partner. Lanes l and l + 16 end with column l.
+__device__ __forceinline__ float column_sums(float (&v)[16], int lane) {
+#pragma unroll
+    for (int w = 8; w; w >>= 1) {
+        const bool upper = lane & w;
+#pragma unroll
+        for (int i = 0; i < w; i++) {
+            const float keep = upper ? v[i + w] : v[i], send = upper ? v[i] : v[i + w];
+            v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, send, w);
+        }
+    }
+    return v[0] + __shfl_xor_sync(0xFFFFFFFFu, v[0], 16);
 }
 
 template <typename T, bool GRAD>
@@ -93,7 +108,7 @@ __global__ void __launch_bounds__(narrow_threads(GRAD), 1) ce_narrow_kernel(cons
         tc::bar_init(s_empty(0), GRAD ? 8 : 4);
         tc::bar_init(s_empty(1), GRAD ? 1 : 4);
         tc::bar_init(dx_full, 1);
-        tc::bar_init(dx_empty, 8);
+        tc::bar_init(dx_empty, 4);
         tc::bar_init(w_full, 1);
         tc::bar_init(done, 1);
         tc::bar_init(drained, 1);
@@ -231,8 +246,11 @@ __global__ void __launch_bounds__(narrow_threads(GRAD), 1) ce_narrow_kernel(cons
     } else if (GRAD && warp >= 4 && warp < 12) {   // softmax - target; two warps share a row's classes
         const int quarter = warp & 3, share = warp - 4 >> 2, half = g.vb / 2, line = quarter * 32 + lane;
         const uint32_t acc = tmem + share * half + ((uint32_t)(quarter * 32) << 16);
-        constexpr int kStrips = kNarrowClasses / 32;   // of 16 classes
-        float cols[kStrips] = {};   // column sums, in both halves of the lanes
+        constexpr int kStrips = kNarrowClasses / 32, kKept = 3;   // of 16 classes
+        // Column sums: a lane adds up what it has of every tile, and the lanes join theirs at the end; of a fourth strip, for which there
+        // are no registers left, after every tile.
+        float2 kept[kKept][8] = {};
+        float last = 0.0f;
         const bool dirty = *g.dirty, zero_rows = want_dw && dirty;
         int it = 0, first = 0;
         // what does not depend on the products is on its way a tile ahead
@@ -305,18 +323,12 @@ __global__ void __launch_bounds__(narrow_threads(GRAD), 1) ce_narrow_kernel(cons
                     st_shared16(dz0 + (piece >> 3) * kChunkBytes + line * 128 + (((piece & 7) ^ (line & 7)) << 4), pack8<T>(v + 8 * i));
                 }
                 if (g.want_db) {
-                    // Column sums over the warp's rows: at every step a lane keeps the half of its columns that its own
-                    // number's next bit names and hands the other half to its partner. Lanes l and l + 16 end with column l.
+                    if (c < kKept) {
 #pragma unroll
-                    for (int w = 8; w; w >>= 1) {
-                        const bool upper = lane & w;
-#pragma unroll
-                        for (int i = 0; i < w; i++) {
-                            const float keep = upper ? v[i + w] : v[i], send = upper ? v[i] : v[i + w];
-                            v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, send, w);
-                        }
+                        for (int i = 0; i < 8; i++) kept[c < kKept ? c : 0][i] = add2(kept[c < kKept ? c : 0][i], make_float2(v[2 * i], v[2 * i + 1]));
+                    } else {
+                        last += column_sums(v, lane);
                     }
-                    cols[c] += v[0];
                 }
             }
             tc::fence_before();
@@ -333,7 +345,16 @@ __global__ void __launch_bounds__(narrow_threads(GRAD), 1) ce_narrow_kernel(cons
         if (g.want_db && __all_sync(0xFFFFFFFFu, tc::bar_wait(done, 0, patience))) {   // nothing reads dz any more: [4][128] column sums
 #pragma unroll
             for (int c = 0; c < kStrips; c++) {
-                const float s = cols[c] + __shfl_xor_sync(0xFFFFFFFFu, cols[c], 16);
+                float s = last;
+                if (c < kKept) {
+                    float v[16];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        v[2 * i] = kept[c < kKept ? c : 0][i].x;
+                        v[2 * i + 1] = kept[c < kKept ? c : 0][i].y;
+                    }
+                    s = column_sums(v, lane);
+                }
                 if (c * 16 < half && lane < 16)
                     asm volatile("st.shared.f32 [%0], %1;" ::"r"(dz0 + (quarter * kNarrowClasses + share * half + c * 16 + lane) * 4), "f"(s) : "memory");
             }
@@ -450,8 +471,8 @@ __global__ void __launch_bounds__(narrow_threads(GRAD), 1) ce_narrow_kernel(cons
             counts_s[1][warp - 4] = dirts;
         }
     } else if (GRAD && warp >= 12) {
-        const int quarter = warp & 3, share = warp - 12 >> 2;   // 64 columns of a piece
-        const uint32_t area = stage0 + (warp - 12) * kStageBytes, lanes = (uint32_t)(quarter * 32) << 16;
+        const int quarter = warp & 3;
+        const uint32_t area = stage0 + quarter * kStageBytes, lanes = (uint32_t)(quarter * 32) << 16;
         const float scale = g.scale.value();
         int pieces = 0;
         bool ok = true;
@@ -461,44 +482,46 @@ __global__ void __launch_bounds__(narrow_threads(GRAD), 1) ce_narrow_kernel(cons
                 ok = __all_sync(0xFFFFFFFFu, tc::bar_wait(dx_full, pieces & 1, patience));
                 if (!ok) break;
                 tc::fence_after();
-                uint4 out[8];
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    uint32_t raw[16];
-                    tc::tmem_load16(tmem + kNarrowDx + share * 64 + q * 16 + lanes, raw);
+                for (int q = 0; q < 2; q++) {
+                    uint32_t raw[2][32];
+                    tc::tmem_load32(tmem + kNarrowDx + q * 64 + lanes, raw[0]);
+                    tc::tmem_load32(tmem + kNarrowDx + q * 64 + 32 + lanes, raw[1]);
                     tc::tmem_wait();
-                    float v[16];
+                    if (q == 1) {   // the accumulator is in registers
+                        tc::fence_before();
+                        __syncwarp();
+                        if (lane == 0) tc::bar_arrive_relaxed(dx_empty);
+                    }
 #pragma unroll
-                    for (int i = 0; i < 16; i++) v[i] = __uint_as_float(raw[i]) * scale;
-                    out[2 * q] = pack8<T>(v);
-                    out[2 * q + 1] = pack8<T>(v + 8);
-                }
-                tc::fence_before();   // the accumulator is in registers
-                __syncwarp();
-                if (lane == 0) tc::bar_arrive_relaxed(dx_empty);
+                    for (int s = 0; s < 2; s++) {
+                        const int col = h * 128 + q * 64 + s * 32, count = g.features - col;
+                        if (count <= 0 || row0 >= g.rows) continue;
+                        float v[32];
 #pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    const int col = h * 128 + share * 64 + s * 32, count = g.features - col;
-                    if (count <= 0 || row0 >= g.rows) continue;
-                    __syncwarp();   // the staging area is free: the strip before has been read
+                        for (int i = 0; i < 32; i++) v[i] = __uint_as_float(raw[s][i]) * scale;
+                        __syncwarp();   // the staging area is free: the strip before has been read
 #pragma unroll
-                    for (int i = 0; i < 4; i++) st_shared16(staged(area, lane, i), out[4 * s + i]);
-                    __syncwarp();
-                    copy_strip(area, reinterpret_cast<T*>(g.dx), g.lddx, g.vec_dx, col, min(32, count), row0, g.rows - row0, lane);
+                        for (int i = 0; i < 4; i++) st_shared16(staged(area, lane, i), pack8<T>(v + 8 * i));
+                        __syncwarp();
+                        copy_strip(area, reinterpret_cast<T*>(g.dx), g.lddx, g.vec_dx, col, min(32, count), row0, g.rows - row0, lane);
+                    }
                 }
             }
         }
         if (want_dw && ok && __all_sync(0xFFFFFFFFu, tc::bar_wait(done, 0, patience))) {   // the CTA's sums: lanes are features, columns classes
             tc::fence_after();
-            const int feature = share * 128 + quarter * 32 + lane;
-            for (int c = 0; c < g.classes && share < halves; c += 16) {
-                uint32_t raw[16];
-                tc::tmem_load16(tmem + kNarrowDw + share * 128 + c + lanes, raw);
-                tc::tmem_wait();
-                float* out = g.dw_part + ((long long)blockIdx.x * g.classes + c) * g.ldpart + feature;
+            for (int h = 0; h < halves; h++) {
+                const int feature = h * 128 + quarter * 32 + lane;
+                for (int c = 0; c < g.classes; c += 32) {
+                    uint32_t raw[32];
+                    tc::tmem_load32(tmem + kNarrowDw + h * 128 + c + lanes, raw);
+                    tc::tmem_wait();
+                    float* out = g.dw_part + ((long long)blockIdx.x * g.classes + c) * g.ldpart + feature;
 #pragma unroll
-                for (int i = 0; i < 16; i++)
-                    if (c + i < g.classes && feature < g.features) out[i * g.ldpart] = __uint_as_float(raw[i]);
+                    for (int i = 0; i < 32; i++)
+                        if (c + i < g.classes && feature < g.features) out[i * g.ldpart] = __uint_as_float(raw[i]);
+                }
             }
         }
         __syncwarp();
