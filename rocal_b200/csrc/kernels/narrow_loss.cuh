@@ -3,14 +3,15 @@
 //   W lies in shared memory for the whole launch; a CTA takes tiles of 128 rows, x arriving in chunks of 64 features,
 //   forward   scores into TMEM, a thread per row makes maximum, sum of exponentials and loss,
 //   backward  scores again, a thread per row turns them into (softmax - target) in the element type, written to shared memory as the
-//             tensor cores read it; then dx = dz W leaves at once, and W's gradient (transposed: features x classes) stays in
-//             TMEM over all of the CTA's tiles, with the same chunks of x as its other operand. CTAs' sums are joined by
-//             narrow_join_kernel in a fixed order, with the column sums for the bias.
+//             tensor cores read it; then dx = dz W leaves at once, and W's gradient stays in TMEM over all of the CTA's tiles,
+//             with the same chunks of x as its other operand. CTAs' sums are joined by narrow_join_kernel in a fixed
+//             order, with the column sums for the bias.
 // Against the general way (scores' gradients through memory, x read for each product), 279424 x 256, 81 classes, bf16: forward
-// 31 us (43), backward 81 us (156). Forward it is bound by the read of x (143 MB at 5 TB/s). Backwards a tile takes 7700 clocks, most
-// of them one after another, since shared memory has no room for a third tile of x: scores 1300, softmax 2600, the other two products
-// 2900 (128 clocks for 16 elements of the contracted axis: operands that are not contiguous along it), handshakes 900. Tried and
-// slower: sixteen softmax warps (91 us), the next scores ahead of dx with the softmax holding its results until dz is read (93 us).
+// 31 us (43), backward 74 us (156). Forward it is bound by the read of x (143 MB at 5 TB/s). Backwards a tile takes 7100 clocks, most
+// of them one after another, since shared memory has no room for a third tile of x: scores 1300, softmax 2000, the other two products
+// 3000, handshakes 800. The products are bound by the read of their operands (some 64 bytes a clock: 128 clocks for 128 x 128 x 16, so
+// W's gradient is made 256 columns at a time: 79 us with 128). Tried and slower: sixteen softmax warps (91 us), the next scores ahead of
+// dx with the softmax holding its results until dz is read (93 us), column sums by shuffles for every tile (2 us).
 // Warps: 0 copies, 1 issues products, 2 allocates TMEM, 4-11 softmax (forward: two groups take turns; backward: two warps share a
 // row), 12-15 dx. Rows that do not count but hold inf or NaN (the forward pass found some) are zeroed in shared memory before W's gradient.
 #pragma once
@@ -57,7 +58,7 @@ struct NarrowArgs {
 };
 
 static __host__ __device__ inline uint32_t narrow_smem(int vb, int chunks, int slots, bool grad) {
-    return (uint32_t)chunks * vb * 128 + slots * kChunkBytes + (grad ? (vb + 63) / 64 * kChunkBytes + 4 * kStageBytes : 0);
+    return (uint32_t)chunks * vb * 128 + slots * kChunkBytes + (grad ? 2 * kChunkBytes + 4 * kStageBytes : 0);
 }
 
 // Sums of 16 columns over the warp's lanes: at every step a lane keeps the half of its columns that its own number's next bit names
@@ -87,7 +88,7 @@ __global__ void __launch_bounds__(narrow_threads(GRAD), 1) ce_narrow_kernel(cons
 
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t w0 = (tc::smem_u32(smem_raw) + 1023u) & ~1023u, w_chunk = (uint32_t)g.vb * 128, x0 = w0 + g.chunks * w_chunk;
-    const uint32_t dz0 = x0 + g.slots * kChunkBytes, stage0 = dz0 + (g.vb + 63) / 64 * kChunkBytes;
+    const uint32_t dz0 = x0 + g.slots * kChunkBytes, stage0 = dz0 + 2 * kChunkBytes;
     const uint32_t bar0 = tc::smem_u32(bars);
     auto full = [&](int s) { return bar0 + 8u * s; };
     auto empty = [&](int s) { return bar0 + 8u * (kNarrowSlots + s); };
@@ -221,13 +222,9 @@ __global__ void __launch_bounds__(narrow_threads(GRAD), 1) ce_narrow_kernel(cons
                     };
                     if (want_dx && !(ok = gradient_of_x(0))) break;
                     if (want_dw) {
-                        const uint64_t b = tc::operand_desc(dz0, true, kChunkBytes);
-                        for (int h = 0; h < halves; h++) {
-                            const uint64_t a = tc::operand_desc(x0 + (first + 2 * h) * kChunkBytes, true, kChunkBytes);
+                        const uint64_t a = tc::operand_desc(dz0, true, kChunkBytes), b = tc::operand_desc(x0 + first * kChunkBytes, true, kChunkBytes);
 #pragma unroll
-                            for (int k = 0; k < 8; k++)
-                                tc::mma_f16<1>(tmem + kNarrowDw + h * 128, a + k * 128, b + k * 128, g.idesc_w, it > 0 || k > 0);
-                        }
+                        for (int k = 0; k < 8; k++) tc::mma_f16<1>(tmem + kNarrowDw, a + k * 128, b + k * 128, g.idesc_w, it > 0 || k > 0);
                     }
                     for (int c = 0; c < g.chunks; c++) tc::mma_commit<1>(empty(first + c));
                     first = first + g.chunks == g.slots ? 0 : first + g.chunks;
@@ -509,19 +506,18 @@ __global__ void __launch_bounds__(narrow_threads(GRAD), 1) ce_narrow_kernel(cons
                 }
             }
         }
-        if (want_dw && ok && __all_sync(0xFFFFFFFFu, tc::bar_wait(done, 0, patience))) {   // the CTA's sums: lanes are features, columns classes
+        if (want_dw && ok && __all_sync(0xFFFFFFFFu, tc::bar_wait(done, 0, patience))) {   // the CTA's sums: lanes are classes
             tc::fence_after();
-            for (int h = 0; h < halves; h++) {
-                const int feature = h * 128 + quarter * 32 + lane;
-                for (int c = 0; c < g.classes; c += 32) {
-                    uint32_t raw[32];
-                    tc::tmem_load32(tmem + kNarrowDw + h * 128 + c + lanes, raw);
-                    tc::tmem_wait();
-                    float* out = g.dw_part + ((long long)blockIdx.x * g.classes + c) * g.ldpart + feature;
+            const int c = quarter * 32 + lane;
+            float* out = g.dw_part + ((long long)blockIdx.x * g.classes + c) * g.ldpart;
+            for (int f = 0; f < g.features && quarter * 32 < g.classes; f += 32) {
+                uint32_t raw[32];
+                tc::tmem_load32(tmem + kNarrowDw + f + lanes, raw);
+                tc::tmem_wait();
 #pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (c + i < g.classes && feature < g.features) out[i * g.ldpart] = __uint_as_float(raw[i]);
-                }
+                for (int i = 0; i < 32; i += 4)   // rows padded to four; the column behind the features is the bias's and written later
+                    if (c < g.classes && f + i < g.features)
+                        *reinterpret_cast<uint4*>(out + f + i) = make_uint4(raw[i], raw[i + 1], raw[i + 2], raw[i + 3]);
             }
         }
         __syncwarp();
@@ -654,7 +650,7 @@ static int narrow_launch(NarrowArgs& g, bool grad, bool bf16, const Operand& x, 
     g.slots = grad ? 2 * g.chunks : kNarrowSlots / g.chunks * g.chunks;
     g.idesc_s = tc::instr_desc(bf16, false, false, kTileM, g.vb);
     g.idesc_x = tc::instr_desc(bf16, false, true, kTileM, 128);
-    g.idesc_w = tc::instr_desc(bf16, true, true, kTileM, (g.vb + 63) / 64 * 64);
+    g.idesc_w = tc::instr_desc(bf16, true, true, kTileM, 64 * g.chunks);
     int rc = make_map(&g.x, x, bf16, kTileM, what);
     if (rc) return rc;
     if ((rc = make_map(&g.w, w, bf16, g.vb, what))) return rc;
