@@ -275,10 +275,11 @@ __global__ void __launch_bounds__(narrow_threads(GRAD), 1) ce_narrow_kernel(cons
             const bool counted = next.counted;
             const int label = counted ? next.label : -1;
             // (softmax - target) * factor = exp(z - top) * mul + add, and at the label
-            // rows that do not count: exp(z - inf) * 0 + 0
+            // rows that do not count: exp(z - inf) * 0 + 0, except where z may be inf or NaN (behind the last row: 0 times W)
             const float factor = counted ? next.coef * 32768.0f : 0.0f, top = counted ? finite_max(next.m) : INFINITY;
             const float mul = counted ? factor / next.s : 0.0f, add = -g.smooth_off * factor;
             const float at_label = exp_diff(next.zl - top) * mul + add - g.smooth_on * factor;
+            const bool clear = !counted && (dirty || t * kTileM + line >= g.rows);
             fetch(t + gridDim.x);
             // the lanes leave together: what follows needs whole warps
             if (!__all_sync(0xFFFFFFFFu, tc::bar_wait(s_full(0), it & 1, patience) && tc::bar_wait(dz_empty, (it & 1) ^ 1, patience))) break;
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(narrow_threads(GRAD), 1) ce_narrow_kernel(cons
 #pragma unroll
             for (int c = 0; c < kStrips; c++) {
                 if (c * 16 >= half) break;
-                const int col = share * half + c * 16, count = counted || !dirty ? g.classes - col : 0, l = label - col;
+                const int col = share * half + c * 16, count = clear ? 0 : g.classes - col, l = label - col;
                 uint32_t raw[16];
                 tc::tmem_load16(acc + c * 16, raw);
                 tc::tmem_wait();
@@ -310,7 +311,7 @@ __global__ void __launch_bounds__(narrow_threads(GRAD), 1) ce_narrow_kernel(cons
 #pragma unroll
                     for (int i = 0; i < 16; i++) v[i] = i == l ? at_label : v[i];
                 }
-                if (count < 16) {   // beyond the classes; rows that do not count and may hold anything
+                if (count < 16) {   // beyond the classes; rows that may hold anything
 #pragma unroll
                     for (int i = 0; i < 16; i++) v[i] = i < count ? v[i] : 0.0f;
                 }

@@ -151,3 +151,26 @@ def test_statistics_in_pieces_of_the_classes(cuda):
         s = slice(i, i + 100000)
         wants, tols = _reference(x[s], w, b, labels[s], 0.1, "none", g[s], "fp16")
         _close(got[s], wants[0], tols[0], "loss")
+
+
+@pytest.mark.parametrize("n,k,v", [(130, 64, 40), (128, 64, 40), (333, 200, 81), (333, 300, 200)])
+def test_a_weight_of_inf_that_masks_a_class(cuda, n, k, v):
+    """Where an infinite weight makes a class' scores -inf in every row, the other gradients are those of the class masked by its
+    bias, to the bit; the rows that fill up the last tile (zeros times that weight) must not show."""
+    from rocal_b200.plugin import pytorch as P
+    x, w, b, labels, _ = _make(n + v, n, k, v, "bf16", True, cuda, ignored=0.0)
+    x[:, 3] = -x[:, 3].abs() - 0.5
+    labels[labels == 5] = 6
+
+    def grads(weight, bias):
+        leaves = [weight.clone().requires_grad_(True), bias.clone().requires_grad_(True)]
+        loss = P.linear_cross_entropy(x, leaves[0], labels, leaves[1], reduction="sum")
+        return [loss.detach()] + list(torch.autograd.grad(loss, leaves))
+    w[5] = 0
+    b_masked = b.clone()
+    b_masked[5] = float("-inf")
+    want = grads(w, b_masked)
+    w_inf = w.clone()
+    w_inf[5, 3] = float("inf")
+    for got, expect in zip(grads(w_inf, b), want):
+        assert bool(torch.isfinite(expect).all()) and torch.equal(got, expect)
