@@ -86,7 +86,7 @@ int make_map(CUtensorMap* map, const Operand& o, bool bf16, int box_rows, const 
 //   the last tile's epilogue is not hidden, and pieces of the contracted axis have to be joined by another launch (about 8000,
 //   half of it on the host). Clusters whose CTAs join their pieces through distributed shared memory were tried instead: 14 us against
 //   9 us for one row of 2048 x 1000, because clusters of full-size CTAs do not fill the GPU.
-GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed, bool may_split) {
+GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed, bool may_split, int bn_most) {
     GemmPlan best = {};
     double best_cost = 0;
     const int kblocks = (k + kTileK - 1) / kTileK, a_rows = m < kTileM ? m : kTileM;
@@ -94,7 +94,7 @@ GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed
         if (cg == 2 && m <= kTileM) continue;
         const int unit = (b_transposed ? 64 : 32) * cg, slots = dev.sms / cg;
         const int tiles_m = (m + kTileM * cg - 1) / (kTileM * cg);
-        for (int bn = kTileNMax; bn >= unit; bn -= unit) {
+        for (int bn = bn_most; bn >= unit; bn -= unit) {
             const int tiles_n = (n + bn - 1) / bn;
             if (bn > unit && (n + bn - unit - 1) / (bn - unit) == tiles_n && bn - unit >= n) continue;   // wider than the matrix
             const long long tiles = (long long)tiles_m * tiles_n;

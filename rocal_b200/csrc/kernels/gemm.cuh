@@ -839,7 +839,7 @@ static inline bool map_ready(const Operand& o) {
 struct GemmPlan {
     int bn, cg, splits, tiles_m, tiles_n, kblocks, kblocks_per_split;
 };
-GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed, bool may_split);
+GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed, bool may_split, int bn_most = kTileNMax);
 
 template <typename T, bool A_MN, bool B_MN, int EPI, int CG>
 int gemm_launch_as(const GemmArgs& g, const DeviceInfo& dev, cudaStream_t stream, const char* what) {

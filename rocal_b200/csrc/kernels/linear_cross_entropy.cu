@@ -308,8 +308,12 @@ struct StatsPlan {
     double* block_sums;
     size_t bytes;
 };
+// The loss is made of 32-bit scores, which drift with the length of one accumulator's sum (the loss by 0.35e-6 at 2048 features, 0.65e-6
+// at 4096, with scores of variance 1; three times that with large ones). Longer sums take tiles that leave TMEM columns for a second
+// accumulator (gemm.cuh): 0.31e-6 at 4096, for 12% of time (8192 x 4096, 16384 classes: 738 -> 829 us).
+constexpr int kLongSum = 2048;
 static GemmPlan stats_gemm(const rb200_linear_ce_params& p, const DeviceInfo& dev, int classes) {
-    return gemm_plan(dev, (int)p.rows, classes, (int)p.features, false, false);
+    return gemm_plan(dev, (int)p.rows, classes, (int)p.features, false, false, p.features > kLongSum ? kTileNMax / 2 : kTileNMax);
 }
 static StatsPlan plan_stats(const rb200_linear_ce_params& p, const DeviceInfo& dev, void* ws) {
     StatsPlan s = {};

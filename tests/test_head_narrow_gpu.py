@@ -174,3 +174,10 @@ def test_a_weight_of_inf_that_masks_a_class(cuda, n, k, v):
     w_inf[5, 3] = float("inf")
     for got, expect in zip(grads(w_inf, b), want):
         assert bool(torch.isfinite(expect).all()) and torch.equal(got, expect)
+
+
+@pytest.mark.parametrize("n,k,v", [(300, 4096, 700), (1000, 2056, 300), (64, 3301, 1000)])
+def test_long_sums(cuda, n, k, v):
+    """More than 2048 features: the scores' sums are spread over two accumulators, which the epilogue adds."""
+    x, w, b, labels, g = _make(n + k, n, k, v, "fp16", True, cuda)
+    _check(x, w, b, labels, 0.1, "none", g, "fp16")
