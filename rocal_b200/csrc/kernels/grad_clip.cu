@@ -307,6 +307,7 @@ __global__ void __launch_bounds__(kClipThreads) __cluster_dims__(kClipCluster, 1
     __shared__ double shared[kClipThreads / 32];
     __shared__ double sums[kClipCluster];
     __shared__ float factor_s;
+    tc::cluster_arrive();
     pdl_launch_dependents();
     pdl_wait();
     double s = 0.0;
@@ -316,6 +317,8 @@ __global__ void __launch_bounds__(kClipThreads) __cluster_dims__(kClipCluster, 1
         s += square_piece(e, begin, (int)min((long long)t.chunk, e.count - begin));
     }
     s = block_sum(s, shared);
+    __syncwarp();
+    tc::cluster_wait();   // all eight blocks have started: their shared memory may be written
     if (threadIdx.x == 0) {
         const uint32_t mine = tc::smem_u32(&sums[tc::cta_rank()]);
 #pragma unroll

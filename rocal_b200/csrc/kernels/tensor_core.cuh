@@ -25,6 +25,10 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The same barrier in two halves: every CTA of the cluster has started once the wait is over, and only then may its shared memory
+// be touched by the others.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // True in one thread of a converged warp, the same one every time. Code under it is known to run in one thread, which the
 // copy and product instructions (their operands live in uniform registers) need to issue without a loop over lanes.

@@ -1,0 +1,34 @@
+"""Rules of the programming model that the head operators' kernels have to keep and that no run can show to be kept: read from
+the sources."""
+import os
+import re
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+KERNELS = os.path.join(ROOT, "rocal_b200", "csrc", "kernels")
+
+
+def _body(file, name):
+    """The body of function `name`, comments taken out."""
+    with open(os.path.join(KERNELS, file)) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    at = text.index("{", text.index(" " + name + "("))
+    depth = 0
+    for end in range(at, len(text)):
+        depth += {"{": 1, "}": -1}.get(text[end], 0)
+        if depth == 0:
+            return text[at:end + 1]
+    raise AssertionError(name)
+
+
+@pytest.mark.parametrize("file,kernel,remote", [("grad_clip.cu", "clip_few_kernel", "st.shared::cluster"),
+                                                ("gemm.cuh", "gemm_kernel", "tc::map_to_rank")])
+def test_clusters_meet_before_they_touch_each_other(file, kernel, remote):
+    """A block's shared memory may be touched by another one only once it is known to have started: a cluster barrier lies
+    before the first access, and another behind the last one, so that no block has left by then."""
+    body = _body(file, kernel)
+    barriers = [m.start() for m in re.finditer(r"tc::cluster_(sync|wait)\(\)", body)]
+    accesses = [m.start() for m in re.finditer(re.escape(remote), body)]
+    assert accesses and barriers and barriers[0] < accesses[0] and accesses[-1] < barriers[-1], (kernel, barriers, accesses)
+    assert body.count("tc::cluster_arrive()") == body.count("tc::cluster_wait()")
