@@ -81,7 +81,15 @@ template <>
 struct Values<__nv_bfloat16> : Values16<__nv_bfloat16> {};
 
 // ---- sum of squares ---------------------------------------------------------------------------------------
-template <typename T>
+// STAYS: nothing writes the gradients while the kernel runs, so that they may be read past the coherent path.
+template <bool STAYS>
+__device__ __forceinline__ uint4 load_vector(const uint4* p) {
+    if constexpr (STAYS)
+        return __ldg(p);
+    else
+        return *p;
+}
+template <bool STAYS, typename T>
 __device__ __forceinline__ double square_sum(const T* p, int count) {
     constexpr int N = Values<T>::N;
     double s = 0.0;
@@ -104,11 +112,11 @@ __device__ __forceinline__ double square_sum(const T* p, int count) {
     for (; i + 3 * kClipThreads < vectors; i += 4 * kClipThreads) {   // four vectors in flight
         uint4 w[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) w[k] = __ldg(q + i + k * kClipThreads);
+        for (int k = 0; k < 4; k++) w[k] = load_vector<STAYS>(q + i + k * kClipThreads);
 #pragma unroll
         for (int k = 0; k < 4; k++) add(w[k]);
     }
-    for (; i < vectors; i += kClipThreads) add(__ldg(q + i));
+    for (; i < vectors; i += kClipThreads) add(load_vector<STAYS>(q + i));
     const int tail = vectors * N + threadIdx.x;
     if (tail < count) {
         const double v = Values<T>::to_float(p[tail]);
@@ -117,10 +125,11 @@ __device__ __forceinline__ double square_sum(const T* p, int count) {
     return s;
 }
 
+template <bool STAYS>
 __device__ __forceinline__ double square_piece(const ClipEntry& e, long long begin, int count) {
-    if (e.grad_dtype == RB200_FP32) return square_sum(reinterpret_cast<const float*>(e.grad) + begin, count);
-    if (e.grad_dtype == RB200_FP16) return square_sum(reinterpret_cast<const __half*>(e.grad) + begin, count);
-    return square_sum(reinterpret_cast<const __nv_bfloat16*>(e.grad) + begin, count);
+    if (e.grad_dtype == RB200_FP32) return square_sum<STAYS>(reinterpret_cast<const float*>(e.grad) + begin, count);
+    if (e.grad_dtype == RB200_FP16) return square_sum<STAYS>(reinterpret_cast<const __half*>(e.grad) + begin, count);
+    return square_sum<STAYS>(reinterpret_cast<const __nv_bfloat16*>(e.grad) + begin, count);
 }
 
 // The block's sum, in thread 0.
@@ -144,7 +153,7 @@ __global__ void __launch_bounds__(kClipThreads) clip_norm_kernel(const __grid_co
         const ClipEntry& e = t.e[find_tensor(t, c)];
         const long long begin = (long long)(c - e.chunk0) * t.chunk;
         const int count = (int)min((long long)t.chunk, e.count - begin);
-        s += square_piece(e, begin, count);
+        s += square_piece<true>(e, begin, count);
     }
     s = block_sum(s, shared);
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
@@ -314,7 +323,7 @@ __global__ void __launch_bounds__(kClipThreads) __cluster_dims__(kClipCluster, 1
     for (int c = blockIdx.x; c < t.chunks; c += kClipCluster) {
         const ClipEntry& e = t.e[find_tensor(t, c)];
         const long long begin = (long long)(c - e.chunk0) * t.chunk;
-        s += square_piece(e, begin, (int)min((long long)t.chunk, e.count - begin));
+        s += square_piece<false>(e, begin, (int)min((long long)t.chunk, e.count - begin));   // written below, in place
     }
     s = block_sum(s, shared);
     __syncwarp();

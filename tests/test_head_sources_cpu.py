@@ -13,7 +13,7 @@ def _body(file, name):
     """The body of function `name`, comments taken out."""
     with open(os.path.join(KERNELS, file)) as f:
         text = re.sub(r"//[^\n]*", "", f.read())
-    at = text.index("{", text.index(" " + name + "("))
+    at = text.index("{", re.search(r"\s%s\((?=[^;]*\{)" % name, text).start())
     depth = 0
     for end in range(at, len(text)):
         depth += {"{": 1, "}": -1}.get(text[end], 0)
@@ -32,3 +32,13 @@ def test_clusters_meet_before_they_touch_each_other(file, kernel, remote):
     accesses = [m.start() for m in re.finditer(re.escape(remote), body)]
     assert accesses and barriers and barriers[0] < accesses[0] and accesses[-1] < barriers[-1], (kernel, barriers, accesses)
     assert body.count("tc::cluster_arrive()") == body.count("tc::cluster_wait()")
+
+
+def test_what_a_kernel_writes_it_reads_coherently():
+    """__ldg is for data that no one writes while the kernel runs. The clipping of few elements reads its gradients and writes them
+    in place in one launch: the sum of squares that it makes asks for plain loads, the loads of the norm's own launch may be __ldg."""
+    few, norm = _body("grad_clip.cu", "clip_few_kernel"), _body("grad_clip.cu", "clip_norm_kernel")
+    assert "square_piece<false>" in few and "square_piece<true>" in norm and "__ldg" not in few
+    assert "__ldg" not in _body("grad_clip.cu", "square_sum") and "square_sum<STAYS>" in _body("grad_clip.cu", "square_piece")
+    for name in ("scale_vectors", "scale_chunk", "load_words"):          # these write the same tensors
+        assert "__ldg" not in _body("grad_clip.cu", name)
