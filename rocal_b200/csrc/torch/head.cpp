@@ -229,6 +229,12 @@ std::vector<Tensor> linear_backward_run(const Tensor& dout_, const Tensor& x_, c
     return g;
 }
 
+// The kernels see values only: a dual tensor's tangent (forward-mode differentiation) would be lost, and count as zero.
+void refuse_tangents(const char* what, std::initializer_list<const Tensor*> tensors) {
+    for (const Tensor* t : tensors)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative: an input carries a tangent");
+}
+
 constexpr const char* kOnce = " is differentiable once: create_graph is not supported";
 
 struct Linear : torch::autograd::Function<Linear> {
@@ -249,6 +255,7 @@ struct Linear : torch::autograd::Function<Linear> {
         const Tensor& dout = grads[0];
         const int64_t rows = ctx->saved_data["rows"].toInt();
         if (!dout.defined()) return torch::autograd::variable_list(5);
+        refuse_tangents("linear's backward pass", {&dout});
         const bool has_bias = ctx->saved_data["bias"].toBool();
         std::array<bool, 4> need = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), has_bias && ctx->needs_input_grad(2),
                                     rows > 0 && ctx->needs_input_grad(has_bias ? 3 : 2)};
@@ -284,6 +291,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const MaybeTensor& bias_, c
     TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1), "x ", x.sizes(), " does not go with weight ", weight.sizes());
     const Tensor bias = or_undefined(bias_);
     Tensor residual = or_undefined(residual_);
+    refuse_tangents("linear", {&x, &weight, &bias, &residual});
     const int64_t m = weight.size(0);
     std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
     shape.back() = m;
@@ -408,6 +416,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "linear_cross_entropy", kOnce);
         if (!grads[0].defined()) return torch::autograd::variable_list(7);
+        refuse_tangents("linear_cross_entropy's backward pass", {&grads[0]});
         const auto s = ctx->get_saved_variables();
         const auto g = ce_backward_run(grads[0], s[0], s[1], s[2], s[4], s[5], s[3], ctx->saved_data["ignore"].toInt(),
                                        ctx->saved_data["smoothing"].toDouble(), (int)ctx->saved_data["reduce"].toInt(),
@@ -423,6 +432,7 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
                           std::equal(labels.sizes().begin(), labels.sizes().end(), x.sizes().begin()),
                       "x ", x.sizes(), ", weight ", weight.sizes(), " and labels ", labels.sizes(), " do not go together");
     const Tensor bias = or_undefined(bias_);
+    refuse_tangents("linear_cross_entropy", {&x, &weight, &bias});
     const bool flat = x.dim() == 2;
     const Tensor x2 = flat ? x : x.reshape({-1, x.size(-1)}), l1 = flat ? labels : labels.reshape({-1});
     Tensor loss;
@@ -466,6 +476,7 @@ Tensor grad_clip(const py::object& grads_, double max_norm, const py::object& ou
     const TensorList grads(grads_, "grads"), out = apart ? TensorList(out_, "out") : grads;
     TORCH_CHECK_VALUE(grads.size() > 0, "no gradients");
     TORCH_CHECK_VALUE(out.size() == grads.size(), out.size(), " outputs for ", grads.size(), " gradients");
+    for (size_t i = 0; i < grads.size(); i++) refuse_tangents("grad_clip", {&grads[i], &out[i]});
     TORCH_CHECK_VALUE(grads[0].is_cuda(), "the gradients are on ", grads[0].device(), ": the head operators run on a GPU");
     TORCH_CHECK_VALUE(max_norm >= 0 && inv_scale > 0, "max_norm ", max_norm, ", inv_scale ", inv_scale);
     at::NoGradGuard no_grad;

@@ -79,8 +79,8 @@ class ROCALClassificationIterator(ROCALGenericIterator):
 
 
 # ---- the head of a training or serving step, on the batches above -----------------------------------
-# Float16 and bfloat16 CUDA tensors; differentiable by torch.autograd, once (create_graph is refused). Everything runs on the
-# tensors' device, on its current stream.
+# Float16 and bfloat16 CUDA tensors; differentiable by torch.autograd, once (create_graph is refused, and so are the tangents of
+# forward-mode differentiation). Everything runs on the tensors' device, on its current stream.
 _head = None
 
 
