@@ -12,8 +12,10 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <array>
 #include <cstring>
+#include <functional>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -471,6 +473,85 @@ struct TensorList {
     const Tensor& operator[](size_t i) const { return THPVariable_Unpack(PyTuple_GET_ITEM(items.ptr(), i)); }
 };
 
+// The memory of tensors that the library sees a dense copy of: it compares ranges of addresses, and theirs are the copies'. Whether such
+// a tensor meets another one is decided here, by the elements themselves.
+struct Extent {
+    const Tensor* t;
+    uintptr_t begin, end;   // first byte, and the one behind the last element
+    explicit Extent(const Tensor& tensor) : t(&tensor), begin((uintptr_t)tensor.data_ptr()), end(begin) {
+        if (!tensor.numel()) return;
+        int64_t reach = 1;
+        for (int64_t d = 0; d < tensor.dim(); d++) reach += (tensor.size(d) - 1) * tensor.stride(d);
+        end += (uintptr_t)reach * tensor.element_size();
+    }
+};
+// Whether sum c_k v_k = rest has a solution with 0 <= v_k <= most_k; the c_k fall, reach[k] = sum of c_j most_j from k on. Strides of
+// slices of one array leave one or two candidates a step. Gives up, and says yes, when `steps` are spent.
+bool reaches(const std::vector<std::pair<int64_t, int64_t>>& terms, const std::vector<int64_t>& reach, size_t k, int64_t rest, int64_t& steps) {
+    if (rest < 0 || rest > reach[k]) return false;
+    if (k == terms.size() || --steps <= 0) return true;   // k == size: reach is 0, and so is the rest
+    const auto [c, most] = terms[k];
+    const int64_t low = rest > reach[k + 1] ? (rest - reach[k + 1] + c - 1) / c : 0, high = std::min(most, rest / c);
+    for (int64_t v = low; v <= high; v++)
+        if (reaches(terms, reach, k + 1, rest - v * c, steps)) return true;
+    return false;
+}
+// Whether an element of `a` and one of `b` share a byte: begin_a + sum x_i s_i + i = begin_b + sum y_j t_j + j, bytes of elements included; y
+// is counted from its end, so that every coefficient is positive.
+bool share_memory(const Extent& a, const Extent& b) {
+    if (a.begin >= b.end || b.begin >= a.end || a.begin == a.end || b.begin == b.end) return false;
+    std::vector<std::pair<int64_t, int64_t>> terms;
+    for (const Extent* e : {&a, &b}) {
+        const int64_t size = (int64_t)e->t->element_size();
+        terms.emplace_back(1, size - 1);
+        for (int64_t d = 0; d < e->t->dim(); d++)
+            if (e->t->size(d) > 1 && e->t->stride(d)) terms.emplace_back(e->t->stride(d) * size, e->t->size(d) - 1);
+    }
+    std::sort(terms.begin(), terms.end(), std::greater<>());
+    size_t n = 0;
+    for (size_t i = 1; i < terms.size(); i++)   // equal strides are one term
+        if (terms[i].first == terms[n].first)
+            terms[n].second += terms[i].second;
+        else
+            terms[++n] = terms[i];
+    terms.resize(n + 1);
+    std::vector<int64_t> reach(terms.size() + 1, 0);
+    for (size_t k = terms.size(); k-- > 0;) reach[k] = reach[k + 1] + terms[k].first * terms[k].second;
+    int64_t steps = 100000;
+    return reaches(terms, reach, 0, (int64_t)(b.end - 1) - (int64_t)a.begin, steps);
+}
+// Every stride steps over all that the smaller ones reach.
+bool overlaps_itself(const Tensor& t) {
+    if (!t.numel()) return false;
+    std::vector<std::pair<int64_t, int64_t>> dims;
+    for (int64_t d = 0; d < t.dim(); d++)
+        if (t.size(d) > 1) dims.emplace_back(t.stride(d), t.size(d));
+    std::sort(dims.begin(), dims.end());
+    int64_t reach = 0;
+    for (const auto& [stride, size] : dims) {
+        if (stride <= reach) return true;
+        reach += stride * (size - 1);
+    }
+    return false;
+}
+// No output meets itself, another output or another tensor's gradients. copied[i]: the library sees a copy of tensor i; those that
+// it sees as they are it compares by itself.
+void refuse_overlaps(const TensorList& grads, const TensorList& out, bool apart, const std::vector<bool>& copied) {
+    std::vector<Extent> outs, ins;
+    for (size_t i = 0; i < out.size(); i++) {
+        outs.emplace_back(out[i]);
+        if (apart) ins.emplace_back(grads[i]);
+    }
+    for (size_t i = 0; i < outs.size(); i++) {
+        bool meets = copied[i] && overlaps_itself(out[i]);
+        for (size_t j = 0; j < outs.size() && !meets; j++) {
+            if (j == i || !(copied[i] || copied[j])) continue;
+            meets = (j > i && share_memory(outs[i], outs[j])) || (apart && share_memory(outs[i], ins[j]));
+        }
+        if (meets) throw LibraryError("grad_clip: an output overlaps itself, another output or another tensor's gradients");
+    }
+}
+
 Tensor grad_clip(const py::object& grads_, double max_norm, const py::object& out_, double inv_scale) {
     const bool apart = !out_.is_none();
     const TensorList grads(grads_, "grads"), out = apart ? TensorList(out_, "out") : grads;
@@ -484,6 +565,7 @@ Tensor grad_clip(const py::object& grads_, double max_norm, const py::object& ou
     const size_t n = grads.size();
     std::vector<rb200_grad_tensor> table(n);
     std::vector<Tensor> held;                              // dense copies of tensors with gaps
+    std::vector<bool> copied(n);
     std::vector<std::pair<Tensor, Tensor>> back;           // (the tensor with gaps, its dense result)
     for (size_t i = 0; i < n; i++) {
         const Tensor& g = grads[i];
@@ -501,12 +583,14 @@ Tensor grad_clip(const py::object& grads_, double max_norm, const py::object& ou
             continue;
         }
         TORCH_CHECK_VALUE(o.sizes() == g.sizes(), "an output has shape ", o.sizes(), " for a gradient ", g.sizes());
+        copied[i] = true;
         Tensor dense = g.contiguous(), result = !apart ? dense : o.is_contiguous() ? o : at::empty(o.sizes(), o.options());
         if (!result.is_same(o)) back.emplace_back(o, result);
         t.grad = dense.data_ptr();
         t.out = result.data_ptr();
         held.push_back(std::move(dense));
     }
+    if (!held.empty()) refuse_overlaps(grads, out, apart, copied);
     const Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
     const uint64_t bytes = api.clip_bytes((int)n);
     const Tensor ws = workspace(bytes, grads[0]);
@@ -547,6 +631,8 @@ PYBIND11_MODULE(_head, m) {
     m.def("linear", &linear);
     m.def("linear_cross_entropy", &linear_cross_entropy);
     m.def("grad_clip", &grad_clip);
+    m.def("share_memory", [](const Tensor& a, const Tensor& b) { return share_memory(Extent(a), Extent(b)); });
+    m.def("overlaps_itself", &overlaps_itself);
     m.def("linear_raw", &linear_raw);
     m.def("linear_backward_raw", [](const Tensor& dout, const Tensor& x, const Tensor& weight, const MaybeTensor& preact, const std::string& act,
                                     int64_t residual_rows, std::array<bool, 4> need, const MaybeTensor& status) {

@@ -122,7 +122,7 @@ def clip_grad_norm(grads, max_norm, out=None, inv_scale=1.0):
     gradients' types, or float32 copies for a 32-bit optimiser; contiguous ones need only the same number of elements).
     Float32, float16 and bfloat16 CUDA tensors of any shapes, mixed, on one device. Returns the norm, a float32 scalar on
     the device; nothing is read back. A gradient with inf gives the norm inf and the factor 0, one with NaN gives NaN, as
-    torch.nn.utils.clip_grad_norm_. No output may overlap another output or another tensor's gradients."""
+    torch.nn.utils.clip_grad_norm_. An output that overlaps itself, another output or another tensor's gradients is refused."""
     return (_head or _binding()).grad_clip(grads if isinstance(grads, list) else list(grads), max_norm, out, inv_scale)
 
 
