@@ -108,6 +108,31 @@ int32_t* status_word(const MaybeTensor& status, const Tensor& like) {
                       like.device());
     return status->data_ptr<int32_t>();
 }
+// Waits inside the products are bounded: one that gives up leaves its results unfinished and raises a status word. Calls for which
+// the caller gives no word of his own through the kernel layer (single launches: the library-wide word) raise this one, which lies
+// in pinned host memory: the host reads it without waiting, and the next call says what has happened. Kept for the whole process; captured
+// graphs hold its address.
+int32_t* unfinished_word() {
+    static int32_t* const word = [] {
+        c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+        const auto* kept = new Tensor(at::empty({1}, at::TensorOptions().dtype(at::kInt).pinned_memory(true)));
+        int32_t* w = kept->data_ptr<int32_t>();
+        __atomic_store_n(w, 0, __ATOMIC_RELAXED);
+        return w;
+    }();
+    return word;
+}
+void check_unfinished() {
+    if (__atomic_load_n(unfinished_word(), __ATOMIC_RELAXED) && __atomic_exchange_n(unfinished_word(), 0, __ATOMIC_RELAXED))
+        throw LibraryError("a bounded wait of an earlier head operator ran out: its results, and what was made from them, are unfinished");
+}
+struct Status {
+    MaybeTensor given;      // the caller's word, or none: the library-wide one
+    bool watched = false;   // unfinished_word()
+};
+constexpr bool kWatched = true;
+int32_t* status_word(const Status& s, const Tensor& like) { return s.watched ? unfinished_word() : status_word(s.given, like); }
+
 // The library has written to a tensor of the caller's: autograd's version check has to know.
 void written(const Tensor& t) {
     if (!t.is_inference()) torch::autograd::impl::bump_version(t);
@@ -131,7 +156,7 @@ int reduction(const std::string& name) {
 // ---- linear -----------------------------------------------------------------------------------------------
 // x, weight and residual are matrices, bias a vector.
 Tensor linear_run(const Tensor& x_, const Tensor& weight_, const Tensor& bias_, const Tensor& residual_, int act, Tensor out, Tensor* preact,
-                  const MaybeTensor& status, std::optional<std::pair<uint64_t, int>> probe) {
+                  const Status& status, std::optional<std::pair<uint64_t, int>> probe) {
     rb200_linear_params p = {};
     p.dtype = head_dtype(x_);
     c10::cuda::CUDAGuard guard(x_.device());
@@ -187,7 +212,7 @@ Tensor linear_run(const Tensor& x_, const Tensor& weight_, const Tensor& bias_, 
 }
 
 std::vector<Tensor> linear_backward_run(const Tensor& dout_, const Tensor& x_, const Tensor& weight_, const Tensor& preact_, int act,
-                                        int64_t residual_rows, std::array<bool, 4> need, const MaybeTensor& status) {
+                                        int64_t residual_rows, std::array<bool, 4> need, const Status& status) {
     rb200_linear_backward_params p = {};
     p.dtype = head_dtype(x_);
     c10::cuda::CUDAGuard guard(x_.device());
@@ -244,7 +269,7 @@ struct Linear : torch::autograd::Function<Linear> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight, const MaybeTensor& bias_,
                           const MaybeTensor& residual_, int64_t act) {
         Tensor preact, bias = or_undefined(bias_), residual = or_undefined(residual_);
-        const Tensor y = linear_run(x, weight, bias, residual, (int)act, Tensor(), act != RB200_ACT_NONE ? &preact : nullptr, {}, {});
+        const Tensor y = linear_run(x, weight, bias, residual, (int)act, Tensor(), act != RB200_ACT_NONE ? &preact : nullptr, {{}, kWatched}, {});
         ctx->save_for_backward({x, weight, preact});
         ctx->saved_data["act"] = act;
         ctx->saved_data["rows"] = residual.defined() ? residual.size(0) : (int64_t)0;
@@ -265,7 +290,7 @@ struct Linear : torch::autograd::Function<Linear> {
         if (whole) need[3] = false;
         std::vector<Tensor> g(4);
         if (need[0] || need[1] || need[2] || need[3])
-            g = linear_backward_run(dout, saved[0], saved[1], saved[2], (int)ctx->saved_data["act"].toInt(), rows, need, {});
+            g = linear_backward_run(dout, saved[0], saved[1], saved[2], (int)ctx->saved_data["act"].toInt(), rows, need, {{}, kWatched});
         return {g[0], g[1], g[2], whole ? dout : g[3], Tensor()};
     }
 };
@@ -295,6 +320,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const MaybeTensor& bias_, c
     Tensor residual = or_undefined(residual_);
     refuse_tangents("linear", {&x, &weight, &bias, &residual});
     const int64_t m = weight.size(0);
+    if (x.is_cuda()) check_unfinished();
     std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
     shape.back() = m;
     if (residual.defined()) {
@@ -311,7 +337,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const MaybeTensor& bias_, c
         refuse_stale_leaves({&x, &weight, &bias, &residual});
         y = Linear::apply(x2, weight, or_absent(bias), or_absent(residual), (int64_t)act);
     } else {
-        y = linear_run(x2, weight, bias, residual, act, Tensor(), nullptr, {}, {});
+        y = linear_run(x2, weight, bias, residual, act, Tensor(), nullptr, {{}, kWatched}, {});
     }
     return flat ? y : y.reshape(shape);
 }
@@ -353,7 +379,7 @@ CeArgs ce_args(const Tensor& x, const Tensor& weight, const Tensor& labels, cons
 
 // (loss, stats, info)
 std::array<Tensor, 3> ce_run(const Tensor& x, const Tensor& weight, const Tensor& labels, const Tensor& bias, int64_t ignore_index, double smoothing,
-                             int reduce, const MaybeTensor& status) {
+                             int reduce, const Status& status) {
     head_dtype(x);
     c10::cuda::CUDAGuard guard(x.device());
     CeArgs a = ce_args(x, weight, labels, bias, ignore_index, smoothing, reduce);
@@ -374,7 +400,7 @@ std::array<Tensor, 3> ce_run(const Tensor& x, const Tensor& weight, const Tensor
 
 std::vector<Tensor> ce_backward_run(const Tensor& dloss_, const Tensor& x, const Tensor& weight, const Tensor& labels, const Tensor& stats,
                                     const Tensor& info, const Tensor& bias, int64_t ignore_index, double smoothing, int reduce,
-                                    std::array<bool, 3> need, const MaybeTensor& status) {
+                                    std::array<bool, 3> need, const Status& status) {
     head_dtype(x);
     c10::cuda::CUDAGuard guard(x.device());
     CeArgs a = ce_args(x, weight, labels, bias, ignore_index, smoothing, reduce);
@@ -408,7 +434,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& labels,
                           const MaybeTensor& bias_, int64_t ignore_index, double smoothing, int64_t reduce) {
         const Tensor bias = or_undefined(bias_);
-        const auto r = ce_run(x, weight, labels, bias, ignore_index, smoothing, (int)reduce, {});
+        const auto r = ce_run(x, weight, labels, bias, ignore_index, smoothing, (int)reduce, {{}, kWatched});
         ctx->save_for_backward({x, weight, labels, bias, r[1], r[2]});
         ctx->saved_data["ignore"] = ignore_index;
         ctx->saved_data["smoothing"] = smoothing;
@@ -422,7 +448,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         const auto s = ctx->get_saved_variables();
         const auto g = ce_backward_run(grads[0], s[0], s[1], s[2], s[4], s[5], s[3], ctx->saved_data["ignore"].toInt(),
                                        ctx->saved_data["smoothing"].toDouble(), (int)ctx->saved_data["reduce"].toInt(),
-                                       {ctx->needs_input_grad(0), ctx->needs_input_grad(1), s[3].defined() && ctx->needs_input_grad(3)}, {});
+                                       {ctx->needs_input_grad(0), ctx->needs_input_grad(1), s[3].defined() && ctx->needs_input_grad(3)}, {{}, kWatched});
         return {g[0], g[1], Tensor(), g[2], Tensor(), Tensor(), Tensor()};
     }
 };
@@ -435,6 +461,7 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
                       "x ", x.sizes(), ", weight ", weight.sizes(), " and labels ", labels.sizes(), " do not go together");
     const Tensor bias = or_undefined(bias_);
     refuse_tangents("linear_cross_entropy", {&x, &weight, &bias});
+    if (x.is_cuda()) check_unfinished();
     const bool flat = x.dim() == 2;
     const Tensor x2 = flat ? x : x.reshape({-1, x.size(-1)}), l1 = flat ? labels : labels.reshape({-1});
     Tensor loss;
@@ -442,7 +469,7 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
         refuse_stale_leaves({&x, &weight, &bias});
         loss = LinearCrossEntropy::apply(x2, weight, l1, or_absent(bias), ignore_index, smoothing, (int64_t)reduce);
     } else {
-        loss = ce_run(x2, weight, l1, bias, ignore_index, smoothing, reduce, {})[0];
+        loss = ce_run(x2, weight, l1, bias, ignore_index, smoothing, reduce, {{}, kWatched})[0];
     }
     return flat || reduce != RB200_REDUCE_NONE ? loss : loss.reshape(labels.sizes());
 }
@@ -559,6 +586,7 @@ Tensor grad_clip(const py::object& grads_, double max_norm, const py::object& ou
     TORCH_CHECK_VALUE(out.size() == grads.size(), out.size(), " outputs for ", grads.size(), " gradients");
     for (size_t i = 0; i < grads.size(); i++) refuse_tangents("grad_clip", {&grads[i], &out[i]});
     TORCH_CHECK_VALUE(grads[0].is_cuda(), "the gradients are on ", grads[0].device(), ": the head operators run on a GPU");
+    check_unfinished();
     TORCH_CHECK_VALUE(max_norm >= 0 && inv_scale > 0, "max_norm ", max_norm, ", inv_scale ", inv_scale);
     at::NoGradGuard no_grad;
     c10::cuda::CUDAGuard guard(grads[0].device());
@@ -604,10 +632,10 @@ Tensor grad_clip(const py::object& grads_, double max_norm, const py::object& ou
 // ---- single launches (rocal_b200.kernels) -----------------------------------------------------------------------
 std::pair<Tensor, MaybeTensor> linear_raw(const Tensor& x, const Tensor& weight, const MaybeTensor& bias, const MaybeTensor& residual,
                                           const std::string& act, const MaybeTensor& out, bool want_preact, const MaybeTensor& status,
-                                          std::optional<std::pair<uint64_t, int>> probe) {
+                                          std::optional<std::pair<uint64_t, int>> probe, bool watched) {
     Tensor preact;
     Tensor y = linear_run(x, weight, or_undefined(bias), or_undefined(residual), activation(act), or_undefined(out), want_preact ? &preact : nullptr,
-                          status, probe);
+                          Status{status, watched}, probe);
     return {y, want_preact ? MaybeTensor(preact) : std::nullopt};
 }
 template <typename G>
@@ -633,19 +661,21 @@ PYBIND11_MODULE(_head, m) {
     m.def("grad_clip", &grad_clip);
     m.def("share_memory", [](const Tensor& a, const Tensor& b) { return share_memory(Extent(a), Extent(b)); });
     m.def("overlaps_itself", &overlaps_itself);
-    m.def("linear_raw", &linear_raw);
+    m.def("check_unfinished", &check_unfinished);
+    m.def("linear_raw", &linear_raw, py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(),
+          py::arg("watched") = false);
     m.def("linear_backward_raw", [](const Tensor& dout, const Tensor& x, const Tensor& weight, const MaybeTensor& preact, const std::string& act,
                                     int64_t residual_rows, std::array<bool, 4> need, const MaybeTensor& status) {
-        return listed(linear_backward_run(dout, x, weight, or_undefined(preact), activation(act), residual_rows, need, status));
+        return listed(linear_backward_run(dout, x, weight, or_undefined(preact), activation(act), residual_rows, need, Status{status}));
     });
     m.def("linear_ce_raw", [](const Tensor& x, const Tensor& weight, const Tensor& labels, const MaybeTensor& bias, int64_t ignore_index,
                               double smoothing, const std::string& reduce, const MaybeTensor& status) {
-        return listed(ce_run(x, weight, labels, or_undefined(bias), ignore_index, smoothing, reduction(reduce), status));
+        return listed(ce_run(x, weight, labels, or_undefined(bias), ignore_index, smoothing, reduction(reduce), Status{status}));
     });
     m.def("linear_ce_backward_raw", [](const Tensor& dloss, const Tensor& x, const Tensor& weight, const Tensor& labels, const Tensor& stats,
                                        const Tensor& info, const MaybeTensor& bias, int64_t ignore_index, double smoothing,
                                        const std::string& reduce, std::array<bool, 3> need, const MaybeTensor& status) {
         return listed(ce_backward_run(dloss, x, weight, labels, stats, info, or_undefined(bias), ignore_index, smoothing, reduction(reduce), need,
-                                      status));
+                                      {status}));
     });
 }

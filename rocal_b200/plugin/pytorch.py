@@ -81,6 +81,9 @@ class ROCALClassificationIterator(ROCALGenericIterator):
 # ---- the head of a training or serving step, on the batches above -----------------------------------
 # Float16 and bfloat16 CUDA tensors; differentiable by torch.autograd, once (create_graph is refused, and so are the tangents of
 # forward-mode differentiation). Everything runs on the tensors' device, on its current stream.
+#
+# Waits inside the kernels are bounded (about a second, longer for long sums); one that runs out leaves its results unfinished. The next of these
+# calls then raises Rb200Error, and check_unfinished() does so behind the last one.
 _head = None
 
 
@@ -133,3 +136,10 @@ def clip_grad_norm_(parameters, max_norm, inv_scale=1.0):
     if not grads:
         return torch.zeros((), device=parameters[0].device if parameters else "cuda")
     return clip_grad_norm(grads, max_norm, inv_scale=inv_scale)
+
+
+def check_unfinished():
+    """Waits for the current device and raises Rb200Error if a call of this section gave up on a bounded wait since the last
+    of these calls: its results, and what was made from them, are unfinished."""
+    torch.cuda.synchronize()
+    (_head or _binding()).check_unfinished()

@@ -1,0 +1,43 @@
+"""Waits that run out, in calls through the torch binding: nothing faults, and the caller is told."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+WAIT_CYCLES = 2_000_000      # about a millisecond of SM clock
+
+
+def test_a_wait_that_ran_out_is_told_by_the_next_call(cuda):
+    """A product whose copies from the third block of the contracted axis on are left out gives up. Whichever operator is
+    called next says so, once; the library-wide word is not touched."""
+    import rocal_b200
+    from rocal_b200._lib import lib
+    from rocal_b200._torch import head
+    from rocal_b200.plugin import pytorch as P
+    g = torch.Generator(device=cuda).manual_seed(5)
+    x, w = (torch.randn((n, 512), generator=g, device=cuda).half() for n in (40, 200))
+    labels, grad = torch.zeros(40, dtype=torch.int32, device=cuda), torch.ones(10, device=cuda)
+    want = P.linear(x, w)
+
+    def gives_up():
+        head.linear_raw(x, w, None, None, "none", None, False, None, (WAIT_CYCLES, 2), watched=True)
+        torch.cuda.synchronize()
+    for call in (lambda: P.linear(x, w), lambda: P.linear_cross_entropy(x, w, labels), lambda: P.clip_grad_norm([grad], 0.5), P.check_unfinished):
+        gives_up()
+        with pytest.raises(rocal_b200.Rb200Error, match="unfinished"):
+            call()
+        call()
+        assert bool((grad == grad[0]).all()) and torch.equal(P.linear(x, w), want)
+        grad.fill_(1)
+    # in a captured graph, too, whose replays raise the same word
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        head.linear_raw(x, w, None, None, "none", None, False, None, (WAIT_CYCLES, 2), watched=True)
+    P.check_unfinished()
+    for _ in range(2):
+        graph.replay()
+        with pytest.raises(rocal_b200.Rb200Error, match="unfinished"):
+            P.check_unfinished()
+    assert lib.rb200k_device_status() == 0
+
