@@ -166,7 +166,9 @@ int gemm_args(GemmArgs* g, const DeviceInfo& dev, int epi, bool bf16, const Oper
     g->stages = kRingBytes / (g->stage_blocks * g->block_bytes);
     if (g->stages > 12) g->stages = 12;
     g->status = wait.status ? wait.status : dev.status;
-    g->wait_cycles = wait.cycles ? wait.cycles : kDefaultWaitCycles;
+    // The longest wait is for all products of a tile. A contracted block takes 290 clocks at least, some 2000 when every SM reads its operands
+    // from memory; with 8192 for each, the ordinary limit holds for sums of any length.
+    g->wait_cycles = wait.cycles ? wait.cycles : kDefaultWaitCycles + 8192ull * plan.kblocks_per_split;
     g->skip_block = wait.skip_block;
     return RB200_OK;
 }

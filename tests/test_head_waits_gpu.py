@@ -41,3 +41,18 @@ def test_a_wait_that_ran_out_is_told_by_the_next_call(cuda):
             P.check_unfinished()
     assert lib.rb200k_device_status() == 0
 
+
+
+def test_the_longest_sums_are_waited_for(cuda):
+    """A tile's products of 2^29 contracted elements (within the documented extents) take more than a second of SM clock, the
+    limit of ordinary waits: 8.4 million blocks of 64 elements at 290 clocks or more. Values are zero but for a few, so that the
+    sums are exact."""
+    from rocal_b200 import kernels as K
+    k = 1 << 29
+    x, w = torch.zeros((1, k), dtype=torch.bfloat16, device=cuda), torch.zeros((2, k), dtype=torch.bfloat16, device=cuda)
+    x[0, 0], x[0, k // 2 + 1], x[0, -1] = 3.0, 5.0, 7.0
+    w[0, 0], w[0, k // 2 + 1], w[1, -1], w[1, 5] = 2.0, 1.0, 1.5, 9.0
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    loss, stats, info = K.linear_cross_entropy(x, w, torch.ones(1, dtype=torch.int64, device=cuda), reduction="sum", status=status)
+    assert int(status) == 0 and float(stats[0]) == 11.0 and float(stats[2]) == 10.5                # scores 11 and 10.5
+    assert abs(float(loss) - (11.0 - 10.5 + torch.log1p(torch.exp(torch.tensor(-0.5, dtype=torch.float64))).item())) <= 1e-6
