@@ -8,6 +8,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
@@ -19,6 +20,7 @@
 #include <optional>
 #include <stdexcept>
 #include <string>
+#include <unordered_set>
 #include <vector>
 
 #include "rb200_kernels.h"
@@ -300,16 +302,28 @@ bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 // A leaf's gradient node lives as long as any graph that holds it, and belongs to the stream that was current when it was
 // made. In a capture, autograd would make the legacy default stream wait for the capturing one if an eager graph of
 // the same leaf were still alive there: CUDA does not allow that, and the error ends the process. Refused here, before anything is
-// captured.
+// captured. A leaf may also lie behind operations of the capture itself (a cast, a view): the graph is followed through nodes of other
+// streams than the default one.
 void refuse_stale_leaves(std::initializer_list<const Tensor*> tensors) {
     if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
-    for (const Tensor* t : tensors) {
-        if (!wants_grad(*t) || !t->is_leaf()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-        if (!node || !node->stream()) continue;
-        TORCH_CHECK(*node->stream() != c10::cuda::getDefaultCUDAStream(t->device().index()).unwrap(),
+    using torch::autograd::Node;
+    std::vector<std::shared_ptr<Node>> todo;
+    std::unordered_set<const Node*> seen;
+    auto take = [&](std::shared_ptr<Node> node) {
+        if (node && seen.insert(node.get()).second) todo.push_back(std::move(node));
+    };
+    for (const Tensor* t : tensors)
+        if (wants_grad(*t)) take(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
+    while (!todo.empty()) {
+        const std::shared_ptr<Node> node = std::move(todo.back());
+        todo.pop_back();
+        const auto stream = node->stream();
+        const bool eager = stream && *stream == c10::cuda::getDefaultCUDAStream(stream->device_index()).unwrap();
+        TORCH_CHECK(!eager || !dynamic_cast<torch::autograd::AccumulateGrad*>(node.get()),
                     "capture with gradients: a graph of the same leaf, made on the default stream, is still alive; drop it "
                     "(its outputs and losses) before the capture, or make it on another stream");
+        if (!eager)
+            for (const auto& edge : node->next_edges()) take(edge.function);
     }
 }
 
