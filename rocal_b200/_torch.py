@@ -11,6 +11,16 @@ _PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_head.so")
 if not os.path.exists(_PATH):
     raise ImportError("rocal_b200: %s not found. Build it with `python -m rocal_b200.build` (needs nvcc, g++ and torch's headers)" % _PATH)
 
+from . import build as _build  # noqa: E402
+
+# The binding uses torch's C++ classes: another torch than the one that it was compiled against must not load it.
+if os.path.exists(_build.HEAD_STAMP):
+    with open(_build.HEAD_STAMP) as _f:
+        _for = _f.readline().strip()
+    if _for != _build.head_versions():
+        raise ImportError("rocal_b200: %s was built for %s, this is %s. Build it anew with `python -m rocal_b200.build`" %
+                          (_PATH, _for, _build.head_versions()))
+
 from . import _head as head  # noqa: E402
 
 # the order of struct Api in csrc/torch/head.cpp

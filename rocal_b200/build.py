@@ -42,6 +42,26 @@ HEAD_SRC = os.path.join(CSRC, "torch", "head.cpp")
 HEAD_LIB = os.path.join(PKG, "_head.so")
 
 
+HEAD_STAMP = os.path.join(OBJ_DIR, "_head.stamp")     # what _head.so was compiled against
+
+
+def head_versions():
+    """The torch and Python that _head.so has to be compiled against, or None without a torch that has CUDA. (torch is not
+    imported: that takes longer than looking whether anything has to be built.)"""
+    import importlib.metadata
+    import importlib.util
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not os.path.exists(os.path.join(os.path.dirname(spec.origin), "lib", "libc10_cuda.so")):
+        return None
+    return "torch %s, Python %d.%d" % ((importlib.metadata.version("torch"),) + sys.version_info[:2])
+
+
+def head_stamp():
+    """The versions, and on further lines where they lie."""
+    import importlib.util
+    return "\n".join([head_versions(), os.path.dirname(importlib.util.find_spec("torch").origin), sys.prefix, NVCC]) + "\n"
+
+
 def head_command():
     """The compiler call that makes _head.so, the torch binding of the head operators. It calls the library through
     addresses it is given at import, so it does not link to it."""
@@ -60,9 +80,18 @@ def head_command():
 
 
 def build_head(force=False):
-    """Starts the build of _head.so where it is out of date; returns the process to wait for, or None."""
+    """Starts the build of _head.so where it is out of date - with its sources, or with the torch or the Python that it was compiled
+    against; returns the process to wait for, or None. Without a torch that has CUDA there is no binding to build: the library
+    itself does not need one."""
+    if head_versions() is None:
+        sys.stderr.write("rocal_b200: no torch with CUDA is installed, the torch binding of the head operators is not built\n")
+        return None
     newest = max(os.path.getmtime(f) for f in (HEAD_SRC, os.path.join(ROOT, "include", "rb200_kernels.h"), __file__))
-    if not force and os.path.exists(HEAD_LIB) and os.path.getmtime(HEAD_LIB) > newest:
+    stamp = ""
+    if os.path.exists(HEAD_STAMP):
+        with open(HEAD_STAMP) as f:
+            stamp = f.read()
+    if not force and os.path.exists(HEAD_LIB) and os.path.getmtime(HEAD_LIB) > newest and stamp == head_stamp():
         return None
     return subprocess.Popen(head_command(), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
 
@@ -99,6 +128,9 @@ def build(force=False, verbose=False, debug_bounds=False):
         if head.returncode != 0:
             failed = True
             sys.stderr.write(out + "g++ failed for %s\n" % HEAD_SRC)
+        else:
+            with open(HEAD_STAMP, "w") as f:
+                f.write(head_stamp())
     if failed:
         raise RuntimeError("rocal_b200: nvcc build failed")
     if procs or force or not os.path.exists(lib):
