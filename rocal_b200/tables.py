@@ -4,8 +4,6 @@ import numpy as np
 FP32, FP16, UINT8 = 0, 1, 2
 BF16 = 16                       # element type of the head operators (rb200k_linear, ...)
 NHWC, NCHW = 0, 1
-REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
-ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 COLOR_NONE, COLOR_BRIGHTNESS, COLOR_CONTRAST, COLOR_TWIST, COLOR_GAMMA, COLOR_BLEND = 0, 1, 2, 3, 4, 5
 
 RESAMPLE_SAMPLE = np.dtype([
