@@ -152,19 +152,22 @@ __device__ __forceinline__ void window(const uint32_t (&w)[2 * W], uint32_t (&ou
     for (int k = 0; k < W; k++) out[k] = __funnelshift_r(w[SHIFT + k], w[(SHIFT + k + 1) % (2 * W)], bits);
 }
 
-// Upper tail of the normal distribution over its density shape: R(a) = Q(a) exp(a^2 / 2) for a in [0, 6]. Q falls like
-// 1 / a times the density, so R is smooth in t = 1 / (1 + p a): a polynomial t, ..., t^6, fitted here together with p for the least
-// relative error (1.0e-6 evaluated in fp32, and the reciprocal's 1e-7). Beyond 6, where Q is below 1e-9, R(6) stands in.
-// (A polynomial in a takes degree 12 for 2e-6, and in packed pairs its coefficients sit in 26 registers: the epilogues
+// Upper tail of the normal distribution over its density shape: R(a) = Q(a) exp(a^2 / 2) for a in [0, 14]. Q falls like
+// 1 / a times the density, so R is smooth in t = 1 / (1 + p a): a polynomial t, ..., t^7, fitted here together with p for the least
+// relative error (1.0e-6 evaluated in fp32, and the reciprocal's 1e-7). Beyond 13.2 the exponential that it goes with is flushed to zero.
+// (A polynomial in a takes degree 12 for 2e-6 up to 6, and in packed pairs its coefficients sit in 26 registers: the epilogues
 // spilled, and the spills took half of the L1's stores.)
+constexpr float kTailEnd = 14.0f, kTailScale = 0.264f;
+__device__ constexpr float tail_term(int i) {   // of t^(i + 1); folded where the loops below are unrolled
+    constexpr float c[7] = {0.105179973f, 0.107738927f, 0.0808872133f, 0.147553459f, -0.0746941119f, 0.202287167f, -0.0689526573f};
+    return c[i];
+}
 __device__ __forceinline__ float tail_ratio(float a) {
     float t;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(fminf(a, 6.0f), 0.294f, 1.0f)));
-    float r = fmaf(t, -0.0888040438f, 0.272132337f);
-    r = fmaf(r, t, -0.0816512033f);
-    r = fmaf(r, t, 0.177665651f);
-    r = fmaf(r, t, 0.102016911f);
-    r = fmaf(r, t, 0.118640058f);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(a, kTailScale, 1.0f)));
+    float r = tail_term(6);
+#pragma unroll
+    for (int i = 5; i >= 0; i--) r = fmaf(r, t, tail_term(i));
     return r * t;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -172,10 +175,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// z Phi(z) = max(z, 0) - |z| Q(|z|): one exponential and one reciprocal, accurate in the negative tail as well: beyond 6,
-// |z| R(|z|) is within 2% of what it is at 6. Infinities give 0 and inf (the exponential is 0 there), NaN stays.
+// z Phi(z) = max(z, 0) - |z| Q(|z|): one exponential and one reciprocal, accurate down the whole negative tail.
+// Infinities give 0 and inf (the exponential is 0 there), NaN stays.
 __device__ __forceinline__ float gelu(float z) {
-    const float a = fminf(fabsf(z), 6.0f), e = exp2_fast(z * (z * -0.72134752f));
+    const float a = fminf(fabsf(z), kTailEnd), e = exp2_fast(z * (z * -0.72134752f));
     return (z < 0.0f ? 0.0f : z) - a * e * tail_ratio(a);
 }
 // Phi(z) + z phi(z), two at a time (fma.f32x2: the sweep over a gradient that this is for is bound by issue as much as by memory;
@@ -185,15 +188,13 @@ __device__ __forceinline__ float2 gelu_slopes(float2 z) {
     asm("min.NaN.f32 %0, %1, 0f42200000;" : "=f"(a.x) : "f"(fabsf(z.x)));
     asm("min.NaN.f32 %0, %1, 0f42200000;" : "=f"(a.y) : "f"(fabsf(z.y)));
     const float2 x = mul2(a, mul2(a, make_float2(-0.72134752f, -0.72134752f))), e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-    const float2 b = fma2(make_float2(fminf(a.x, 6.0f), fminf(a.y, 6.0f)), make_float2(0.294f, 0.294f), make_float2(1.0f, 1.0f));
+    const float2 b = fma2(make_float2(fminf(a.x, kTailEnd), fminf(a.y, kTailEnd)), make_float2(kTailScale, kTailScale), make_float2(1.0f, 1.0f));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t.x) : "f"(b.x));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t.y) : "f"(b.y));
     auto both = [](float c) { return make_float2(c, c); };
-    float2 r = fma2(t, both(0.0888040438f), both(-0.272132337f));   // -R: tail_ratio's polynomial
-    r = fma2(r, t, both(0.0816512033f));
-    r = fma2(r, t, both(-0.177665651f));
-    r = fma2(r, t, both(-0.102016911f));
-    r = fma2(r, t, both(-0.118640058f));
+    float2 r = both(-tail_term(6));   // -R: tail_ratio's polynomial
+#pragma unroll
+    for (int i = 5; i >= 0; i--) r = fma2(r, t, both(-tail_term(i)));
     // |z| phi - Q, which the sign of z turns into the distance from 1 or from 0
     const float2 d = mul2(e, fma2(a, both(0.39894228f), mul2(r, t)));
     auto turn = [](float v, float dist) {
@@ -202,7 +203,17 @@ __device__ __forceinline__ float2 gelu_slopes(float2 z) {
     };
     return make_float2(turn(z.x, d.x), turn(z.y, d.y));
 }
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + exp2_fast(z * -1.4426950408889634f)); }
+// sigmoid(z) = h (h r) and 1 - sigmoid(z) = r from h = exp(z / 2), r = 1 / (1 + h^2): the root, because exp(z) itself and its reciprocal
+// leave the range of normal numbers while z sigmoid(z) is still a number of the result's type. z is held at 60, where
+// sigmoid is 1; NaN passes.
+struct Sigmoid {
+    float z, h, r;
+    __device__ __forceinline__ explicit Sigmoid(float v) {
+        asm("min.NaN.f32 %0, %1, 0f42700000;" : "=f"(z) : "f"(v));
+        h = exp2_fast(z * 0.72134752f);
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(h, h, 1.0f)));
+    }
+};
 
 // N values at a time: one branch on the activation, and N independent chains of operations behind it.
 template <int N>
@@ -215,7 +226,10 @@ __device__ __forceinline__ void act_values(float* v, int act) {
         for (int i = 0; i < N; i++) v[i] = gelu(v[i]);
     } else if (act == ACT_SILU) {
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] *= sigmoid(v[i]);
+        for (int i = 0; i < N; i++) {
+            const Sigmoid g(v[i]);
+            v[i] = v[i] * g.h * (g.h * g.r);
+        }
     }
 }
 template <int N>
@@ -233,8 +247,8 @@ __device__ __forceinline__ void act_slopes(float* v, int act) {   // z -> slope
     } else if (act == ACT_SILU) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const float g = sigmoid(v[i]);
-            v[i] = g * fmaf(v[i], 1.0f - g, 1.0f);
+            const Sigmoid g(v[i]);
+            v[i] = fmaf(g.z, g.r, 1.0f) * g.h * (g.h * g.r);
         }
     } else {
 #pragma unroll
