@@ -458,7 +458,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     }
                 }
             }
-            if (!ok && rank == 0) {   // copies still on their way into this CTA's (and its peer's) stages
+            // Copies still on their way into this CTA's (and its peer's) stages. The products wait for every one of them, but may have
+            // given up, also when this warp is through.
+            if (rank == 0) {
                 for (int i = 0; i < S && i < filled; i++) {
                     if (s == 0) {
                         s = S;
@@ -514,7 +516,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 buf ^= 1;
                 acc_phase ^= buf == 0;
             }
-            if (!ok && issued) {   // products still running when the CTA gives up
+            if (issued) {   // products still running: the epilogues wait for all of them, but may have given up
                 tc::mma_commit<CG>(drained);
                 tc::bar_drain(drained, 0, g.wait_cycles);
             }
@@ -823,6 +825,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         __syncthreads();
     tc::fence_after();
     if (warp == 2) tc::tmem_free<CG>(tmem);
+    // the last arrival that the other CTA's products bring here (what it needs is read anew: kept, it costs the epilogues spills)
+    if (CG == 2 && threadIdx.x == 32 && tc::cta_rank() == 1) tc::bar_drain(tc::smem_u32(&bars[36]), 0, g.wait_cycles);
 }
 
 // ---- host side -----------------------------------------------------------------------------------------

@@ -156,16 +156,16 @@ __global__ void __launch_bounds__(narrow_threads(GRAD), 1) ce_narrow_kernel(cons
                     }
                 }
             }
-            if (!ok) {   // copies still on their way into this CTA
-                tc::bar_drain(w_full, 0, g.wait_cycles);
-                for (int i = 0; i < g.slots && i < filled; i++) {
-                    if (s == 0) {
-                        s = g.slots;
-                        phase ^= 1;
-                    }
-                    s--;
-                    tc::bar_drain(full(s), phase, g.wait_cycles);
+            // Copies still on their way into this CTA. The products wait for every one of them, but may have given up, also when this
+            // warp is through.
+            tc::bar_drain(w_full, 0, g.wait_cycles);
+            for (int i = 0; i < g.slots && i < filled; i++) {
+                if (s == 0) {
+                    s = g.slots;
+                    phase ^= 1;
                 }
+                s--;
+                tc::bar_drain(full(s), phase, g.wait_cycles);
             }
         }
         __syncwarp();
@@ -234,10 +234,8 @@ __global__ void __launch_bounds__(narrow_threads(GRAD), 1) ce_narrow_kernel(cons
                 }
                 if (ok) tc::mma_commit<1>(done);
             }
-            if (!ok) {   // products still running when the CTA gives up
-                tc::mma_commit<1>(drained);
-                tc::bar_drain(drained, 0, g.wait_cycles);
-            }
+            tc::mma_commit<1>(drained);   // products still running: the other warps wait for all of them, but may have given up
+            tc::bar_drain(drained, 0, g.wait_cycles);
         }
         __syncwarp();
     } else if (GRAD && warp >= 4 && warp < 12) {   // softmax - target; two warps share a row's classes

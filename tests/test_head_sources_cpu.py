@@ -42,3 +42,21 @@ def test_what_a_kernel_writes_it_reads_coherently():
     assert "__ldg" not in _body("grad_clip.cu", "square_sum") and "square_sum<STAYS>" in _body("grad_clip.cu", "square_piece")
     for name in ("scale_vectors", "scale_chunk", "load_words"):          # these write the same tensors
         assert "__ldg" not in _body("grad_clip.cu", name)
+
+
+@pytest.mark.parametrize("waits_for", [r"full\(s\)", "drained"])
+@pytest.mark.parametrize("file,kernel", [("gemm.cuh", "gemm_kernel"), ("narrow_loss.cuh", "ce_narrow_kernel")])
+def test_copies_and_products_in_flight_are_waited_for(file, kernel, waits_for):
+    """A block must not end while a copy into its shared memory is on its way, or a product that it has issued. Where another warp gives up
+    on a wait, the warp that issues the copies (the products) may have issued its last one already: its own wait for them must not
+    depend on whether it has been told."""
+    body = _body(file, kernel)
+    loops = [m.start() for m in re.finditer(r"tc::bar_drain\(" + waits_for, body)]
+    assert loops
+    at, depth, conditions = loops[0], 0, []
+    for i in range(at, body.index("tc::elect_one()"), -1):      # the blocks that the wait lies in
+        depth += {"}": 1, "{": -1}.get(body[i], 0)
+        if body[i] == "{" and depth < 0:
+            conditions.append(re.split(r"[;{}]", body[:i])[-1] if "for" not in body[max(0, i - 80):i] else "for")
+            depth = 0
+    assert conditions and not any(re.search(r"\bok\b|gave_up", c) for c in conditions), conditions
