@@ -2,6 +2,7 @@
 import os
 import subprocess
 import sys
+import time
 
 import pytest
 
@@ -19,7 +20,7 @@ def build(monkeypatch, tmp_path):
     monkeypatch.setattr(B, "HEAD_LIB", str(tmp_path / "_head.so"))
     monkeypatch.setattr(B.subprocess, "Popen", lambda command, **kw: started.append(command) or "process")
     (tmp_path / "_head.so").write_bytes(b"")
-    future = max(os.path.getmtime(f) for f in (B.HEAD_SRC, B.__file__)) + 1000
+    future = time.time() + 1000
     os.utime(tmp_path / "_head.so", (future, future))
     return B, started
 
