@@ -501,6 +501,9 @@ RB200_API int rb200k_linear_ce(const rb200_linear_ce_params* params, void* strea
  * type (pieces of the classes, or of the rows where there are more of those). */
 RB200_API uint64_t rb200k_linear_ce_backward_workspace_bytes(const rb200_linear_ce_params* params);
 RB200_API int rb200k_linear_ce_backward(const rb200_linear_ce_params* params, void* stream);
+/* Self-test of the bounded waits, as rb200k_linear_probe: every product of the forward (backward = 0) or the backward pass leaves
+ * out the copies of the contracted axis' blocks from skip_block on, and gives up after wait_cycles. */
+RB200_API int rb200k_linear_ce_probe(const rb200_linear_ce_params* params, void* stream, int backward, uint64_t wait_cycles, int skip_block);
 
 /* Global norm of a step's gradients and clipping. With N = inv_scale * sqrt(sum of all squares over all tensors) and
  * c = min(1, max_norm / (N + 1e-6)), every tensor's out = grad * (inv_scale * c), and *norm = N. inv_scale undoes the loss scale

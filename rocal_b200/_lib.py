@@ -100,6 +100,8 @@ lib.rb200k_grad_clip.argtypes = [c_void_p, c_int, ctypes.c_float, ctypes.c_float
 lib.rb200k_grad_clip.restype = c_int
 lib.rb200k_linear_probe.argtypes = [ctypes.POINTER(LinearParams), c_void_p, c_uint64, c_int]
 lib.rb200k_linear_probe.restype = c_int
+lib.rb200k_linear_ce_probe.argtypes = [ctypes.POINTER(LinearCeParams), c_void_p, c_int, c_uint64, c_int]
+lib.rb200k_linear_ce_probe.restype = c_int
 lib.rb200k_normalize_scratch_bytes.argtypes = [c_int, c_int, c_int, c_int]
 lib.rb200k_normalize_scratch_bytes.restype = ctypes.c_size_t
 lib.rb200k_normalize.argtypes = [c_void_p, c_void_p, c_void_p, c_int, ctypes.POINTER(NormalizeParams), c_void_p, ctypes.c_size_t, c_void_p]

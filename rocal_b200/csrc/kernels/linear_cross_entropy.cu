@@ -282,7 +282,7 @@ static EpiArgs label_args(const rb200_linear_ce_params& p) {
     e.smooth_off = p.label_smoothing / (float)p.classes;
     return e;
 }
-static NarrowArgs narrow_args(const rb200_linear_ce_params& p) {
+static NarrowArgs narrow_args(const rb200_linear_ce_params& p, const GemmWait& wait) {
     NarrowArgs g = {};
     g.bias = p.bias;
     g.labels = p.labels;
@@ -293,6 +293,8 @@ static NarrowArgs narrow_args(const rb200_linear_ce_params& p) {
     g.smooth_off = p.label_smoothing / (float)p.classes;
     g.stats = p.stats;
     g.status = p.status;
+    g.wait_cycles = wait.cycles;
+    g.skip_chunk = wait.skip_block;
     return g;
 }
 static const uint8_t* at_row(const void* p, long long ld, long long row) { return (const uint8_t*)p + row * ld * 2; }
@@ -344,7 +346,7 @@ static StatsPlan plan_stats(const rb200_linear_ce_params& p, const DeviceInfo& d
     return s;
 }
 
-static int ce_forward(const rb200_linear_ce_params* p, cudaStream_t stream) {
+static int ce_forward(const rb200_linear_ce_params* p, cudaStream_t stream, GemmWait wait) {
     const char* what = "rb200k_linear_ce";
     if (!p) {
         set_error("%s: params is null", what);
@@ -369,7 +371,7 @@ static int ce_forward(const rb200_linear_ce_params* p, cudaStream_t stream) {
     const bool bf16 = p->dtype == RB200_BF16;
     if ((rc = pack_operands(&s.x, &s.w, stream, what))) return rc;
     if (s.narrow) {
-        NarrowArgs g = narrow_args(*p);
+        NarrowArgs g = narrow_args(*p, wait);
         g.loss = p->loss;
         g.none = p->reduction == RB200_REDUCE_NONE;
         g.sums = s.block_sums;
@@ -382,7 +384,7 @@ static int ce_forward(const rb200_linear_ce_params* p, cudaStream_t stream) {
         count_launch();
         return RB200_OK;
     }
-    const GemmWait wait = {p->status, 0, -1};
+    wait.status = p->status;
     for (long long c0 = 0; c0 < p->classes; c0 += s.piece) {
         const int classes = (int)(p->classes - c0 < s.piece ? p->classes - c0 : s.piece);
         const GemmPlan plan = stats_gemm(*p, dev, classes);
@@ -512,7 +514,7 @@ static int narrow_join(const NarrowArgs& a, const rb200_linear_ce_params& p, con
     count_launch();
     return RB200_OK;
 }
-static int ce_backward(const rb200_linear_ce_params* p, cudaStream_t stream) {
+static int ce_backward(const rb200_linear_ce_params* p, cudaStream_t stream, GemmWait wait) {
     const char* what = "rb200k_linear_ce_backward";
     if (!p) {
         set_error("%s: params is null", what);
@@ -540,13 +542,13 @@ static int ce_backward(const rb200_linear_ce_params* p, cudaStream_t stream) {
     const GradPlan g = plan_grad(*p, dev, p->workspace);
     if ((rc = check_workspace(what, p->workspace, p->workspace_bytes, g.bytes))) return rc;
     const bool bf16 = p->dtype == RB200_BF16;
-    const GemmWait wait = {p->status, 0, -1};
+    wait.status = p->status;
     if ((rc = pack_operands(&g.x, &g.w, stream, what))) return rc;
     const bool none = p->reduction == RB200_REDUCE_NONE;
     if (none && (rc = factors_launch(*p, g.tops, g.coef, g.factor, stream, what))) return rc;
     const Scale scale(1.0f / 32768.0f, none ? g.factor : p->dloss, p->reduction == RB200_REDUCE_MEAN ? p->info : nullptr);
     if (g.narrow) {
-        NarrowArgs a = narrow_args(*p);
+        NarrowArgs a = narrow_args(*p, wait);
         a.coef = none ? g.coef : nullptr;
         a.dirty = p->info + 1;
         a.dx = p->dx;
@@ -646,15 +648,21 @@ static int ce_backward(const rb200_linear_ce_params* p, cudaStream_t stream) {
 
 using namespace rb200;
 
+static const GemmWait kNoProbe = {nullptr, 0, -1};
+
 extern "C" uint64_t rb200k_linear_ce_workspace_bytes(const rb200_linear_ce_params* p) {
     DeviceInfo dev;
     if (!p || check_sizes("rb200k_linear_ce_workspace_bytes", *p) || p->rows == 0 || device_info(&dev)) return 0;
     return plan_stats(*p, dev, nullptr).bytes;
 }
-extern "C" int rb200k_linear_ce(const rb200_linear_ce_params* p, void* stream) { return ce_forward(p, (cudaStream_t)stream); }
+extern "C" int rb200k_linear_ce(const rb200_linear_ce_params* p, void* stream) { return ce_forward(p, (cudaStream_t)stream, kNoProbe); }
 extern "C" uint64_t rb200k_linear_ce_backward_workspace_bytes(const rb200_linear_ce_params* p) {
     DeviceInfo dev;
     if (!p || check_sizes("rb200k_linear_ce_backward_workspace_bytes", *p) || p->rows == 0 || device_info(&dev)) return 0;
     return plan_grad(*p, dev, nullptr).bytes;
 }
-extern "C" int rb200k_linear_ce_backward(const rb200_linear_ce_params* p, void* stream) { return ce_backward(p, (cudaStream_t)stream); }
+extern "C" int rb200k_linear_ce_backward(const rb200_linear_ce_params* p, void* stream) { return ce_backward(p, (cudaStream_t)stream, kNoProbe); }
+extern "C" int rb200k_linear_ce_probe(const rb200_linear_ce_params* p, void* stream, int backward, uint64_t wait_cycles, int skip_block) {
+    const GemmWait wait = {nullptr, wait_cycles, skip_block};
+    return backward ? ce_backward(p, (cudaStream_t)stream, wait) : ce_forward(p, (cudaStream_t)stream, wait);
+}

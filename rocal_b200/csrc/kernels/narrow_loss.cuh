@@ -54,7 +54,8 @@ struct NarrowArgs {
     long long ldpart;
     int want_dw, want_db;
     int* status;
-    unsigned long long wait_cycles;
+    unsigned long long wait_cycles;   // 0: the ordinary limit
+    int skip_chunk;           // copies of x's chunks from this one on are left out (-1: none)
 };
 
 static __host__ __device__ inline uint32_t narrow_smem(int vb, int chunks, int slots, bool grad) {
@@ -148,7 +149,7 @@ __global__ void __launch_bounds__(narrow_threads(GRAD), 1) ce_narrow_kernel(cons
                     ok = tc::bar_wait(empty(s), phase ^ 1, patience);
                     if (!ok) break;
                     tc::bar_expect(full(s), kChunkBytes);
-                    tc::tma_load<1>(x0 + s * kChunkBytes, &g.x, c * kTileK, t * kTileM, full(s));
+                    if (g.skip_chunk < 0 || c < g.skip_chunk) tc::tma_load<1>(x0 + s * kChunkBytes, &g.x, c * kTileK, t * kTileM, full(s));
                     filled++;
                     if (++s == g.slots) {
                         s = 0;
@@ -654,7 +655,7 @@ static int narrow_launch(NarrowArgs& g, bool grad, bool bf16, const Operand& x, 
     if (rc) return rc;
     if ((rc = make_map(&g.w, w, bf16, g.vb, what))) return rc;
     if (!g.status) g.status = dev.status;
-    g.wait_cycles = kDefaultWaitCycles;
+    if (!g.wait_cycles) g.wait_cycles = kDefaultWaitCycles;
     if (grad) return bf16 ? narrow_launch_as<__nv_bfloat16, true>(g, dev, stream, what) : narrow_launch_as<__half, true>(g, dev, stream, what);
     return bf16 ? narrow_launch_as<__nv_bfloat16, false>(g, dev, stream, what) : narrow_launch_as<__half, false>(g, dev, stream, what);
 }

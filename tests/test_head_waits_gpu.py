@@ -56,3 +56,39 @@ def test_the_longest_sums_are_waited_for(cuda):
     loss, stats, info = K.linear_cross_entropy(x, w, torch.ones(1, dtype=torch.int64, device=cuda), reduction="sum", status=status)
     assert int(status) == 0 and float(stats[0]) == 11.0 and float(stats[2]) == 10.5                # scores 11 and 10.5
     assert abs(float(loss) - (11.0 - 10.5 + torch.log1p(torch.exp(torch.tensor(-0.5, dtype=torch.float64))).item())) <= 1e-6
+
+
+@pytest.mark.parametrize("backward", [False, True])
+@pytest.mark.parametrize("n,k,v", [(100, 256, 90), (40000, 256, 90), (40000, 128, 128), (300, 512, 200), (2000, 640, 3000)])
+def test_waits_of_the_loss_run_out(cuda, n, k, v, backward):
+    """Copies from the second block of the features on are left out, in the way for few classes (tiles fewer and more than the SMs) and in the
+    general one: every role gives up, the status word reads 1, and the next call on the same buffers is right."""
+    import ctypes
+    from rocal_b200 import kernels as K
+    from rocal_b200._lib import LinearCeParams, lib
+    g = torch.Generator(device=cuda).manual_seed(n + k + v)
+    x, w = (torch.randn((r, k), generator=g, device=cuda).half() / 8 for r in (n, v))
+    labels = torch.randint(0, v, (n,), generator=g, device=cuda)
+    loss, stats, info = K.linear_cross_entropy(x, w, labels, reduction="sum")
+    grads = K.linear_cross_entropy_backward(torch.ones_like(loss), x, w, labels, stats, info, reduction="sum")
+    status, one = torch.zeros(1, dtype=torch.int32, device=cuda), torch.ones((), device=cuda)
+    outs = [torch.zeros_like(t) for t in (loss, stats, info) + grads]
+    p = LinearCeParams()
+    p.dtype, p.reduction, p.rows, p.features, p.classes, p.label_bytes, p.ignore_index = 1, 2, n, k, v, 8, -100
+    p.x, p.ldx, p.weight, p.ldw, p.labels = x.data_ptr(), k, w.data_ptr(), k, labels.data_ptr()
+    p.loss, p.stats, p.info, p.dloss = outs[0].data_ptr(), outs[1].data_ptr(), outs[2].data_ptr(), one.data_ptr()
+    p.dx, p.lddx, p.dweight, p.lddw, p.dbias, p.status = outs[3].data_ptr(), k, outs[4].data_ptr(), k, outs[5].data_ptr(), status.data_ptr()
+    need = (lib.rb200k_linear_ce_backward_workspace_bytes if backward else lib.rb200k_linear_ce_workspace_bytes)(ctypes.byref(p))
+    ws = torch.empty(need, dtype=torch.uint8, device=cuda)
+    p.workspace, p.workspace_bytes = ws.data_ptr(), need
+    stream = torch.cuda.current_stream().cuda_stream
+    if backward:
+        outs[1].copy_(stats)
+        outs[2].copy_(info)
+    for skip, cycles, told in ((1, WAIT_CYCLES, 1), (0, WAIT_CYCLES, 1), (-1, WAIT_CYCLES * 1000, 0)):
+        status.zero_()
+        assert lib.rb200k_linear_ce_probe(ctypes.byref(p), stream, int(backward), cycles, skip) == 0
+        torch.cuda.synchronize()
+        assert int(status) == told, skip
+    for got, want in zip(outs[3:], grads) if backward else zip(outs[:2], (loss, stats)):
+        assert torch.equal(got, want)
