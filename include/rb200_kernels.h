@@ -386,8 +386,10 @@ RB200_API int rb200k_transpose(const uint8_t* arena, const rb200_pointwise_sampl
  * Matrices are row-major: element (i, j) at data[i * ld + j], ld in elements. All pointers are device pointers. Rows
  * that start on 16-byte boundaries (base address and ld * element size multiples of 16) are read in place; any other
  * operand of a matrix product is first copied into the workspace (not for up to four rows of rb200k_linear). Workspaces hold nothing of value between calls and
- * need no initialisation; two calls that can run at the same time need two workspaces. Results do not depend on
- * timing: no floating-point atomics are used. Every wait inside these kernels is bounded (see "Bounded waits"); trouble
+ * need no initialisation (the backward pass of the loss reserves room for a copy of x: rows that do not count but hold inf or NaN
+ * are found on the device); two calls that can run at the same time need two workspaces. Results do not depend on
+ * timing: no floating-point atomics are used. Every wait inside these kernels is bounded (see "Bounded waits"; the limit grows with
+ * the contracted axis); trouble
  * goes to `status` or, where that is NULL, to the library-wide status word. Outputs overlap neither inputs nor one
  * another (rb200k_grad_clip says where it allows that). The calls may be captured into a graph; make the first call on a device
  * before any capture (it looks up the device's properties and the status word's address). Launches overlap the tail of
@@ -463,7 +465,9 @@ RB200_API int rb200k_linear_backward(const rb200_linear_backward_params* params,
  * A row whose label equals ignore_index does not count: its loss is 0 and nothing flows back from or into it, whatever its
  * features hold (the padding of a last batch, anchors that matched nothing). A label that is neither ignore_index nor
  * a class makes the row's loss NaN. Classes may be masked by a bias of -inf or of the type's lowest value. Reductions:
- * NONE = one loss a row, SUM, MEAN = over the rows that count, 0 if none does. 32-bit sums; loss and stats are fp32. */
+ * NONE = one loss a row, SUM, MEAN = over the rows that count, 0 if none does. 32-bit sums; loss and stats are fp32. The scores'
+ * gradients are rounded to the element type (relative to the largest loss gradient G of a row with NONE) before they are multiplied with
+ * x and weight: in fp16 with G above 2^15, rows whose loss gradient is 2^-24 of G or less lose digits of their dx. */
 enum { RB200_REDUCE_NONE = 0, RB200_REDUCE_MEAN = 1, RB200_REDUCE_SUM = 2 };
 typedef struct rb200_linear_ce_params {
     int32_t dtype;               /* RB200_FP16 or RB200_BF16, of x, weight, bias and their gradients */
@@ -509,7 +513,7 @@ RB200_API int rb200k_linear_ce_probe(const rb200_linear_ce_params* params, void*
  * c = min(1, max_norm / (N + 1e-6)), every tensor's out = grad * (inv_scale * c), and *norm = N. inv_scale undoes the loss scale
  * of float16 training (1 otherwise). out may be grad itself (same type; nothing is written when inv_scale * c is 1) or
  * another array; no two outputs overlap, and no output overlaps another tensor's gradients (refused). Squares are added
- * in 64 bits, in an order that only depends on the tensors' sizes. A gradient with inf gives N = inf and c = 0, one
+ * in 64 bits, in an order that only depends on the tensors' sizes, on where they start within 16 bytes and on the device. A gradient with inf gives N = inf and c = 0, one
  * with NaN gives NaN everywhere. No alignment beyond the elements' own is needed; 16-byte boundaries are faster. Empty
  * tensors are skipped. `tensors` is a HOST array, not retained after return. */
 typedef struct rb200_grad_tensor {

@@ -12,10 +12,13 @@
 //               it took 900 to 2500 clocks and bounded products of up to 1024 contracted elements.
 // CG = 2: two CTAs (a cluster) work on one tile of 256 rows; each holds its 128 rows of A and half of the B tile, so a
 // tile of 256 columns takes 128 bytes of operands per SM and clock at the full rate of the tensor cores instead of 192.
-// The tensor cores cut the sums they add to where they do not fit 32 bits, always to the same side, so a long sum drifts (measured:
-// 3e-6 relative after 4096 products). That is far below a 16-bit result's rounding, but not below an fp32 loss': where that is
-// made, tiles of up to 128 columns, which leave TMEM columns free, spread the contracted axis over several accumulators,
-// 512 elements at least in each, and the epilogue adds them with correct rounding.
+// The tensor cores cut the sums they add to where they do not fit 32 bits, always towards zero, so a long sum drifts (measured, one
+// accumulator, relative to the root mean square of the sums: 0.7e-6 after 2048 products of normal numbers, 1.4e-6 after 4096, 3.0e-6
+// after 8192; of numbers of one sign 1.7e-6, 4.3e-6 and 11e-6). That is far below a 16-bit result's rounding, but not below an fp32
+// loss': where that is made, tiles of up to 128 columns, which leave TMEM columns free, spread the contracted axis over several
+// accumulators, 512 elements at least in each, and the epilogue adds them with correct rounding. And a sum near zero may come out on
+// its other side: a relu then passes or stops a gradient that it should not, for 0.3e-6 of the elements at 2048 products and 0.7e-6 at
+// 4096 (sums rounded to nearest: 0.1e-6 and 0.2e-6).
 // Either operand may have the contracted axis contiguous (K-major) or the other one (MN-major): the backward products
 // need no transposed copies. Rows and columns beyond the matrices arrive as zeros and are not stored.
 #pragma once
@@ -337,7 +340,8 @@ struct RunningSoftmax {
 };
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
 constexpr float kLog2e = 1.4426950408889634f;
-// exp(d) for a difference d <= 0 (or NaN): one special-function operation, 2^-22 relative.
+// exp(d) for a difference d <= 0 (or NaN): one special-function operation, 2^-22 relative, and the rounding of its argument,
+// |d| 2^-24 relative (a term that weighs exp(d) in a sum with one of 1).
 __device__ __forceinline__ float exp_diff(float d) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * kLog2e));
@@ -663,7 +667,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     copy_strip(area, reinterpret_cast<T*>(out), ld, vec, col, min(32, count), row0, g.m - row0, lane);
                 };
                 if constexpr (EPI == EPI_LINEAR || EPI == EPI_LINEAR_ADD) {
-                    if (g.e.preact) {
+                    if (g.e.preact) {   // in the element type: kept in 32 bits, z would add 4 bytes a value each way to a pass bound by memory
                         leave(g.e.preact, g.e.ldp, g.e.vec_pre);
                         __syncwarp();
                     }
@@ -785,6 +789,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     }
 #pragma unroll
                     for (int i = 0; i < 32; i++) v[i] = counted ? v[i] : 0.0f;   // whatever the row held
+                    // rounded to the element type, as an operand of two products has to be; column sums are made of what it was before
 #pragma unroll
                     for (int i = 0; i < 4; i++) st_shared16(staged(area, lane, i), pack8<T>(v + 8 * i));
                     if (g.e.col_part) {

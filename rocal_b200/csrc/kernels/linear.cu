@@ -8,7 +8,8 @@ namespace rb200 {
 // ---- sweeps over a gradient matrix ------------------------------------------------------------------------
 // Rows j, j + period, j + 2 period, ... of `src` are summed into partial sums [chunk][j][column] in 32 bits; with
 // `preact` the elements are first multiplied by the activation's slope, and with `dst` what was read (multiplied) is
-// written, in the element type. A block takes up to 256 columns (8 a thread, as many threads side by side as the columns
+// written, in the element type: dz is an operand of two products on the tensor cores, which take 16 bits, and splitting it into two
+// such numbers would double both (dx and dW are 1.4 times as far from 64 bits as with dz in 32 bits). A block takes up to 256 columns (8 a thread, as many threads side by side as the columns
 // need, the others on further rows) and a chunk of the repeats; a thread has two or four rows in flight. The row sums meet in
 // shared memory, chunks meet in sum_chunks_kernel, always in the same order. Bound by memory.
 struct RowsArgs {
@@ -613,12 +614,12 @@ static int backward_run(const rb200_linear_backward_params* p, void* stream_v) {
     if (p->dx) {
         e.out = p->dx;
         e.ldo = p->lddx;
-            if ((rc = gemm_store_joined(GEMM_KN, bf16, l.dz, l.w.use, nullptr, nullptr, l.gx, e, l.px, wait, stream, what))) return rc;
+        if ((rc = gemm_store_joined(GEMM_KN, bf16, l.dz, l.w.use, nullptr, nullptr, l.gx, e, l.px, wait, stream, what))) return rc;
     }
     if (p->dweight) {
         e.out = p->dweight;
         e.ldo = p->lddw;
-            Operand dzt = l.dz;
+        Operand dzt = l.dz;
         dzt.transposed = true;
         if ((rc = gemm_store_joined(GEMM_NN, bf16, dzt, l.x.use, nullptr, nullptr, l.gw, e, l.pw, wait, stream, what))) return rc;
     }

@@ -5,7 +5,10 @@
 //             that piece times W and transposed times x. Pieces are cut along the longer of classes and rows; the
 //             gradient that sums over pieces is accumulated in 32 bits.
 // Pieces hold (softmax - target) * c_i * 2^15 with |c_i| <= 1, so that a probability of 2^-29 is still a normal fp16;
-// the common factor (2^-15, the loss gradient, 1 / count) is applied to the 32-bit sums.
+// the common factor (2^-15, the loss gradient, 1 / count) is applied to the 32-bit sums. They are rounded to the element type once, as
+// operands of two products have to be. What fp16 loses of a row far below the largest is half of its least
+// step, 2^-25, for each class: 2^-40 G times the norm of a feature's weights in dx, with the common factor G. For G up to 2^15 that is about
+// half of dx' own least step; larger gradients of single rows' losses (reduction NONE) are named in rb200_kernels.h.
 // Few classes and features take one sweep over x each way instead (narrow_loss.cuh).
 #include "narrow_loss.cuh"
 
@@ -310,9 +313,11 @@ struct StatsPlan {
     double* block_sums;
     size_t bytes;
 };
-// The loss is made of 32-bit scores, which drift with the length of one accumulator's sum (the loss by 0.35e-6 at 2048 features, 0.65e-6
-// at 4096, with scores of variance 1; three times that with large ones). Longer sums take tiles that leave TMEM columns for a second
-// accumulator (gemm.cuh): 0.31e-6 at 4096, for 12% of time (8192 x 4096, 16384 classes: 738 -> 829 us).
+// The loss is made of 32-bit scores, which drift with the length of one accumulator's sum (gemm.cuh). The border is where the loss would
+// come off 64 bits by more than 1e-6 of itself: with scores of spread 2 (8192 rows, 16384 classes, fp16) it is off by 0.45e-6 at 1024
+// features, 0.87e-6 at 2048, 1.7e-6 at 4096. Longer sums take tiles that leave TMEM columns for a second accumulator: 0.85e-6 at 4096,
+// for 12 to 17% of time (714 -> 838 us). A border at 1024 would halve the error at 2048 (0.44e-6) for 19% of it (373 -> 442 us), four
+// accumulators beyond 4096 that at 8192 (1.7e-6 -> 0.83e-6) for 55%.
 constexpr int kLongSum = 2048;
 static GemmPlan stats_gemm(const rb200_linear_ce_params& p, const DeviceInfo& dev, int classes) {
     return gemm_plan(dev, (int)p.rows, classes, (int)p.features, false, false, p.features > kLongSum ? kTileNMax / 2 : kTileNMax);

@@ -314,6 +314,7 @@ __global__ void __launch_bounds__(narrow_threads(GRAD), 1) ce_narrow_kernel(cons
 #pragma unroll
                     for (int i = 0; i < 16; i++) v[i] = i < count ? v[i] : 0.0f;
                 }
+                // rounded to the element type: an operand of two products (column sums are made of what it was before)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {   // piece j of line r lies at j ^ (r % 8): the 128-byte swizzle
                     const int piece = col / 8 + i;

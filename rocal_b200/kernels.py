@@ -240,7 +240,9 @@ def transpose(arena, samples, perm, out_dims, out=None, d_samples=None, stream=N
 
 # ---- head operators -----------------------------------------------------------------------------
 # Tensors may live on any device; a call runs there, on `stream` or that device's current stream, and takes its workspace from
-# torch's allocator on that stream. Arguments are checked in the binding (ValueError); a failed library call is Rb200Error.
+# torch's allocator on that stream. Arguments are checked in the binding (ValueError); a failed library call is Rb200Error. These are
+# single launches outside autograd; a wait that ran out is read from `status` or rb200k_device_status(). plugin.pytorch has the
+# differentiable forms.
 
 
 class _on:

@@ -80,7 +80,9 @@ class ROCALClassificationIterator(ROCALGenericIterator):
 
 # ---- the head of a training or serving step, on the batches above -----------------------------------
 # Float16 and bfloat16 CUDA tensors; differentiable by torch.autograd, once (create_graph is refused, and so are the tangents of
-# forward-mode differentiation). Everything runs on the tensors' device, on its current stream.
+# forward-mode differentiation). Everything runs on the tensors' device, on its current stream. The calls are C++ functions, not
+# registered operators: torch.compile breaks its graph at them, and dispatch modes and the functions of tensor subclasses do not see
+# them.
 #
 # Waits inside the kernels are bounded (about a second, longer for long sums); one that runs out leaves its results unfinished. The next of these
 # calls then raises Rb200Error, and check_unfinished() does so behind the last one.
