@@ -66,7 +66,8 @@ struct EpiArgs {
     int label_bytes, classes, class0;
     long long ignore_index;
     float smooth_on, smooth_off;   // 1 - smoothing, smoothing / classes
-    float* part;              // STATS: [parts][m] maxima, then [parts][m] sums, then (smoothing) [parts][m] sums of z;
+    float inv_classes;
+    float* part;              // STATS: [parts][m] maxima, then [parts][m] sums, then (smoothing) [parts][m] sums of z / classes;
                               // two parts a tile
     int parts, want_zsum;
     float* zlabel;            // STATS: [m] the label's z
@@ -738,15 +739,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                             for (int i = 0; i < w; i++) a[i] = l & w ? a[i + w] : a[i];
                         if (label < g.n) g.e.zlabel[row] = a[0];
                     }
-                    if (g.e.want_zsum) {   // four sums, not one chain of 32
+                    // four sums, not one chain of 32; of z / classes: two classes that the type's lowest value masks add up to more than
+                    // fp32 holds, their mean does not
+                    if (g.e.want_zsum) {
+                        const float2 inv = make_float2(g.e.inv_classes, g.e.inv_classes);
                         float2 sum[2] = {};
                         if (count >= 32) {
 #pragma unroll
-                            for (int i = 0; i < 32; i += 2) sum[i >> 1 & 1] = add2(sum[i >> 1 & 1], make_float2(v[i], v[i + 1]));
+                            for (int i = 0; i < 32; i += 2) sum[i >> 1 & 1] = fma2(make_float2(v[i], v[i + 1]), inv, sum[i >> 1 & 1]);
                         } else {
 #pragma unroll
                             for (int i = 0; i < 32; i += 2)
-                                sum[i >> 1 & 1] = add2(sum[i >> 1 & 1], make_float2(i < count ? v[i] : 0.0f, i + 1 < count ? v[i + 1] : 0.0f));
+                                sum[i >> 1 & 1] = fma2(make_float2(i < count ? v[i] : 0.0f, i + 1 < count ? v[i + 1] : 0.0f), inv, sum[i >> 1 & 1]);
                         }
                         zsum += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                     }

@@ -19,7 +19,7 @@ constexpr size_t kPieceBytes = 256u << 20;   // scores' gradients of one piece
 
 // ---- forward: joining the partial statistics ----------------------------------------------------------------
 struct MergeArgs {
-    const float* part;      // [parts][rows] maxima, sums, sums of z
+    const float* part;      // [parts][rows] maxima, sums, sums of z / classes
     int parts, want_zsum;
     const void* labels;
     int label_bytes, classes, rows, reduction;
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(256) ce_merge_kernel(MergeArgs a) {
                 } else {
                     const float lse = logf(r.s);   // above the maximum
                     loss = (1.0f - a.smoothing) * (lse + (r.m - at_label));
-                    if (a.want_zsum) loss += a.smoothing * (lse + (r.m - z / (float)a.classes));
+                    if (a.want_zsum) loss += a.smoothing * (lse + (r.m - z));
                 }
             } else {
                 dirty_mine |= !(isfinite(r.m) && isfinite(r.s));
@@ -283,6 +283,7 @@ static EpiArgs label_args(const rb200_linear_ce_params& p) {
     e.ignore_index = p.ignore_index;
     e.smooth_on = 1.0f - p.label_smoothing;
     e.smooth_off = p.label_smoothing / (float)p.classes;
+    e.inv_classes = 1.0f / (float)p.classes;
     return e;
 }
 static NarrowArgs narrow_args(const rb200_linear_ce_params& p, const GemmWait& wait) {
@@ -294,6 +295,7 @@ static NarrowArgs narrow_args(const rb200_linear_ce_params& p, const GemmWait& w
     g.smoothing = p.label_smoothing;
     g.smooth_on = 1.0f - p.label_smoothing;
     g.smooth_off = p.label_smoothing / (float)p.classes;
+    g.inv_classes = 1.0f / (float)p.classes;
     g.stats = p.stats;
     g.status = p.status;
     g.wait_cycles = wait.cycles;

@@ -38,7 +38,7 @@ struct NarrowArgs {
     const void* labels;
     int label_bytes;
     long long ignore_index;
-    float smoothing, smooth_on, smooth_off;   // s, 1 - s, s / classes
+    float smoothing, smooth_on, smooth_off, inv_classes;   // s, 1 - s, s / classes, 1 / classes
     int none;                 // forward: a loss for every row
     float* stats;             // [3][rows]
     float* loss;              // forward, none: [rows]
@@ -401,15 +401,16 @@ __global__ void __launch_bounds__(narrow_threads(GRAD), 1) ce_narrow_kernel(cons
                         for (int i = 0; i < w; i++) a[i] = l & w ? a[i + w] : a[i];
                     z_label = a[0];
                 }
-                if (g.smoothing > 0.0f) {   // four sums, not one chain of 32
+                if (g.smoothing > 0.0f) {   // four sums, not one chain of 32; of z / classes, as in gemm.cuh
+                    const float2 inv = make_float2(g.inv_classes, g.inv_classes);
                     float2 sum[2] = {};
                     if (count >= 32) {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) sum[i >> 1 & 1] = add2(sum[i >> 1 & 1], make_float2(v[i], v[i + 1]));
+                        for (int i = 0; i < 32; i += 2) sum[i >> 1 & 1] = fma2(make_float2(v[i], v[i + 1]), inv, sum[i >> 1 & 1]);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 32; i += 2)
-                            sum[i >> 1 & 1] = add2(sum[i >> 1 & 1], make_float2(i < count ? v[i] : 0.0f, i + 1 < count ? v[i + 1] : 0.0f));
+                            sum[i >> 1 & 1] = fma2(make_float2(i < count ? v[i] : 0.0f, i + 1 < count ? v[i + 1] : 0.0f), inv, sum[i >> 1 & 1]);
                     }
                     zsum += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 }
@@ -447,7 +448,7 @@ __global__ void __launch_bounds__(narrow_threads(GRAD), 1) ce_narrow_kernel(cons
                     } else {
                         const float lse = logf(run.s);   // above the maximum
                         loss = g.smooth_on * (lse + (run.m - z_label));
-                        if (g.smoothing > 0.0f) loss += g.smoothing * (lse + (run.m - zsum / (float)g.classes));
+                        if (g.smoothing > 0.0f) loss += g.smoothing * (lse + (run.m - zsum));
                     }
                 } else {
                     dirts |= !(isfinite(run.m) && isfinite(run.s));
