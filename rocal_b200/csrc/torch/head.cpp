@@ -83,18 +83,22 @@ bool has_rows(const Tensor& t) {
 }
 int64_t pitch(const Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
 
+// What the kernels read are the bytes: a view whose negation is still to come (the imaginary part of a conjugate) is made first.
+Tensor settled(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // A matrix of the input's type and device, its rows contiguous (copied if need be).
 Tensor matrix(const Tensor& t, const char* name, const Tensor& like, int64_t rows, int64_t cols) {
     TORCH_CHECK_VALUE(t.dim() == 2, name, " has ", t.dim(), " dimensions, a matrix is needed");
     same_kind(t, name, like);
     TORCH_CHECK_VALUE(cols < 0 || t.size(1) == cols, name, " has ", t.size(1), " columns, ", cols, " are needed");
     TORCH_CHECK_VALUE(rows < 0 || t.size(0) == rows, name, " has ", t.size(0), " rows, ", rows, " are needed");
-    return has_rows(t) ? t : t.contiguous();
+    const Tensor s = settled(t);
+    return has_rows(s) ? s : s.contiguous();
 }
 Tensor vector(const Tensor& t, const char* name, const Tensor& like, int64_t n) {
     TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == n, name, " has shape ", t.sizes(), ", (", n, ",) is needed");
     same_kind(t, name, like);
-    return t.contiguous();
+    return settled(t).contiguous();
 }
 bool given(const MaybeTensor& t) { return t.has_value() && t->defined(); }
 Tensor or_undefined(const MaybeTensor& t) { return given(t) ? *t : Tensor(); }
@@ -186,7 +190,7 @@ Tensor linear_run(const Tensor& x_, const Tensor& weight_, const Tensor& bias_, 
         p.residual_rows = r;
     }
     if (out.defined()) {
-        TORCH_CHECK_VALUE(out.dim() == 2 && out.size(0) == n && out.size(1) == m && has_rows(out), "out has shape ", out.sizes(), ", strides ",
+        TORCH_CHECK_VALUE(out.dim() == 2 && out.size(0) == n && out.size(1) == m && has_rows(out) && !out.is_neg(), "out has shape ", out.sizes(), ", strides ",
                           out.strides(), "; (", n, ", ", m, ") with contiguous rows is needed");
         same_kind(out, "out", x);
         written(out);
@@ -426,7 +430,7 @@ std::vector<Tensor> ce_backward_run(const Tensor& dloss_, const Tensor& x, const
                           stats.device() == x.device() && info.dim() == 1 && info.size(0) == 4 && info.scalar_type() == at::kInt &&
                           info.is_contiguous() && info.device() == x.device(),
                       "stats and info are not those of this forward pass");
-    const Tensor dloss = dloss_.contiguous();
+    const Tensor dloss = settled(dloss_).contiguous();
     std::vector<Tensor> g(3);
     if (need[0]) a.p.dx = (g[0] = at::empty({n, k}, x.options())).data_ptr();
     if (need[1]) a.p.dweight = (g[1] = at::empty({v, k}, x.options())).data_ptr();
@@ -618,15 +622,15 @@ Tensor grad_clip(const py::object& grads_, double max_norm, const py::object& ou
         t.count = g.numel();
         TORCH_CHECK_VALUE(o.numel() == t.count, "an output has ", o.numel(), " elements for a gradient of ", t.count);
         TORCH_CHECK_VALUE(t.out_dtype == t.grad_dtype || t.out_dtype == RB200_FP32, "an output is ", o.scalar_type(), " for a gradient ", g.scalar_type());
-        const bool plain = g.is_contiguous() && (!apart || o.is_contiguous());
-        if (plain || (g.is_non_overlapping_and_dense() && (!apart || (o.sizes() == g.sizes() && o.strides() == g.strides())))) {
+        const bool settled_both = !g.is_neg() && !o.is_neg(), plain = g.is_contiguous() && (!apart || o.is_contiguous());
+        if (settled_both && (plain || (g.is_non_overlapping_and_dense() && (!apart || (o.sizes() == g.sizes() && o.strides() == g.strides()))))) {
             t.grad = g.data_ptr();
             t.out = o.data_ptr();
             continue;
         }
         TORCH_CHECK_VALUE(o.sizes() == g.sizes(), "an output has shape ", o.sizes(), " for a gradient ", g.sizes());
         copied[i] = true;
-        Tensor dense = g.contiguous(), result = !apart ? dense : o.is_contiguous() ? o : at::empty(o.sizes(), o.options());
+        Tensor dense = settled(g).contiguous(), result = !apart ? dense : o.is_contiguous() && !o.is_neg() ? o : at::empty(o.sizes(), o.options());
         if (!result.is_same(o)) back.emplace_back(o, result);
         t.grad = dense.data_ptr();
         t.out = result.data_ptr();
