@@ -86,10 +86,14 @@ int make_map(CUtensorMap* map, const Operand& o, bool bf16, int box_rows, const 
 //   the last tile's epilogue is not hidden, and pieces of the contracted axis have to be joined by another launch (about 8000,
 //   half of it on the host). Clusters whose CTAs join their pieces through distributed shared memory were tried instead: 14 us against
 //   9 us for one row of 2048 x 1000, because clusters of full-size CTAs do not fill the GPU.
+// A sum of very many products is cut whatever the model says, so that what the tensor cores cut off stays small (gemm.cuh): 32768 products of
+// one sign in one accumulator come off by 1e-4, a fifth of half an fp16 step. (524288 rows in one: 3e-3.)
+constexpr int kLongestSum = 32768;
 GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed, bool may_split, int bn_most) {
     GemmPlan best = {};
     double best_cost = 0;
     const int kblocks = (k + kTileK - 1) / kTileK, a_rows = m < kTileM ? m : kTileM;
+    const long long least = may_split ? (k + (long long)kLongestSum - 1) / kLongestSum : 1;
     for (int cg = 2; cg >= 1; cg--) {
         if (cg == 2 && m <= kTileM) continue;
         const int unit = (b_transposed ? 64 : 32) * cg, slots = dev.sms / cg;
@@ -100,12 +104,12 @@ GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed
             const long long tiles = (long long)tiles_m * tiles_n;
             const double products = 2.0 * bn > 290 ? 2.0 * bn : 290, epilogue = 16.0 * bn + 500;
             // one piece, or as many as the free SMs take in one or two rounds
-            long long choices[3] = {1, 1, 1};
+            long long choices[3] = {least, least, least};
             if (may_split && kblocks >= 16) {
                 for (int r = 1; r <= 2; r++) {
                     long long s = r * slots / tiles;
                     if (s > kblocks / 8) s = kblocks / 8;
-                    choices[r] = s > 1 ? s : 1;
+                    choices[r] = s > least ? s : least;
                 }
             }
             for (long long s : choices) {

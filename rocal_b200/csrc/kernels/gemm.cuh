@@ -14,8 +14,8 @@
 // tile of 256 columns takes 128 bytes of operands per SM and clock at the full rate of the tensor cores instead of 192.
 // The tensor cores cut the sums they add to where they do not fit 32 bits, always towards zero, so a long sum drifts (measured, one
 // accumulator, relative to the root mean square of the sums: 0.7e-6 after 2048 products of normal numbers, 1.4e-6 after 4096, 3.0e-6
-// after 8192; of numbers of one sign 1.7e-6, 4.3e-6 and 11e-6). That is far below a 16-bit result's rounding, but not below an fp32
-// loss': where that is made, tiles of up to 128 columns, which leave TMEM columns free, spread the contracted axis over several
+// after 8192, 26e-6 after 65536; of numbers of one sign 1.7e-6, 4.3e-6, 11e-6 and 0.19e-3, and 3e-3 after 524288). Up to 32768 products, which
+// is where sums are split (gemm_plan), that is well below a 16-bit result's rounding, but not below an fp32 loss': where that is made, tiles of up to 128 columns, which leave TMEM columns free, spread the contracted axis over several
 // accumulators, 512 elements at least in each, and the epilogue adds them with correct rounding. And a sum near zero may come out on
 // its other side: a relu then passes or stops a gradient that it should not, for 0.3e-6 of the elements at 2048 products and 0.7e-6 at
 // 4096 (sums rounded to nearest: 0.1e-6 and 0.2e-6).

@@ -132,3 +132,26 @@ def test_drift_of_long_sums(cuda, dtype):
         loss = K.linear_cross_entropy(x, w, labels, reduction="none")[0].double()
         drift[k] = float((loss - exact).sum() / exact.sum())
     assert abs(drift[2048]) <= 1.0e-6 and abs(drift[4096]) <= 1.0e-6, drift
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_sums_over_very_many_rows(cuda, dtype):
+    """Products of one sign, the worst that cutting can meet: a long sum in one accumulator drifts by 2.9e-9 of itself for every product (measured
+    up to 65536 of them), 524288 rows by 3e-3. Split as they are, they must not drift by more than 2.44e-4, half of an fp16 result's half
+    step. (The tiles alone nearly fill the GPU, so that nothing else splits the sum.)"""
+    from rocal_b200 import kernels as K
+    g = torch.Generator(device=cuda).manual_seed(4)
+    n, m, k = 524288, 2048, 2048
+    x = torch.rand((n, k), generator=g, device=cuda, dtype=torch.float32).to(TYPES[dtype])
+    dout = (torch.rand((n, m), generator=g, device=cuda, dtype=torch.float32) / 16).to(TYPES[dtype])
+    dw = K.linear_backward(dout, x, torch.zeros((m, k), dtype=TYPES[dtype], device=cuda), need=(False, True, False, False))[1].double()
+    exact = torch.zeros((m, k), dtype=torch.float64, device=cuda)
+    for a, b in zip(dout.split(65536), x.split(65536)):
+        exact += a.double().t() @ b.double()
+    off = (dw - exact) / exact
+    half = torch.finfo(TYPES[dtype]).eps / 2
+    assert float(off.abs().max()) <= half + 2.44e-4, float(off.abs().max())
+    # the mean, but for the roundings' own: the sums are 8192 with a spread of 10, bfloat16's step is 32 below and 64 above it, so that its
+    # roundings all go to 8192 and do not cancel
+    rounded = (exact.to(TYPES[dtype]).double() - exact) / exact
+    assert abs(float((off - rounded).mean())) <= 2.44e-4, float((off - rounded).mean())
