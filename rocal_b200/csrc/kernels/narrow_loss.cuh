@@ -618,9 +618,12 @@ static inline bool narrow_fits(long long classes, long long features) {
     const int chunks = (int)((features + 127) / 128) * 2;
     return narrow_smem((int)round_up(classes, 32), chunks, 2 * chunks, true) <= kNarrowSmem;
 }
+// One for every SM - or as many as it takes for none to add up more than 32768 rows: sums on the tensor cores drift (gemm.cuh; 2^25 rows of
+// one sign over 148 CTAs: 1.1e-3).
+constexpr int kNarrowTiles = 32768 / kTileM;
 static inline int narrow_ctas(long long rows, int sms) {
-    const long long tiles = (rows + kTileM - 1) / kTileM;
-    return (int)(tiles < sms ? tiles : sms);
+    const long long tiles = (rows + kTileM - 1) / kTileM, least = (tiles + kNarrowTiles - 1) / kNarrowTiles, most = tiles < sms ? tiles : sms;
+    return (int)(least > most ? least : most);
 }
 
 template <typename T, bool GRAD>

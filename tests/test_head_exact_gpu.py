@@ -155,3 +155,24 @@ def test_sums_over_very_many_rows(cuda, dtype):
     # roundings all go to 8192 and do not cancel
     rounded = (exact.to(TYPES[dtype]).double() - exact) / exact
     assert abs(float((off - rounded).mean())) <= 2.44e-4, float((off - rounded).mean())
+
+
+def test_few_classes_over_very_many_rows(cuda):
+    """The same for the way of few classes, where a block adds up all of its rows: weights of zero and one label for all rows make the other
+    class' gradient half the sum of the features, all of one sign. 2^25 rows are 226720 for each of 148 blocks, which drift by 6.6e-4 and
+    more. Features of 64 sizes within a binade, so that the mean of the 64 roundings is within 2^-11 / 3 ** 0.5 / 8 = 3.5e-5 (one spread)."""
+    from rocal_b200 import kernels as K
+    g = torch.Generator(device=cuda).manual_seed(6)
+    n, k = 1 << 25, 64
+    x = torch.empty((n, k), dtype=torch.float16, device=cuda)
+    exact = torch.zeros(k, dtype=torch.float64, device=cuda)
+    for part in x.split(1 << 21):
+        part.copy_(torch.rand(part.shape, generator=g, device=cuda) * (1 + torch.arange(k, device=cuda) / k))
+        exact += part.double().sum(0) / 2
+    w, labels = torch.zeros((2, k), dtype=torch.float16, device=cuda), torch.zeros(n, dtype=torch.int32, device=cuda)
+    loss, stats, info = K.linear_cross_entropy(x, w, labels, reduction="sum")
+    dw = K.linear_cross_entropy_backward(torch.full_like(loss, 2.0 ** -12), x, w, labels, stats, info, reduction="sum", need=(False, True, False))[1].double()
+    exact *= 2.0 ** -12
+    assert torch.equal(dw[0], -dw[1])
+    off = (dw[1] - exact) / exact
+    assert float(off.abs().max()) <= 2.0 ** -11 + 2.44e-4 and abs(float(off.mean())) <= 2.44e-4, (float(off.abs().max()), float(off.mean()))
