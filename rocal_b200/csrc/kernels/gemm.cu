@@ -87,7 +87,8 @@ int make_map(CUtensorMap* map, const Operand& o, bool bf16, int box_rows, const 
 //   half of it on the host). Clusters whose CTAs join their pieces through distributed shared memory were tried instead: 14 us against
 //   9 us for one row of 2048 x 1000, because clusters of full-size CTAs do not fill the GPU.
 // A sum of very many products is cut whatever the model says, so that what the tensor cores cut off stays small (gemm.cuh): 32768 products of
-// one sign in one accumulator come off by 1e-4, a fifth of half an fp16 step. (524288 rows in one: 3e-3.)
+// one sign in one accumulator come off by 1e-4, a fifth of half an fp16 step. (524288 rows in one: 3e-3. Split, 524288 x 2048 x 2048 takes
+// 3.6 -> 3.8 ms; 131072 x 4096 x 1024 and 65536 x 4096 x 4096 as long as before, within the 5% that runs differ by.)
 constexpr int kLongestSum = 32768;
 GemmPlan gemm_plan(const DeviceInfo& dev, int m, int n, int k, bool b_transposed, bool may_split, int bn_most) {
     GemmPlan best = {};
