@@ -48,12 +48,14 @@ HEAD_STAMP = os.path.join(OBJ_DIR, "_head.stamp")     # what _head.so was compil
 def head_versions():
     """The torch and Python that _head.so has to be compiled against, or None without a torch that has CUDA. (torch is not
     imported: that takes longer than looking whether anything has to be built.)"""
-    import importlib.metadata
     import importlib.util
+    import re
     spec = importlib.util.find_spec("torch")
     if spec is None or not os.path.exists(os.path.join(os.path.dirname(spec.origin), "lib", "libc10_cuda.so")):
         return None
-    return "torch %s, Python %d.%d" % ((importlib.metadata.version("torch"),) + sys.version_info[:2])
+    with open(os.path.join(os.path.dirname(spec.origin), "version.py")) as f:     # there without a package's metadata, too
+        version = re.search(r"__version__\s*=\s*['\"]([^'\"]+)", f.read())
+    return "torch %s, Python %d.%d" % ((version.group(1) if version else "of no version",) + sys.version_info[:2])
 
 
 def head_stamp():

@@ -51,6 +51,19 @@ def test_the_library_builds_without_torch(build, monkeypatch, capsys):
     assert "not built" in capsys.readouterr().err
 
 
+def test_the_version_is_torch_s_own(monkeypatch):
+    """Also where torch has no package metadata (a build from sources on the path)."""
+    import importlib.metadata
+
+    import torch
+    from rocal_b200 import build as B
+
+    def missing(name):
+        raise importlib.metadata.PackageNotFoundError(name)
+    monkeypatch.setattr(importlib.metadata, "version", missing)
+    assert B.head_versions() == "torch %s, Python %d.%d" % ((torch.__version__,) + sys.version_info[:2])
+
+
 def test_a_torch_without_cuda_has_no_binding(build, monkeypatch, tmp_path):
     import importlib.machinery
     import importlib.util
