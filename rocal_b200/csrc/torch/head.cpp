@@ -588,10 +588,11 @@ void refuse_overlaps(const TensorList& grads, const TensorList& out, bool apart,
         if (apart) ins.emplace_back(grads[i]);
     }
     for (size_t i = 0; i < outs.size(); i++) {
-        bool meets = copied[i] && overlaps_itself(out[i]);
+        if (!copied[i]) continue;
+        bool meets = overlaps_itself(out[i]);
         for (size_t j = 0; j < outs.size() && !meets; j++) {
-            if (j == i || !(copied[i] || copied[j])) continue;
-            meets = (j > i && share_memory(outs[i], outs[j])) || (apart && share_memory(outs[i], ins[j]));
+            if (j == i || (copied[j] && j < i)) continue;   // that pair has been looked at
+            meets = share_memory(outs[i], outs[j]) || (apart && (share_memory(outs[i], ins[j]) || share_memory(outs[j], ins[i])));
         }
         if (meets) throw LibraryError("grad_clip: an output overlaps itself, another output or another tensor's gradients");
     }
