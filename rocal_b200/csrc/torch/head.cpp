@@ -115,7 +115,7 @@ int32_t* status_word(const MaybeTensor& status, const Tensor& like) {
     return status->data_ptr<int32_t>();
 }
 // Waits inside the products are bounded: one that gives up leaves its results unfinished and raises a status word. Calls for which
-// the caller gives no word of his own through the kernel layer (single launches: the library-wide word) raise this one, which lies
+// the caller gives no word of their own through the kernel layer (single launches: the library-wide word) raise this one, which lies
 // in pinned host memory: the host reads it without waiting, and the next call says what has happened. Kept for the whole process; captured
 // graphs hold its address.
 int32_t* unfinished_word() {
