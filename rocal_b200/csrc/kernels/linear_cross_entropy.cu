@@ -315,11 +315,12 @@ struct StatsPlan {
     double* block_sums;
     size_t bytes;
 };
-// The loss is made of 32-bit scores, which drift with the length of one accumulator's sum (gemm.cuh). The border is where the loss would
-// come off 64 bits by more than 1e-6 of itself: with scores of spread 2 (8192 rows, 16384 classes, fp16) it is off by 0.45e-6 at 1024
-// features, 0.87e-6 at 2048, 1.7e-6 at 4096. Longer sums take tiles that leave TMEM columns for a second accumulator: 0.85e-6 at 4096,
-// for 12 to 17% of time (714 -> 838 us). A border at 1024 would halve the error at 2048 (0.44e-6) for 19% of it (373 -> 442 us), four
-// accumulators beyond 4096 that at 8192 (1.7e-6 -> 0.83e-6) for 55%.
+// The loss is made of 32-bit scores, which drift with the length of one accumulator's sum (gemm.cuh). The border is where the loss comes
+// off 64 bits by some 1e-6 of itself: with scores of spread 2 (8192 rows, 16384 classes, fp16) it is off by 0.45e-6 at 1024 features,
+// 0.87e-6 at 2048, 1.7e-6 at 4096; a loss that is small beside its scores by more, 1.2e-6 with 227 classes at 1875. Longer sums take
+// tiles that leave TMEM columns for a second accumulator: 0.85e-6 at 4096, for 12 to 17% of time (714 -> 838 us). A border at 1024 would
+// halve the error at 2048 (0.44e-6), for 4.5% of a training step (8192 x 2048, 128000 classes: 13.3 -> 13.9 ms) and 16% of an evaluation
+// (64 x 2048, 21841 classes: 25.1 -> 29.2 us); four accumulators beyond 4096 that at 8192 (1.7e-6 -> 0.83e-6), for 55% of the forward pass.
 constexpr int kLongSum = 2048;
 static GemmPlan stats_gemm(const rb200_linear_ce_params& p, const DeviceInfo& dev, int classes) {
     return gemm_plan(dev, (int)p.rows, classes, (int)p.features, false, false, p.features > kLongSum ? kTileNMax / 2 : kTileNMax);
